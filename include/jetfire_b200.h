@@ -482,6 +482,71 @@ jf_status_t jf_alloc_mapped_on_node(uint64_t bytes, int32_t node, void** host_pt
 jf_status_t jf_set_cpu_attn_node(int32_t node);
 int32_t     jf_get_cpu_attn_node(void);
 
+/* ---- attention over a cache of 8-bit codes with one scale per block and head ---------------------
+ * No counterpart in the reference, whose release modes hold 2 to 4 bits per element.  The format for
+ * layers that need more than that, without a host mirror and its correction:
+ *
+ *   k_data, v_data     (H_kv, num_blocks * 16, 128) codes: signed 8-bit integers, or e4m3
+ *   k_scales, v_scales (H_kv, num_blocks) fp32, one per block of 16 positions and KV head
+ *
+ * An element is code * scale.  With a = max(largest finite magnitude written, 2^-100):
+ *   int8  scale = a / 127 rounded to fp32; code = rint(fp32(x * fp32(1 / scale))), half to even
+ *   e4m3  scale = the smallest power of two with a <= 448 * scale; code = e4m3(x / scale), half to even
+ * NaN is stored as 0, an infinity as the largest code.
+ *
+ * jf_block8_append writes the new tokens of n_seqs sequences: rows query_start_loc[i] .. [i+1] of key /
+ * value (T, H_kv, 128) are the last positions below seq_lens[i], which counts them already.  A block
+ * that holds earlier positions of its sequence keeps the larger of its scale and the one that its new
+ * rows ask for; where the scale grows the earlier rows become round(code * fp32(old / new)).  A block
+ * begun by the call takes nothing from what it held before.  Rows behind query_start_loc[n_seqs],
+ * positions below 0, and positions without a valid block of the table are skipped; rows of a block
+ * behind the last position are left alone.  The blocks written by one call belong to one sequence each.
+ *
+ * jf_block8_attn attends with one query token per sequence, at position seq_lens[b] - 1:
+ *   s_j = attn_scale * q.k_j, then softcap * tanh(s_j / softcap) if softcap > 0, then
+ *   - alibi_slopes[head] * (seq_lens[b] - 1 - j) if alibi_slopes is given;
+ *   out = softmax(s).v, lse = log sum exp(s),
+ * over the positions j of [seq_lens[b] - window, seq_lens[b]) and [0, prefix_lens[b]) (all of them if
+ * window is 0) whose block id is valid; out = 0 and lse = -inf where there is none.  seq_lens is cut to
+ * [0, min(max_S, 16 * max_blocks)].  q, out (B, H_q, 128), lse (B, H_q) f32 or null, all contiguous.
+ * Two launches at most; workspace as for the entry points above (jf_block8_workspace_bytes, 0 = bad
+ * shape), needed no longer than the call's launches.  Block ids are 64-bit or 32-bit integers, rows
+ * bt_stride ids apart. */
+enum { JF_CODES_INT8 = 0, JF_CODES_E4M3 = 1 };
+
+typedef struct jf_block8_attn_args {
+  int32_t codes, q_dtype;
+  int32_t B, H_q, H_kv, max_S;
+  int32_t max_blocks, bt_is_i32;
+  int32_t window;                 /* 0: none */
+  float   attn_scale, softcap;    /* softcap 0: none */
+  int32_t reserved;
+  int64_t num_blocks, bt_stride;
+  const void*    q;
+  const void*    k_data;
+  const float*   k_scales;
+  const void*    v_data;
+  const float*   v_scales;
+  const void*    block_table;
+  const int32_t* seq_lens;
+  const int32_t* prefix_lens;     /* (B,) or null */
+  const float*   alibi_slopes;    /* (H_q,) or null */
+  void*          out;
+  float*         lse;             /* may be null */
+  void*          workspace;
+  uint64_t       workspace_bytes;
+} jf_block8_attn_args;
+
+jf_status_t jf_block8_append(const void* key, const void* value, int32_t dtype, int64_t T, int32_t H_kv,
+                             int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                             int64_t v_stride_h, const int32_t* query_start_loc,
+                             const int32_t* seq_lens, int32_t n_seqs, const void* block_table,
+                             int32_t bt_is_i32, int64_t bt_stride, int32_t max_blocks, int32_t codes,
+                             void* k_data, float* k_scales, void* v_data, float* v_scales,
+                             int64_t num_blocks, jf_stream_t stream);
+uint64_t    jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S);
+jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,7 @@ JF_DTYPE_BF16, JF_DTYPE_FP16 = 0, 1
 JF_MODE_K3V2, JF_MODE_K4V4 = 0, 1
 JF_SCAN_ALL, JF_SCAN_K_ONLY, JF_SCAN_V_ONLY = 0, 1, 2
 JF_STAGE_B_FP32, JF_STAGE_B_INT8P = 0, 1
+JF_CODES_INT8, JF_CODES_E4M3 = 0, 1
 
 
 class JetFireError(RuntimeError):
@@ -44,6 +45,20 @@ class DecodeArgs(C.Structure):
         ("softmax_m", C.c_void_p), ("softmax_inv_z", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
         ("topk_slots_i32", C.c_void_p),
+    ]
+
+
+class Block8AttnArgs(C.Structure):
+    _fields_ = [
+        ("codes", C.c_int32), ("q_dtype", C.c_int32),
+        ("B", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32), ("max_S", C.c_int32),
+        ("max_blocks", C.c_int32), ("bt_is_i32", C.c_int32), ("window", C.c_int32),
+        ("attn_scale", C.c_float), ("softcap", C.c_float), ("reserved", C.c_int32),
+        ("num_blocks", C.c_int64), ("bt_stride", C.c_int64),
+        ("q", C.c_void_p), ("k_data", C.c_void_p), ("k_scales", C.c_void_p),
+        ("v_data", C.c_void_p), ("v_scales", C.c_void_p), ("block_table", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("prefix_lens", C.c_void_p), ("alibi_slopes", C.c_void_p),
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -146,6 +161,11 @@ _SIGS = {
     "jf_submit_ctx_set_rows": (C.c_int32, [C.c_int64, C.c_int64, C.c_int64]),
     "jf_stream_signal_host": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "jf_stream_wait_host_flag": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "jf_block8_append": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32] + [C.c_int64] * 4 +
+                         [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32] +
+                         [C.c_void_p] * 4 + [C.c_int64, C.c_void_p]),
+    "jf_block8_workspace_bytes": (C.c_uint64, [C.c_int32] * 4),
+    "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
     "jf_alloc_mapped": (C.c_int32, [C.c_uint64, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "jf_free_mapped": (C.c_int32, [C.c_void_p]),
 }

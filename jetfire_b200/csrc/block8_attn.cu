@@ -1,0 +1,579 @@
+// Decode attention over the cache of 8-bit codes with one scale per block of 16 positions and KV head.
+//
+//   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(f(attn_scale * q.k_j) + bias_j)
+//
+// Both products run on the tensor cores with fp16 operands that hold the codes exactly (an int8 code is an integer
+// below 2^7; an e4m3 code times 2^-8 is a bit shift of itself); the scales stay outside, in fp32.  q goes to fp16 by a power of two
+// per head that brings its largest element to [2^13, 2^14): what that rounds is 2^-38 of it.  The tile of a product
+// is one block: scores as K (16 positions) x q^T (8 heads of the group, NT times), outputs as V^T (8 x 16 dims) x p^T.
+// Channels and positions are contracted in whatever order the lanes hold them, so each lane takes 16-byte pieces of the
+// rows as they lie in memory and turns them into operands in its own registers: no transposition, and shared memory
+// holds only what the lane itself copied there.
+//
+// A warp goes through its blocks with a running reference m for every head, the sum of its weights and the output
+// unnormalised.  The V scale of a block joins the exponent: w = exp2(s + log2(vs) - m) is what meets the codes, in
+// fp16 (rounded to 11 bits: relative 2^-12 per weight, unbiased), and w / vs in fp32 what the sum gets.  m may lag the
+// maximum by up to kLag, so that most blocks need one vote and no reduction.
+//
+// Work: the blocks of every sequence are cut into pieces of one length for the whole batch, chosen on the device from the lengths
+// so that the pieces of a KV head fill about one wave; the pieces' partial results meet in a second kernel.  A
+// sequence of one piece is written by the first kernel itself.
+//
+// Bound: memory, 256 bytes per (position, KV head).
+#include "jf_common.cuh"
+
+#include <algorithm>
+
+namespace jf {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kStages = 3;                    // blocks of K and V in flight per warp
+constexpr int kStageBytes = 2 * JF_BLOCK_SIZE * JF_HEAD_DIM;
+// The reference of the fp16 weights lies 2^kLift below the maximum it was taken from and may lag the present one by
+// 2^kLag: weights stay below 2^15, and what fp16 flushes to zero is below 2^-33 of the largest (a long row's many small weights add up).
+constexpr float kLift = 9.0f, kLag = 6.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
+  const void* q;
+  const uint8_t *k_data, *v_data;
+  const float *k_scales, *v_scales;
+  const void* table;
+  const int32_t *seq_lens, *prefix_lens;
+  const float* slopes;
+  void* out;
+  float* lse;
+  float *part_o, *part_ml;      // [piece][kv head, group of heads][8 * NT][128] and [..][2]
+  int64_t num_blocks, bt_stride;
+  int32_t B, H_q, H_kv, G, groups, max_S, max_blocks, window, target, min_piece, pieces;
+  float scale, softcap;
+  bool bt_i32;
+};
+
+// What of a sequence is scanned: its first `head` blocks and the `count - head` blocks that end with its last position.
+struct Span { int len, prefix, lo, head, first, count; };
+__device__ __forceinline__ Span span_of(const AttnParams& P, int b) {
+  Span s;
+  s.len = max(0, min(P.seq_lens[b], min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
+  const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
+  s.prefix = s.lo = s.head = s.first = 0;
+  s.count = blocks;
+  if (P.window > 0 && P.window < s.len) {
+    s.lo = s.len - P.window;
+    s.prefix = P.prefix_lens ? max(0, min(P.prefix_lens[b], s.lo)) : 0;
+    s.first = s.lo / JF_BLOCK_SIZE;
+    s.head = min((s.prefix + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, s.first);
+    s.count = s.head + blocks - s.first;
+  }
+  return s;
+}
+// Blocks per piece, and whose piece `x` is: the first piece of sequence b is the sum of those before.
+struct Cut { int piece, b, index, n; };
+__device__ __forceinline__ int piece_length(const AttnParams& P, int total) {
+  return max(P.min_piece, (total + P.target - 1) / P.target);
+}
+// All lanes of a warp; b = -1 if there is no such piece.
+__device__ __forceinline__ Cut find_piece(const AttnParams& P, int x) {
+  const int lane = threadIdx.x & 31;
+  int total = 0, mine = 0;
+  for (int b0 = 0; b0 < P.B; b0 += 32) {
+    mine = b0 + lane < P.B ? span_of(P, b0 + lane).count : 0;
+    total += __reduce_add_sync(0xFFFFFFFFu, mine);
+  }
+  Cut c{piece_length(P, total), -1, 0, 0};
+  int before = 0;
+  for (int b0 = 0; b0 < P.B; b0 += 32) {
+    if (P.B > 32) mine = b0 + lane < P.B ? span_of(P, b0 + lane).count : 0;
+    const int n = b0 + lane < P.B ? max(1, (mine + c.piece - 1) / c.piece) : 0;   // an empty sequence is written by a piece too
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const unsigned past = __ballot_sync(0xFFFFFFFFu, before + sum > x);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      c.b = b0 + l;
+      c.n = __shfl_sync(0xFFFFFFFFu, n, l);
+      c.index = x - before - (__shfl_sync(0xFFFFFFFFu, sum, l) - c.n);
+      return c;
+    }
+    before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  return c;
+}
+
+__device__ __forceinline__ int64_t block_id(const AttnParams& P, int64_t at) {
+  return P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
+}
+
+// Two bytes of a pair of operands as fp16: bytes (a, b) -> code a, code b.  `w` holds four codes, SEL picks two.
+template <int CODES> __device__ __forceinline__ uint32_t bias(uint32_t w) { return CODES == JF_CODES_INT8 ? w ^ 0x80808080u : w; }
+template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
+  uint32_t d;
+  if (CODES == JF_CODES_INT8) {   // 0x6400 + u is 1024 + u
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(w, 0x64646464u, HIGH ? 0x4342u : 0x4140u)), "r"(0x64806480u));
+    return d;
+  }
+  const uint32_t h = prmt(w, 0u, HIGH ? 0x3424u : 0x1404u);
+  return (h & 0x80008000u) | (h >> 1 & 0x3F803F80u);
+}
+
+template <int CODES, int DT, int NT, bool FEAT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kernel(const __grid_constant__ AttnParams P) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y / P.groups, grp = blockIdx.y % P.groups;
+  const int first_head = kvh * P.G + grp * 8 * NT, heads = min(8 * NT, P.G - grp * 8 * NT);
+  pdl_wait();
+  pdl_trigger();
+  const Cut cut = find_piece(P, blockIdx.x);
+  if (cut.b < 0) return;
+  const int b = cut.b;
+  const Span span = span_of(P, b);
+  const int begin = cut.index * cut.piece, end = min(begin + cut.piece, span.count);
+
+  // q of the lane's head (column g of each tile), scaled to fp16
+  uint32_t qf[NT][16];
+  float sfac[NT][2], slope[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int head = n * 8 + g;
+    uint4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (head < heads)
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) +
+                                                      (static_cast<int64_t>(b) * P.H_q + first_head + head) * JF_HEAD_DIM +
+                                                      (i >> 1) * 64 + t * 16 + (i & 1) * 8));
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        amax = fmaxf(amax, fmaxf(fabsf(Elem<DT>::to_f32(static_cast<uint16_t>(w[k]))), fabsf(Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)))));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+    // 2^(13 - exponent of amax); below 2^-113 it stays 2^126, an infinite q keeps its scale
+    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    if (e == 128) e = 13;
+    e = max(e, -113);
+    const float up = __uint_as_float(static_cast<uint32_t>(13 - e + 127) << 23);   // 13 - e in [-114, 126]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __half2 h = __floats2half2_rn(Elem<DT>::to_f32(static_cast<uint16_t>(w[k])) * up, Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)) * up);
+        qf[n][i * 4 + k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    // what brings a sum of products back, for the heads of the lane's score columns 2t and 2t + 1
+    const float down = __uint_as_float(static_cast<uint32_t>(e - 13 + 127 + (CODES == JF_CODES_E4M3 ? 8 : 0)) << 23);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      sfac[n][c] = __shfl_sync(0xFFFFFFFFu, down, (2 * t + c) * 4) * P.scale * (FEAT ? 1.0f : kLog2e);
+      const int head_c = n * 8 + 2 * t + c;
+      slope[n][c] = FEAT && P.slopes && head_c < heads ? P.slopes[first_head + head_c] : 0.0f;
+    }
+  }
+
+  float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[n][i][k] = 0.0f;
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+  }
+
+  // The warp's blocks: begin + warp, + kWarps, ...; 32 of them are looked up at a time, a lane each.
+  const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;
+  const int64_t table_row = static_cast<int64_t>(b) * P.bt_stride, head_row = static_cast<int64_t>(kvh) * P.num_blocks;
+  auto position_of = [&](int i) {   // first position of the warp's i-th block
+    const int at = begin + warp + i * kWarps;
+    return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
+  };
+  struct Look { int64_t id; float ks, vs; };
+  auto look_up = [&](int i0) {
+    Look r{-1, 0.0f, 1.0f};
+    if (i0 + lane < mine) {
+      r.id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
+      if (r.id < 0 || r.id >= P.num_blocks) r.id = -1;
+      if (r.id >= 0) {
+        r.ks = P.k_scales[head_row + r.id];
+        r.vs = P.v_scales[head_row + r.id];
+        if (r.vs == 0.0f) r.vs = 0x1p-100f;   // weightless, but its positions count
+      }
+    }
+    return r;
+  };
+  unsigned char* ring = smem + warp * kStages * kStageBytes + lane * 16;
+  const uint32_t k_off = g * JF_HEAD_DIM + t * 16, v_off = 2 * t * JF_HEAD_DIM + g * 16;
+  auto fetch = [&](int64_t id, int stage) {
+    if (id >= 0) {
+      unsigned char* dst = ring + stage * kStageBytes;
+      const uint8_t* k = P.k_data + (head_row + id) * (JF_BLOCK_SIZE * JF_HEAD_DIM) + k_off;
+      const uint8_t* v = P.v_data + (head_row + id) * (JF_BLOCK_SIZE * JF_HEAD_DIM) + v_off;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cp_async_16(dst + i * 512, k + (i & 1) * 8 * JF_HEAD_DIM + (i >> 1) * 64);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cp_async_16(dst + 2048 + i * 512, v + ((i & 1) + (i >> 1) * 8) * JF_HEAD_DIM);
+    }
+    cp_async_commit();
+  };
+  Look look = look_up(0), next = look;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i < mine ? __shfl_sync(0xFFFFFFFFu, look.id, i) : -1, i);
+  int stage = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int i32 = i & 31;
+    if (i32 == 0 && i > 0) look = next;
+    if (i32 == 0) next = look_up((i & ~31) + 32);
+    {
+      const int ahead = i + kStages - 1;
+      const int64_t id = __shfl_sync(0xFFFFFFFFu, (ahead & ~31) == (i & ~31) ? look.id : next.id, ahead & 31);
+      fetch(ahead < mine ? id : -1, stage == 0 ? kStages - 1 : stage - 1);
+    }
+    cp_async_wait_group<kStages - 1>();
+    const int64_t id = __shfl_sync(0xFFFFFFFFu, look.id, i32);
+    const unsigned char* at = ring + stage * kStageBytes;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (id < 0) continue;
+    const float ks = __shfl_sync(0xFFFFFFFFu, look.ks, i32), vs = __shfl_sync(0xFFFFFFFFu, look.vs, i32);
+    const int pos = position_of(i);
+
+    float s[NT][4];
+    {
+      float c2[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[n][k] = c2[n][k] = 0.0f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint4 lo = *reinterpret_cast<const uint4*>(at + half * 1024), hi = *reinterpret_cast<const uint4*>(at + half * 1024 + 512);
+        const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, c[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = bias<CODES>(a[w]), y = bias<CODES>(c[w]);
+          const uint32_t a0 = widen<CODES, false>(x), a1 = widen<CODES, false>(y), a2 = widen<CODES, true>(x), a3 = widen<CODES, true>(y);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(half ? c2[n] : s[n], a0, a1, a2, a3, qf[n][half * 8 + w * 2], qf[n][half * 8 + w * 2 + 1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[n][k] = (s[n][k] + c2[n][k]) * (sfac[n][k & 1] * ks);
+    }
+    if (FEAT) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float x = s[n][k];
+          if (P.softcap > 0.0f) x = P.softcap * tanhf(x / P.softcap);
+          x -= slope[n][k & 1] * static_cast<float>(span.len - 1 - (pos + g + (k >> 1) * 8));
+          s[n][k] = x * kLog2e;
+        }
+    }
+    const bool whole = pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix);
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int p = pos + g + k * 8;
+        const bool seen = p < span.len && (p >= span.lo || p < span.prefix);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[n][2 * k] = seen ? s[n][2 * k] : -INFINITY;
+          s[n][2 * k + 1] = seen ? s[n][2 * k + 1] : -INFINITY;
+        }
+      }
+    }
+    float lvs;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
+    const float ivs = ex2(-lvs);
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[n][k] += lvs;
+        above |= s[n][k] > m[n][k & 1] + (kLift + kLag);
+      }
+    if (__any_sync(0xFFFFFFFFu, above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = fmaxf(s[n][c], s[n][2 + c]);
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+          const float to = fmaxf(m[n][c], top - kLift);
+          const float f = to == m[n][c] ? 1.0f : ex2(m[n][c] - to);
+          m[n][c] = to;
+          l[n][c] *= f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            o[n][j][c] *= f;
+            o[n][j][2 + c] *= f;
+          }
+        }
+    }
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+      const float p0 = ex2(s[n][0] - m0), p1 = ex2(s[n][1] - m1), p2 = ex2(s[n][2] - m0), p3 = ex2(s[n][3] - m1);
+      l[n][0] = fmaf(p0 + p2, ivs, l[n][0]);
+      l[n][1] = fmaf(p1 + p3, ivs, l[n][1]);
+      const __half2 a = __floats2half2_rn(p0, p1), c = __floats2half2_rn(p2, p3);
+      pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&a));
+      pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&c));
+    }
+    {
+      uint32_t r[4][4];
+#pragma unroll
+      for (int i2 = 0; i2 < 4; ++i2) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at + 2048 + i2 * 512);
+        r[i2][0] = bias<CODES>(x.x); r[i2][1] = bias<CODES>(x.y); r[i2][2] = bias<CODES>(x.z); r[i2][3] = bias<CODES>(x.w);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int hl = 0; hl < 2; ++hl) {   // channels 16g + 4w + 2hl (row g of the tile) and the next (row g + 8)
+          const uint32_t x = prmt(r[0][w], r[1][w], hl ? 0x7362u : 0x5140u), y = prmt(r[2][w], r[3][w], hl ? 0x7362u : 0x5140u);
+          const uint32_t a0 = widen<CODES, false>(x), a1 = widen<CODES, true>(x), a2 = widen<CODES, false>(y), a3 = widen<CODES, true>(y);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + hl], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
+    }
+  }
+  cp_async_wait_all();
+
+  // The warps' results meet: references first, then the sums under the common one.
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float x = l[n][c];
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+      x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+      if (g == 0) {
+        sm_m[warp][n * 8 + 2 * t + c] = m[n][c];
+        sm_l[warp][n * 8 + 2 * t + c] = x;
+      }
+    }
+  __syncthreads();   // (also: every warp is through with its ring)
+  float* so = reinterpret_cast<float*>(smem);   // [warp][head][128]
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float f[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][n * 8 + 2 * t + c]);
+      f[c] = m[n][c] == -INFINITY ? 0.0f : ex2(m[n][c] - top);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)   // tile j: channels 16g + 2j (registers 0, 1) and 16g + 2j + 1
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<float2*>(so + (warp * 8 * NT + n * 8 + 2 * t + c) * JF_HEAD_DIM + 16 * g + 2 * j) =
+            make_float2(o[n][j][c] * f[c], o[n][j][2 + c] * f[c]);
+  }
+  __syncthreads();
+  constexpr float kBack = CODES == JF_CODES_E4M3 ? 256.0f : 1.0f;
+  for (int i = threadIdx.x; i < heads * JF_HEAD_DIM; i += kWarps * 32) {
+    const int head = i / JF_HEAD_DIM, d = i % JF_HEAD_DIM;
+    float top = -INFINITY, sum = 0.0f, z = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][head]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      sum += so[(w * 8 * NT + head) * JF_HEAD_DIM + d];
+      if (sm_m[w][head] != -INFINITY) z = fmaf(sm_l[w][head], ex2(sm_m[w][head] - top), z);
+    }
+    sum *= kBack;
+    if (cut.n == 1) {
+      const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
+      static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + d] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : sum / z);
+      if (d == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
+    } else {
+      const int64_t row = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (8 * NT) + head;
+      P.part_o[row * JF_HEAD_DIM + d] = sum;
+      if (d == 0) {
+        P.part_ml[row * 2] = top;
+        P.part_ml[row * 2 + 1] = z;
+      }
+    }
+  }
+}
+
+// The pieces of a sequence: one block per (head, sequence), four threads share an output channel.
+constexpr int kJoin = 4;
+template <int DT>
+__global__ void __launch_bounds__(JF_HEAD_DIM * kJoin) block8_join_kernel(const __grid_constant__ AttnParams P, int width, int grid_y) {
+  __shared__ float sm_o[kJoin][JF_HEAD_DIM], sm_z[kJoin], sm_top[kJoin * 4];
+  __shared__ int sm_first, sm_n;
+  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {   // pieces before this sequence's
+    int total = 0, before = 0, own = 0;
+    for (int i = lane; i < P.B; i += 32) total += span_of(P, i).count;
+    const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total));
+    for (int i = lane; i <= b; i += 32) {
+      const int n = max(1, (span_of(P, i).count + piece - 1) / piece);
+      if (i < b) before += n; else own = n;
+    }
+    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    own = __reduce_add_sync(0xFFFFFFFFu, own);
+    if (lane == 0) { sm_first = before; sm_n = own; }
+  }
+  __syncthreads();
+  const int n = sm_n;
+  if (n == 1) return;
+  const int kvh = h / P.G, in_group = h % P.G, y = kvh * P.groups + in_group / width;
+  auto row_of = [&](int i) { return (static_cast<int64_t>(sm_first + i) * grid_y + y) * width + in_group % width; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += JF_HEAD_DIM * kJoin) top = fmaxf(top, P.part_ml[row_of(i) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  if (lane == 0) sm_top[warp] = top;
+  __syncthreads();
+  top = sm_top[0];
+#pragma unroll
+  for (int w = 1; w < kJoin * 4; ++w) top = fmaxf(top, sm_top[w]);
+  const int part = threadIdx.x / JF_HEAD_DIM, d = threadIdx.x % JF_HEAD_DIM;
+  float sum = 0.0f, z = 0.0f;
+#pragma unroll 8
+  for (int i = part; i < n; i += kJoin) {
+    const int64_t row = row_of(i);
+    const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + row * 2);
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum = fmaf(P.part_o[row * JF_HEAD_DIM + d], f, sum);
+    z = fmaf(ml.y, f, z);
+  }
+  sm_o[part][d] = sum;
+  if (d == 0) sm_z[part] = z;
+  __syncthreads();
+  if (part == 0) {
+    sum = sm_o[0][d];
+    z = sm_z[0];
+#pragma unroll
+    for (int k = 1; k < kJoin; ++k) { sum += sm_o[k][d]; z += sm_z[k]; }
+    const int64_t row = static_cast<int64_t>(b) * P.H_q + h;
+    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + d] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : sum / z);
+    if (d == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
+  }
+}
+
+struct Plan { int G, nt, groups, target, min_piece, pieces; uint64_t bytes; };
+constexpr int kMinPiece = 8;   // blocks
+
+// Pieces per KV head: one wave of blocks where the batch leaves room for it, several where it does not.
+bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
+  if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_S <= 0 || H_q % H_kv != 0) return false;
+  p.G = H_q / H_kv;
+  p.nt = p.G <= 8 ? 1 : 2;
+  p.groups = (p.G + 8 * p.nt - 1) / (8 * p.nt);
+  const int64_t columns = static_cast<int64_t>(H_kv) * p.groups;
+  const int64_t most = (static_cast<int64_t>(max_S) + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;       // blocks of a sequence
+  if (columns > 65535 || most * B > INT32_MAX / 2) return false;
+  const int64_t wave = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1) / columns);
+  p.target = static_cast<int>(2 * B <= wave ? wave - B : 3 * wave);
+  p.target = std::max(p.target, 1);
+  p.min_piece = kMinPiece;
+  const int64_t each = (most + p.min_piece - 1) / p.min_piece;
+  p.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.target) + B, each * B));
+  p.bytes = static_cast<uint64_t>(p.pieces) * columns * 8 * p.nt * (JF_HEAD_DIM + 2) * sizeof(float);
+  return true;
+}
+
+template <int CODES, int DT, int NT, bool FEAT>
+jf_status_t launch_attn(const AttnParams& P, dim3 grid, cudaStream_t s) {
+  constexpr int smem = std::max(kWarps * kStages * kStageBytes, kWarps * 8 * NT * JF_HEAD_DIM * 4);
+  auto* kernel = block8_attn_kernel<CODES, DT, NT, FEAT>;
+  JF_ENSURE_SMEM(kernel, smem);
+  JF_CUDA_TRY(launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, P));
+  return JF_OK;
+}
+template <int CODES, int DT> jf_status_t launch_attn(const AttnParams& P, int nt, bool feat, dim3 grid, cudaStream_t s) {
+  if (nt == 1) return feat ? launch_attn<CODES, DT, 1, true>(P, grid, s) : launch_attn<CODES, DT, 1, false>(P, grid, s);
+  return feat ? launch_attn<CODES, DT, 2, true>(P, grid, s) : launch_attn<CODES, DT, 2, false>(P, grid, s);
+}
+
+}  // namespace
+}  // namespace jf
+
+extern "C" uint64_t jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S) {
+  jf::Plan p;
+  return jf::make_plan(B, H_q, H_kv, max_S, p) ? p.bytes : 0;
+}
+
+extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t stream) {
+  using namespace jf;
+  if (!a) return JF_ERR_ARG;
+  if ((a->q_dtype != JF_DTYPE_BF16 && a->q_dtype != JF_DTYPE_FP16) || (a->codes != JF_CODES_INT8 && a->codes != JF_CODES_E4M3)) return JF_ERR_ARG;
+  if (a->B < 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->window < 0 || !(a->softcap >= 0.0f) || a->softcap > 3.0e38f) return JF_ERR_ARG;
+  if (a->B == 0) return JF_OK;
+  Plan p;
+  if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;
+  if (!a->q || !a->k_data || !a->v_data || !a->k_scales || !a->v_scales || !a->block_table || !a->seq_lens || !a->out) return JF_ERR_ARG;
+  if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 2)) return JF_ERR_ARG;
+  if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE) return JF_ERR_UNSUPPORTED;
+  if (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)) return JF_ERR_WORKSPACE;
+  AttnParams P{};
+  P.q = a->q;
+  P.k_data = static_cast<const uint8_t*>(a->k_data);
+  P.v_data = static_cast<const uint8_t*>(a->v_data);
+  P.k_scales = a->k_scales;
+  P.v_scales = a->v_scales;
+  P.table = a->block_table;
+  P.seq_lens = a->seq_lens;
+  P.prefix_lens = a->prefix_lens;
+  P.slopes = a->alibi_slopes;
+  P.out = a->out;
+  P.lse = a->lse;
+  const int64_t rows = static_cast<int64_t>(p.pieces) * a->H_kv * p.groups * 8 * p.nt;
+  P.part_o = static_cast<float*>(a->workspace);
+  P.part_ml = P.part_o + rows * JF_HEAD_DIM;
+  P.num_blocks = a->num_blocks;
+  P.bt_stride = a->bt_stride;
+  P.B = a->B; P.H_q = a->H_q; P.H_kv = a->H_kv; P.G = p.G; P.groups = p.groups;
+  P.max_S = a->max_S; P.max_blocks = a->max_blocks; P.window = a->window;
+  P.target = p.target; P.min_piece = p.min_piece; P.pieces = p.pieces;
+  P.scale = a->attn_scale; P.softcap = a->softcap;
+  P.bt_i32 = a->bt_is_i32 != 0;
+  const bool feat = a->softcap > 0.0f || a->alibi_slopes;
+  const auto s = static_cast<cudaStream_t>(stream);
+  const dim3 grid(p.pieces, a->H_kv * p.groups);
+  jf_status_t st;
+  if (a->q_dtype == JF_DTYPE_BF16)
+    st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_BF16>(P, p.nt, feat, grid, s)
+                                   : launch_attn<JF_CODES_E4M3, JF_DTYPE_BF16>(P, p.nt, feat, grid, s);
+  else
+    st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_FP16>(P, p.nt, feat, grid, s)
+                                   : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
+  if (st != JF_OK || p.pieces == a->B) return st;   // one piece per sequence: nothing to join
+  const dim3 jgrid(a->H_q, a->B);
+  if (a->B > 65535) return JF_ERR_UNSUPPORTED;
+  JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
+                  ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16>, jgrid, dim3(JF_HEAD_DIM * kJoin), 0, s, P, 8 * p.nt, a->H_kv * p.groups)
+                  : launch_pdl(block8_join_kernel<JF_DTYPE_FP16>, jgrid, dim3(JF_HEAD_DIM * kJoin), 0, s, P, 8 * p.nt, a->H_kv * p.groups));
+  return JF_OK;
+}

@@ -667,10 +667,189 @@ PyObject* step_run(PyObject*, PyObject* const* p, Py_ssize_t n) {
   });
 }
 
+// ---- the cache of 8-bit codes -------------------------------------------------------------
+
+// The launch goes to the current device's stream: a tensor elsewhere is refused.
+void here(const at::Tensor& t, const char* name, const char* what) {
+  if (t.is_cuda() && t.device().index() == c10::cuda::current_device()) return;
+  PyErr_Format(PyExc_RuntimeError, "%s: %s must be a CUDA tensor of the current device", name, what);
+  throw ArgError();
+}
+
+struct Block8 {
+  int32_t codes = 0, h_kv = 0;
+  int64_t num_blocks = 0;
+
+  void side(const at::Tensor& data, const at::Tensor& scales, bool k_side, const char* name) {
+    here(data, name, k_side ? "k_data" : "v_data");
+    here(scales, name, k_side ? "k_scales" : "v_scales");
+    const auto type = data.scalar_type();
+    require(type == at::kChar || type == at::kFloat8_e4m3fn, name, "k_data / v_data must be int8 or float8_e4m3fn");
+    require(data.is_contiguous() && data.dim() == 3 && data.size(2) == JF_HEAD_DIM && data.size(1) % JF_BLOCK_SIZE == 0, name,
+            "k_data / v_data must be contiguous (H_kv, num_blocks * 16, 128)");
+    const int32_t c = type == at::kChar ? JF_CODES_INT8 : JF_CODES_E4M3;
+    if (k_side) {
+      codes = c;
+      require(data.size(0) > 0 && data.size(0) <= INT32_MAX, name, "the cache has no heads");
+      h_kv = static_cast<int32_t>(data.size(0));
+      num_blocks = data.size(1) / JF_BLOCK_SIZE;
+    }
+    require(c == codes && data.size(0) == h_kv && data.size(1) == num_blocks * JF_BLOCK_SIZE, name, "K and V caches differ in type or shape");
+    require(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 2 && scales.size(0) == h_kv &&
+                scales.size(1) == num_blocks,
+            name, "k_scales / v_scales must be contiguous float32 (H_kv, num_blocks)");
+  }
+};
+
+struct Table {
+  const void* at;
+  int32_t is_i32, width;
+  int64_t stride;
+};
+Table block_table(const at::Tensor& t, int64_t n, const char* name) {
+  here(t, name, "block_table");
+  require((t.scalar_type() == at::kLong || t.scalar_type() == at::kInt) && t.dim() == 2 && t.size(0) == n, name,
+          "block_table must be (sequences, max_blocks) int64 or int32");
+  require(t.size(1) <= 1 || t.stride(1) == 1, name, "block_table rows must be contiguous");
+  require(t.size(1) <= INT32_MAX, name, "block_table is too wide");
+  return {ptr(t), t.scalar_type() == at::kInt, static_cast<int32_t>(t.size(1)), n > 1 ? t.stride(0) : t.size(1)};
+}
+const int32_t* int32_vector(const at::Tensor& t, int64_t n, const char* name, const char* what) {
+  here(t, name, what);
+  if (!(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous())) {
+    PyErr_Format(PyExc_RuntimeError, "%s: %s must be contiguous int32 with %lld entries", name, what, static_cast<long long>(n));
+    throw ArgError();
+  }
+  return static_cast<const int32_t*>(ptr(t));
+}
+
+// block8_append(name, key, value, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales)
+PyObject* block8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 10, "block8_append");
+    const char* name = text(a[0]);
+    const at::Tensor &key = tensor(a[1], name, "key_tok"), &value = tensor(a[2], name, "value_tok"),
+                     &start = tensor(a[3], name, "query_start_loc"), &lens = tensor(a[4], name, "seq_lens"),
+                     &bt = tensor(a[5], name, "block_table"), &kd = tensor(a[6], name, "k_data"), &ks = tensor(a[7], name, "k_scales"),
+                     &vd = tensor(a[8], name, "v_data"), &vs = tensor(a[9], name, "v_scales");
+    Block8 c;
+    c.side(kd, ks, true, name);
+    c.side(vd, vs, false, name);
+    here(key, name, "key_tok");
+    here(value, name, "value_tok");
+    require(key.dim() == 3 && key.size(1) == c.h_kv && key.size(2) == JF_HEAD_DIM && value.sizes() == key.sizes(), name,
+            "key_tok / value_tok must be (T, H_kv, 128)");
+    require(key.scalar_type() == value.scalar_type(), name, "key_tok / value_tok differ in dtype");
+    require(key.stride(2) == 1 && value.stride(2) == 1, name, "key_tok / value_tok innermost dim must be contiguous");
+    const int dt = dtype_id(key);
+    const int64_t seqs = lens.dim() == 1 ? lens.size(0) : -1;
+    require(seqs >= 0 && seqs < INT32_MAX, name, "seq_lens must be (sequences,) int32");
+    const int32_t* lp = int32_vector(lens, seqs, name, "seq_lens");
+    const int32_t* sp = int32_vector(start, seqs + 1, name, "query_start_loc");
+    const Table tb = block_table(bt, seqs, name);
+    const jf_stream_t st = current_stream();
+    const void *kp = ptr(key), *vp = ptr(value);
+    const int64_t T = key.size(0), k_t = key.stride(0), k_h = key.stride(1), v_t = value.stride(0), v_h = value.stride(1);
+    void *kdp = out_ptr(kd), *vdp = out_ptr(vd);
+    auto *ksp = static_cast<float*>(out_ptr(ks)), *vsp = static_cast<float*>(out_ptr(vs));
+    return PyLong_FromLong(unlocked([&] {
+      return jf_block8_append(kp, vp, dt, T, c.h_kv, k_t, k_h, v_t, v_h, sp, lp, static_cast<int32_t>(seqs), tb.at, tb.is_i32, tb.stride,
+                              tb.width, c.codes, kdp, ksp, vdp, vsp, c.num_blocks, st);
+    }));
+  });
+}
+
+// block8_attn(name, q, k_data, k_scales, v_data, v_scales, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale,
+//             softcap, alibi_slopes | None, window (0: none), prefix_lens | None, workspace | None, out | None)
+//   -> (status, out, lse)
+PyObject* block8_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 19, "block8_attn");
+    const char* name = text(p[0]);
+    const at::Tensor &q_in = tensor(p[1], name, "q"), &kd = tensor(p[2], name, "k_data"), &ks = tensor(p[3], name, "k_scales"),
+                     &vd = tensor(p[4], name, "v_data"), &vs = tensor(p[5], name, "v_scales"), &bt = tensor(p[6], name, "block_table"),
+                     &lens = tensor(p[7], name, "seq_lens");
+    Block8 c;
+    c.side(kd, ks, true, name);
+    c.side(vd, vs, false, name);
+    const int32_t max_S = as_int32(p[8]), h_q = as_int32(p[9]), h_kv = as_int32(p[10]);
+    require(as_int32(p[11]) == JF_BLOCK_SIZE, name, "block_size must be 16");
+    require(h_kv == c.h_kv, name, "H_kv differs from the cache's");
+    require(h_q > 0 && h_q % h_kv == 0, name, "H_q must be a multiple of H_kv");
+    require(max_S > 0, name, "max_S must be positive");
+    here(q_in, name, "q");
+    const int64_t B = lens.dim() == 1 ? lens.size(0) : -1;
+    require(B >= 0 && B <= INT32_MAX, name, "seq_lens must be (B,) int32");
+    require(q_in.dim() == 3 && q_in.size(0) == B && q_in.size(1) == h_q && q_in.size(2) == JF_HEAD_DIM, name, "q must be (B, H_q, 128)");
+    at::Tensor keep;
+    const at::Tensor* qc = &contiguous(q_in, keep);
+    if (reinterpret_cast<uintptr_t>(ptr(*qc)) % 16 != 0) qc = &(keep = qc->clone());
+    jf_block8_attn_args a{};
+    a.codes = c.codes;
+    a.q_dtype = dtype_id(q_in);
+    a.B = static_cast<int32_t>(B); a.H_q = h_q; a.H_kv = h_kv; a.max_S = max_S;
+    const Table tb = block_table(bt, B, name);
+    a.max_blocks = tb.width; a.bt_is_i32 = tb.is_i32; a.bt_stride = tb.stride; a.block_table = tb.at;
+    a.attn_scale = static_cast<float>(real(p[12]));
+    const double cap = real(p[13]);
+    require(cap >= 0.0 && cap < 1e30, name, "softcap must be 0 (none) or positive");
+    a.softcap = static_cast<float>(cap);
+    a.window = as_int32(p[15]);
+    require(a.window >= 0, name, "window must be positive, or None");
+    a.num_blocks = c.num_blocks;
+    a.seq_lens = int32_vector(lens, B, name, "seq_lens");
+    if (p[14] != Py_None) {
+      const at::Tensor& s = tensor(p[14], name, "alibi_slopes");
+      here(s, name, "alibi_slopes");
+      require(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == h_q && s.is_contiguous(), name, "alibi_slopes must be contiguous float32 (H_q,)");
+      a.alibi_slopes = static_cast<const float*>(ptr(s));
+    }
+    if (p[16] != Py_None) a.prefix_lens = int32_vector(tensor(p[16], name, "prefix_lens"), B, name, "prefix_lens");
+    const c10::Device device = q_in.device();
+    at::Tensor out;
+    if (p[18] != Py_None) {
+      out = tensor(p[18], name, "out");
+      here(out, name, "out");
+      require(out.is_contiguous() && out.scalar_type() == q_in.scalar_type() && out.sizes() == q_in.sizes(), name,
+              "out must be contiguous, of q's dtype and shape");
+    } else {
+      out = at::detail::empty_cuda({B, h_q, JF_HEAD_DIM}, q_in.scalar_type(), device, c10::nullopt);
+    }
+    at::Tensor lse = at::detail::empty_cuda({B, h_q}, at::kFloat, device, c10::nullopt), scratch;
+    jf_status_t r = JF_OK;
+    if (B > 0) {
+      const uint64_t bytes = jf_block8_workspace_bytes(a.B, h_q, h_kv, max_S);
+      require(bytes > 0, name, "bad shape");
+      if (p[17] != Py_None) {
+        scratch = tensor(p[17], name, "workspace");
+        here(scratch, name, "workspace");
+        require(scratch.is_contiguous(), name, "workspace must be contiguous");
+      } else {
+        scratch = workspace(bytes, device);
+      }
+      const auto base = reinterpret_cast<uintptr_t>(out_ptr(scratch)), at = (base + 255) / 256 * 256;
+      const uint64_t size = static_cast<uint64_t>(scratch.numel()) * scratch.element_size();
+      a.workspace = reinterpret_cast<void*>(at);
+      a.workspace_bytes = size > at - base ? size - (at - base) : 0;
+      a.q = ptr(*qc);
+      a.k_data = ptr(kd);
+      a.v_data = ptr(vd);
+      a.k_scales = static_cast<const float*>(ptr(ks));
+      a.v_scales = static_cast<const float*>(ptr(vs));
+      a.out = out_ptr(out);
+      a.lse = static_cast<float*>(out_ptr(lse));
+      const jf_stream_t st = current_stream();
+      r = unlocked([&] { return jf_block8_attn(&a, st); });
+    }
+    return tuple_of(r, {out, lse});
+  });
+}
+
 #define JF_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     JF_METHOD(quant_write), JF_METHOD(quant_write_kv), JF_METHOD(fused_attn), JF_METHOD(stage_a), JF_METHOD(stage_b),
     JF_METHOD(decode), JF_METHOD(get_workspace), JF_METHOD(blend), JF_METHOD(step_create), JF_METHOD(step_run),
+    JF_METHOD(block8_append), JF_METHOD(block8_attn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "tensor-taking half of jetfire_b200.ops", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -521,6 +521,58 @@ def int8tc_softmax_v_with_pre_corr_reg_stats(scores, softmax_m, softmax_inv_z, v
 
 
 # ---------------------------------------------------------------------------------------
+# cache of 8-bit codes with one scale per block and head
+# ---------------------------------------------------------------------------------------
+
+BLOCK8_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def block8_append(key_tok, value_tok, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales) -> None:
+    """In place: the new tokens of a step into a paged cache of 8-bit codes.
+
+    ``key_tok / value_tok (T, H_kv, 128)`` bf16 or fp16 (any strides with a contiguous innermost dim);
+    ``query_start_loc (n + 1,)`` int32: rows of sequence i; ``seq_lens (n,)`` int32: lengths that count these
+    tokens already, so that the rows are the sequence's last positions; ``block_table (n, max_blocks)`` int64 or
+    int32; ``k_data / v_data (H_kv, num_blocks * 16, 128)`` int8 or float8_e4m3fn; ``k_scales / v_scales
+    (H_kv, num_blocks)`` float32.  An element is ``code * scale``; int8 scales are ``amax / 127``, e4m3 scales the
+    smallest power of two that brings amax to at most 448.  A block that holds earlier positions of its sequence
+    keeps the larger scale, its codes rounded to it where it grew.  NaN becomes 0, an infinity the largest code, and neither
+    counts in amax.  Rows behind the last sequence and positions without a valid block are skipped.  Every
+    block is written for one sequence only (blocks that sequences share are full and are not written)."""
+    check("block8_append", _host.block8_append("block8_append", key_tok, value_tok, query_start_loc, seq_lens, block_table,
+                                               k_data, k_scales, v_data, v_scales))
+
+
+def block8_workspace_bytes(B, H_q, H_kv, max_S) -> int:
+    """Scratch of ``block8_decode_attn`` for calls of these sizes."""
+    return int(lib.jf_block8_workspace_bytes(B, H_q, H_kv, max_S))
+
+
+def _window(window, name) -> int:
+    """Positions a token sees including its own; None: all.  0 would see nothing and is refused."""
+    if window is None:
+        return 0
+    _require(int(window) > 0, f"{name}: window must be positive, or None")
+    return min(int(window), 2**31 - 1)
+
+
+def block8_decode_attn(q, k_data, k_scales, v_data, v_scales, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale, *,
+                       softcap=0.0, alibi_slopes=None, window=None, prefix_lens=None, workspace=None, out=None):
+    """Attention of one query token per sequence over the cache that ``block8_append`` fills.
+
+    ``q (B, H_q, 128)`` stands at position ``seq_lens[b] - 1``.  Scores are ``attn_scale * q.k``, then
+    ``softcap * tanh(s / softcap)`` where ``softcap`` is not 0, then ``- alibi_slopes[h] * distance``.  A query sees the
+    last ``window`` positions and the first ``prefix_lens[b]``, or everything.  Positions whose block id is not
+    in the cache are not seen; a sequence that sees nothing (length 0) gets zeros and ``lse = -inf``.  ``max_S``
+    bounds the lengths (longer ones are cut to it).  Returns ``(out (B, H_q, 128) like q, lse (B, H_q) float32)``."""
+    name = "block8_decode_attn"
+    st, out, lse = _host.block8_attn(name, q, k_data, k_scales, v_data, v_scales, block_table, seq_lens, max_S, H_q, H_kv, block_size,
+                                     attn_scale, softcap, alibi_slopes, _window(window, name), prefix_lens, workspace, out)
+    check(name, st)
+    return out, lse
+
+
+# ---------------------------------------------------------------------------------------
 # correction merge
 # ---------------------------------------------------------------------------------------
 

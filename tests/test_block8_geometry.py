@@ -1,0 +1,81 @@
+"""Which warp of the append writes which rows, and how the decode kernel cuts a batch into pieces: the device
+arithmetic restated line for line, over random batches."""
+import random
+
+
+def _append_writes(start, lens, T, chunk, max_blocks):
+    """(sequence, block, first row of the call, rows, row in the block) of every warp's writes of one head and side."""
+    out, n = [], len(lens)
+    for t0 in range(0, T, chunk):
+        t, end = t0, min(t0 + chunk, T)
+        s = sum(start[i + 1] <= t for i in range(n))
+        while t < end:
+            while s < n and start[s + 1] <= t:
+                s += 1
+            if s >= n:
+                break
+            a, b = start[s], min(start[s + 1], T)
+            if t < a:
+                t = a
+                continue
+            pos = lens[s] - (b - t)
+            if pos < 0:
+                t += min(b - t, -pos)
+                continue
+            step = 0 if t == a else (16 - (pos & 15)) & 15
+            t, pos = t + step, pos + step
+            if t >= b:
+                t = b
+                continue
+            if t >= end:
+                break
+            r = pos & 15
+            cnt = min(16 - r, b - t)
+            if pos >> 4 < max_blocks:
+                out.append((s, pos >> 4, t, cnt, r))
+            t += cnt
+    return out
+
+
+def test_every_row_is_written_once_and_every_block_by_one_warp():
+    rng = random.Random(5)
+    for _ in range(4000):
+        n = rng.randint(1, 9)
+        new = [rng.choice((0, 1, 1, rng.randint(1, 80))) for _ in range(n)]
+        old = [rng.choice((0, rng.randint(0, 70), -rng.randint(1, 20) if rng.random() < 0.1 else 3)) for _ in range(n)]
+        gap = rng.choice((0, 0, 3))
+        start = [gap]
+        for x in new:
+            start.append(start[-1] + x)
+        lens = [o + x for o, x in zip(old, new)]
+        T = start[-1] + rng.choice((0, 0, 5))
+        writes = _append_writes(start, lens, T, rng.choice((1, 4, 16)), 1000)
+        want = {(s, old[s] + i, start[s] + i) for s in range(n) for i in range(new[s]) if old[s] + i >= 0}
+        got = [(s, blk * 16 + r + i, t + i) for s, blk, t, cnt, r in writes for i in range(cnt)]
+        assert len(got) == len(set(got)) and set(got) == want
+        assert len({(s, blk) for s, blk, *_ in writes}) == len(writes)
+        for s, blk, t, cnt, r in writes:
+            assert cnt >= 1 and r + cnt <= 16 and 0 <= t and t + cnt <= T
+            assert r == 0 or (t == start[s] and old[s] % 16 == r)     # rows in front of it were there before the call
+
+
+def _pieces(counts, target, min_piece):
+    piece = max(min_piece, -(-sum(counts) // target))
+    return piece, [max(1, -(-c // piece)) for c in counts]
+
+
+def test_pieces_fit_the_grid_and_cover_every_block():
+    rng = random.Random(6)
+    for _ in range(4000):
+        B = rng.randint(1, 70)
+        most = rng.choice((1, 5, 40, 700, 8192))
+        counts = [rng.choice((0, most, rng.randint(0, most))) for _ in range(B)]
+        wave = rng.choice((1, 18, 37, 74, 296))
+        target = max(1, wave - B if 2 * B <= wave else 3 * wave)
+        min_piece = 8
+        piece, n = _pieces(counts, target, min_piece)
+        grid = min(target + B, -(-most // min_piece) * B)
+        assert sum(n) <= grid
+        for c, k in zip(counts, n):
+            covered = [min(i * piece + piece, c) - i * piece for i in range(k)]
+            assert sum(max(0, x) for x in covered) == c and (c == 0 or min(covered) > 0)
