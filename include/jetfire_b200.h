@@ -547,6 +547,40 @@ jf_status_t jf_block8_append(const void* key, const void* value, int32_t dtype, 
 uint64_t    jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S);
 jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
 
+/* ---- attention of packed prompts over their own keys and values -----------------------------------
+ * What a library's variable-length attention does for the prefill rows of a step (the call of
+ * jetfire_vllm/adapter/decode_path.py:1500-1517), in a kernel of this library.
+ *
+ *   q (T, H_q, 128), k / v (T, H_kv, 128), 16-bit, strides in elements, the innermost contiguous;
+ *   sequence i owns the rows cu_seqlens[i] .. cu_seqlens[i + 1]; out (T, H_q, 128) contiguous; lse
+ *   (T, H_q) f32 or null.  Rows of no sequence are not written.
+ *
+ * Scores as in jf_block8_attn, the distance being |i - j|.  Row i of a sequence sees j <= i (causal) with
+ * |i - j| < window (if window > 0), and j < prefix_lens[sequence] (if given).  What a row does not see
+ * has no influence on it, not even as an infinity or a NaN.
+ *
+ * Base addresses 16-byte aligned, row and head strides positive multiples of 8 elements (strides of a
+ * dimension of size 1 are ignored).  status_record: 16 bytes in device memory, or null; an error that the
+ * kernel meets (a wait that ran out) is written there as jf_decode_status_of_copy reads it. */
+typedef struct jf_varlen_attn_args {
+  int32_t dtype, n_seqs, H_q, H_kv;
+  int32_t causal, window;         /* window 0: none */
+  float   attn_scale, softcap;    /* softcap 0: none */
+  int64_t T;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const void*    q;
+  const void*    k;
+  const void*    v;
+  const int32_t* cu_seqlens;      /* n_seqs + 1 */
+  const int32_t* prefix_lens;     /* (n_seqs,) or null */
+  const float*   alibi_slopes;    /* (H_q,) or null */
+  void*          out;
+  float*         lse;
+  void*          status_record;
+} jf_varlen_attn_args;
+
+jf_status_t jf_varlen_attn(const jf_varlen_attn_args* args, jf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

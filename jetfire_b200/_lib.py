@@ -62,6 +62,19 @@ class Block8AttnArgs(C.Structure):
     ]
 
 
+class VarlenAttnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_seqs", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32),
+        ("causal", C.c_int32), ("window", C.c_int32), ("attn_scale", C.c_float), ("softcap", C.c_float),
+        ("T", C.c_int64),
+        ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("prefix_lens", C.c_void_p), ("alibi_slopes", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("status_record", C.c_void_p),
+    ]
+
+
 _SIGS = {
     "jf_status_string": (C.c_char_p, [C.c_int32]),
     "jf_version": (C.c_int32, []),
@@ -166,6 +179,7 @@ _SIGS = {
                          [C.c_void_p] * 4 + [C.c_int64, C.c_void_p]),
     "jf_block8_workspace_bytes": (C.c_uint64, [C.c_int32] * 4),
     "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
+    "jf_varlen_attn": (C.c_int32, [C.POINTER(VarlenAttnArgs), C.c_void_p]),
     "jf_alloc_mapped": (C.c_int32, [C.c_uint64, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "jf_free_mapped": (C.c_int32, [C.c_void_p]),
 }

@@ -845,11 +845,95 @@ PyObject* block8_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   });
 }
 
+// ---- packed prompts -------------------------------------------------------------------------
+
+// (T, H, 128) as the kernel's tensor copies can address it, or a contiguous copy.
+const at::Tensor& addressable(const at::Tensor& t, at::Tensor& keep) {
+  auto ok = [&](int64_t d) { return t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0); };
+  if (t.stride(2) == 1 && ok(0) && ok(1) && reinterpret_cast<uintptr_t>(ptr(t)) % 16 == 0) return t;
+  keep = at::empty(t.sizes(), t.options());
+  keep.copy_(t);
+  return keep;
+}
+
+// varlen_attn(name, q, k, v, cu_seqlens, attn_scale, causal, window (0: none), softcap, alibi_slopes | None, prefix_lens | None,
+//             out | None, status_record | None) -> (status, out, lse)
+PyObject* varlen_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 13, "varlen_attn");
+    const char* name = text(p[0]);
+    const at::Tensor &q_in = tensor(p[1], name, "q"), &k_in = tensor(p[2], name, "k"), &v_in = tensor(p[3], name, "v"),
+                     &cu = tensor(p[4], name, "cu_seqlens");
+    here(q_in, name, "q");
+    here(k_in, name, "k");
+    here(v_in, name, "v");
+    require(q_in.dim() == 3 && q_in.size(2) == JF_HEAD_DIM, name, "q must be (T, H_q, 128)");
+    require(k_in.dim() == 3 && k_in.size(0) == q_in.size(0) && k_in.size(2) == JF_HEAD_DIM && v_in.sizes() == k_in.sizes(), name,
+            "k / v must be (T, H_kv, 128)");
+    require(k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type(), name, "q, k and v differ in dtype");
+    const int64_t T = q_in.size(0), h_q = q_in.size(1), h_kv = k_in.size(1);
+    require(h_kv > 0 && h_q > 0 && h_q % h_kv == 0 && h_q <= 65535, name, "H_q must be a multiple of H_kv");
+    jf_varlen_attn_args a{};
+    a.dtype = dtype_id(q_in);
+    const int64_t n_seqs = cu.dim() == 1 ? cu.size(0) - 1 : -1;
+    require(n_seqs >= 0 && n_seqs < INT32_MAX, name, "cu_seqlens must be (sequences + 1,) int32");
+    a.cu_seqlens = int32_vector(cu, n_seqs + 1, name, "cu_seqlens");
+    a.n_seqs = static_cast<int32_t>(n_seqs);
+    a.H_q = static_cast<int32_t>(h_q);
+    a.H_kv = static_cast<int32_t>(h_kv);
+    a.T = T;
+    a.attn_scale = static_cast<float>(real(p[5]));
+    a.causal = truth(p[6]);
+    a.window = as_int32(p[7]);
+    require(a.window >= 0, name, "window must be positive, or None");
+    const double cap = real(p[8]);
+    require(cap >= 0.0 && cap < 1e30, name, "softcap must be 0 (none) or positive");
+    a.softcap = static_cast<float>(cap);
+    if (p[9] != Py_None) {
+      const at::Tensor& s = tensor(p[9], name, "alibi_slopes");
+      here(s, name, "alibi_slopes");
+      require(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == h_q && s.is_contiguous(), name, "alibi_slopes must be contiguous float32 (H_q,)");
+      a.alibi_slopes = static_cast<const float*>(ptr(s));
+    }
+    if (p[10] != Py_None) a.prefix_lens = int32_vector(tensor(p[10], name, "prefix_lens"), n_seqs, name, "prefix_lens");
+    at::Tensor out, keep[3];
+    if (p[11] != Py_None) {
+      out = tensor(p[11], name, "out");
+      here(out, name, "out");
+      require(out.is_contiguous() && out.scalar_type() == q_in.scalar_type() && out.sizes() == q_in.sizes() &&
+                  reinterpret_cast<uintptr_t>(ptr(out)) % 16 == 0,
+              name, "out must be contiguous, 16-byte aligned, of q's dtype and shape");
+    } else {
+      out = at::detail::empty_cuda({T, h_q, JF_HEAD_DIM}, q_in.scalar_type(), q_in.device(), c10::nullopt);
+    }
+    if (p[12] != Py_None) {
+      const at::Tensor& r = tensor(p[12], name, "status_record");
+      here(r, name, "status_record");
+      require(r.is_contiguous() && r.numel() * r.element_size() >= JF_STATUS_RECORD_BYTES && reinterpret_cast<uintptr_t>(ptr(r)) % 8 == 0, name,
+              "status_record must hold 16 bytes, 8-byte aligned");
+      a.status_record = out_ptr(r);
+    }
+    at::Tensor lse = at::detail::empty_cuda({T, h_q}, at::kFloat, q_in.device(), c10::nullopt);
+    jf_status_t r = JF_OK;
+    if (T > 0 && n_seqs > 0) {
+      const at::Tensor &q = addressable(q_in, keep[0]), &k = addressable(k_in, keep[1]), &v = addressable(v_in, keep[2]);
+      a.q = ptr(q); a.q_stride_t = q.stride(0); a.q_stride_h = q.stride(1);
+      a.k = ptr(k); a.k_stride_t = k.stride(0); a.k_stride_h = k.stride(1);
+      a.v = ptr(v); a.v_stride_t = v.stride(0); a.v_stride_h = v.stride(1);
+      a.out = out_ptr(out);
+      a.lse = static_cast<float*>(out_ptr(lse));
+      const jf_stream_t st = current_stream();
+      r = unlocked([&] { return jf_varlen_attn(&a, st); });
+    }
+    return tuple_of(r, {out, lse});
+  });
+}
+
 #define JF_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     JF_METHOD(quant_write), JF_METHOD(quant_write_kv), JF_METHOD(fused_attn), JF_METHOD(stage_a), JF_METHOD(stage_b),
     JF_METHOD(decode), JF_METHOD(get_workspace), JF_METHOD(blend), JF_METHOD(step_create), JF_METHOD(step_run),
-    JF_METHOD(block8_append), JF_METHOD(block8_attn),
+    JF_METHOD(block8_append), JF_METHOD(block8_attn), JF_METHOD(varlen_attn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "tensor-taking half of jetfire_b200.ops", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

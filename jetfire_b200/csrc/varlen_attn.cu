@@ -1,0 +1,687 @@
+// Attention of packed prompts over their own keys and values (forward), on the fifth-generation tensor cores.
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(f(scale q_i.k_j) - slope |i - j|) where i sees j
+//
+// One pass over the keys per row with a running reference m_i and sum l_i; nothing of size rows x keys leaves the chip.
+// A work item is 256 query rows of one head of one sequence: two tiles of 128 rows that share every tile of 128 keys
+// brought into shared memory.  S = Q K^T (fp32) stands in tensor memory, 128 columns per row tile; a thread owns a row: it
+// reads its 128 scores, turns them into weights and writes them back, 16 bits each, over the scores, where they
+// are the first operand of O += P V.  While one row tile's weights are computed the tensor core works on the other's products.
+//
+//   warps 0-3, 4-7   scores -> weights of row tile 0, 1; the rescaling of O when a reference moves; the result
+//   warp 8           TMA loads: Q of an item, then K and V tiles through a ring of five 32 KB buffers
+//   warp 9           issues the matrix products
+//   warp 10          finds this block's work items (longest rows of all sequences first) ahead of the others
+//   warp 11          clears values that are no numbers out of V tiles with masked entries
+//
+// The reference of a row lags its maximum by up to 2^kLag, so that O is rescaled rarely (both factors are exact
+// powers in the exponent; the sum uses the same ones).  A masked entry's weight is 0, but 0 * inf in the product
+// would not be: warp 11 looks at every V tile that has masked entries and zeroes infinities and NaN in it; rows that do see
+// them get them back at the end (never, with finite inputs).
+//
+// Bound: the exponentials -- 128 x 128 of them a tile at 16 a cycle and multiprocessor are 1024 cycles, the two products of a tile
+// 512.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "decode_common.cuh"
+
+namespace jf {
+namespace {
+
+constexpr int kRows = 128, kKeys = 128;               // of a tile
+constexpr int kPairRows = 2 * kRows;
+constexpr int kKvStages = 5;
+constexpr int kTileBytes = kKeys * JF_HEAD_DIM * 2;   // 32 KB: two slabs of 64 channels, 128-byte swizzle
+constexpr int kSlabBytes = kTileBytes / 2;
+constexpr int kItems = 2;                             // work items looked up ahead
+constexpr int kClean = 4;
+constexpr int kThreads = 384;
+// Registers: the warpgroups of rows take kRowRegs a thread, the other one is left kRoleRegs; together no more than the
+// block is launched with (launch() checks that of the compiled kernel).
+constexpr int kRowRegs = 216, kRoleRegs = 64;
+constexpr float kLag = 8.0f;                          // log2
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Params {
+  const int32_t *cu, *prefix;
+  const float* slopes;
+  const uint16_t* v;
+  uint16_t* out;
+  float* lse;
+  int32_t* status;
+  int64_t v_stride_t, v_stride_h;
+  int32_t T, n_seqs, H_q, H_kv, window;
+  float scale, softcap;
+  bool causal;
+};
+
+struct Item { int row0, len, pair, head, prefix; };   // row0: first row of the sequence; len < 0: no more items
+
+struct Shared {
+  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2], o_full[2], item_full[kItems], item_empty[kItems],
+      cleaned[kClean];
+  Item item[kItems];
+  int bad[kItems];       // V tiles of the item held values that are no numbers
+  uint32_t tmem;
+};
+constexpr int kSmemBytes = 2 * kTileBytes + kKvStages * kTileBytes + 1024;
+
+// ---- tcgen05 ------------------------------------------------------------------------------
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// all products issued so far by this thread, on `bar`
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+#define JF_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
+#define JF_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+// 32 columns of the lane's row
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* x) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : JF_R8(x, 0), JF_R8(x, 8), JF_R8(x, 16), JF_R8(x, 24)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::JF_W8(x, 0), JF_W8(x, 8), JF_W8(x, 16), JF_W8(x, 24), "r"(at)
+      : "memory");
+}
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, kWaitNs); }
+// by a whole warp, which goes on or gives up together
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, kWaitNs)); }
+
+// Shared-memory operand: 128-byte swizzle, rows of 128 bytes in groups of eight (1024 bytes).  K-major operands (Q, K) step
+// through a row's 128 bytes; the MN-major one (V: rows are keys, the contraction) has its 64-channel slabs kSlabBytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t smem, uint32_t lead_bytes) {
+  return static_cast<uint64_t>(smem >> 4 & 0x3FFFu) | static_cast<uint64_t>(lead_bytes >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+         1ull << 46 | 2ull << 61;
+}
+template <int DT> __device__ constexpr uint32_t instruction(bool b_mn_major) {
+  constexpr uint32_t type = DT == JF_DTYPE_BF16 ? 1u : 0u;
+  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
+}
+
+// ---- which keys a row sees ----------------------------------------------------------------
+__device__ __forceinline__ int first_key(const Params& P, int row) { return P.window > 0 ? max(0, row - P.window + 1) : 0; }
+__device__ __forceinline__ int end_key(const Params& P, const Item& it, int row) {
+  if (P.causal) return row + 1;
+  return P.window > 0 ? static_cast<int>(min(static_cast<int64_t>(it.len), static_cast<int64_t>(row) + P.window)) : it.len;
+}
+// The key tiles of an item, prefix first: tiles 0 .. a, then first, first + 1, ...
+struct Keys { int a, first, count; };
+__device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
+  const int r0 = it.pair * kPairRows, r1 = min(r0 + kPairRows, it.len) - 1;
+  const int np = (it.prefix + kKeys - 1) / kKeys, from = first_key(P, r0) / kKeys, to = (end_key(P, it, r1) + kKeys - 1) / kKeys;
+  Keys k;
+  k.a = min(np, from);
+  k.first = from;
+  k.count = k.a + max(to, np) - from;
+  return k;
+}
+__device__ __forceinline__ int tile_of(const Keys& k, int i) { return i < k.a ? i : k.first + i - k.a; }
+// does any row of the tile that starts at row q0 see a key of tile `t`; does every one see all of it
+__device__ __forceinline__ bool uses(const Params& P, const Item& it, int q0, int t) {
+  if (q0 >= it.len) return false;
+  const int k0 = t * kKeys, r1 = min(q0 + kRows, it.len) - 1;
+  return k0 < it.prefix || (k0 < end_key(P, it, r1) && k0 + kKeys > first_key(P, q0));
+}
+__device__ __forceinline__ bool masked(const Params& P, const Item& it, int q0, int t) {
+  const int k0 = t * kKeys, r1 = min(q0 + kRows, it.len) - 1;
+  return !(k0 + kKeys <= it.prefix || (k0 + kKeys <= end_key(P, it, q0) && k0 + kKeys <= it.len && k0 >= first_key(P, r1)));
+}
+__device__ __forceinline__ bool needs_clean(const Params& P, const Item& it, int t) {
+  const int q0 = it.pair * kPairRows;
+  return (uses(P, it, q0, t) && masked(P, it, q0, t)) || (uses(P, it, q0 + kRows, t) && masked(P, it, q0 + kRows, t));
+}
+__device__ __forceinline__ bool sees(const Params& P, const Item& it, int row, int j) {
+  return j < it.len && (j < it.prefix || (j >= first_key(P, row) && j < end_key(P, it, row)));
+}
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+template <int DT> __device__ __forceinline__ bool no_number(uint32_t half) {
+  constexpr uint32_t inf = DT == JF_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  return (half & inf) == inf;
+}
+
+// ---- the roles ------------------------------------------------------------------------------
+
+// Work items of this block: level by level (the l-th 256 rows of every sequence that has them, from the last), heads
+// fastest, so that long rows come first and heads that share keys run at the same time; every gridDim.x-th is this block's.
+__device__ __forceinline__ bool schedule(const Params& P, Shared& S) {
+  const int lane = threadIdx.x & 31;
+  int slot = 0, uses_of_slot = 0;
+  auto emit = [&](int row0, int len, int pair, int head, int prefix) {
+    bool ok = true;
+    if (uses_of_slot > 0) ok = wait_warp(&S.item_empty[slot], (uses_of_slot - 1) & 1);
+    if (!ok) return false;
+    if (lane == 0) {
+      S.item[slot] = Item{row0, len, pair, head, prefix};
+      S.bad[slot] = 0;
+      mbar_arrive(&S.item_full[slot]);
+    }
+    __syncwarp();
+    if (++slot == kItems) { slot = 0; ++uses_of_slot; }
+    return true;
+  };
+  auto bounds = [&](int s, int& row0, int& len) {
+    row0 = len = 0;
+    if (s < P.n_seqs) {
+      row0 = min(max(P.cu[s], 0), P.T);
+      len = min(max(P.cu[s + 1], row0), P.T) - row0;
+    }
+  };
+  int row0, len, most = 0;
+  for (int c = 0; c < P.n_seqs; c += 32) {
+    bounds(c + lane, row0, len);
+    most = max(most, static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(len))));
+  }
+  int64_t want = blockIdx.x, before = 0;
+  for (int level = (most + kPairRows - 1) / kPairRows - 1; level >= 0; --level)
+    for (int c = 0; c < P.n_seqs; c += 32) {
+      if (P.n_seqs > 32) bounds(c + lane, row0, len);
+      const unsigned has = __ballot_sync(0xFFFFFFFFu, len > level * kPairRows);
+      const int64_t n = static_cast<int64_t>(__popc(has)) * P.H_q;
+      while (want < before + n) {
+        const int at = static_cast<int>(want - before), src = __fns(has, 0, at / P.H_q + 1);
+        const int r = __shfl_sync(0xFFFFFFFFu, row0, src), l = __shfl_sync(0xFFFFFFFFu, len, src);
+        const int prefix = P.prefix ? min(max(P.prefix[c + src], 0), l) : 0;
+        if (!emit(r, l, level, at % P.H_q, prefix)) return false;
+        want += gridDim.x;
+      }
+      before += n;
+    }
+  return emit(0, -1, 0, 0, 0);
+}
+
+struct ItemReader {
+  int slot = 0, round = 0;
+  template <bool WARP = false> __device__ __forceinline__ bool next(Shared& S, Item& it) {
+    if (!(WARP ? wait_warp(&S.item_full[slot], round & 1) : wait(&S.item_full[slot], round & 1))) return false;
+    it = S.item[slot];
+    return true;
+  }
+  __device__ __forceinline__ void release(Shared& S) {   // by one thread for its warp
+    mbar_arrive(&S.item_empty[slot]);
+    if (++slot == kItems) { slot = 0; ++round; }
+  }
+};
+struct Ring {   // position in the ring of K and V tiles
+  int stage = 0, round = 0;
+  __device__ __forceinline__ void step(int n = 1) {
+    stage += n;
+    if (stage >= kKvStages) { stage -= kKvStages; ++round; }
+  }
+};
+
+__device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, const CUtensorMap* qm, const CUtensorMap* km,
+                                     const CUtensorMap* vm) {
+  ItemReader items;
+  Item it;
+  Ring ring;
+  const int group = P.H_q / P.H_kv;
+  for (int n = 0;; ++n) {
+    if (!items.next(S, it)) return false;
+    if (it.len < 0) return true;
+    const Keys keys = keys_of(P, it);
+    const int q0 = it.pair * kPairRows, kvh = it.head / group;
+    const bool two = q0 + kRows < it.len;
+    if (n > 0 && !wait(&S.q_empty, (n - 1) & 1)) return false;
+    mbar_expect_tx(&S.q_full, two ? 2 * kTileBytes : kTileBytes);
+    for (int t = 0; t < (two ? 2 : 1); ++t)
+      for (int slab = 0; slab < 2; ++slab)
+        tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head, it.row0 + q0 + t * kRows, &S.q_full);
+    for (int i = 0; i < keys.count; ++i) {
+      const int row = it.row0 + tile_of(keys, i) * kKeys;
+      for (int side = 0; side < 2; ++side) {
+        if (ring.round > 0 && !wait(&S.kv_empty[ring.stage], (ring.round - 1) & 1)) return false;
+        mbar_expect_tx(&S.kv_full[ring.stage], kTileBytes);
+        for (int slab = 0; slab < 2; ++slab)
+          tma_load(kv_smem + ring.stage * kTileBytes + slab * kSlabBytes, side ? vm : km, slab * 64, kvh, row, &S.kv_full[ring.stage]);
+        ring.step();
+      }
+    }
+    items.release(S);
+  }
+}
+
+template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, uint32_t tmem) {
+  constexpr uint32_t qk = instruction<DT>(false), pv = instruction<DT>(true);
+  ItemReader items;
+  Item it;
+  Ring ring;
+  int p_count[2] = {0, 0}, clean = 0;
+  for (int n = 0;; ++n) {
+    if (!items.next(S, it)) return false;
+    if (it.len < 0) return true;
+    const Keys keys = keys_of(P, it);
+    const int q0 = it.pair * kPairRows;
+    int last[2];
+    for (int t = 0; t < 2; ++t) {
+      last[t] = keys.count - 1;
+      while (last[t] >= 0 && !uses(P, it, q0 + t * kRows, tile_of(keys, last[t]))) --last[t];
+    }
+    if (!wait(&S.q_full, n & 1)) return false;
+    auto scores = [&](int t, int stage) {
+      const uint32_t a = q_smem + t * kTileBytes, b = kv_smem + stage * kTileBytes;
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t off = (k >> 2) * kSlabBytes + (k & 3) * 32;
+        mma_ss(tmem + t * 128, operand(a + off, 16), operand(b + off, 16), qk, k > 0);
+      }
+      tc_commit(&S.s_full[t]);
+    };
+    bool started[2] = {false, false};
+    for (int i = -1; i < keys.count; ++i) {
+      // products with V of tile i and scores of tile i + 1, row tile by row tile
+      Ring v_ring = ring, k_ring = ring;
+      if (i >= 0) k_ring.step();
+      bool v_here = false, k_here = false;
+      for (int t = 0; t < 2; ++t) {
+        if (i >= 0 && uses(P, it, q0 + t * kRows, tile_of(keys, i))) {
+          if (!v_here) {
+            if (!wait(&S.kv_full[v_ring.stage], v_ring.round & 1)) return false;
+            if (needs_clean(P, it, tile_of(keys, i))) {
+              if (!wait(&S.cleaned[clean % kClean], clean / kClean & 1)) return false;
+              ++clean;
+            }
+            v_here = true;
+          }
+          if (!wait(&S.p_full[t], p_count[t]++ & 1)) return false;
+          tc_fence_after();
+          const uint32_t b = kv_smem + v_ring.stage * kTileBytes;
+          for (int k = 0; k < 8; ++k)
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, operand(b + k * 2048, kSlabBytes), pv, started[t] || k > 0);
+          started[t] = true;
+          if (i == last[t]) tc_commit(&S.o_full[t]);
+        }
+        if (i + 1 < keys.count && uses(P, it, q0 + t * kRows, tile_of(keys, i + 1))) {
+          if (!k_here) {
+            if (!wait(&S.kv_full[k_ring.stage], k_ring.round & 1)) return false;
+            k_here = true;
+          }
+          tc_fence_after();
+          scores(t, k_ring.stage);
+        }
+      }
+      if (i >= 0) tc_commit(&S.kv_empty[v_ring.stage]);
+      if (i + 1 < keys.count) tc_commit(&S.kv_empty[k_ring.stage]);
+      if (i + 2 == keys.count) tc_commit(&S.q_empty);
+      ring = k_ring;
+      ring.step();
+    }
+    // (the last step moved past a K tile that does not exist)
+    ring.stage = ring.stage == 0 ? (--ring.round, kKvStages - 1) : ring.stage - 1;
+    items.release(S);
+  }
+}
+
+template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, Shared& S, unsigned char* kv) {
+  constexpr uint32_t inf = DT == JF_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  const int lane = threadIdx.x & 31;
+  ItemReader items;
+  Item it;
+  Ring ring;
+  int clean = 0;
+  for (;;) {
+    if (!items.next<true>(S, it)) return false;
+    if (it.len < 0) return true;
+    const Keys keys = keys_of(P, it);
+    for (int i = 0; i < keys.count; ++i) {
+      // every buffer is waited for and passed on, so that none is filled twice in between
+      if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
+      if (lane == 0) mbar_arrive(&S.kv_empty[ring.stage]);
+      ring.step();
+      if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
+      const int t = tile_of(keys, i);
+      if (needs_clean(P, it, t)) {
+        uint4* tile = reinterpret_cast<uint4*>(kv + ring.stage * kTileBytes);
+        uint32_t top = 0;
+#pragma unroll 8
+        for (int n = lane; n < kTileBytes / 16; n += 32) {
+          const uint4 x = tile[n];
+          top = __vmaxu2(__vmaxu2(top, __vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu)), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+        }
+        if (__any_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16) >= inf)) {
+          bool own = false;   // among the sequence's own rows
+          for (int n = lane; n < kTileBytes / 4; n += 32) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(tile) + n;
+            const uint32_t x = *w, y = (no_number<DT>(x) ? 0u : x & 0xFFFFu) | (no_number<DT>(x >> 16) ? 0u : x & 0xFFFF0000u);
+            if (x != y) {
+              *w = y;
+              own |= t * kKeys + (n * 4 % kSlabBytes) / 128 < it.len;
+            }
+          }
+          fence_proxy_async();
+          if (__any_sync(0xFFFFFFFFu, own) && lane == 0) S.bad[items.slot] = 1;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.cleaned[clean % kClean]);
+        ++clean;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.kv_empty[ring.stage]);
+      ring.step();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.item_empty[items.slot]);
+    if (++items.slot == kItems) { items.slot = 0; ++items.round; }
+  }
+}
+
+template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params& P, Shared& S, uint32_t tmem, int t) {
+  constexpr float kLift = DT == JF_DTYPE_FP16 ? 7.0f : 0.0f;   // fp16 weights use the range up to 2^15
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, r = warp * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+  const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+  const float sl2 = P.scale * kLog2e;
+  ItemReader items;
+  Item it;
+  int s_count = 0, o_count = 0;
+  for (;;) {
+    if (!items.next<true>(S, it)) return false;
+    if (it.len < 0) return true;
+    const Keys keys = keys_of(P, it);
+    const int q0 = it.pair * kPairRows + t * kRows, row = q0 + r;
+    const float slope = FEAT && P.slopes ? P.slopes[it.head] : 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    bool have = false;
+    for (int i = 0; i < keys.count; ++i) {
+      const int tile = tile_of(keys, i), k0 = tile * kKeys;
+      if (!uses(P, it, q0, tile)) continue;
+      if (!wait_warp(&S.s_full[t], s_count++ & 1)) return false;
+      tc_fence_after();
+      uint32_t u[128];
+      float* s = reinterpret_cast<float*>(u);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, u + c * 32);
+      tc_wait_ld();
+      if (FEAT) {
+        const float cap = P.softcap, to_e = cap > 0.0f ? 2.0f * sl2 / cap : 0.0f;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          float x;
+          if (cap > 0.0f) {   // cap * tanh(x / cap) = cap - 2 cap / (e^(2x / cap) + 1)
+            x = (cap - __fdividef(2.0f * cap, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f)) * kLog2e;
+          } else {
+            x = s[c] * sl2;
+          }
+          s[c] = x - slope * kLog2e * fabsf(static_cast<float>(row - k0 - c));
+        }
+      }
+      if (masked(P, it, q0, tile)) {
+        const int a = first_key(P, row) - k0, b = min(end_key(P, it, row), it.len) - k0, p = it.prefix - k0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t bits = (below(b - 32 * w) & ~below(a - 32 * w)) | below(p - 32 * w);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[w * 32 + c] = bits >> c & 1u ? s[w * 32 + c] : -INFINITY;
+        }
+      }
+      float top4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 128; ++c) top4[c & 3] = fmaxf(top4[c & 3], s[c]);
+      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * (FEAT ? 1.0f : sl2);
+      if (__any_sync(0xFFFFFFFFu, top > m + kLag)) {
+        const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
+        m = to;
+        l *= f;
+        if (have) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st32(o_at + c * 32, o);
+          }
+        }
+      }
+      have = true;
+      const float ref = m == -INFINITY ? 0.0f : m - kLift;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 128; ++c) {
+        s[c] = ex2(FEAT ? s[c] - ref : fmaf(s[c], sl2, -ref));
+        sum[c & 3] += s[c];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[c]) : "f"(s[h * 64 + 2 * c + 1]), "f"(s[h * 64 + 2 * c]));
+          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c]) : "f"(s[h * 64 + 2 * c + 1]), "f"(s[h * 64 + 2 * c]));
+        }
+        tmem_st32(s_at + h * 32, p);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.p_full[t]);
+    }
+    if (have) {
+      if (!wait_warp(&S.o_full[t], o_count++ & 1)) return false;
+      tc_fence_after();
+      const int64_t at = (static_cast<int64_t>(it.row0) + row) * P.H_q + it.head;
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const bool bad = S.bad[items.slot] != 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_at + c * 32, o);
+        tc_wait_ld();
+        if (bad && row < it.len) {
+          for (int i = 0; i < keys.count; ++i) {
+            const int tile = tile_of(keys, i);
+            if (!needs_clean(P, it, tile)) continue;
+            for (int j = tile * kKeys; j < min((tile + 1) * kKeys, it.len); ++j) {
+              if (!sees(P, it, row, j)) continue;
+              const uint16_t* v = P.v + (static_cast<int64_t>(it.row0) + j) * P.v_stride_t + it.head / (P.H_q / P.H_kv) * P.v_stride_h + c * 32;
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (no_number<DT>(v[k])) o[k] = __float_as_uint(__uint_as_float(o[k]) + Elem<DT>::to_f32(v[k]));
+            }
+          }
+        }
+        if (row < it.len) {
+          uint4* out = reinterpret_cast<uint4*>(P.out + at * JF_HEAD_DIM + c * 32);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = __uint_as_float(o[k * 8 + e * 2]) * inv, y = __uint_as_float(o[k * 8 + e * 2 + 1]) * inv;
+              w[e] = Elem<DT>::from_f32(x) | static_cast<uint32_t>(Elem<DT>::from_f32(y)) << 16;
+            }
+            out[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before();
+      if (row < it.len && P.lse) P.lse[at] = l > 0.0f || l != l ? (m - kLift + __log2f(l)) * kLn2 : -INFINITY;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.item_empty[items.slot]);
+    if (++items.slot == kItems) { items.slot = 0; ++items.round; }
+  }
+}
+
+template <int DT, bool FEAT>
+__global__ void __launch_bounds__(kThreads, 1)
+varlen_attn_kernel(const Params P, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                   const __grid_constant__ CUtensorMap vm) {
+  extern __shared__ unsigned char raw[];
+  __shared__ Shared S;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t q_smem = smem_u32(smem), kv_smem = q_smem + 2 * kTileBytes;
+  if (threadIdx.x == 0) {
+    mbar_init(&S.q_full, 1);
+    mbar_init(&S.q_empty, 1);
+    for (int i = 0; i < kKvStages; ++i) { mbar_init(&S.kv_full[i], 1); mbar_init(&S.kv_empty[i], 2); }   // empty: products done, looked over
+    for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t], 4); mbar_init(&S.o_full[t], 1); }
+    for (int i = 0; i < kItems; ++i) { mbar_init(&S.item_full[i], 1); mbar_init(&S.item_empty[i], 11); }   // 8 + loads, products, cleaning
+    for (int i = 0; i < kClean; ++i) mbar_init(&S.cleaned[i], 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem;
+  pdl_wait();
+  pdl_trigger();
+  // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
+  bool ok = true;
+  if (warp >= 8) {
+    regs_dec<kRoleRegs>();
+    if (warp == 8) {
+      if (lane == 0) ok = load(P, S, q_smem, kv_smem, &qm, &km, &vm);
+    } else if (warp == 9) {
+      if (lane == 0) ok = multiply<DT>(P, S, q_smem, kv_smem, tmem);
+    } else if (warp == 10) {
+      ok = schedule(P, S);
+    } else {
+      ok = clean_values<DT>(P, S, smem + 2 * kTileBytes);
+    }
+  } else {
+    regs_inc<kRowRegs>();
+    ok = soften<DT, FEAT>(P, S, tmem, warp >> 2);
+  }
+  if (!ok && P.status) report_status(P.status, JF_ERR_TIMEOUT);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess)
+      sym = nullptr;
+    return reinterpret_cast<EncodeFn>(sym);
+  }();
+  return fn;
+}
+
+// (rows, heads, 128) as boxes of 128 rows of one head, 64 channels wide; rows past the end read as zeros.
+jf_status_t rows_map(const void* base, int dtype, int64_t T, int32_t H, int64_t stride_t, int64_t stride_h, CUtensorMap* out) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return JF_ERR_CUDA;
+  const cuuint64_t dims[3] = {JF_HEAD_DIM, static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(T)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(H > 1 ? stride_h : JF_HEAD_DIM) * 2,
+                                 static_cast<cuuint64_t>(T > 1 ? stride_t : JF_HEAD_DIM) * 2};
+  const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, dtype == JF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { g_last_cuda_error = static_cast<int32_t>(r); return JF_ERR_CUDA; }
+  return JF_OK;
+}
+
+template <int DT, bool FEAT>
+jf_status_t launch(const Params& P, int grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
+  auto* kernel = varlen_attn_kernel<DT, FEAT>;
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, varlen_attn_kernel<DT, FEAT>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  // (a warpgroup that asks for more than the block has waits for good)
+  if (regs * kThreads < 256 * kRowRegs + 128 * kRoleRegs) return JF_ERR_UNSUPPORTED;
+  JF_ENSURE_SMEM(kernel, kSmemBytes);
+  JF_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmemBytes, s, P, q, k, v));
+  return JF_OK;
+}
+
+}  // namespace
+}  // namespace jf
+
+extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t stream) {
+  using namespace jf;
+  if (!a) return JF_ERR_ARG;
+  if (a->dtype != JF_DTYPE_BF16 && a->dtype != JF_DTYPE_FP16) return JF_ERR_ARG;
+  if (a->T < 0 || a->n_seqs < 0 || a->H_q <= 0 || a->H_kv <= 0 || a->H_q % a->H_kv != 0 || a->window < 0) return JF_ERR_ARG;
+  if (!(a->softcap >= 0.0f) || a->softcap > 3.0e38f) return JF_ERR_ARG;
+  if (a->T > INT32_MAX / 2) return JF_ERR_UNSUPPORTED;
+  if (a->T == 0 || a->n_seqs == 0) return JF_OK;
+  if (!a->q || !a->k || !a->v || !a->cu_seqlens || !a->out) return JF_ERR_ARG;
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || !aligned(a->status_record, 8)) return JF_ERR_ARG;
+  auto stride_ok = [](int64_t size, int64_t stride) { return size == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  if (!stride_ok(a->T, a->q_stride_t) || !stride_ok(a->H_q, a->q_stride_h) || !stride_ok(a->T, a->k_stride_t) || !stride_ok(a->H_kv, a->k_stride_h) ||
+      !stride_ok(a->T, a->v_stride_t) || !stride_ok(a->H_kv, a->v_stride_h))
+    return JF_ERR_ARG;
+  CUtensorMap q, k, v;
+  jf_status_t st = rows_map(a->q, a->dtype, a->T, a->H_q, a->q_stride_t, a->q_stride_h, &q);
+  if (st == JF_OK) st = rows_map(a->k, a->dtype, a->T, a->H_kv, a->k_stride_t, a->k_stride_h, &k);
+  if (st == JF_OK) st = rows_map(a->v, a->dtype, a->T, a->H_kv, a->v_stride_t, a->v_stride_h, &v);
+  if (st != JF_OK) return st;
+  Params P{};
+  P.cu = a->cu_seqlens;
+  P.prefix = a->prefix_lens;
+  P.slopes = a->alibi_slopes;
+  P.v = static_cast<const uint16_t*>(a->v);
+  P.out = static_cast<uint16_t*>(a->out);
+  P.lse = a->lse;
+  P.status = static_cast<int32_t*>(a->status_record);
+  P.v_stride_t = a->v_stride_t;
+  P.v_stride_h = a->v_stride_h;
+  P.T = static_cast<int32_t>(a->T);
+  P.n_seqs = a->n_seqs;
+  P.H_q = a->H_q;
+  P.H_kv = a->H_kv;
+  P.window = a->window;
+  P.scale = a->attn_scale;
+  P.softcap = a->softcap;
+  P.causal = a->causal != 0;
+  const int64_t most = (a->T / kPairRows + std::min<int64_t>(a->n_seqs, a->T)) * a->H_q;   // work items
+  const int grid = static_cast<int>(std::min<int64_t>(num_sms(), most));
+  const bool feat = a->softcap > 0.0f || a->alibi_slopes || !(a->attn_scale > 0.0f);   // (the plain form takes the maximum before it scales)
+  const auto s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == JF_DTYPE_BF16) return feat ? launch<JF_DTYPE_BF16, true>(P, grid, s, q, k, v) : launch<JF_DTYPE_BF16, false>(P, grid, s, q, k, v);
+  return feat ? launch<JF_DTYPE_FP16, true>(P, grid, s, q, k, v) : launch<JF_DTYPE_FP16, false>(P, grid, s, q, k, v);
+}

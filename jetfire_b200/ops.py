@@ -572,6 +572,24 @@ def block8_decode_attn(q, k_data, k_scales, v_data, v_scales, block_table, seq_l
     return out, lse
 
 
+def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=None, softcap=0.0, alibi_slopes=None,
+                        prefix_lens=None, out=None, status_record=None):
+    """Attention of packed prompts over their own keys and values, each sequence (document) by itself.
+
+    ``q (T, H_q, 128)``, ``k / v (T, H_kv, 128)`` bf16 or fp16; any strides, copied first where tensor copies cannot
+    address them (innermost dim not contiguous, rows not 16-byte aligned).  Sequence i owns the rows ``cu_seqlens[i] ..
+    cu_seqlens[i + 1]`` (int32).  Scores as in ``block8_decode_attn``, with ``|i - j|`` for the distance.  Row i
+    sees ``j <= i`` (``causal``) closer than ``window``, and the first ``prefix_lens[sequence]`` positions from anywhere;
+    what it does not see has no influence, not even as an infinity or a NaN.  Rows of no sequence are not written.
+    Returns ``(out (T, H_q, 128), lse (T, H_q) float32)``.  ``status_record``: 16 cleared bytes on the device in which the
+    kernel notes a wait that ran out (``decode_status_of_copy`` reads a host copy)."""
+    name = "varlen_prefill_attn"
+    st, out, lse = _host.varlen_attn(name, q, k, v, cu_seqlens, attn_scale, causal, _window(window, name), softcap, alibi_slopes,
+                                     prefix_lens, out, status_record)
+    check(name, st)
+    return out, lse
+
+
 # ---------------------------------------------------------------------------------------
 # correction merge
 # ---------------------------------------------------------------------------------------

@@ -108,3 +108,48 @@ def test_ops_refuse_wrong_shapes_and_types(L):
                dict(out=z(1, 4, 256, dtype=bf)[..., ::2])):
         with pytest.raises(RuntimeError):
             ops.block8_decode_attn(*call.values(), **kw)
+
+
+# ---- packed prompts -----------------------------------------------------------------------
+
+
+def _varlen(L, **kw):
+    a = L.VarlenAttnArgs()
+    a.dtype, a.n_seqs, a.H_q, a.H_kv, a.causal, a.attn_scale, a.T = 0, 2, 8, 2, 1, 0.1, 40
+    a.q_stride_t, a.q_stride_h, a.k_stride_t, a.k_stride_h, a.v_stride_t, a.v_stride_h = 1024, 128, 256, 128, 256, 128
+    for n in ("q", "k", "v", "cu_seqlens", "out"):
+        setattr(a, n, 4096)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return L.lib.jf_varlen_attn(C.byref(a), None)
+
+
+def test_varlen_status(L):
+    assert C.sizeof(L.VarlenAttnArgs) == 8 * 4 + 7 * 8 + 9 * 8
+    assert L.lib.jf_varlen_attn(None, None) == L.JF_ERR_ARG
+    for bad in (dict(dtype=3), dict(n_seqs=-1), dict(H_q=0), dict(H_q=7), dict(H_kv=0), dict(window=-1), dict(softcap=-1.0),
+                dict(softcap=float("nan")), dict(T=-1), dict(q=None), dict(k=None), dict(v=None), dict(cu_seqlens=None), dict(out=None), dict(q=4104),
+                dict(k=4098), dict(v=4100), dict(out=4104), dict(status_record=4100), dict(q_stride_t=1028), dict(k_stride_h=0), dict(v_stride_t=-256)):
+        assert _varlen(L, **bad) == L.JF_ERR_ARG, bad
+    assert _varlen(L, T=2 ** 31) == L.JF_ERR_UNSUPPORTED
+    assert _varlen(L, T=0) == L.JF_OK and _varlen(L, n_seqs=0) == L.JF_OK
+
+
+@pytest.mark.gpu
+def test_varlen_refuses_wrong_shapes_and_types(L):
+    from jetfire_b200 import ops
+    def z(*s, dtype=torch.bfloat16):
+        return torch.zeros(*s, dtype=dtype, device="cuda")
+    i32 = torch.int32
+    good = dict(q=z(9, 4, 128), k=z(9, 2, 128), v=z(9, 2, 128), cu=torch.tensor([0, 9], dtype=i32, device="cuda"), scale=0.1)
+    ops.varlen_prefill_attn(*good.values())
+    for kw in (dict(q=z(9, 3, 128)), dict(q=z(9, 4, 64)), dict(k=z(8, 2, 128)), dict(v=z(9, 1, 128)), dict(v=z(9, 2, 128, dtype=torch.float16)),
+               dict(q=z(9, 4, 128, dtype=torch.float32)), dict(cu=torch.tensor([0, 9], device="cuda")), dict(cu=torch.tensor([0, 9], dtype=i32)),
+               dict(cu=z(1, 2, dtype=i32)), dict(q=torch.zeros(9, 4, 128, dtype=torch.bfloat16))):
+        with pytest.raises(RuntimeError):
+            ops.varlen_prefill_attn(*{**good, **kw}.values())
+    for kw in (dict(window=0), dict(window=-3), dict(softcap=-1.0), dict(softcap=float("nan")), dict(alibi_slopes=z(4)), dict(alibi_slopes=z(3, dtype=torch.float32)),
+               dict(prefix_lens=z(2, dtype=i32)), dict(out=z(9, 4, 128, dtype=torch.float16)), dict(out=z(9, 4, 256)[..., ::2]),
+               dict(status_record=z(4)), dict(out=z(8, 4, 128))):
+        with pytest.raises(RuntimeError):
+            ops.varlen_prefill_attn(*good.values(), **kw)
