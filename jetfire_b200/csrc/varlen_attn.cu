@@ -40,8 +40,9 @@ constexpr int kClean = 4;
 constexpr int kThreads = 384;
 // Registers: the warpgroups of rows take kRowRegs a thread, the other one is left kRoleRegs; together no more than the
 // block is launched with (launch() checks that of the compiled kernel).
-constexpr int kRowRegs = 216, kRoleRegs = 64;
+constexpr int kRowRegs = 208, kRoleRegs = 80;
 constexpr float kLag = 8.0f;                          // log2
+constexpr int kPoly = 1;                              // of four pairs of exponentials, on the multiply-add units
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -61,7 +62,7 @@ struct Params {
 struct Item { int row0, len, pair, head, prefix; };   // row0: first row of the sequence; len < 0: no more items
 
 struct Shared {
-  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2], o_full[2], item_full[kItems], item_empty[kItems],
+  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], o_full[2], item_full[kItems], item_empty[kItems],
       cleaned[kClean];
   Item item[kItems];
   int bad[kItems];       // V tiles of the item held values that are no numbers
@@ -118,9 +119,15 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, kWaitNs); }
+// Bounded.  Most waits end within a few attempts; the clock that bounds the others is read only after that (a read of it
+// in front of every wait that did not end at once took 0.4 us of each step).
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < 1000; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, kWaitNs);
+}
 // by a whole warp, which goes on or gives up together
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, kWaitNs)); }
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
 
 // Shared-memory operand: 128-byte swizzle, rows of 128 bytes in groups of eight (1024 bytes).  K-major operands (Q, K) step
 // through a row's 128 bytes; the MN-major one (V: rows are keys, the contraction) has its 64-channel slabs kSlabBytes apart.
@@ -139,7 +146,28 @@ __device__ __forceinline__ int end_key(const Params& P, const Item& it, int row)
   if (P.causal) return row + 1;
   return P.window > 0 ? static_cast<int>(min(static_cast<int64_t>(it.len), static_cast<int64_t>(row) + P.window)) : it.len;
 }
-// The key tiles of an item, prefix first: tiles 0 .. a, then first, first + 1, ...
+__device__ __forceinline__ bool sees(const Params& P, const Item& it, int row, int j) {
+  return j < it.len && (j < it.prefix || (j >= first_key(P, row) && j < end_key(P, it, row)));
+}
+// Key tiles of a row tile: some row sees some of tile t if t < some_p or lo <= t < hi; every row sees all of it if
+// t < all_p or all_lo <= t < all_hi.
+struct Tiles {
+  int some_p, lo, hi, all_p, all_lo, all_hi;
+  __device__ __forceinline__ bool uses(int t) const { return t < some_p || (t >= lo && t < hi); }
+  __device__ __forceinline__ bool masked(int t) const { return t >= all_p && (t < all_lo || t >= all_hi); }
+  __device__ __forceinline__ bool partly(int t) const { return uses(t) && masked(t); }
+};
+__device__ __forceinline__ Tiles tiles_of(const Params& P, const Item& it, int q0) {
+  if (q0 >= it.len) return Tiles{0, 0, 0, 0, 0, 0};
+  const int r1 = min(q0 + kRows, it.len) - 1;
+  return Tiles{(it.prefix + kKeys - 1) / kKeys,
+               first_key(P, q0) / kKeys,
+               (end_key(P, it, r1) + kKeys - 1) / kKeys,
+               it.prefix / kKeys,
+               (first_key(P, r1) + kKeys - 1) / kKeys,
+               min(end_key(P, it, q0), it.len) / kKeys};
+}
+// The key tiles of an item, prefix first: tiles 0 .. a, then first, first + 1, ...  Each is used by one of its row tiles.
 struct Keys { int a, first, count; };
 __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
   const int r0 = it.pair * kPairRows, r1 = min(r0 + kPairRows, it.len) - 1;
@@ -151,23 +179,6 @@ __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
   return k;
 }
 __device__ __forceinline__ int tile_of(const Keys& k, int i) { return i < k.a ? i : k.first + i - k.a; }
-// does any row of the tile that starts at row q0 see a key of tile `t`; does every one see all of it
-__device__ __forceinline__ bool uses(const Params& P, const Item& it, int q0, int t) {
-  if (q0 >= it.len) return false;
-  const int k0 = t * kKeys, r1 = min(q0 + kRows, it.len) - 1;
-  return k0 < it.prefix || (k0 < end_key(P, it, r1) && k0 + kKeys > first_key(P, q0));
-}
-__device__ __forceinline__ bool masked(const Params& P, const Item& it, int q0, int t) {
-  const int k0 = t * kKeys, r1 = min(q0 + kRows, it.len) - 1;
-  return !(k0 + kKeys <= it.prefix || (k0 + kKeys <= end_key(P, it, q0) && k0 + kKeys <= it.len && k0 >= first_key(P, r1)));
-}
-__device__ __forceinline__ bool needs_clean(const Params& P, const Item& it, int t) {
-  const int q0 = it.pair * kPairRows;
-  return (uses(P, it, q0, t) && masked(P, it, q0, t)) || (uses(P, it, q0 + kRows, t) && masked(P, it, q0 + kRows, t));
-}
-__device__ __forceinline__ bool sees(const Params& P, const Item& it, int row, int j) {
-  return j < it.len && (j < it.prefix || (j >= first_key(P, row) && j < end_key(P, it, row)));
-}
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
 template <int DT> __device__ __forceinline__ bool no_number(uint32_t half) {
@@ -227,13 +238,14 @@ __device__ __forceinline__ bool schedule(const Params& P, Shared& S) {
 
 struct ItemReader {
   int slot = 0, round = 0;
-  template <bool WARP = false> __device__ __forceinline__ bool next(Shared& S, Item& it) {
-    if (!(WARP ? wait_warp(&S.item_full[slot], round & 1) : wait(&S.item_full[slot], round & 1))) return false;
+  __device__ __forceinline__ bool next(Shared& S, Item& it) {
+    if (!wait_warp(&S.item_full[slot], round & 1)) return false;
     it = S.item[slot];
     return true;
   }
-  __device__ __forceinline__ void release(Shared& S) {   // by one thread for its warp
-    mbar_arrive(&S.item_empty[slot]);
+  __device__ __forceinline__ void release_warp(Shared& S) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&S.item_empty[slot]);
     if (++slot == kItems) { slot = 0; ++round; }
   }
 };
@@ -257,27 +269,34 @@ __device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem
     const Keys keys = keys_of(P, it);
     const int q0 = it.pair * kPairRows, kvh = it.head / group;
     const bool two = q0 + kRows < it.len;
-    if (n > 0 && !wait(&S.q_empty, (n - 1) & 1)) return false;
-    mbar_expect_tx(&S.q_full, two ? 2 * kTileBytes : kTileBytes);
-    for (int t = 0; t < (two ? 2 : 1); ++t)
-      for (int slab = 0; slab < 2; ++slab)
-        tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head, it.row0 + q0 + t * kRows, &S.q_full);
+    if (n > 0 && !wait_warp(&S.q_empty, (n - 1) & 1)) return false;
+    if (elect_one()) {
+      mbar_expect_tx(&S.q_full, two ? 2 * kTileBytes : kTileBytes);
+      for (int t = 0; t < (two ? 2 : 1); ++t)
+        for (int slab = 0; slab < 2; ++slab)
+          tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head, it.row0 + q0 + t * kRows, &S.q_full);
+    }
+    __syncwarp();
     for (int i = 0; i < keys.count; ++i) {
       const int row = it.row0 + tile_of(keys, i) * kKeys;
       for (int side = 0; side < 2; ++side) {
-        if (ring.round > 0 && !wait(&S.kv_empty[ring.stage], (ring.round - 1) & 1)) return false;
-        mbar_expect_tx(&S.kv_full[ring.stage], kTileBytes);
-        for (int slab = 0; slab < 2; ++slab)
-          tma_load(kv_smem + ring.stage * kTileBytes + slab * kSlabBytes, side ? vm : km, slab * 64, kvh, row, &S.kv_full[ring.stage]);
+        if (ring.round > 0 && !wait_warp(&S.kv_empty[ring.stage], (ring.round - 1) & 1)) return false;
+        if (elect_one()) {
+          mbar_expect_tx(&S.kv_full[ring.stage], kTileBytes);
+          for (int slab = 0; slab < 2; ++slab)
+            tma_load(kv_smem + ring.stage * kTileBytes + slab * kSlabBytes, side ? vm : km, slab * 64, kvh, row, &S.kv_full[ring.stage]);
+        }
+        __syncwarp();
         ring.step();
       }
     }
-    items.release(S);
+    items.release_warp(S);
   }
 }
 
 template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, uint32_t tmem) {
   constexpr uint32_t qk = instruction<DT>(false), pv = instruction<DT>(true);
+  const uint64_t q_op = operand(q_smem, 16), k_op = operand(kv_smem, 16), v_op = operand(kv_smem, kSlabBytes);
   ItemReader items;
   Item it;
   Ring ring;
@@ -287,62 +306,82 @@ template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shar
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
     const int q0 = it.pair * kPairRows;
+    const Tiles tiles[2] = {tiles_of(P, it, q0), tiles_of(P, it, q0 + kRows)};
     int last[2];
+#pragma unroll
     for (int t = 0; t < 2; ++t) {
       last[t] = keys.count - 1;
-      while (last[t] >= 0 && !uses(P, it, q0 + t * kRows, tile_of(keys, last[t]))) --last[t];
+      while (last[t] >= 0 && !tiles[t].uses(tile_of(keys, last[t]))) --last[t];
     }
-    if (!wait(&S.q_full, n & 1)) return false;
-    auto scores = [&](int t, int stage) {
-      const uint32_t a = q_smem + t * kTileBytes, b = kv_smem + stage * kTileBytes;
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t off = (k >> 2) * kSlabBytes + (k & 3) * 32;
-        mma_ss(tmem + t * 128, operand(a + off, 16), operand(b + off, 16), qk, k > 0);
-      }
-      tc_commit(&S.s_full[t]);
-    };
+    if (!wait_warp(&S.q_full, n & 1)) return false;
     bool started[2] = {false, false};
+    bool now[2] = {false, false};   // row tile t uses key tile i
     for (int i = -1; i < keys.count; ++i) {
       // products with V of tile i and scores of tile i + 1, row tile by row tile
       Ring v_ring = ring, k_ring = ring;
       if (i >= 0) k_ring.step();
+      const int tile = i >= 0 ? tile_of(keys, i) : 0, then = tile_of(keys, i + 1);
+      const bool more = i + 1 < keys.count, look = i >= 0 && (tiles[0].partly(tile) || tiles[1].partly(tile));
+      const bool next[2] = {more && tiles[0].uses(then), more && tiles[1].uses(then)};
       bool v_here = false, k_here = false;
+#pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (i >= 0 && uses(P, it, q0 + t * kRows, tile_of(keys, i))) {
+        if (now[t]) {
           if (!v_here) {
-            if (!wait(&S.kv_full[v_ring.stage], v_ring.round & 1)) return false;
-            if (needs_clean(P, it, tile_of(keys, i))) {
-              if (!wait(&S.cleaned[clean % kClean], clean / kClean & 1)) return false;
+            if (!wait_warp(&S.kv_full[v_ring.stage], v_ring.round & 1)) return false;
+            if (look) {
+              if (!wait_warp(&S.cleaned[clean % kClean], clean / kClean & 1)) return false;
               ++clean;
             }
             v_here = true;
           }
-          if (!wait(&S.p_full[t], p_count[t]++ & 1)) return false;
-          tc_fence_after();
-          const uint32_t b = kv_smem + v_ring.stage * kTileBytes;
-          for (int k = 0; k < 8; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, operand(b + k * 2048, kSlabBytes), pv, started[t] || k > 0);
+          const uint64_t b = v_op + v_ring.stage * (kTileBytes >> 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {   // the weights come in two halves
+            if (!wait_warp(&S.p_full[t][h], p_count[t] & 1)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = h * 4; k < h * 4 + 4; ++k)
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, started[t] || k > 0);
+              if (h == 1 && i == last[t]) tc_commit(&S.o_full[t]);
+            }
+            __syncwarp();
+          }
+          ++p_count[t];
           started[t] = true;
-          if (i == last[t]) tc_commit(&S.o_full[t]);
         }
-        if (i + 1 < keys.count && uses(P, it, q0 + t * kRows, tile_of(keys, i + 1))) {
+        if (next[t]) {
           if (!k_here) {
-            if (!wait(&S.kv_full[k_ring.stage], k_ring.round & 1)) return false;
+            if (!wait_warp(&S.kv_full[k_ring.stage], k_ring.round & 1)) return false;
             k_here = true;
           }
           tc_fence_after();
-          scores(t, k_ring.stage);
+          const uint64_t a = q_op + t * (kTileBytes >> 4), b = k_op + k_ring.stage * (kTileBytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = ((k >> 2) * kSlabBytes + (k & 3) * 32) >> 4;
+              mma_ss(tmem + t * 128, a + off, b + off, qk, k > 0);
+            }
+            tc_commit(&S.s_full[t]);
+          }
+          __syncwarp();
         }
+        now[t] = next[t];
       }
-      if (i >= 0) tc_commit(&S.kv_empty[v_ring.stage]);
-      if (i + 1 < keys.count) tc_commit(&S.kv_empty[k_ring.stage]);
-      if (i + 2 == keys.count) tc_commit(&S.q_empty);
+      if (elect_one()) {
+        if (i >= 0) tc_commit(&S.kv_empty[v_ring.stage]);
+        if (more) tc_commit(&S.kv_empty[k_ring.stage]);
+        if (i + 2 == keys.count) tc_commit(&S.q_empty);
+      }
+      __syncwarp();
       ring = k_ring;
       ring.step();
     }
     // (the last step moved past a K tile that does not exist)
     ring.stage = ring.stage == 0 ? (--ring.round, kKvStages - 1) : ring.stage - 1;
-    items.release(S);
+    items.release_warp(S);
   }
 }
 
@@ -354,9 +393,10 @@ template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, 
   Ring ring;
   int clean = 0;
   for (;;) {
-    if (!items.next<true>(S, it)) return false;
+    if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
+    const Tiles upper = tiles_of(P, it, it.pair * kPairRows), lower = tiles_of(P, it, it.pair * kPairRows + kRows);
     for (int i = 0; i < keys.count; ++i) {
       // every buffer is waited for and passed on, so that none is filled twice in between
       if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
@@ -364,7 +404,7 @@ template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, 
       ring.step();
       if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
       const int t = tile_of(keys, i);
-      if (needs_clean(P, it, t)) {
+      if (upper.partly(t) || lower.partly(t)) {
         uint4* tile = reinterpret_cast<uint4*>(kv + ring.stage * kTileBytes);
         uint32_t top = 0;
 #pragma unroll 8
@@ -393,13 +433,146 @@ template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, 
       if (lane == 0) mbar_arrive(&S.kv_empty[ring.stage]);
       ring.step();
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&S.item_empty[items.slot]);
-    if (++items.slot == kItems) { items.slot = 0; ++items.round; }
+    items.release_warp(S);
   }
 }
 
-template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params& P, Shared& S, uint32_t tmem, int t) {
+// ---- arithmetic on pairs ----------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the largest of three, a NaN if there is one
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of a pair on the multiply-add units: the nearest integer leaves by an addition of 1.5 * 2^23, 2^f on [-1/2, 1/2] is a
+// polynomial fitted here for the least largest relative error (7.5e-5 at degree 3, against a bf16 weight's half step of 2e-3;
+// 2.6e-6 at degree 4, against fp16's 2.4e-4), the integer goes to the exponent.  x below -126 counts as -126.
+template <int DT> __device__ __forceinline__ void exp2_pair(float& a, float& b) {
+  const uint64_t x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t magic = pair(12582912.0f, 12582912.0f), back = pair(-12582912.0f, -12582912.0f), minus = pair(-1.0f, -1.0f);
+  const uint64_t y = add2(x, magic), f = fma2(add2(y, back), minus, x);
+  uint64_t p;
+  if (DT == JF_DTYPE_BF16) {
+    p = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.242611125f, 0.242611125f));
+    p = fma2(p, f, pair(0.693260968f, 0.693260968f));
+    p = fma2(p, f, pair(0.999928057f, 0.999928057f));
+  } else {
+    p = fma2(f, pair(0.0095701021f, 0.0095701021f), pair(0.0559178591f, 0.0559178591f));
+    p = fma2(p, f, pair(0.240247443f, 0.240247443f));
+    p = fma2(p, f, pair(0.693121791f, 0.693121791f));
+    p = fma2(p, f, pair(0.999999285f, 0.999999285f));
+  }
+  float ya, yb, pa, pb;
+  split(y, ya, yb);
+  split(p, pa, pb);
+  a = __uint_as_float((__float_as_uint(ya) << 23) + __float_as_uint(pa));
+  b = __uint_as_float((__float_as_uint(yb) << 23) + __float_as_uint(pb));
+}
+
+// 128 scores -> softened and biased ones, in units of log2.  `lin`: 1 if every key of the tile stands before every row, -1 if
+// behind, 0 if neither.
+template <bool CAP> __device__ __forceinline__ void reshape(float* s, const Params& P, float slope2, int apart, int lin) {
+  const float sl2 = P.scale * kLog2e;
+  if (CAP) {
+    const float in = P.scale / P.softcap, cap2 = P.softcap * kLog2e;
+    float most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 128; ++c) most = fmaxf(most, fabsf(s[c]));
+    if (__all_sync(0xFFFFFFFFu, most * fabsf(in) <= 1.0f)) {
+      // tanh z = z (1 + w q(w)), w = z^2 <= 1, q fitted here for the least relative error of the whole: 6.6e-7
+      const uint64_t in2 = pair(in, in), c2 = pair(cap2, cap2);
+#pragma unroll
+      for (int c = 0; c < 128; c += 2) {
+        const uint64_t z = mul2(pair(s[c], s[c + 1]), in2), w = mul2(z, z);
+        uint64_t q = fma2(w, pair(-0.00312657771f, -0.00312657771f), pair(0.0169064086f, 0.0169064086f));
+        q = fma2(q, w, pair(-0.0517682843f, -0.0517682843f));
+        q = fma2(q, w, pair(0.132884905f, 0.132884905f));
+        q = fma2(q, w, pair(-0.333302796f, -0.333302796f));
+        q = fma2(q, w, pair(1.0f, 1.0f));
+        split(mul2(mul2(z, c2), q), s[c], s[c + 1]);
+      }
+    } else {   // cap tanh z = cap - 2 cap / (e^(2z) + 1)
+      const float to_e = 2.0f * in * kLog2e;
+#pragma unroll
+      for (int c = 0; c < 128; ++c) s[c] = cap2 - __fdividef(2.0f * cap2, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f);
+    }
+  }
+  const float mul = CAP ? 1.0f : sl2;
+  if (lin != 0) {
+    // -slope |i - j| = lin * slope * (j - i): a small integer, exact, times the slope
+    const float k = lin * slope2, a = static_cast<float>(-apart);
+    const uint64_t k2 = pair(k, k), a2 = pair(a, a), m2 = pair(mul, mul);
+#pragma unroll
+    for (int c = 0; c < 128; c += 2) {
+      const uint64_t x = pair(s[c], s[c + 1]);
+      split(fma2(add2(a2, pair(static_cast<float>(c), static_cast<float>(c + 1))), k2, CAP ? x : mul2(x, m2)), s[c], s[c + 1]);
+    }
+  } else {
+    const float a = static_cast<float>(apart);
+#pragma unroll
+    for (int c = 0; c < 128; ++c) s[c] = fmaf(fabsf(a - static_cast<float>(c)), -slope2, CAP ? s[c] : s[c] * mul);
+  }
+}
+
+// Weights of 64 scores, 16 bits each, and their sum.  Of every eight, 2 * POLY are worked out on the multiply-add units: the
+// special function unit takes 8 cycles for a warp's 32 and would bound the kernel alone.
+template <int DT, bool SCALED, int POLY> __device__ __forceinline__ void weigh(float* s, uint32_t* p, uint64_t* sum, float sl2, float ref) {
+  const uint64_t m2 = pair(sl2, sl2), r2 = pair(-ref, -ref);
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    float a, b;
+    split(SCALED ? add2(pair(s[c], s[c + 1]), r2) : fma2(pair(s[c], s[c + 1]), m2, r2), a, b);
+    if ((c & 7) / 2 >= 4 - POLY) {
+      exp2_pair<DT>(a, b);
+    } else {
+      a = ex2(a);
+      b = ex2(b);
+    }
+    sum[c / 2 & 1] = add2(sum[c / 2 & 1], pair(a, b));
+    if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
+  }
+}
+
+// Adds to a row of the result what the cleaned tiles' infinities and NaN do to it.
+template <int DT> __device__ __noinline__ void give_back(const Params& P, const Item it, int row, uint16_t* out) {
+  const Keys keys = keys_of(P, it);
+  const Tiles upper = tiles_of(P, it, it.pair * kPairRows), lower = tiles_of(P, it, it.pair * kPairRows + kRows);
+  for (int i = 0; i < keys.count; ++i) {
+    const int tile = tile_of(keys, i);
+    if (!upper.partly(tile) && !lower.partly(tile)) continue;
+    for (int j = tile * kKeys; j < min((tile + 1) * kKeys, it.len); ++j) {
+      if (!sees(P, it, row, j)) continue;
+      const uint16_t* v = P.v + (static_cast<int64_t>(it.row0) + j) * P.v_stride_t + it.head / (P.H_q / P.H_kv) * P.v_stride_h;
+      for (int k = 0; k < JF_HEAD_DIM; ++k)
+        if (no_number<DT>(v[k])) out[k] = Elem<DT>::from_f32(Elem<DT>::to_f32(out[k]) + Elem<DT>::to_f32(v[k]));
+    }
+  }
+}
+
+// FEAT: 0 plain, 1 bias (and scores that are scaled before their maximum is taken), 2 cap, with or without bias
+template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params& P, Shared& S, uint32_t tmem, int t) {
   constexpr float kLift = DT == JF_DTYPE_FP16 ? 7.0f : 0.0f;   // fp16 weights use the range up to 2^15
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, r = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
@@ -409,16 +582,18 @@ template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params
   Item it;
   int s_count = 0, o_count = 0;
   for (;;) {
-    if (!items.next<true>(S, it)) return false;
+    if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
     const int q0 = it.pair * kPairRows + t * kRows, row = q0 + r;
-    const float slope = FEAT && P.slopes ? P.slopes[it.head] : 0.0f;
+    const Tiles tiles = tiles_of(P, it, q0);
+    const float slope2 = FEAT && P.slopes ? P.slopes[it.head] * kLog2e : 0.0f;
     float m = -INFINITY, l = 0.0f;
     bool have = false;
     for (int i = 0; i < keys.count; ++i) {
       const int tile = tile_of(keys, i), k0 = tile * kKeys;
-      if (!uses(P, it, q0, tile)) continue;
+      if (!tiles.uses(tile)) continue;
+      const bool masked = tiles.masked(tile);
       if (!wait_warp(&S.s_full[t], s_count++ & 1)) return false;
       tc_fence_after();
       uint32_t u[128];
@@ -426,20 +601,8 @@ template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, u + c * 32);
       tc_wait_ld();
-      if (FEAT) {
-        const float cap = P.softcap, to_e = cap > 0.0f ? 2.0f * sl2 / cap : 0.0f;
-#pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          float x;
-          if (cap > 0.0f) {   // cap * tanh(x / cap) = cap - 2 cap / (e^(2x / cap) + 1)
-            x = (cap - __fdividef(2.0f * cap, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f)) * kLog2e;
-          } else {
-            x = s[c] * sl2;
-          }
-          s[c] = x - slope * kLog2e * fabsf(static_cast<float>(row - k0 - c));
-        }
-      }
-      if (masked(P, it, q0, tile)) {
+      if (FEAT) reshape<FEAT == 2>(s, P, slope2, row - k0, k0 + kKeys <= q0 + 1 ? 1 : k0 >= q0 + kRows - 1 ? -1 : 0);
+      if (masked) {
         const int a = first_key(P, row) - k0, b = min(end_key(P, it, row), it.len) - k0, p = it.prefix - k0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -450,8 +613,13 @@ template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params
       }
       float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < 128; ++c) top4[c & 3] = fmaxf(top4[c & 3], s[c]);
-      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * (FEAT ? 1.0f : sl2);
+      for (int c = 4; c < 124; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[c + k], s[c + 4 + k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[124 + k], s[124 + k]);
+      const float top = max3(max3(top4[0], top4[1], top4[2]), top4[3], top4[3]) * (FEAT ? 1.0f : sl2);
+      if (top != top) l = top;   // a NaN among the scores is all that is left of the row
       if (__any_sync(0xFFFFFFFFu, top > m + kLag)) {
         const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
         m = to;
@@ -470,52 +638,34 @@ template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params
       }
       have = true;
       const float ref = m == -INFINITY ? 0.0f : m - kLift;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int c = 0; c < 128; ++c) {
-        s[c] = ex2(FEAT ? s[c] - ref : fmaf(s[c], sl2, -ref));
-        sum[c & 3] += s[c];
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t p[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[c]) : "f"(s[h * 64 + 2 * c + 1]), "f"(s[h * 64 + 2 * c]));
-          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c]) : "f"(s[h * 64 + 2 * c + 1]), "f"(s[h * 64 + 2 * c]));
-        }
+        // (masked entries have to become zeros exactly)
+        if (masked) weigh<DT, FEAT != 0, 0>(s + h * 64, p, sum, sl2, ref);
+        else weigh<DT, FEAT != 0, kPoly>(s + h * 64, p, sum, sl2, ref);
         tmem_st32(s_at + h * 32, p);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[t][h]);
       }
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.p_full[t]);
+      float a, b, c, d;
+      split(sum[0], a, b);
+      split(sum[1], c, d);
+      l += (a + b) + (c + d);
     }
     if (have) {
       if (!wait_warp(&S.o_full[t], o_count++ & 1)) return false;
       tc_fence_after();
       const int64_t at = (static_cast<int64_t>(it.row0) + row) * P.H_q + it.head;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      const bool bad = S.bad[items.slot] != 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         tmem_ld32(o_at + c * 32, o);
         tc_wait_ld();
-        if (bad && row < it.len) {
-          for (int i = 0; i < keys.count; ++i) {
-            const int tile = tile_of(keys, i);
-            if (!needs_clean(P, it, tile)) continue;
-            for (int j = tile * kKeys; j < min((tile + 1) * kKeys, it.len); ++j) {
-              if (!sees(P, it, row, j)) continue;
-              const uint16_t* v = P.v + (static_cast<int64_t>(it.row0) + j) * P.v_stride_t + it.head / (P.H_q / P.H_kv) * P.v_stride_h + c * 32;
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (no_number<DT>(v[k])) o[k] = __float_as_uint(__uint_as_float(o[k]) + Elem<DT>::to_f32(v[k]));
-            }
-          }
-        }
         if (row < it.len) {
           uint4* out = reinterpret_cast<uint4*>(P.out + at * JF_HEAD_DIM + c * 32);
 #pragma unroll
@@ -529,30 +679,31 @@ template <int DT, bool FEAT> __device__ __forceinline__ bool soften(const Params
             out[k] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        __syncwarp();
       }
       tc_fence_before();
+      if (S.bad[items.slot] && row < it.len) give_back<DT>(P, it, row, P.out + at * JF_HEAD_DIM);
+      __syncwarp();
       if (row < it.len && P.lse) P.lse[at] = l > 0.0f || l != l ? (m - kLift + __log2f(l)) * kLn2 : -INFINITY;
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&S.item_empty[items.slot]);
-    if (++items.slot == kItems) { items.slot = 0; ++items.round; }
+    items.release_warp(S);
   }
 }
 
-template <int DT, bool FEAT>
+template <int DT, int FEAT>
 __global__ void __launch_bounds__(kThreads, 1)
-varlen_attn_kernel(const Params P, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+varlen_attn_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                    const __grid_constant__ CUtensorMap vm) {
   extern __shared__ unsigned char raw[];
   __shared__ Shared S;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // (known to be the same for all lanes)
   unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t q_smem = smem_u32(smem), kv_smem = q_smem + 2 * kTileBytes;
   if (threadIdx.x == 0) {
     mbar_init(&S.q_full, 1);
     mbar_init(&S.q_empty, 1);
     for (int i = 0; i < kKvStages; ++i) { mbar_init(&S.kv_full[i], 1); mbar_init(&S.kv_empty[i], 2); }   // empty: products done, looked over
-    for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t], 4); mbar_init(&S.o_full[t], 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t][0], 4); mbar_init(&S.p_full[t][1], 4); mbar_init(&S.o_full[t], 1); }
     for (int i = 0; i < kItems; ++i) { mbar_init(&S.item_full[i], 1); mbar_init(&S.item_empty[i], 11); }   // 8 + loads, products, cleaning
     for (int i = 0; i < kClean; ++i) mbar_init(&S.cleaned[i], 1);
     fence_barrier_init();
@@ -572,9 +723,9 @@ varlen_attn_kernel(const Params P, const __grid_constant__ CUtensorMap qm, const
   if (warp >= 8) {
     regs_dec<kRoleRegs>();
     if (warp == 8) {
-      if (lane == 0) ok = load(P, S, q_smem, kv_smem, &qm, &km, &vm);
+      ok = load(P, S, q_smem, kv_smem, &qm, &km, &vm);
     } else if (warp == 9) {
-      if (lane == 0) ok = multiply<DT>(P, S, q_smem, kv_smem, tmem);
+      ok = multiply<DT>(P, S, q_smem, kv_smem, tmem);
     } else if (warp == 10) {
       ok = schedule(P, S);
     } else {
@@ -624,7 +775,7 @@ jf_status_t rows_map(const void* base, int dtype, int64_t T, int32_t H, int64_t 
   return JF_OK;
 }
 
-template <int DT, bool FEAT>
+template <int DT, int FEAT>
 jf_status_t launch(const Params& P, int grid, cudaStream_t s, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
   auto* kernel = varlen_attn_kernel<DT, FEAT>;
   static const int regs = [] {
@@ -680,8 +831,12 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   P.causal = a->causal != 0;
   const int64_t most = (a->T / kPairRows + std::min<int64_t>(a->n_seqs, a->T)) * a->H_q;   // work items
   const int grid = static_cast<int>(std::min<int64_t>(num_sms(), most));
-  const bool feat = a->softcap > 0.0f || a->alibi_slopes || !(a->attn_scale > 0.0f);   // (the plain form takes the maximum before it scales)
+  // (the plain form takes the maximum before it scales, so it needs a positive scale)
+  const int feat = a->softcap > 0.0f ? 2 : a->alibi_slopes || !(a->attn_scale > 0.0f) ? 1 : 0;
   const auto s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == JF_DTYPE_BF16) return feat ? launch<JF_DTYPE_BF16, true>(P, grid, s, q, k, v) : launch<JF_DTYPE_BF16, false>(P, grid, s, q, k, v);
-  return feat ? launch<JF_DTYPE_FP16, true>(P, grid, s, q, k, v) : launch<JF_DTYPE_FP16, false>(P, grid, s, q, k, v);
+  if (a->dtype == JF_DTYPE_BF16)
+    return feat == 0 ? launch<JF_DTYPE_BF16, 0>(P, grid, s, q, k, v) : feat == 1 ? launch<JF_DTYPE_BF16, 1>(P, grid, s, q, k, v)
+                                                                            : launch<JF_DTYPE_BF16, 2>(P, grid, s, q, k, v);
+  return feat == 0 ? launch<JF_DTYPE_FP16, 0>(P, grid, s, q, k, v) : feat == 1 ? launch<JF_DTYPE_FP16, 1>(P, grid, s, q, k, v)
+                                                                          : launch<JF_DTYPE_FP16, 2>(P, grid, s, q, k, v);
 }
