@@ -24,6 +24,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "decode_common.cuh"
 
@@ -42,7 +43,6 @@ constexpr int kThreads = 384;
 // block is launched with (launch() checks that of the compiled kernel).
 constexpr int kRowRegs = 208, kRoleRegs = 80;
 constexpr float kLag = 8.0f;                          // log2
-constexpr int kPoly = 1;                              // of four pairs of exponentials, on the multiply-add units
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -62,7 +62,7 @@ struct Params {
 struct Item { int row0, len, pair, head, prefix; };   // row0: first row of the sequence; len < 0: no more items
 
 struct Shared {
-  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], o_full[2], item_full[kItems], item_empty[kItems],
+  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], half_done[2], o_full[2], item_full[kItems], item_empty[kItems],
       cleaned[kClean];
   Item item[kItems];
   int bad[kItems];       // V tiles of the item held values that are no numbers
@@ -344,7 +344,8 @@ template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shar
 #pragma unroll
               for (int k = h * 4; k < h * 4 + 4; ++k)
                 mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, started[t] || k > 0);
-              if (h == 1 && i == last[t]) tc_commit(&S.o_full[t]);
+              if (h == 0) tc_commit(&S.half_done[t]);
+              else if (i == last[t]) tc_commit(&S.o_full[t]);
             }
             __syncwarp();
           }
@@ -465,45 +466,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x of a pair on the multiply-add units: the nearest integer leaves by an addition of 1.5 * 2^23, 2^f on [-1/2, 1/2] is a
-// polynomial fitted here for the least largest relative error (7.5e-5 at degree 3, against a bf16 weight's half step of 2e-3;
-// 2.6e-6 at degree 4, against fp16's 2.4e-4), the integer goes to the exponent.  x below -126 counts as -126.
-template <int DT> __device__ __forceinline__ void exp2_pair(float& a, float& b) {
-  const uint64_t x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t magic = pair(12582912.0f, 12582912.0f), back = pair(-12582912.0f, -12582912.0f), minus = pair(-1.0f, -1.0f);
-  const uint64_t y = add2(x, magic), f = fma2(add2(y, back), minus, x);
-  uint64_t p;
-  if (DT == JF_DTYPE_BF16) {
-    p = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.242611125f, 0.242611125f));
-    p = fma2(p, f, pair(0.693260968f, 0.693260968f));
-    p = fma2(p, f, pair(0.999928057f, 0.999928057f));
-  } else {
-    p = fma2(f, pair(0.0095701021f, 0.0095701021f), pair(0.0559178591f, 0.0559178591f));
-    p = fma2(p, f, pair(0.240247443f, 0.240247443f));
-    p = fma2(p, f, pair(0.693121791f, 0.693121791f));
-    p = fma2(p, f, pair(0.999999285f, 0.999999285f));
-  }
-  float ya, yb, pa, pb;
-  split(y, ya, yb);
-  split(p, pa, pb);
-  a = __uint_as_float((__float_as_uint(ya) << 23) + __float_as_uint(pa));
-  b = __uint_as_float((__float_as_uint(yb) << 23) + __float_as_uint(pb));
-}
-
-// 128 scores -> softened and biased ones, in units of log2.  `lin`: 1 if every key of the tile stands before every row, -1 if
-// behind, 0 if neither.
+// 64 scores -> softened and biased ones, in units of log2.  `apart`: the row's position minus the first key's; `lin`: 1 if
+// every key stands before every row of the tile, -1 if behind, 0 if neither.
 template <bool CAP> __device__ __forceinline__ void reshape(float* s, const Params& P, float slope2, int apart, int lin) {
   const float sl2 = P.scale * kLog2e;
   if (CAP) {
     const float in = P.scale / P.softcap, cap2 = P.softcap * kLog2e;
     float most = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 128; ++c) most = fmaxf(most, fabsf(s[c]));
+    for (int c = 0; c < 64; ++c) most = fmaxf(most, fabsf(s[c]));
     if (__all_sync(0xFFFFFFFFu, most * fabsf(in) <= 1.0f)) {
       // tanh z = z (1 + w q(w)), w = z^2 <= 1, q fitted here for the least relative error of the whole: 6.6e-7
       const uint64_t in2 = pair(in, in), c2 = pair(cap2, cap2);
 #pragma unroll
-      for (int c = 0; c < 128; c += 2) {
+      for (int c = 0; c < 64; c += 2) {
         const uint64_t z = mul2(pair(s[c], s[c + 1]), in2), w = mul2(z, z);
         uint64_t q = fma2(w, pair(-0.00312657771f, -0.00312657771f), pair(0.0169064086f, 0.0169064086f));
         q = fma2(q, w, pair(-0.0517682843f, -0.0517682843f));
@@ -515,46 +491,67 @@ template <bool CAP> __device__ __forceinline__ void reshape(float* s, const Para
     } else {   // cap tanh z = cap - 2 cap / (e^(2z) + 1)
       const float to_e = 2.0f * in * kLog2e;
 #pragma unroll
-      for (int c = 0; c < 128; ++c) s[c] = cap2 - __fdividef(2.0f * cap2, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f);
+      for (int c = 0; c < 64; ++c) s[c] = cap2 - __fdividef(2.0f * cap2, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f);
     }
   }
   const float mul = CAP ? 1.0f : sl2;
   if (lin != 0) {
-    // -slope |i - j| = lin * slope * (j - i): a small integer, exact, times the slope
-    const float k = lin * slope2, a = static_cast<float>(-apart);
+    // -slope |i - j| = lin * slope * (j - i) = k c - k apart for the tile's c-th key; what its two roundings lose is 2^-23 of
+    // the bias itself
+    const float k = lin * slope2, a = -k * static_cast<float>(apart);
     const uint64_t k2 = pair(k, k), a2 = pair(a, a), m2 = pair(mul, mul);
 #pragma unroll
-    for (int c = 0; c < 128; c += 2) {
-      const uint64_t x = pair(s[c], s[c + 1]);
-      split(fma2(add2(a2, pair(static_cast<float>(c), static_cast<float>(c + 1))), k2, CAP ? x : mul2(x, m2)), s[c], s[c + 1]);
+    for (int c = 0; c < 64; c += 2) {
+      const uint64_t x = pair(s[c], s[c + 1]), bias = fma2(pair(static_cast<float>(c), static_cast<float>(c + 1)), k2, a2);
+      split(CAP ? add2(x, bias) : fma2(x, m2, bias), s[c], s[c + 1]);
     }
   } else {
     const float a = static_cast<float>(apart);
 #pragma unroll
-    for (int c = 0; c < 128; ++c) s[c] = fmaf(fabsf(a - static_cast<float>(c)), -slope2, CAP ? s[c] : s[c] * mul);
+    for (int c = 0; c < 64; ++c) s[c] = fmaf(fabsf(a - static_cast<float>(c)), -slope2, CAP ? s[c] : s[c] * mul);
   }
 }
 
-// Weights of 64 scores, 16 bits each, and their sum.  Of every eight, 2 * POLY are worked out on the multiply-add units: the
-// special function unit takes 8 cycles for a warp's 32 and would bound the kernel alone.
-template <int DT, bool SCALED, int POLY> __device__ __forceinline__ void weigh(float* s, uint32_t* p, uint64_t* sum, float sl2, float ref) {
+// Weights of 64 scores, 16 bits each, and their sum (added to `sum`).  A polynomial on the multiply-add units for a
+// quarter of the exponentials gained nothing here (8192 tokens 949 -> 977 us).
+template <int DT, bool SCALED> __device__ __forceinline__ void weigh(const float* s, uint32_t* p, uint64_t* sum, float sl2, float ref) {
   const uint64_t m2 = pair(sl2, sl2), r2 = pair(-ref, -ref);
 #pragma unroll
   for (int c = 0; c < 64; c += 2) {
     float a, b;
     split(SCALED ? add2(pair(s[c], s[c + 1]), r2) : fma2(pair(s[c], s[c + 1]), m2, r2), a, b);
-    if ((c & 7) / 2 >= 4 - POLY) {
-      exp2_pair<DT>(a, b);
-    } else {
-      a = ex2(a);
-      b = ex2(b);
-    }
+    a = ex2(a);
+    b = ex2(b);
     sum[c / 2 & 1] = add2(sum[c / 2 & 1], pair(a, b));
     if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
   }
 }
 
+// Largest of N scores; a NaN if there is one.
+template <int N> __device__ __forceinline__ float largest(const float* s) {
+  float x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = s[k];
+#pragma unroll
+  for (int c = 4; c < N - 4; c += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = max3(x[k], s[c + k], s[c + 4 + k]);
+  return max3(max3(x[0], x[1], s[N - 4]), max3(x[2], x[3], s[N - 3]), max3(s[N - 2], s[N - 1], s[N - 1]));
+}
+
+// A row's output so far goes to another reference.
+__device__ __forceinline__ void rescale(uint32_t o_at, float f) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t o[32];
+    tmem_ld32(o_at + c * 32, o);
+    tc_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+    tmem_st32(o_at + c * 32, o);
+  }
+}
 // Adds to a row of the result what the cleaned tiles' infinities and NaN do to it.
 template <int DT> __device__ __noinline__ void give_back(const Params& P, const Item it, int row, uint16_t* out) {
   const Keys keys = keys_of(P, it);
@@ -596,61 +593,63 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
       const bool masked = tiles.masked(tile);
       if (!wait_warp(&S.s_full[t], s_count++ & 1)) return false;
       tc_fence_after();
-      uint32_t u[128];
-      float* s = reinterpret_cast<float*>(u);
+      uint64_t sum[2] = {0, 0};
+      // KEYS keys of the tile from key `from` on, a step of the online softmax: maximum, reference, weights
+      auto step = [&](auto keys_tag, int from) {
+        constexpr int N = decltype(keys_tag)::value;
+        uint32_t u[N], p[32];
+        float* s = reinterpret_cast<float*>(u);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, u + c * 32);
-      tc_wait_ld();
-      if (FEAT) reshape<FEAT == 2>(s, P, slope2, row - k0, k0 + kKeys <= q0 + 1 ? 1 : k0 >= q0 + kRows - 1 ? -1 : 0);
-      if (masked) {
-        const int a = first_key(P, row) - k0, b = min(end_key(P, it, row), it.len) - k0, p = it.prefix - k0;
+        for (int c = 0; c < N; c += 32) tmem_ld32(s_at + from + c, u + c);
+        tc_wait_ld();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t bits = (below(b - 32 * w) & ~below(a - 32 * w)) | below(p - 32 * w);
+        for (int c = 0; c < N; c += 64) {
+          const int k1 = k0 + from + c;
+          if (FEAT) reshape<FEAT == 2>(s + c, P, slope2, row - k1, k0 + kKeys <= q0 + 1 ? 1 : k0 >= q0 + kRows - 1 ? -1 : 0);
+          if (masked) {
+            const int a = first_key(P, row) - k1, b = min(end_key(P, it, row), it.len) - k1, e = it.prefix - k1;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[w * 32 + c] = bits >> c & 1u ? s[w * 32 + c] : -INFINITY;
-        }
-      }
-      float top4[4] = {s[0], s[1], s[2], s[3]};
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t bits = (below(b - 32 * w) & ~below(a - 32 * w)) | below(e - 32 * w);
 #pragma unroll
-      for (int c = 4; c < 124; c += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[c + k], s[c + 4 + k]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[124 + k], s[124 + k]);
-      const float top = max3(max3(top4[0], top4[1], top4[2]), top4[3], top4[3]) * (FEAT ? 1.0f : sl2);
-      if (top != top) l = top;   // a NaN among the scores is all that is left of the row
-      if (__any_sync(0xFFFFFFFFu, top > m + kLag)) {
-        const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
-        m = to;
-        l *= f;
-        if (have) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c * 32, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st32(o_at + c * 32, o);
+              for (int k = 0; k < 32; ++k) s[c + w * 32 + k] = bits >> k & 1u ? s[c + w * 32 + k] : -INFINITY;
+            }
           }
         }
+        const float top = largest<N>(s) * (FEAT ? 1.0f : sl2);
+        if (__any_sync(0xFFFFFFFFu, !(top <= m + kLag))) {
+          // (the output holds this tile's first half only when its product is through)
+          if (from > 0 && !wait_warp(&S.half_done[t], (s_count - 1) & 1)) return false;
+          if (from > 0) tc_fence_after();
+          if (top != top) l = top;   // a NaN among the scores is all that is left of the row
+          const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
+          m = to;
+          l *= f;
+          sum[0] = mul2(sum[0], pair(f, f));
+          sum[1] = mul2(sum[1], pair(f, f));
+          if (have || from > 0) rescale(o_at, f);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m - kLift;
+#pragma unroll
+        for (int c = 0; c < N; c += 64) {
+          weigh<DT, FEAT != 0>(s + c, p, sum, sl2, ref);
+          const int h = from / 64 + c / 64;
+          tmem_st32(s_at + h * 32, p);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.p_full[t][h]);
+        }
+        return true;
+      };
+      if (FEAT == 2) {   // half a tile at a time: what the cap takes of registers and code
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h)
+          if (!step(std::integral_constant<int, 64>(), h * 64)) return false;
+      } else {
+        if (!step(std::integral_constant<int, 128>(), 0)) return false;
       }
       have = true;
-      const float ref = m == -INFINITY ? 0.0f : m - kLift;
-      uint64_t sum[2] = {0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
-        // (masked entries have to become zeros exactly)
-        if (masked) weigh<DT, FEAT != 0, 0>(s + h * 64, p, sum, sl2, ref);
-        else weigh<DT, FEAT != 0, kPoly>(s + h * 64, p, sum, sl2, ref);
-        tmem_st32(s_at + h * 32, p);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.p_full[t][h]);
-      }
       float a, b, c, d;
       split(sum[0], a, b);
       split(sum[1], c, d);
@@ -703,7 +702,7 @@ varlen_attn_kernel(const __grid_constant__ Params P, const __grid_constant__ CUt
     mbar_init(&S.q_full, 1);
     mbar_init(&S.q_empty, 1);
     for (int i = 0; i < kKvStages; ++i) { mbar_init(&S.kv_full[i], 1); mbar_init(&S.kv_empty[i], 2); }   // empty: products done, looked over
-    for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t][0], 4); mbar_init(&S.p_full[t][1], 4); mbar_init(&S.o_full[t], 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t][0], 4); mbar_init(&S.p_full[t][1], 4); mbar_init(&S.half_done[t], 1); mbar_init(&S.o_full[t], 1); }
     for (int i = 0; i < kItems; ++i) { mbar_init(&S.item_full[i], 1); mbar_init(&S.item_empty[i], 11); }   // 8 + loads, products, cleaning
     for (int i = 0; i < kClean; ++i) mbar_init(&S.cleaned[i], 1);
     fence_barrier_init();
