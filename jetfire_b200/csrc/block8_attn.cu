@@ -2,13 +2,14 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(f(attn_scale * q.k_j) + bias_j)
 //
-// Both products run on the tensor cores with fp16 operands that hold the codes exactly (an int8 code is an integer
-// below 2^7; an e4m3 code times 2^-8 is a bit shift of itself); the scales stay outside, in fp32.  q goes to fp16 by a power of two
-// per head that brings its largest element to [2^13, 2^14): what that rounds is 2^-38 of it.  The tile of a product
-// is one block: scores as K (16 positions) x q^T (8 heads of the group, NT times), outputs as V^T (8 x 16 dims) x p^T.
-// Channels and positions are contracted in whatever order the lanes hold them, so each lane takes 16-byte pieces of the
-// rows as they lie in memory and turns them into operands in its own registers: no transposition, and shared memory
-// holds only what the lane itself copied there.
+// Both products run on the tensor cores, the scales stay outside of them, in fp32.  int8 scores are exact integer sums: q of a
+// head is a number of 22 bits below a power of two, cut into three signed bytes, and each meets the codes as they lie
+// in memory (no conversion; what the 22 bits round is 2^-22 of the head's largest element).  e4m3 codes are converted to fp16, which
+// holds them exactly, and meet q as fp16 numbers under a power of two per head that brings its largest element to [2^13,
+// 2^14): what that rounds is 2^-38 of it.  V's codes become fp16 in either case.  The tile of a product is one block: scores as K (16
+// positions) x q^T (8 heads of the group, NT times), outputs as V^T (8 x 16 channels) x p^T.  Channels and positions are
+// contracted in whatever order the lanes hold them, so each lane takes 16-byte pieces of the rows as they lie in memory
+// and turns them into operands in its own registers: no transposition, and shared memory holds only what the lane itself copied there.
 //
 // A warp goes through its blocks with a running reference m for every head, the sum of its weights and the output
 // unnormalised.  The V scale of a block joins the exponent: w = exp2(s + log2(vs) - m) is what meets the codes, in
@@ -109,16 +110,43 @@ __device__ __forceinline__ int64_t block_id(const AttnParams& P, int64_t at) {
   return P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
 }
 
-// Two bytes of a pair of operands as fp16: bytes (a, b) -> code a, code b.  `w` holds four codes, SEL picks two.
+// The lower or upper two of four codes as fp16.  int8: `w` has its sign bits turned over, 0x6400 + u is 1024 + u.
 template <int CODES> __device__ __forceinline__ uint32_t bias(uint32_t w) { return CODES == JF_CODES_INT8 ? w ^ 0x80808080u : w; }
 template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
   uint32_t d;
-  if (CODES == JF_CODES_INT8) {   // 0x6400 + u is 1024 + u
+  if (CODES == JF_CODES_INT8)
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(w, 0x64646464u, HIGH ? 0x4342u : 0x4140u)), "r"(0x64806480u));
-    return d;
+  else if (HIGH)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// cap * tanh(x / cap) of four scores, for the whole warp the same way: up to |x| = cap by a polynomial fitted for the least
+// relative error (6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).
+__device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap) {
+  float most = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[k]));
+  if (__all_sync(0xFFFFFFFFu, most <= cap)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float z = x[k] * inv_cap, w = z * z;
+      float q = fmaf(w, -0.00312657771f, 0.0169064086f);
+      q = fmaf(q, w, -0.0517682843f);
+      q = fmaf(q, w, 0.132884905f);
+      q = fmaf(q, w, -0.333302796f);
+      x[k] = x[k] * fmaf(q, w, 1.0f);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = cap - __fdividef(2.0f * cap, ex2(fminf(x[k] * inv_cap * (2.0f * kLog2e), 126.0f)) + 1.0f);
   }
-  const uint32_t h = prmt(w, 0u, HIGH ? 0x3424u : 0x1404u);
-  return (h & 0x80008000u) | (h >> 1 & 0x3F803F80u);
 }
 
 template <int CODES, int DT, int NT, bool FEAT>
@@ -136,8 +164,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   const Span span = span_of(P, b);
   const int begin = cut.index * cut.piece, end = min(begin + cut.piece, span.count);
 
-  // q of the lane's head (column g of each tile), scaled to fp16
-  uint32_t qf[NT][16];
+  // q of the lane's head (column g of each tile): fp16 pairs, or the three bytes of four elements at a time
+  constexpr bool INT = CODES == JF_CODES_INT8;
+  uint32_t qf[NT][INT ? 24 : 16];
   float sfac[NT][2], slope[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -151,32 +180,53 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
                                                       (static_cast<int64_t>(b) * P.H_q + first_head + head) * JF_HEAD_DIM +
                                                       (i >> 1) * 64 + t * 16 + (i & 1) * 8));
     }
-    float amax = 0.0f;
+    float x[32], amax = 0.0f, odd = 0.0f;   // odd: NaN if an element is no number, else 0
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        amax = fmaxf(amax, fmaxf(fabsf(Elem<DT>::to_f32(static_cast<uint16_t>(w[k]))), fabsf(Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)))));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float y = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16 * e));
+          x[i * 8 + k * 2 + e] = y;
+          amax = fmaxf(amax, fabsf(y));
+          odd = fmaf(y, 0.0f, odd);
+        }
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-    // 2^(13 - exponent of amax); below 2^-113 it stays 2^126, an infinite q keeps its scale
-    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-    if (e == 128) e = 13;
-    e = max(e, -113);
-    const float up = __uint_as_float(static_cast<uint32_t>(13 - e + 127) << 23);   // 13 - e in [-114, 126]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    for (int o = 1; o < 4; o <<= 1) {
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+      odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+    }
+    // a power of two that brings the largest element to [2^TOP, 2^(TOP + 1)); 2^126 at most
+    constexpr int TOP = INT ? 21 : 13;
+    const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127, 127), TOP - 126);
+    const float up = __uint_as_float(static_cast<uint32_t>(TOP - e + 127) << 23);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const __half2 h = __floats2half2_rn(Elem<DT>::to_f32(static_cast<uint16_t>(w[k])) * up, Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)) * up);
-        qf[n][i * 4 + k] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int w = 0; w < 8; ++w) {   // word w of the lane's 32 channels
+      if (INT) {
+        uint32_t lo = 0, mid = 0, hi = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int v = __float2int_rn(x[w * 4 + k] * up), a = static_cast<int8_t>(v), r = (v - a) >> 8, c = static_cast<int8_t>(r);
+          lo |= (static_cast<uint32_t>(a) & 255u) << 8 * k;
+          mid |= (static_cast<uint32_t>(c) & 255u) << 8 * k;
+          hi |= (static_cast<uint32_t>((r - c) >> 8) & 255u) << 8 * k;
+        }
+        qf[n][w] = lo;
+        qf[n][8 + w] = mid;
+        qf[n][16 + w] = hi;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const __half2 h = __floats2half2_rn(x[w * 4 + k * 2] * up, x[w * 4 + k * 2 + 1] * up);
+          qf[n][w * 2 + k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
       }
     }
     // what brings a sum of products back, for the heads of the lane's score columns 2t and 2t + 1
-    const float down = __uint_as_float(static_cast<uint32_t>(e - 13 + 127 + (CODES == JF_CODES_E4M3 ? 8 : 0)) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) + odd;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       sfac[n][c] = __shfl_sync(0xFFFFFFFFu, down, (2 * t + c) * 4) * P.scale * (FEAT ? 1.0f : kLog2e);
@@ -203,12 +253,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     const int at = begin + warp + i * kWarps;
     return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
   };
-  struct Look { int64_t id; float ks, vs; };
+  struct Look { int id; float ks, vs; };
   auto look_up = [&](int i0) {
     Look r{-1, 0.0f, 1.0f};
     if (i0 + lane < mine) {
-      r.id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
-      if (r.id < 0 || r.id >= P.num_blocks) r.id = -1;
+      const int64_t id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
+      r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
       if (r.id >= 0) {
         r.ks = P.k_scales[head_row + r.id];
         r.vs = P.v_scales[head_row + r.id];
@@ -218,12 +268,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     return r;
   };
   unsigned char* ring = smem + warp * kStages * kStageBytes + lane * 16;
-  const uint32_t k_off = g * JF_HEAD_DIM + t * 16, v_off = 2 * t * JF_HEAD_DIM + g * 16;
-  auto fetch = [&](int64_t id, int stage) {
+  const uint8_t* k_base = P.k_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + g * JF_HEAD_DIM + t * 16;
+  const uint8_t* v_base = P.v_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + 2 * t * JF_HEAD_DIM + g * 16;
+  auto fetch = [&](int id, int stage) {
     if (id >= 0) {
       unsigned char* dst = ring + stage * kStageBytes;
-      const uint8_t* k = P.k_data + (head_row + id) * (JF_BLOCK_SIZE * JF_HEAD_DIM) + k_off;
-      const uint8_t* v = P.v_data + (head_row + id) * (JF_BLOCK_SIZE * JF_HEAD_DIM) + v_off;
+      const uint8_t* k = k_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
+      const uint8_t* v = v_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
 #pragma unroll
       for (int i = 0; i < 4; ++i) cp_async_16(dst + i * 512, k + (i & 1) * 8 * JF_HEAD_DIM + (i >> 1) * 64);
 #pragma unroll
@@ -234,6 +285,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   Look look = look_up(0), next = look;
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i < mine ? __shfl_sync(0xFFFFFFFFu, look.id, i) : -1, i);
+  const float inv_cap = FEAT && P.softcap > 0.0f ? 1.0f / P.softcap : 0.0f;
   int stage = 0;
   for (int i = 0; i < mine; ++i) {
     const int i32 = i & 31;
@@ -241,11 +293,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     if (i32 == 0) next = look_up((i & ~31) + 32);
     {
       const int ahead = i + kStages - 1;
-      const int64_t id = __shfl_sync(0xFFFFFFFFu, (ahead & ~31) == (i & ~31) ? look.id : next.id, ahead & 31);
+      const int id = __shfl_sync(0xFFFFFFFFu, (ahead & ~31) == (i & ~31) ? look.id : next.id, ahead & 31);
       fetch(ahead < mine ? id : -1, stage == 0 ? kStages - 1 : stage - 1);
     }
     cp_async_wait_group<kStages - 1>();
-    const int64_t id = __shfl_sync(0xFFFFFFFFu, look.id, i32);
+    const int id = __shfl_sync(0xFFFFFFFFu, look.id, i32);
     const unsigned char* at = ring + stage * kStageBytes;
     stage = stage + 1 == kStages ? 0 : stage + 1;
     if (id < 0) continue;
@@ -253,7 +305,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     const int pos = position_of(i);
 
     float s[NT][4];
-    {
+    if (INT) {
+      int d[NT][3][4] = {};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint4 a = *reinterpret_cast<const uint4*>(at + half * 1024), c = *reinterpret_cast<const uint4*>(at + half * 1024 + 512);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            mma_s8_16832(d[n][k], a.x, c.x, a.y, c.y, qf[n][k * 8 + half * 4], qf[n][k * 8 + half * 4 + 1]);
+            mma_s8_16832(d[n][k], a.z, c.z, a.w, c.w, qf[n][k * 8 + half * 4 + 2], qf[n][k * 8 + half * 4 + 3]);
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // (the upper two together stay below 2^29)
+          s[n][k] = fmaf(static_cast<float>(d[n][2][k] * 256 + d[n][1][k]), 256.0f, static_cast<float>(d[n][0][k])) * (sfac[n][k & 1] * ks);
+    } else {
       float c2[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -265,10 +335,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
         const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, c[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t x = bias<CODES>(a[w]), y = bias<CODES>(c[w]);
-          const uint32_t a0 = widen<CODES, false>(x), a1 = widen<CODES, false>(y), a2 = widen<CODES, true>(x), a3 = widen<CODES, true>(y);
+          const uint32_t a0 = widen<CODES, false>(a[w]), a1 = widen<CODES, false>(c[w]), a2 = widen<CODES, true>(a[w]), a3 = widen<CODES, true>(c[w]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(half ? c2[n] : s[n], a0, a1, a2, a3, qf[n][half * 8 + w * 2], qf[n][half * 8 + w * 2 + 1]);
+          for (int n = 0; n < NT; ++n) mma_f16_16816(half ? c2[n] : s[n], a0, a1, a2, a3, qf[n][(half * 8 + w * 2) % 16], qf[n][(half * 8 + w * 2 + 1) % 16]);
         }
       }
 #pragma unroll
@@ -278,14 +347,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     }
     if (FEAT) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        if (P.softcap > 0.0f) soften4(s[n], P.softcap, inv_cap);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float x = s[n][k];
-          if (P.softcap > 0.0f) x = P.softcap * tanhf(x / P.softcap);
-          x -= slope[n][k & 1] * static_cast<float>(span.len - 1 - (pos + g + (k >> 1) * 8));
-          s[n][k] = x * kLog2e;
-        }
+        for (int k = 0; k < 4; ++k)
+          s[n][k] = (s[n][k] - slope[n][k & 1] * static_cast<float>(span.len - 1 - (pos + g + (k >> 1) * 8))) * kLog2e;
+      }
     }
     const bool whole = pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix);
     if (!whole) {
@@ -348,6 +415,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       for (int i2 = 0; i2 < 4; ++i2) {
         const uint4 x = *reinterpret_cast<const uint4*>(at + 2048 + i2 * 512);
         r[i2][0] = bias<CODES>(x.x); r[i2][1] = bias<CODES>(x.y); r[i2][2] = bias<CODES>(x.z); r[i2][3] = bias<CODES>(x.w);
+        if (CODES == JF_CODES_E4M3 && !whole) {   // a weight of 0 does not make up for a row of NaN codes
+          const int p = pos + 2 * t + (i2 & 1) + (i2 >> 1) * 8;
+          if (p >= span.len || (p < span.lo && p >= span.prefix)) r[i2][0] = r[i2][1] = r[i2][2] = r[i2][3] = 0;
+        }
       }
 #pragma unroll
       for (int w = 0; w < 4; ++w)
@@ -396,7 +467,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
             make_float2(o[n][j][c] * f[c], o[n][j][2 + c] * f[c]);
   }
   __syncthreads();
-  constexpr float kBack = CODES == JF_CODES_E4M3 ? 256.0f : 1.0f;
   for (int i = threadIdx.x; i < heads * JF_HEAD_DIM; i += kWarps * 32) {
     const int head = i / JF_HEAD_DIM, d = i % JF_HEAD_DIM;
     float top = -INFINITY, sum = 0.0f, z = 0.0f;
@@ -407,7 +477,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       sum += so[(w * 8 * NT + head) * JF_HEAD_DIM + d];
       if (sm_m[w][head] != -INFINITY) z = fmaf(sm_l[w][head], ex2(sm_m[w][head] - top), z);
     }
-    sum *= kBack;
     if (cut.n == 1) {
       const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
       static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + d] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : sum / z);
@@ -535,6 +604,7 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;
   if (!a->q || !a->k_data || !a->v_data || !a->k_scales || !a->v_scales || !a->block_table || !a->seq_lens || !a->out) return JF_ERR_ARG;
   if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 2)) return JF_ERR_ARG;
+  if (a->num_blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
   if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE) return JF_ERR_UNSUPPORTED;
   if (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)) return JF_ERR_WORKSPACE;
   AttnParams P{};
