@@ -9,7 +9,7 @@
 // 2^14): what that rounds is 2^-38 of it.  V's codes become fp16 in either case.  The tile of a product is one block: scores as K (16
 // positions) x q^T (8 heads of the group, NT times), outputs as V^T (8 x 16 channels) x p^T.  Channels and positions are
 // contracted in whatever order the lanes hold them, so each lane takes 16-byte pieces of the rows as they lie in memory
-// and turns them into operands in its own registers: no transposition, and shared memory holds only what the lane itself copied there.
+// and turns them into operands in its own registers: no transposition.
 //
 // A warp goes through its blocks with a running reference m for every head, the sum of its weights and the output
 // unnormalised.  The V scale of a block joins the exponent: w = exp2(s + log2(vs) - m) is what meets the codes, in
@@ -69,7 +69,8 @@ __device__ __forceinline__ Span span_of(const AttnParams& P, int b) {
   }
   return s;
 }
-// Blocks per piece, and whose piece `x` is: the first piece of sequence b is the sum of those before.
+// Whose piece `x` is: n pieces of `piece` blocks (the last may be shorter) make up sequence b, the index-th is x.  The first
+// piece of a sequence is the sum of those before it.
 struct Cut { int piece, b, index, n; };
 __device__ __forceinline__ int piece_length(const AttnParams& P, int total) {
   return max(P.min_piece, (total + P.target - 1) / P.target);
@@ -99,6 +100,7 @@ __device__ __forceinline__ Cut find_piece(const AttnParams& P, int x) {
       c.b = b0 + l;
       c.n = __shfl_sync(0xFFFFFFFFu, n, l);
       c.index = x - before - (__shfl_sync(0xFFFFFFFFu, sum, l) - c.n);
+      c.piece = (__shfl_sync(0xFFFFFFFFu, mine, l) + c.n - 1) / c.n;   // as many blocks in each
       return c;
     }
     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -253,63 +255,61 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     const int at = begin + warp + i * kWarps;
     return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
   };
-  struct Look { int id; float ks, vs; };
+  struct Look { int id; float ks, vs; };   // vs: its log2
   auto look_up = [&](int i0) {
-    Look r{-1, 0.0f, 1.0f};
+    Look r{-1, 0.0f, 0.0f};
     if (i0 + lane < mine) {
       const int64_t id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
       r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
       if (r.id >= 0) {
         r.ks = P.k_scales[head_row + r.id];
         r.vs = P.v_scales[head_row + r.id];
-        if (r.vs == 0.0f) r.vs = 0x1p-100f;   // weightless, but its positions count
+        // weightless where 0, but its positions count
+        asm("lg2.approx.f32 %0, %1;" : "=f"(r.vs) : "f"(r.vs == 0.0f ? 0x1p-100f : r.vs));
       }
     }
     return r;
   };
-  unsigned char* ring = smem + warp * kStages * kStageBytes + lane * 16;
-  const uint8_t* k_base = P.k_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + g * JF_HEAD_DIM + t * 16;
-  const uint8_t* v_base = P.v_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + 2 * t * JF_HEAD_DIM + g * 16;
-  auto fetch = [&](int id, int stage) {
-    if (id >= 0) {
-      unsigned char* dst = ring + stage * kStageBytes;
-      const uint8_t* k = k_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
-      const uint8_t* v = v_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
+  // Rings of K and V blocks, kStages each; K runs one block ahead, since the scores of a block are worked out beside the
+  // outputs of the one before it.
+  unsigned char* k_ring = smem + warp * kStages * kStageBytes;
+  unsigned char* v_ring = k_ring + kStages * (kStageBytes / 2);
+  // A copy moves 512 consecutive bytes, four rows (pieces of rows that the lanes need were 130 us where this takes 102:
+  // four sequences of 65536 positions, 8 KV heads, copies alone).  In shared memory the 16-byte chunks of a row change places
+  // so that eight lanes which read together meet no bank twice: K's by the row's parity, V's by its pair.
+  const int row4 = lane >> 3, chunk = lane & 7;
+  const uint8_t* k_base = P.k_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
+  const uint8_t* v_base = P.v_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
+  const int k_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 & 1) << 2) << 4), v_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 >> 1) << 1) << 4);
+  const int k_at = g * JF_HEAD_DIM + ((t ^ (g & 1) << 2) << 4), v_at = 2 * t * JF_HEAD_DIM + ((g ^ t << 1) << 4);
+  auto fetch_k = [&](int id, int slot) {
+    if (id < 0) return;
+    const uint8_t* k = k_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) cp_async_16(dst + i * 512, k + (i & 1) * 8 * JF_HEAD_DIM + (i >> 1) * 64);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cp_async_16(dst + 2048 + i * 512, v + ((i & 1) + (i >> 1) * 8) * JF_HEAD_DIM);
-    }
-    cp_async_commit();
+    for (int i = 0; i < 4; ++i) cp_async_16(k_ring + slot * 2048 + i * 512 + k_to, k + i * 512);
   };
-  Look look = look_up(0), next = look;
+  auto fetch_v = [&](int id, int slot) {
+    if (id < 0) return;
+    const uint8_t* v = v_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i < mine ? __shfl_sync(0xFFFFFFFFu, look.id, i) : -1, i);
+    for (int i = 0; i < 4; ++i) cp_async_16(v_ring + slot * 2048 + i * 512 + (v_to ^ (i & 1) << 6), v + i * 512);
+  };
   const float inv_cap = FEAT && P.softcap > 0.0f ? 1.0f / P.softcap : 0.0f;
-  int stage = 0;
-  for (int i = 0; i < mine; ++i) {
-    const int i32 = i & 31;
-    if (i32 == 0 && i > 0) look = next;
-    if (i32 == 0) next = look_up((i & ~31) + 32);
-    {
-      const int ahead = i + kStages - 1;
-      const int id = __shfl_sync(0xFFFFFFFFu, (ahead & ~31) == (i & ~31) ? look.id : next.id, ahead & 31);
-      fetch(ahead < mine ? id : -1, stage == 0 ? kStages - 1 : stage - 1);
+  auto whole = [&](int pos) { return pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix); };
+  // Scores of the warp's i-th block, in units of log2 and with log2 of its V scale on top; -inf where there is nothing to see.
+  auto score = [&](float (&s)[NT][4], int id, float ks, float lvs, int pos, const unsigned char* at) {
+    if (id < 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[n][k] = -INFINITY;
+      return;
     }
-    cp_async_wait_group<kStages - 1>();
-    const int id = __shfl_sync(0xFFFFFFFFu, look.id, i32);
-    const unsigned char* at = ring + stage * kStageBytes;
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (id < 0) continue;
-    const float ks = __shfl_sync(0xFFFFFFFFu, look.ks, i32), vs = __shfl_sync(0xFFFFFFFFu, look.vs, i32);
-    const int pos = position_of(i);
-
-    float s[NT][4];
     if (INT) {
       int d[NT][3][4] = {};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint4 a = *reinterpret_cast<const uint4*>(at + half * 1024), c = *reinterpret_cast<const uint4*>(at + half * 1024 + 512);
+        const uint4 a = *reinterpret_cast<const uint4*>(at + (k_at ^ half << 6)), c = *reinterpret_cast<const uint4*>(at + (k_at ^ half << 6) + 1024);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
         for (int k = 0; k < 4; ++k) s[n][k] = c2[n][k] = 0.0f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint4 lo = *reinterpret_cast<const uint4*>(at + half * 1024), hi = *reinterpret_cast<const uint4*>(at + half * 1024 + 512);
+        const uint4 lo = *reinterpret_cast<const uint4*>(at + (k_at ^ half << 6)), hi = *reinterpret_cast<const uint4*>(at + (k_at ^ half << 6) + 1024);
         const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, c[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -354,8 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           s[n][k] = (s[n][k] - slope[n][k & 1] * static_cast<float>(span.len - 1 - (pos + g + (k >> 1) * 8))) * kLog2e;
       }
     }
-    const bool whole = pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix);
-    if (!whole) {
+    if (!whole(pos)) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int p = pos + g + k * 8;
@@ -367,15 +366,57 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
         }
       }
     }
-    float lvs;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] += lvs;
+  };
+  Look look = look_up(0), next = look;
+  int base = 0;   // first of the blocks that `look` holds; `next` holds the 32 after them
+  auto id_of = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.id : next.id, j & 31); };
+  auto k_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.ks : next.ks, j & 31); };
+  auto log_v_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.vs : next.vs, j & 31); };
+  // (copies arrive in the order of their groups: K of block j is in group j, V of block j in group j + 1)
+  const int id0 = mine > 0 ? id_of(0) : -1, id1 = mine > 1 ? id_of(1) : -1, id2 = mine > 2 ? id_of(2) : -1;
+  fetch_k(id0, 0);
+  cp_async_commit();
+  fetch_k(id1, 1);
+  fetch_v(id0, 0);
+  cp_async_commit();
+  fetch_k(id2, 2);
+  fetch_v(id1, 1);
+  cp_async_commit();
+  cp_async_wait_group<2>();
+  __syncwarp();
+  float s[NT][4];
+  float lvs = mine > 0 ? log_v_scale(0) : 0.0f;
+  score(s, id0, mine > 0 ? k_scale(0) : 0.0f, lvs, mine > 0 ? position_of(0) : 0, k_ring);
+  int ids[4] = {id0, id1, id2, -1};   // of blocks i .. i + 3
+  int slot = 0;                       // i % kStages
+  for (int i = 0; i < mine; ++i) {
+    if ((i & 31) == 0) {
+      if (i > 0) { look = next; base = i; }
+      next = look_up(i + 32);
+    }
+    __syncwarp();              // the slots that are filled now were read in the step before
+    const int slot1 = slot + 1 == kStages ? 0 : slot + 1, slot2 = slot1 + 1 == kStages ? 0 : slot1 + 1;
+    ids[3] = i + 3 < mine ? id_of(i + 3) : -1;
+    fetch_k(ids[3], slot);     // (K of block i was read in the step before)
+    fetch_v(ids[2], slot2);
+    cp_async_commit();
+    cp_async_wait_group<2>();
+    __syncwarp();
+    const int id = ids[0], pos = position_of(i);
     const float ivs = ex2(-lvs);
+    float ahead[NT][4];
+    const float lvs1 = log_v_scale(i + 1);
+    score(ahead, ids[1], k_scale(i + 1), lvs1, position_of(i + 1), k_ring + slot1 * 2048);
+    const unsigned char* at = v_ring + slot * 2048;
     bool above = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        s[n][k] += lvs;
         above |= s[n][k] > m[n][k & 1] + (kLift + kLag);
       }
     if (__any_sync(0xFFFFFFFFu, above)) {
@@ -409,13 +450,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&a));
       pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&c));
     }
-    {
+    if (id >= 0) {
       uint32_t r[4][4];
 #pragma unroll
       for (int i2 = 0; i2 < 4; ++i2) {
-        const uint4 x = *reinterpret_cast<const uint4*>(at + 2048 + i2 * 512);
+        const uint4 x = *reinterpret_cast<const uint4*>(at + v_at + (i2 & 1) * JF_HEAD_DIM + (i2 >> 1) * 1024);
         r[i2][0] = bias<CODES>(x.x); r[i2][1] = bias<CODES>(x.y); r[i2][2] = bias<CODES>(x.z); r[i2][3] = bias<CODES>(x.w);
-        if (CODES == JF_CODES_E4M3 && !whole) {   // a weight of 0 does not make up for a row of NaN codes
+        if (CODES == JF_CODES_E4M3 && !whole(pos)) {   // a weight of 0 does not make up for a row of NaN codes
           const int p = pos + 2 * t + (i2 & 1) + (i2 >> 1) * 8;
           if (p >= span.len || (p < span.lo && p >= span.prefix)) r[i2][0] = r[i2][1] = r[i2][2] = r[i2][3] = 0;
         }
@@ -430,6 +471,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + hl], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
     }
+    ids[0] = ids[1];
+    ids[1] = ids[2];
+    ids[2] = ids[3];
+    lvs = lvs1;
+    slot = slot1;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] = ahead[n][k];
   }
   cp_async_wait_all();
 
