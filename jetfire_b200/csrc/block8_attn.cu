@@ -56,13 +56,14 @@ struct AttnParams {
 struct Span { int len, prefix, lo, head, first, count; };
 __device__ __forceinline__ Span span_of(const AttnParams& P, int b) {
   Span s;
-  s.len = max(0, min(P.seq_lens[b], min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
+  const int length = P.seq_lens[b], prefix = P.window > 0 && P.prefix_lens ? P.prefix_lens[b] : 0;
+  s.len = max(0, min(length, min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
   const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
   s.prefix = s.lo = s.head = s.first = 0;
   s.count = blocks;
   if (P.window > 0 && P.window < s.len) {
     s.lo = s.len - P.window;
-    s.prefix = P.prefix_lens ? max(0, min(P.prefix_lens[b], s.lo)) : 0;
+    s.prefix = max(0, min(prefix, s.lo));
     s.first = s.lo / JF_BLOCK_SIZE;
     s.head = min((s.prefix + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, s.first);
     s.count = s.head + blocks - s.first;
@@ -155,6 +156,7 @@ template <int CODES, int DT, int NT, bool FEAT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kernel(const __grid_constant__ AttnParams P) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT];
+  __shared__ float2 sm_ml[8 * NT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y / P.groups, grp = blockIdx.y % P.groups;
   const int first_head = kvh * P.G + grp * 8 * NT, heads = min(8 * NT, P.G - grp * 8 * NT);
@@ -165,27 +167,109 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   const int b = cut.b;
   const Span span = span_of(P, b);
   const int begin = cut.index * cut.piece, end = min(begin + cut.piece, span.count);
-
-  // q of the lane's head (column g of each tile): fp16 pairs, or the three bytes of four elements at a time
-  constexpr bool INT = CODES == JF_CODES_INT8;
-  uint32_t qf[NT][INT ? 24 : 16];
-  float sfac[NT][2], slope[NT][2];
+  // q of the lane's head (column g of each tile), and the slopes of the heads of its score columns 2t and 2t + 1
+  uint4 q_raw[NT][4];
+  float slope[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int head = n * 8 + g;
-    uint4 raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (head < heads)
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) +
-                                                      (static_cast<int64_t>(b) * P.H_q + first_head + head) * JF_HEAD_DIM +
-                                                      (i >> 1) * 64 + t * 16 + (i & 1) * 8));
+      q_raw[n][i] = make_uint4(0, 0, 0, 0);
+      if (n * 8 + g < heads)
+        q_raw[n][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) +
+                                                           (static_cast<int64_t>(b) * P.H_q + first_head + n * 8 + g) * JF_HEAD_DIM +
+                                                           (i >> 1) * 64 + t * 16 + (i & 1) * 8));
     }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) slope[n][c] = FEAT && P.slopes && n * 8 + 2 * t + c < heads ? P.slopes[first_head + n * 8 + 2 * t + c] : 0.0f;
+  }
+
+
+  float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[n][i][k] = 0.0f;
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+  }
+
+  // The warp's blocks: begin + warp, + kWarps, ...; 32 of them are looked up at a time, a lane each.
+  const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;
+  const int64_t table_row = static_cast<int64_t>(b) * P.bt_stride, head_row = static_cast<int64_t>(kvh) * P.num_blocks;
+  auto position_of = [&](int i) {   // first position of the warp's i-th block
+    const int at = begin + warp + i * kWarps;
+    return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
+  };
+  struct Look { int id; float ks, vs; };
+  auto look_up = [&](int i0) {
+    Look r{-1, 0.0f, 0.0f};
+    if (i0 + lane < mine) {
+      const int64_t id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
+      r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
+      if (r.id >= 0) {
+        r.ks = P.k_scales[head_row + r.id];
+        r.vs = P.v_scales[head_row + r.id];
+      }
+    }
+    return r;
+  };
+  // Rings of K and V blocks, kStages each; K runs one block ahead, since the scores of a block are worked out beside the
+  // outputs of the one before it.
+  unsigned char* k_ring = smem + warp * kStages * kStageBytes;
+  unsigned char* v_ring = k_ring + kStages * (kStageBytes / 2);
+  // A copy moves 512 consecutive bytes, four rows (pieces of rows that the lanes need were 130 us where this takes 102:
+  // four sequences of 65536 positions, 8 KV heads, copies alone).  In shared memory the 16-byte chunks of a row change places
+  // so that eight lanes which read together meet no bank twice: K's by the row's parity, V's by its pair.
+  const int row4 = lane >> 3, chunk = lane & 7;
+  const uint8_t* k_base = P.k_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
+  const uint8_t* v_base = P.v_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
+  const int k_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 & 1) << 2) << 4), v_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 >> 1) << 1) << 4);
+  const int k_at = g * JF_HEAD_DIM + ((t ^ (g & 1) << 2) << 4), v_at = 2 * t * JF_HEAD_DIM + ((g ^ t << 1) << 4);
+  auto fetch_k = [&](int id, int slot) {
+    if (id < 0) return;
+    const uint8_t* k = k_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async_16(k_ring + slot * 2048 + i * 512 + k_to, k + i * 512);
+  };
+  auto fetch_v = [&](int id, int slot) {
+    if (id < 0) return;
+    const uint8_t* v = v_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async_16(v_ring + slot * 2048 + i * 512 + (v_to ^ (i & 1) << 6), v + i * 512);
+  };
+  Look look = look_up(0), next = look;
+  int base = 0;   // first of the blocks that `look` holds; `next` holds the 32 after them
+  auto id_of = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.id : next.id, j & 31); };
+  auto k_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.ks : next.ks, j & 31); };
+  auto log_v_scale = [&](int j) {   // (0 is taken for 2^-100: weightless, but its positions count)
+    const float vs = __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.vs : next.vs, j & 31);
+    float lg;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(vs == 0.0f ? 0x1p-100f : vs));
+    return lg;
+  };
+  // (copies arrive in the order of their groups: K of block j is in group j, V of block j in group j + 1)
+  const int id0 = mine > 0 ? id_of(0) : -1, id1 = mine > 1 ? id_of(1) : -1, id2 = mine > 2 ? id_of(2) : -1;
+  fetch_k(id0, 0);
+  cp_async_commit();
+  fetch_k(id1, 1);
+  fetch_v(id0, 0);
+  cp_async_commit();
+  fetch_k(id2, 2);
+  fetch_v(id1, 1);
+  cp_async_commit();
+  // q as operands: fp16 pairs, or the three bytes of four elements at a time
+  constexpr bool INT = CODES == JF_CODES_INT8;
+  uint32_t qf[NT][INT ? 24 : 16];
+  float sfac[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     float x[32], amax = 0.0f, odd = 0.0f;   // odd: NaN if an element is no number, else 0
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      const uint32_t w[4] = {q_raw[n][i].x, q_raw[n][i].y, q_raw[n][i].z, q_raw[n][i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -230,70 +314,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     // what brings a sum of products back, for the heads of the lane's score columns 2t and 2t + 1
     const float down = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) + odd;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      sfac[n][c] = __shfl_sync(0xFFFFFFFFu, down, (2 * t + c) * 4) * P.scale * (FEAT ? 1.0f : kLog2e);
-      const int head_c = n * 8 + 2 * t + c;
-      slope[n][c] = FEAT && P.slopes && head_c < heads ? P.slopes[first_head + head_c] : 0.0f;
-    }
+    for (int c = 0; c < 2; ++c) sfac[n][c] = __shfl_sync(0xFFFFFFFFu, down, (2 * t + c) * 4) * P.scale * (FEAT ? 1.0f : kLog2e);
   }
 
-  float o[NT][8][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[n][i][k] = 0.0f;
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.0f;
-  }
-
-  // The warp's blocks: begin + warp, + kWarps, ...; 32 of them are looked up at a time, a lane each.
-  const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;
-  const int64_t table_row = static_cast<int64_t>(b) * P.bt_stride, head_row = static_cast<int64_t>(kvh) * P.num_blocks;
-  auto position_of = [&](int i) {   // first position of the warp's i-th block
-    const int at = begin + warp + i * kWarps;
-    return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
-  };
-  struct Look { int id; float ks, vs; };   // vs: its log2
-  auto look_up = [&](int i0) {
-    Look r{-1, 0.0f, 0.0f};
-    if (i0 + lane < mine) {
-      const int64_t id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
-      r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
-      if (r.id >= 0) {
-        r.ks = P.k_scales[head_row + r.id];
-        r.vs = P.v_scales[head_row + r.id];
-        // weightless where 0, but its positions count
-        asm("lg2.approx.f32 %0, %1;" : "=f"(r.vs) : "f"(r.vs == 0.0f ? 0x1p-100f : r.vs));
-      }
-    }
-    return r;
-  };
-  // Rings of K and V blocks, kStages each; K runs one block ahead, since the scores of a block are worked out beside the
-  // outputs of the one before it.
-  unsigned char* k_ring = smem + warp * kStages * kStageBytes;
-  unsigned char* v_ring = k_ring + kStages * (kStageBytes / 2);
-  // A copy moves 512 consecutive bytes, four rows (pieces of rows that the lanes need were 130 us where this takes 102:
-  // four sequences of 65536 positions, 8 KV heads, copies alone).  In shared memory the 16-byte chunks of a row change places
-  // so that eight lanes which read together meet no bank twice: K's by the row's parity, V's by its pair.
-  const int row4 = lane >> 3, chunk = lane & 7;
-  const uint8_t* k_base = P.k_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
-  const uint8_t* v_base = P.v_data + head_row * (JF_BLOCK_SIZE * JF_HEAD_DIM) + lane * 16;
-  const int k_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 & 1) << 2) << 4), v_to = row4 * JF_HEAD_DIM + ((chunk ^ (row4 >> 1) << 1) << 4);
-  const int k_at = g * JF_HEAD_DIM + ((t ^ (g & 1) << 2) << 4), v_at = 2 * t * JF_HEAD_DIM + ((g ^ t << 1) << 4);
-  auto fetch_k = [&](int id, int slot) {
-    if (id < 0) return;
-    const uint8_t* k = k_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cp_async_16(k_ring + slot * 2048 + i * 512 + k_to, k + i * 512);
-  };
-  auto fetch_v = [&](int id, int slot) {
-    if (id < 0) return;
-    const uint8_t* v = v_base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cp_async_16(v_ring + slot * 2048 + i * 512 + (v_to ^ (i & 1) << 6), v + i * 512);
-  };
   const float inv_cap = FEAT && P.softcap > 0.0f ? 1.0f / P.softcap : 0.0f;
   auto whole = [&](int pos) { return pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix); };
   // Scores of the warp's i-th block, in units of log2 and with log2 of its V scale on top; -inf where there is nothing to see.
@@ -371,21 +394,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[n][k] += lvs;
   };
-  Look look = look_up(0), next = look;
-  int base = 0;   // first of the blocks that `look` holds; `next` holds the 32 after them
-  auto id_of = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.id : next.id, j & 31); };
-  auto k_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.ks : next.ks, j & 31); };
-  auto log_v_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.vs : next.vs, j & 31); };
-  // (copies arrive in the order of their groups: K of block j is in group j, V of block j in group j + 1)
-  const int id0 = mine > 0 ? id_of(0) : -1, id1 = mine > 1 ? id_of(1) : -1, id2 = mine > 2 ? id_of(2) : -1;
-  fetch_k(id0, 0);
-  cp_async_commit();
-  fetch_k(id1, 1);
-  fetch_v(id0, 0);
-  cp_async_commit();
-  fetch_k(id2, 2);
-  fetch_v(id1, 1);
-  cp_async_commit();
   cp_async_wait_group<2>();
   __syncwarp();
   float s[NT][4];
@@ -516,95 +524,124 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
         *reinterpret_cast<float2*>(so + (warp * 8 * NT + n * 8 + 2 * t + c) * JF_HEAD_DIM + 16 * g + 2 * j) =
             make_float2(o[n][j][c] * f[c], o[n][j][2 + c] * f[c]);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * JF_HEAD_DIM; i += kWarps * 32) {
-    const int head = i / JF_HEAD_DIM, d = i % JF_HEAD_DIM;
-    float top = -INFINITY, sum = 0.0f, z = 0.0f;
+  if (threadIdx.x < 8 * NT) {
+    float top = -INFINITY, z = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][head]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][threadIdx.x]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (sm_m[w][threadIdx.x] != -INFINITY) z = fmaf(sm_l[w][threadIdx.x], ex2(sm_m[w][threadIdx.x] - top), z);
+    sm_ml[threadIdx.x] = make_float2(top, z);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (JF_HEAD_DIM / 4); i += kWarps * 32) {
+    const int head = i / (JF_HEAD_DIM / 4), d = i % (JF_HEAD_DIM / 4) * 4;
+    const float2 ml = sm_ml[head];
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      sum += so[(w * 8 * NT + head) * JF_HEAD_DIM + d];
-      if (sm_m[w][head] != -INFINITY) z = fmaf(sm_l[w][head], ex2(sm_m[w][head] - top), z);
+      const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 * NT + head) * JF_HEAD_DIM + d);
+      sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
     }
     if (cut.n == 1) {
       const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
-      static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + d] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : sum / z);
-      if (d == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
+      const bool none = ml.x == -INFINITY;
+      const float r[4] = {sum.x, sum.y, sum.z, sum.w};
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(none ? 0.0f : r[k] / ml.y);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + row * JF_HEAD_DIM + d) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+      if (d == 0 && P.lse) P.lse[row] = none ? -INFINITY : (ml.x + __log2f(ml.y)) / kLog2e;
     } else {
       const int64_t row = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (8 * NT) + head;
-      P.part_o[row * JF_HEAD_DIM + d] = sum;
-      if (d == 0) {
-        P.part_ml[row * 2] = top;
-        P.part_ml[row * 2 + 1] = z;
-      }
+      *reinterpret_cast<float4*>(P.part_o + row * JF_HEAD_DIM + d) = sum;
+      if (d == 0) *reinterpret_cast<float2*>(P.part_ml + row * 2) = ml;
     }
   }
 }
 
-// The pieces of a sequence: one block per (head, sequence), four threads share an output channel.
-constexpr int kJoin = 4;
-template <int DT>
-__global__ void __launch_bounds__(JF_HEAD_DIM * kJoin) block8_join_kernel(const __grid_constant__ AttnParams P, int width, int grid_y) {
-  __shared__ float sm_o[kJoin][JF_HEAD_DIM], sm_z[kJoin], sm_top[kJoin * 4];
-  __shared__ int sm_first, sm_n;
+// The pieces of a sequence.  A block of WARPS warps per (head, sequence) and 32 * VEC channels; a warp takes every WARPS-th piece.  Rows
+// of many pieces are spread over four blocks of 32 warps (one sequence of 131072 positions, 8 heads, 293
+// pieces: 4 us instead of 10); many rows take one block of 8 warps (32 sequences, 32 heads: 3 us instead of 12).
+template <int DT, int VEC, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_constant__ AttnParams P, int width, int grid_y) {
+  __shared__ float sm_w[WARPS * 32], sm_z[WARPS], sm_top[WARPS], sm_o[WARPS][32 * VEC];
   const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_wait();
-  pdl_trigger();
-  if (warp == 0) {   // pieces before this sequence's
-    int total = 0, before = 0, own = 0;
-    for (int i = lane; i < P.B; i += 32) total += span_of(P, i).count;
-    const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total));
-    for (int i = lane; i <= b; i += 32) {
-      const int n = max(1, (span_of(P, i).count + piece - 1) / piece);
-      if (i < b) before += n; else own = n;
-    }
-    before = __reduce_add_sync(0xFFFFFFFFu, before);
-    own = __reduce_add_sync(0xFFFFFFFFu, own);
-    if (lane == 0) { sm_first = before; sm_n = own; }
+  // The lengths are not written by the kernel in front of this one, whose blocks all wait for what is in front of them before
+  // they let this one start: they may be read at once.  Every warp works out for itself which pieces are the sequence's.
+  int total = 0, first = 0, n = 0;
+  for (int i = lane; i < P.B; i += 32) total += span_of(P, i).count;
+  const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total));
+  for (int i = lane; i <= b; i += 32) {
+    const int k = max(1, (span_of(P, i).count + piece - 1) / piece);
+    if (i < b) first += k; else n = k;
   }
-  __syncthreads();
-  const int n = sm_n;
+  first = __reduce_add_sync(0xFFFFFFFFu, first);
+  n = __reduce_add_sync(0xFFFFFFFFu, n);
+  pdl_wait();   // (also by blocks with nothing to do: who follows this kernel relies on the one before it)
+  pdl_trigger();
   if (n == 1) return;
   const int kvh = h / P.G, in_group = h % P.G, y = kvh * P.groups + in_group / width;
-  auto row_of = [&](int i) { return (static_cast<int64_t>(sm_first + i) * grid_y + y) * width + in_group % width; };
+  const int64_t row0 = (static_cast<int64_t>(first) * grid_y + y) * width + in_group % width, step = static_cast<int64_t>(grid_y) * width;
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += JF_HEAD_DIM * kJoin) top = fmaxf(top, P.part_ml[row_of(i) * 2]);
+  for (int i = threadIdx.x; i < n; i += WARPS * 32) top = fmaxf(top, P.part_ml[(row0 + i * step) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if (lane == 0) sm_top[warp] = top;
   __syncthreads();
   top = sm_top[0];
 #pragma unroll
-  for (int w = 1; w < kJoin * 4; ++w) top = fmaxf(top, sm_top[w]);
-  const int part = threadIdx.x / JF_HEAD_DIM, d = threadIdx.x % JF_HEAD_DIM;
-  float sum = 0.0f, z = 0.0f;
+  for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_top[w]);
+  float sum[VEC] = {}, z = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += WARPS * 32) {
+    const int m = min(WARPS * 32, n - i0);
+    if (threadIdx.x < m) {
+      const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + (row0 + (i0 + threadIdx.x) * step) * 2);
+      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+      sm_w[threadIdx.x] = f;
+      z = fmaf(ml.y, f, z);
+    }
+    __syncthreads();
+    const float* o = P.part_o + (row0 + i0 * step) * JF_HEAD_DIM + (blockIdx.z * 32 + lane) * VEC;
 #pragma unroll 8
-  for (int i = part; i < n; i += kJoin) {
-    const int64_t row = row_of(i);
-    const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + row * 2);
-    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-    sum = fmaf(P.part_o[row * JF_HEAD_DIM + d], f, sum);
-    z = fmaf(ml.y, f, z);
-  }
-  sm_o[part][d] = sum;
-  if (d == 0) sm_z[part] = z;
-  __syncthreads();
-  if (part == 0) {
-    sum = sm_o[0][d];
-    z = sm_z[0];
+    for (int i = warp; i < m; i += WARPS) {
+      const float w = sm_w[i];
+      if (VEC == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(o + i * step * JF_HEAD_DIM);
+        const float e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int k = 1; k < kJoin; ++k) { sum += sm_o[k][d]; z += sm_z[k]; }
+        for (int k = 0; k < VEC; ++k) sum[k] = fmaf(e[k], w, sum[k]);
+      } else {
+        sum[0] = fmaf(o[i * step * JF_HEAD_DIM], w, sum[0]);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sm_o[warp][lane * VEC + k] = sum[k];
+  if (lane == 0) sm_z[warp] = z;
+  __syncthreads();
+  if (threadIdx.x < 32 * VEC) {
+    float x = 0.0f;
+    z = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      x += sm_o[k][threadIdx.x];
+      z += sm_z[k];
+    }
     const int64_t row = static_cast<int64_t>(b) * P.H_q + h;
-    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + d] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : sum / z);
-    if (d == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
+    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + blockIdx.z * 32 * VEC + threadIdx.x] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : x / z);
+    if (threadIdx.x == 0 && blockIdx.z == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
   }
 }
 
 struct Plan { int G, nt, groups, target, min_piece, pieces; uint64_t bytes; };
 constexpr int kMinPiece = 8;   // blocks
+constexpr int kManyPieces = 32;   // of a sequence on average: the join spreads a row over four blocks
 
-// Pieces per KV head: one wave of blocks where the batch leaves room for it, several where it does not.
+// Pieces per KV head: one wave of blocks where the batch leaves room for it, three where it does not.
 bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
   if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_S <= 0 || H_q % H_kv != 0) return false;
   p.G = H_q / H_kv;
@@ -612,11 +649,13 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
   p.groups = (p.G + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t columns = static_cast<int64_t>(H_kv) * p.groups;
   const int64_t most = (static_cast<int64_t>(max_S) + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;       // blocks of a sequence
-  if (columns > 65535 || most * B > INT32_MAX / 2) return false;
+  if (columns > 65535 || H_q > 65535 || B > 65535 || most * B > INT32_MAX / 2) return false;
   const int64_t wave = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1) / columns);
   p.target = static_cast<int>(2 * B <= wave ? wave - B : 3 * wave);
   p.target = std::max(p.target, 1);
-  p.min_piece = kMinPiece;
+  // A sequence is cut where that finds work for idle multiprocessors: down to a block per warp for one sequence, hardly at all where
+  // the batch fills them (64 x 1000 positions, 8 KV heads: 61 -> 45 us; 8 x 500: 16 -> 12).
+  p.min_piece = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(kMinPiece, B * columns / 2)));
   const int64_t each = (most + p.min_piece - 1) / p.min_piece;
   p.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.target) + B, each * B));
   p.bytes = static_cast<uint64_t>(p.pieces) * columns * 8 * p.nt * (JF_HEAD_DIM + 2) * sizeof(float);
@@ -653,7 +692,7 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   Plan p;
   if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;
   if (!a->q || !a->k_data || !a->v_data || !a->k_scales || !a->v_scales || !a->block_table || !a->seq_lens || !a->out) return JF_ERR_ARG;
-  if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 2)) return JF_ERR_ARG;
+  if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 8)) return JF_ERR_ARG;
   if (a->num_blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
   if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE) return JF_ERR_UNSUPPORTED;
   if (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)) return JF_ERR_WORKSPACE;
@@ -690,10 +729,14 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
     st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_FP16>(P, p.nt, feat, grid, s)
                                    : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
   if (st != JF_OK || p.pieces == a->B) return st;   // one piece per sequence: nothing to join
-  const dim3 jgrid(a->H_q, a->B);
-  if (a->B > 65535) return JF_ERR_UNSUPPORTED;
-  JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
-                  ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16>, jgrid, dim3(JF_HEAD_DIM * kJoin), 0, s, P, 8 * p.nt, a->H_kv * p.groups)
-                  : launch_pdl(block8_join_kernel<JF_DTYPE_FP16>, jgrid, dim3(JF_HEAD_DIM * kJoin), 0, s, P, 8 * p.nt, a->H_kv * p.groups));
+  const int width = 8 * p.nt, grid_y = a->H_kv * p.groups;
+  if (p.pieces / a->B >= kManyPieces)
+    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
+                    ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16, 1, 32>, dim3(a->H_q, a->B, 4), dim3(1024), 0, s, P, width, grid_y)
+                    : launch_pdl(block8_join_kernel<JF_DTYPE_FP16, 1, 32>, dim3(a->H_q, a->B, 4), dim3(1024), 0, s, P, width, grid_y));
+  else
+    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
+                    ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16, 4, 8>, dim3(a->H_q, a->B), dim3(256), 0, s, P, width, grid_y)
+                    : launch_pdl(block8_join_kernel<JF_DTYPE_FP16, 4, 8>, dim3(a->H_q, a->B), dim3(256), 0, s, P, width, grid_y));
   return JF_OK;
 }
