@@ -8,7 +8,8 @@ variables kept from the reference: ``JETFIRE_MODE``, ``JETFIRE_TOPK``, ``JETFIRE
 ``JETFIRE_GPU_CORRECTION_SHARE`` (0..0.5: rows of the correction the GPU computes itself from the
 mapped mirror over the host link, stream-ordered steps with flags only) and
 ``JETFIRE_NUMA_NODE`` (``auto`` | ``off`` | a node number: where the host mirrors and the
-correction workers of this rank are placed).
+correction workers of this rank are placed) and ``JETFIRE_BLOCK8`` (``off`` | ``int8`` | ``e4m3``: layers
+keep their keys and values in 8 bits instead, see ``adapter/block8.py``).
 """
 from __future__ import annotations
 
@@ -38,6 +39,7 @@ SCHEME_TO_KERNEL_MODE = {"SymInt3K_SymInt2V": "k3v2", "SymInt4K_SymInt4V": "k4v4
 SUPPORTED_TOP_K = (32, 64, 128, 256, 512, 1024, 2048, 4096)
 
 
+BLOCK8_CODES = ("int8", "e4m3")
 NUMA_AUTO, NUMA_OFF = -2, -1   # the GPU's own node when the host has several / leave it to first touch
 
 
@@ -54,6 +56,7 @@ class JetFireConfig:
     stream_ordered: bool = True           # decode step queued on the stream without a host wait (capturable)
     stream_signal: str = "flags"          # how a stream-ordered step meets the host: "flags" or "callbacks"
     gpu_correction_share: float = 0.0     # fraction of the correction's rows the GPU computes from the mapped mirror
+    block8: str | None = None             # codes of an 8-bit cache in place of the packed one and its mirror
 
     @property
     def scheme(self) -> QuantScheme:
@@ -124,11 +127,14 @@ def get_jetfire_config() -> JetFireConfig:
         raise ValueError("JETFIRE_GPU_CORRECTION_SHARE must be a number between 0 and 0.5") from exc
     if not 0.0 <= share <= 0.5:
         raise ValueError("JETFIRE_GPU_CORRECTION_SHARE must be a number between 0 and 0.5")
+    block8 = (os.environ.get("JETFIRE_BLOCK8") or "off").strip().lower()
+    if block8 not in ("off", *BLOCK8_CODES):
+        raise ValueError(f"JETFIRE_BLOCK8 must be 'off' or one of {BLOCK8_CODES}, got {block8!r}")
     _CONFIG = JetFireConfig(mode=mode, top_k=top_k, group_size=group, cpu_attn_threads=threads,
                             max_batch_size=_int_env("JETFIRE_MAX_BATCH_SIZE", 32),
                             slots_i32=_int_env("JETFIRE_SLOTS_I32", 1) != 0, numa_node=_numa_env(),
                             stream_ordered=_int_env("JETFIRE_STREAM_ORDERED", 1) != 0, stream_signal=signal,
-                            gpu_correction_share=share)
+                            gpu_correction_share=share, block8=None if block8 == "off" else block8)
     return _CONFIG
 
 

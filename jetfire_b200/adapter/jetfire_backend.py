@@ -3,26 +3,28 @@
 vLLM's classes are imported lazily and only here, so the rest of the package works without
 vLLM.  ``JetFireAttentionImplMixin`` holds the routing (decode -> ``try_jetfire_decode``,
 a step with decode and prefill sequences -> ``try_jetfire_mixed``, append ->
-``JetFireCacheStore.write_slots``); ``make_backend()`` binds it to the vLLM FlashAttention
+``JetFireCacheStore.write_slots``; a layer with an 8-bit cache -> ``try_block8_attention``, which
+appends too); ``make_backend()`` binds it to the vLLM FlashAttention
 classes of the installed version, with a metadata builder that notes the scheduler's
 decode/prefill split on the metadata, and returns the backend class to register as ``CUSTOM`` (``register_backend(AttentionBackendEnum.CUSTOM, ...)``, reference
 jetfire_vllm/adapter/registry.py:19, :61).
 """
 from __future__ import annotations
 
+from .block8 import JetFireBlock8Store, try_block8_attention
 from .cache_store import JetFireCacheStore
 from .config import get_jetfire_config
 from .decode_path import try_jetfire_decode
 from .mixed_batch import annotate_split_counts, try_jetfire_mixed
 
-_STORES: dict[str, JetFireCacheStore] = {}
+_STORES: dict[str, JetFireCacheStore | JetFireBlock8Store] = {}
 
 
-def get_layer_store(layer_name: str) -> JetFireCacheStore | None:
+def get_layer_store(layer_name: str) -> JetFireCacheStore | JetFireBlock8Store | None:
     return _STORES.get(layer_name)
 
 
-def register_layer_store(layer_name: str, store: JetFireCacheStore) -> None:
+def register_layer_store(layer_name: str, store: JetFireCacheStore | JetFireBlock8Store) -> None:
     _STORES[layer_name] = store
 
 
@@ -32,7 +34,13 @@ class JetFireAttentionImplMixin:
     def forward(self, layer, query, key, value, kv_cache, attn_metadata, output=None,
                 output_scale=None, output_block_scale=None):
         store = get_layer_store(getattr(layer, "layer_name", ""))
-        if output is not None and attn_metadata is not None:
+        if isinstance(store, JetFireBlock8Store):
+            if output is not None and attn_metadata is not None and key is not None and value is not None:
+                done = try_block8_attention(impl=self, layer=layer, query=query, key=key, value=value,
+                                            attn_metadata=attn_metadata, output=output, store=store)
+                if done is not None:
+                    return done
+        elif output is not None and attn_metadata is not None:
             done = try_jetfire_decode(impl=self, layer=layer, query=query, attn_metadata=attn_metadata,
                                       output=output, store=store, cfg=get_jetfire_config())
             if done is not None:
@@ -48,7 +56,8 @@ class JetFireAttentionImplMixin:
 
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
         store = get_layer_store(getattr(layer, "layer_name", ""))
-        if store is not None:
+        # (an 8-bit cache is filled by forward, which knows the sequences' bounds)
+        if store is not None and not isinstance(store, JetFireBlock8Store):
             n = int(slot_mapping.shape[0])
             store.write_slots(key[:n].view(n, store.num_kv_heads, store.head_dim),
                               value[:n].view(n, store.num_kv_heads, store.head_dim), slot_mapping)

@@ -217,7 +217,8 @@ def _decode_metadata(attn_metadata, seq_lens, block_table, max_seq_len, n, devic
 def try_jetfire_mixed(*, impl, layer, query, key, value, attn_metadata, output, store=None,
                       cfg: JetFireConfig | None = None, prefill_attention: PrefillAttention | None = None,
                       stats: MixedBatchStats | None = None):
-    """A step with both decode and prefill sequences.  Returns ``output`` when both parts were
+    """A step with both decode and prefill sequences.  ``prefill_attention``: what the prompts' rows go to, by default vLLM's
+    flash attention; ``block8.native_varlen_prefill`` is this library's own kernel.  Returns ``output`` when both parts were
     written, None when the step is not one this path serves (the caller then runs its native
     attention over the whole step; nothing has been written to ``output`` in that case).
 

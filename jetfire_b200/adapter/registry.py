@@ -15,6 +15,7 @@ dummy native KV tensors, prefill activation chunking and scheduler changes.
 """
 from __future__ import annotations
 
+from .block8 import JetFireBlock8Store
 from .cache_store import JetFireCacheStore
 from .config import JetFireConfig, get_jetfire_config
 from .jetfire_backend import register_layer_store
@@ -44,8 +45,8 @@ def ensure_jetfire_registered() -> bool:
 def install_layer_stores(layers: dict, *, num_blocks: int, block_size: int = 16, device="cuda", dtype=None,
                          cfg: JetFireConfig | None = None, mirror_append: str = "mapped") -> dict:
     """``layers``: layer name -> object with ``num_kv_heads`` and ``head_size`` (vLLM's ``Attention``
-    modules, or any stand-in).  Creates one ``JetFireCacheStore`` per layer with vLLM's planned
-    ``num_blocks`` (the scheduler hands out block ids in [0, num_blocks), so the cache must cover
+    modules, or any stand-in).  Creates one ``JetFireCacheStore`` (``JetFireBlock8Store`` where the configuration
+    asks for an 8-bit cache) per layer with vLLM's planned ``num_blocks`` (the scheduler hands out block ids in [0, num_blocks), so the cache must cover
     them all) and registers it under the layer's name.  Layers whose geometry the decode path does
     not serve (head size other than 128, block size other than 16) are skipped and fall back to
     vLLM's native attention.  Returns name -> store for the layers that were installed."""
@@ -55,6 +56,12 @@ def install_layer_stores(layers: dict, *, num_blocks: int, block_size: int = 16,
     out = {}
     for name, layer in layers.items():
         if int(getattr(layer, "head_size", 0)) != 128 or int(block_size) != 16:
+            continue
+        if cfg.block8:
+            store = JetFireBlock8Store(num_blocks=int(num_blocks), num_kv_heads=int(layer.num_kv_heads), codes=cfg.block8, device=device,
+                                       block_size=int(block_size))
+            register_layer_store(name, store)
+            out[name] = store
             continue
         store = JetFireCacheStore(num_blocks=int(num_blocks), num_kv_heads=int(layer.num_kv_heads), head_dim=128,
                                   cfg=cfg, device=device, dtype=dtype, block_size=int(block_size),

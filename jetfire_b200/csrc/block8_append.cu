@@ -14,6 +14,8 @@
 #include "jf_common.cuh"
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace jf {
 namespace {
 
@@ -33,9 +35,16 @@ struct AppendParams {
   const void* table;
   int64_t bt_stride, num_blocks;
   int32_t T, H, n_seqs, max_blocks, chunk;
-  bool bt_i32, vec;           // vec: rows may be read 16 bytes at a time
+  bool bt_i32;
 };
 
+// Larger magnitudes of two pairs; NaN wins, the signs are left over.
+template <int DT> __device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if (DT == JF_DTYPE_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 template <int DT> __device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
   if (DT == JF_DTYPE_BF16) {
     lo = __uint_as_float(w << 16);
@@ -47,23 +56,35 @@ template <int DT> __device__ __forceinline__ void unpack2(uint32_t w, float& lo,
   }
 }
 
-// Four scaled values as codes.  int8: adding 1.5 * 2^23 rounds to an integer, half to even, and leaves its two's
-// complement in the low byte; `clean` values cannot leave the range (|x| <= amax, and amax * fp32(1 / fp32(amax / 127))
-// is within 2^-22 of 127).
-template <int CODES> __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, bool clean) {
-  if (!clean) {
-    constexpr float top = CODES == JF_CODES_INT8 ? 127.0f : 448.0f;
-    auto tame = [](float v) { return v != v ? 0.0f : fminf(fmaxf(v, -top), top); };
-    a = tame(a); b = tame(b); c = tame(c); d = tame(d);
-  }
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+
+// Four scaled values (two pairs) as codes; none of them leaves the range.  int8: adding 1.5 * 2^23 rounds to an integer, half to
+// even, and leaves its two's complement in the low byte.
+template <int CODES> __device__ __forceinline__ uint32_t encode4(uint64_t ab, uint64_t cd) {
+  float a, b, c, d;
   if (CODES == JF_CODES_INT8) {
-    const uint32_t i = __float_as_uint(a + 12582912.0f), j = __float_as_uint(b + 12582912.0f);
-    const uint32_t k = __float_as_uint(c + 12582912.0f), l = __float_as_uint(d + 12582912.0f);
-    return prmt(prmt(i, j, 0x0040u), prmt(k, l, 0x0040u), 0x5410u);
+    const uint64_t magic = pair(12582912.0f, 12582912.0f);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(ab) : "l"(magic));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(cd) : "l"(magic));
+    split(ab, a, b);
+    split(cd, c, d);
+    return prmt(prmt(__float_as_uint(a), __float_as_uint(b), 0x0040u), prmt(__float_as_uint(c), __float_as_uint(d), 0x0040u), 0x5410u);
   }
+  split(ab, a, b);
+  split(cd, c, d);
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
+}
+// NaN as 0, what lies beyond the largest code as that
+template <int CODES> __device__ __forceinline__ float tame(float v) {
+  constexpr float top = CODES == JF_CODES_INT8 ? 127.0f : 448.0f;
+  return v != v ? 0.0f : fminf(fmaxf(v, -top), top);
 }
 
 template <int CODES> __device__ __forceinline__ float decode1(uint32_t byte) {
@@ -79,8 +100,8 @@ template <int CODES> __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float((((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 8u) << 23);
 }
 
-template <int DT> __device__ __forceinline__ uint4 load8(const uint16_t* p, bool vec) {
-  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+template <bool VEC> __device__ __forceinline__ uint4 load8(const uint16_t* p) {
+  if constexpr (VEC) return __ldg(reinterpret_cast<const uint4*>(p));
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __ldg(p + 2 * i) | static_cast<uint32_t>(__ldg(p + 2 * i + 1)) << 16;
@@ -88,7 +109,7 @@ template <int DT> __device__ __forceinline__ uint4 load8(const uint16_t* p, bool
 }
 
 // Rows t .. t + cnt of the call into rows r .. r + cnt of block `id`; r rows of its sequence are there already.
-template <int DT, int CODES>
+template <int DT, int CODES, bool VEC>
 __device__ __forceinline__ void write_block(const AppendParams& P, const AppendSide& S, int h, int t, int cnt, int r, int64_t id) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const uint16_t* x = S.x + static_cast<int64_t>(t) * S.stride_t + h * S.stride_h + col;
@@ -96,7 +117,7 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = 2 * i + half;
-    raw[i] = row < cnt ? load8<DT>(x + row * S.stride_t, P.vec) : make_uint4(0, 0, 0, 0);
+    raw[i] = row < cnt ? load8<VEC>(x + row * S.stride_t) : make_uint4(0, 0, 0, 0);
   }
   float* scale_at = S.scales + h * P.num_blocks + id;
   float old = r > 0 ? *scale_at : 0.0f;
@@ -104,9 +125,8 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
   constexpr uint32_t kInf = DT == JF_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    m = __vmaxu2(__vmaxu2(m, __vmaxu2(raw[i].x & 0x7FFF7FFFu, raw[i].y & 0x7FFF7FFFu)),
-                 __vmaxu2(raw[i].z & 0x7FFF7FFFu, raw[i].w & 0x7FFF7FFFu));
+  for (int i = 0; i < 8; ++i) m = absmax2<DT>(m, absmax2<DT>(absmax2<DT>(raw[i].x, raw[i].y), absmax2<DT>(raw[i].z, raw[i].w)));
+  m &= 0x7FFF7FFFu;
   uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(m & 0xFFFFu, m >> 16));
   const bool clean = top < kInf;
   if (!clean) {   // infinities and NaN do not count
@@ -124,34 +144,43 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
   }
   const float s = fmaxf(old, scale_for<CODES>(Elem<DT>::to_f32(static_cast<uint16_t>(top))));
   const float inv = __frcp_rn(s);
+  const uint64_t inv2 = pair(inv, inv);
   uint8_t* rows = S.data + ((h * P.num_blocks + id) * JF_BLOCK_SIZE) * JF_HEAD_DIM + col;
+  // Finite values stay in range: |x| <= amax, and amax * fp32(1 / fp32(amax / 127)) is within 2^-22 of 127.  The products are
+  // rounded to fp32 before the codes are (not fused with what follows).
+  auto store = [&](auto wild) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = 2 * i + half;
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float v[8];
+    for (int i = 0; i < 8; ++i) {
+      const int row = 2 * i + half;
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      uint64_t v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      unpack2<DT>(w[k], v[2 * k], v[2 * k + 1]);
-      v[2 * k] = __fmul_rn(v[2 * k], inv);   // rounded to fp32 before the code is: not fused with what follows
-      v[2 * k + 1] = __fmul_rn(v[2 * k + 1], inv);
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpack2<DT>(w[k], a, b);
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v[k]) : "l"(pair(a, b)), "l"(inv2));
+        if (decltype(wild)::value) {
+          split(v[k], a, b);
+          v[k] = pair(tame<CODES>(a), tame<CODES>(b));
+        }
+      }
+      if (row < cnt) *reinterpret_cast<uint2*>(rows + (r + row) * JF_HEAD_DIM) = make_uint2(encode4<CODES>(v[0], v[1]), encode4<CODES>(v[2], v[3]));
     }
-    if (row < cnt)
-      *reinterpret_cast<uint2*>(rows + (r + row) * JF_HEAD_DIM) =
-          make_uint2(encode4<CODES>(v[0], v[1], v[2], v[3], clean), encode4<CODES>(v[4], v[5], v[6], v[7], clean));
-  }
+  };
+  if (clean) store(std::false_type());
+  else store(std::true_type());
   if (r > 0 && s != old) {
     const float ratio = __fdiv_rn(old, s);
     for (int row = half; row < r; row += 2) {
       uint2* p = reinterpret_cast<uint2*>(rows + row * JF_HEAD_DIM);
       const uint2 c = *p;
-      float v[8];
+      uint64_t v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] = __fmul_rn(decode1<CODES>(c.x >> 8 * k & 255u), ratio);
-        v[4 + k] = __fmul_rn(decode1<CODES>(c.y >> 8 * k & 255u), ratio);
+        const uint32_t two = (k < 2 ? c.x : c.y) >> 16 * (k & 1);
+        v[k] = pair(tame<CODES>(__fmul_rn(decode1<CODES>(two & 255u), ratio)), tame<CODES>(__fmul_rn(decode1<CODES>(two >> 8 & 255u), ratio)));
       }
-      *p = make_uint2(encode4<CODES>(v[0], v[1], v[2], v[3], false), encode4<CODES>(v[4], v[5], v[6], v[7], false));
+      *p = make_uint2(encode4<CODES>(v[0], v[1]), encode4<CODES>(v[2], v[3]));
     }
   }
   __syncwarp();
@@ -159,20 +188,16 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
 }
 
 // A warp per (chunk of tokens, head, side): it writes every block whose first token of the call stands in the chunk.
-template <int DT, int CODES>
+template <int DT, int CODES, bool VEC>   // VEC: rows may be read 16 bytes at a time
 __global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid_constant__ AppendParams P) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int side = item & 1;
-  const int64_t rest = item >> 1;
-  const int h = static_cast<int>(rest % P.H);
-  int t = static_cast<int>(rest / P.H) * P.chunk;
+  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), rest = item >> 1;
+  const int side = item & 1, h = static_cast<int>(rest % static_cast<uint32_t>(P.H));
+  const int64_t from = static_cast<int64_t>(rest / static_cast<uint32_t>(P.H)) * P.chunk;
+  if (from >= P.T) { pdl_wait(); return; }
+  int t = static_cast<int>(from);
   const int end = min(t + P.chunk, P.T);
   const AppendSide& S = P.side[side];
-  // The chunk's rows start on their way to L2 before it is known where they go (nothing is read here): the bounds, the length
-  // and the block id come one after the other.  8192 tokens, 8 KV heads, int8: 14.7 -> 12.3 us.
-  if ((lane >> 1) < P.chunk && t + (lane >> 1) < P.T)
-    prefetch_l2(S.x + static_cast<int64_t>(t + (lane >> 1)) * S.stride_t + h * S.stride_h + (lane & 1) * 64);
   pdl_wait();
   pdl_trigger();
   // sequences that end at or before t
@@ -197,7 +222,7 @@ __global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid
     if (blk < P.max_blocks) {
       const int64_t at = s * P.bt_stride + blk;
       const int64_t id = P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
-      if (id >= 0 && id < P.num_blocks) write_block<DT, CODES>(P, S, h, t, cnt, r, id);
+      if (id >= 0 && id < P.num_blocks) write_block<DT, CODES, VEC>(P, S, h, t, cnt, r, id);
     }
     t += cnt;
   }
@@ -230,18 +255,24 @@ extern "C" jf_status_t jf_block8_append(const void* key, const void* value, int3
   P.n_seqs = n_seqs;
   P.max_blocks = max_blocks;
   P.bt_i32 = bt_is_i32 != 0;
-  P.vec = aligned(key, 16) && aligned(value, 16) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0;
+  const bool vec = aligned(key, 16) && aligned(value, 16) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0;
   const int64_t mean = T / n_seqs;
   P.chunk = mean >= 16 ? 16 : mean >= 4 ? 4 : 1;
   const int64_t items = (T + P.chunk - 1) / P.chunk * H_kv * 2, blocks = (items + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
+  if (items > INT32_MAX) return JF_ERR_UNSUPPORTED;
   const auto s = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(blocks)), block(kWarps * 32);
+  auto launch = [&](auto dt, auto code) {
+    constexpr int D = decltype(dt)::value, C = decltype(code)::value;
+    return vec ? launch_pdl(block8_append_kernel<D, C, true>, grid, block, 0, s, P) : launch_pdl(block8_append_kernel<D, C, false>, grid, block, 0, s, P);
+  };
+  using Bf16 = std::integral_constant<int, JF_DTYPE_BF16>;
+  using Fp16 = std::integral_constant<int, JF_DTYPE_FP16>;
+  using Int8 = std::integral_constant<int, JF_CODES_INT8>;
+  using E4m3 = std::integral_constant<int, JF_CODES_E4M3>;
   if (dtype == JF_DTYPE_BF16)
-    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch_pdl(block8_append_kernel<JF_DTYPE_BF16, JF_CODES_INT8>, grid, block, 0, s, P)
-                                       : launch_pdl(block8_append_kernel<JF_DTYPE_BF16, JF_CODES_E4M3>, grid, block, 0, s, P));
+    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Bf16(), Int8()) : launch(Bf16(), E4m3()));
   else
-    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch_pdl(block8_append_kernel<JF_DTYPE_FP16, JF_CODES_INT8>, grid, block, 0, s, P)
-                                       : launch_pdl(block8_append_kernel<JF_DTYPE_FP16, JF_CODES_E4M3>, grid, block, 0, s, P));
+    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Fp16(), Int8()) : launch(Fp16(), E4m3()));
   return JF_OK;
 }

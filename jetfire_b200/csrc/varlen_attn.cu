@@ -179,6 +179,11 @@ __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
   return k;
 }
 __device__ __forceinline__ int tile_of(const Keys& k, int i) { return i < k.a ? i : k.first + i - k.a; }
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {   // of two unsigned halves
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
 template <int DT> __device__ __forceinline__ bool no_number(uint32_t half) {
@@ -411,7 +416,7 @@ template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, 
 #pragma unroll 8
         for (int n = lane; n < kTileBytes / 16; n += 32) {
           const uint4 x = tile[n];
-          top = __vmaxu2(__vmaxu2(top, __vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu)), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+          top = max2(max2(top, max2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu)), max2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
         }
         if (__any_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16) >= inf)) {
           bool own = false;   // among the sequence's own rows
