@@ -167,7 +167,8 @@ __device__ __forceinline__ Tiles tiles_of(const Params& P, const Item& it, int q
                (first_key(P, r1) + kKeys - 1) / kKeys,
                min(end_key(P, it, q0), it.len) / kKeys};
 }
-// The key tiles of an item, prefix first: tiles 0 .. a, then first, first + 1, ...  Each is used by one of its row tiles.
+// The key tiles of an item, the last first: count - a tiles down to `first`, then the prefix's a - 1 .. 0.  Each is used by one
+// of its row tiles.  (From the row's own position backwards: where nearer keys weigh more, references settle early.)
 struct Keys { int a, first, count; };
 __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
   const int r0 = it.pair * kPairRows, r1 = min(r0 + kPairRows, it.len) - 1;
@@ -178,7 +179,10 @@ __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
   k.count = k.a + max(to, np) - from;
   return k;
 }
-__device__ __forceinline__ int tile_of(const Keys& k, int i) { return i < k.a ? i : k.first + i - k.a; }
+__device__ __forceinline__ int tile_of(const Keys& k, int i) {
+  const int j = k.count - 1 - i;
+  return j < k.a ? j : k.first + j - k.a;
+}
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {   // of two unsigned halves
   uint32_t d;
   asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -533,6 +537,35 @@ template <int DT, bool SCALED> __device__ __forceinline__ void weigh(const float
   }
 }
 
+// The same for scores under a cap whose magnitude stays below it: x = f(s) - ref with f(s) = s (c0 + w q(w)), w = s^2.
+template <int DT> __device__ __forceinline__ void weigh_capped(const float* s, uint32_t* p, uint64_t* sum, const float (&co)[6], float ref) {
+  const uint64_t r2 = pair(-ref, -ref);
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    const uint64_t x = pair(s[c], s[c + 1]), w = mul2(x, x);
+    uint64_t q = fma2(w, pair(co[5], co[5]), pair(co[4], co[4]));
+#pragma unroll
+    for (int k = 3; k >= 0; --k) q = fma2(q, w, pair(co[k], co[k]));
+    float a, b;
+    split(fma2(x, q, r2), a, b);
+    a = ex2(a);
+    b = ex2(b);
+    sum[c / 2 & 1] = add2(sum[c / 2 & 1], pair(a, b));
+    if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[c / 2]) : "f"(b), "f"(a));
+  }
+}
+
+// Smallest of 64 scores, NaN left out of account.
+__device__ __forceinline__ float smallest(const float* s) {
+  float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < 64; c += 4)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = fminf(x[k], s[c + k]);
+  return fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+}
+
 // Largest of N scores; a NaN if there is one.
 template <int N> __device__ __forceinline__ float largest(const float* s) {
   float x[4];
@@ -580,6 +613,19 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
   const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
   const float sl2 = P.scale * kLog2e;
+  // log2(e) cap tanh(scale s / cap) = s (co[0] + co[1] s^2 + ...) while |s| <= cap_in (the fit of reshape(), in s)
+  float co[6], cap_in = 0.0f;
+  if (FEAT == 2) {
+    constexpr float fit[6] = {1.0f, -0.333302796f, 0.132884905f, -0.0517682843f, 0.0169064086f, -0.00312657771f};
+    const float in = P.scale / P.softcap, in2 = in * in;
+    cap_in = in2 < 1e6f ? fabsf(P.softcap / P.scale) : -1.0f;   // (beyond, powers of in2 leave fp32's range)
+    float power = sl2;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      co[k] = fit[k] * power;
+      power *= in2;
+    }
+  }
   ItemReader items;
   Item it;
   int s_count = 0, o_count = 0;
@@ -607,6 +653,46 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
 #pragma unroll
         for (int c = 0; c < N; c += 32) tmem_ld32(s_at + from + c, u + c);
         tc_wait_ld();
+        auto move_to = [&](float top) {
+          // (the output holds this tile's first half only when its product is through)
+          if (from > 0 && !wait_warp(&S.half_done[t], (s_count - 1) & 1)) return false;
+          if (from > 0) tc_fence_after();
+          if (top != top) l = top;   // a NaN among the scores is all that is left of the row
+          const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
+          m = to;
+          l *= f;
+          sum[0] = mul2(sum[0], pair(f, f));
+          sum[1] = mul2(sum[1], pair(f, f));
+          if (have || from > 0) rescale(o_at, f);
+          return true;
+        };
+        auto publish = [&](int h) {
+          tmem_st32(s_at + h * 32, p);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.p_full[t][h]);
+        };
+        if (FEAT == 2 && !masked && slope2 == 0.0f) {
+          // the cap keeps the order of scores: the largest is taken before it, and the reference leaves with the last step of f
+          const float high = largest<64>(s), low = smallest(s);
+          if (__all_sync(0xFFFFFFFFu, fmaxf(fabsf(high), fabsf(low)) <= cap_in)) {
+            const float w = high * high;
+            float q = fmaf(w, co[5], co[4]);
+#pragma unroll
+            for (int k = 3; k >= 0; --k) q = fmaf(q, w, co[k]);
+            // (a negative scale turns the order round)
+            const float lw = low * low;
+            float lq = fmaf(lw, co[5], co[4]);
+#pragma unroll
+            for (int k = 3; k >= 0; --k) lq = fmaf(lq, lw, co[k]);
+            const float top = fmaxf(high * q, low * lq);
+            if (__any_sync(0xFFFFFFFFu, top > m + kLag) && !move_to(top)) return false;
+            weigh_capped<DT>(s, p, sum, co, m - kLift);
+            publish(from / 64);
+            return true;
+          }
+        }
 #pragma unroll
         for (int c = 0; c < N; c += 64) {
           const int k1 = k0 + from + c;
@@ -622,28 +708,12 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
           }
         }
         const float top = largest<N>(s) * (FEAT ? 1.0f : sl2);
-        if (__any_sync(0xFFFFFFFFu, !(top <= m + kLag))) {
-          // (the output holds this tile's first half only when its product is through)
-          if (from > 0 && !wait_warp(&S.half_done[t], (s_count - 1) & 1)) return false;
-          if (from > 0) tc_fence_after();
-          if (top != top) l = top;   // a NaN among the scores is all that is left of the row
-          const float to = fmaxf(m, top), f = to == m ? 1.0f : ex2(m - to);
-          m = to;
-          l *= f;
-          sum[0] = mul2(sum[0], pair(f, f));
-          sum[1] = mul2(sum[1], pair(f, f));
-          if (have || from > 0) rescale(o_at, f);
-        }
+        if (__any_sync(0xFFFFFFFFu, !(top <= m + kLag)) && !move_to(top)) return false;
         const float ref = m == -INFINITY ? 0.0f : m - kLift;
 #pragma unroll
         for (int c = 0; c < N; c += 64) {
           weigh<DT, FEAT != 0>(s + c, p, sum, sl2, ref);
-          const int h = from / 64 + c / 64;
-          tmem_st32(s_at + h * 32, p);
-          tc_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S.p_full[t][h]);
+          publish(from / 64 + c / 64);
         }
         return true;
       };
