@@ -505,14 +505,19 @@ template <bool CAP> __device__ __forceinline__ void reshape(float* s, const Para
   }
   const float mul = CAP ? 1.0f : sl2;
   if (lin != 0) {
-    // -slope |i - j| = lin * slope * (j - i) = k c - k apart for the tile's c-th key; what its two roundings lose is 2^-23 of
-    // the bias itself
-    const float k = lin * slope2, a = -k * static_cast<float>(apart);
-    const uint64_t k2 = pair(k, k), a2 = pair(a, a), m2 = pair(mul, mul);
+    // -slope |i - j| = lin * slope * (j - i) = k (c - apart) for the c-th key: four pairs that go on by 8 k, so that no
+    // constants have to be brought up (what eight additions round is 2^-21 of the bias)
+    const float k = lin * slope2;
+    const uint64_t on = pair(8.0f * k, 8.0f * k), m2 = pair(mul, mul);
+    uint64_t bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = pair(k * static_cast<float>(2 * e - apart), k * static_cast<float>(2 * e + 1 - apart));
 #pragma unroll
     for (int c = 0; c < 64; c += 2) {
-      const uint64_t x = pair(s[c], s[c + 1]), bias = fma2(pair(static_cast<float>(c), static_cast<float>(c + 1)), k2, a2);
-      split(CAP ? add2(x, bias) : fma2(x, m2, bias), s[c], s[c + 1]);
+      uint64_t& b = bias[c / 2 & 3];
+      const uint64_t x = pair(s[c], s[c + 1]);
+      split(CAP ? add2(x, b) : fma2(x, m2, b), s[c], s[c + 1]);
+      b = add2(b, on);
     }
   } else {
     const float a = static_cast<float>(apart);
