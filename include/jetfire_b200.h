@@ -519,7 +519,7 @@ typedef struct jf_block8_attn_args {
   int32_t B, H_q, H_kv, max_S;
   int32_t max_blocks, bt_is_i32;
   int32_t window;                 /* 0: none */
-  float   attn_scale, softcap;    /* softcap 0: none */
+  float   attn_scale, softcap;    /* softcap 0: none, else 1e-30 .. 1e30 */
   int32_t reserved;
   int64_t num_blocks, bt_stride;
   const void*    q;
@@ -565,7 +565,7 @@ jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
 typedef struct jf_varlen_attn_args {
   int32_t dtype, n_seqs, H_q, H_kv;
   int32_t causal, window;         /* window 0: none */
-  float   attn_scale, softcap;    /* softcap 0: none */
+  float   attn_scale, softcap;    /* softcap 0: none, else 1e-30 .. 1e30 */
   int64_t T;
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
   const void*    q;

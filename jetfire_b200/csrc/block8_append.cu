@@ -102,10 +102,12 @@ template <int CODES> __device__ __forceinline__ float scale_for(float amax) {
 
 template <bool VEC> __device__ __forceinline__ uint4 load8(const uint16_t* p) {
   if constexpr (VEC) return __ldg(reinterpret_cast<const uint4*>(p));
-  uint32_t w[4];
+  else {
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __ldg(p + 2 * i) | static_cast<uint32_t>(__ldg(p + 2 * i + 1)) << 16;
-  return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(p + 2 * i) | static_cast<uint32_t>(__ldg(p + 2 * i + 1)) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // Rows t .. t + cnt of the call into rows r .. r + cnt of block `id`; r rows of its sequence are there already.
@@ -257,7 +259,10 @@ extern "C" jf_status_t jf_block8_append(const void* key, const void* value, int3
   P.bt_i32 = bt_is_i32 != 0;
   const bool vec = aligned(key, 16) && aligned(value, 16) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0;
   const int64_t mean = T / n_seqs;
-  P.chunk = mean >= 16 ? 16 : mean >= 4 ? 4 : 1;
+  // Tokens a warp looks through.  16 suit one prompt (8192 tokens, 8 KV heads: 13.7 us, with chunks of four 17.2), but sequences of one
+  // token would wait for one another there (64 of them beside a prompt of 2048: 31.5 us, with chunks of four 10.9), and
+  // which sequences are long is not known here.
+  P.chunk = n_seqs < 4 ? 16 : mean >= 8 ? 4 : mean >= 2 ? 2 : 1;
   const int64_t items = (T + P.chunk - 1) / P.chunk * H_kv * 2, blocks = (items + kWarps - 1) / kWarps;
   if (items > INT32_MAX) return JF_ERR_UNSUPPORTED;
   const auto s = static_cast<cudaStream_t>(stream);

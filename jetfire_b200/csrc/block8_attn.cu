@@ -54,9 +54,8 @@ struct AttnParams {
 
 // What of a sequence is scanned: its first `head` blocks and the `count - head` blocks that end with its last position.
 struct Span { int len, prefix, lo, head, first, count; };
-__device__ __forceinline__ Span span_of(const AttnParams& P, int b) {
+__device__ __forceinline__ Span span_of(const AttnParams& P, int length, int prefix) {
   Span s;
-  const int length = P.seq_lens[b], prefix = P.window > 0 && P.prefix_lens ? P.prefix_lens[b] : 0;
   s.len = max(0, min(length, min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
   const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
   s.prefix = s.lo = s.head = s.first = 0;
@@ -70,24 +69,32 @@ __device__ __forceinline__ Span span_of(const AttnParams& P, int b) {
   }
   return s;
 }
+__device__ __forceinline__ int prefix_of(const AttnParams& P, int b) { return P.window > 0 && P.prefix_lens ? P.prefix_lens[b] : 0; }
+__device__ __forceinline__ int blocks_of(const AttnParams& P, int b) { return span_of(P, P.seq_lens[b], prefix_of(P, b)).count; }
 // Whose piece `x` is: n pieces of `piece` blocks (the last may be shorter) make up sequence b, the index-th is x.  The first
 // piece of a sequence is the sum of those before it.
-struct Cut { int piece, b, index, n; };
+struct Cut { int piece, b, index, n, length, prefix; };
 __device__ __forceinline__ int piece_length(const AttnParams& P, int total) {
   return max(P.min_piece, (total + P.target - 1) / P.target);
 }
 // All lanes of a warp; b = -1 if there is no such piece.
 __device__ __forceinline__ Cut find_piece(const AttnParams& P, int x) {
   const int lane = threadIdx.x & 31;
-  int total = 0, mine = 0;
+  int total = 0, length = 0, prefix = 0, mine = 0;
+  auto look_at = [&](int b) {
+    const bool is = b < P.B;
+    length = is ? P.seq_lens[b] : 0;
+    prefix = is ? prefix_of(P, b) : 0;
+    mine = is ? span_of(P, length, prefix).count : 0;
+  };
   for (int b0 = 0; b0 < P.B; b0 += 32) {
-    mine = b0 + lane < P.B ? span_of(P, b0 + lane).count : 0;
+    look_at(b0 + lane);
     total += __reduce_add_sync(0xFFFFFFFFu, mine);
   }
-  Cut c{piece_length(P, total), -1, 0, 0};
+  Cut c{piece_length(P, total), -1, 0, 0, 0, 0};
   int before = 0;
   for (int b0 = 0; b0 < P.B; b0 += 32) {
-    if (P.B > 32) mine = b0 + lane < P.B ? span_of(P, b0 + lane).count : 0;
+    if (P.B > 32) look_at(b0 + lane);
     const int n = b0 + lane < P.B ? max(1, (mine + c.piece - 1) / c.piece) : 0;   // an empty sequence is written by a piece too
     int sum = n;
 #pragma unroll
@@ -102,6 +109,8 @@ __device__ __forceinline__ Cut find_piece(const AttnParams& P, int x) {
       c.n = __shfl_sync(0xFFFFFFFFu, n, l);
       c.index = x - before - (__shfl_sync(0xFFFFFFFFu, sum, l) - c.n);
       c.piece = (__shfl_sync(0xFFFFFFFFu, mine, l) + c.n - 1) / c.n;   // as many blocks in each
+      c.length = __shfl_sync(0xFFFFFFFFu, length, l);
+      c.prefix = __shfl_sync(0xFFFFFFFFu, prefix, l);
       return c;
     }
     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   const Cut cut = find_piece(P, blockIdx.x);
   if (cut.b < 0) return;
   const int b = cut.b;
-  const Span span = span_of(P, b);
+  const Span span = span_of(P, cut.length, cut.prefix);
   const int begin = cut.index * cut.piece, end = min(begin + cut.piece, span.count);
   // q of the lane's head (column g of each tile), and the slopes of the heads of its score columns 2t and 2t + 1
   uint4 q_raw[NT][4];
@@ -570,10 +579,10 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
   // The lengths are not written by the kernel in front of this one, whose blocks all wait for what is in front of them before
   // they let this one start: they may be read at once.  Every warp works out for itself which pieces are the sequence's.
   int total = 0, first = 0, n = 0;
-  for (int i = lane; i < P.B; i += 32) total += span_of(P, i).count;
+  for (int i = lane; i < P.B; i += 32) total += blocks_of(P, i);
   const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total));
   for (int i = lane; i <= b; i += 32) {
-    const int k = max(1, (span_of(P, i).count + piece - 1) / piece);
+    const int k = max(1, (blocks_of(P, i) + piece - 1) / piece);
     if (i < b) first += k; else n = k;
   }
   first = __reduce_add_sync(0xFFFFFFFFu, first);
@@ -687,7 +696,8 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   using namespace jf;
   if (!a) return JF_ERR_ARG;
   if ((a->q_dtype != JF_DTYPE_BF16 && a->q_dtype != JF_DTYPE_FP16) || (a->codes != JF_CODES_INT8 && a->codes != JF_CODES_E4M3)) return JF_ERR_ARG;
-  if (a->B < 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->window < 0 || !(a->softcap >= 0.0f) || a->softcap > 3.0e38f) return JF_ERR_ARG;
+  if (a->B < 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->window < 0) return JF_ERR_ARG;
+  if (a->softcap != 0.0f && !(a->softcap >= 1.0e-30f && a->softcap <= 1.0e30f)) return JF_ERR_ARG;
   if (a->B == 0) return JF_OK;
   Plan p;
   if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;

@@ -792,7 +792,7 @@ PyObject* block8_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
     a.max_blocks = tb.width; a.bt_is_i32 = tb.is_i32; a.bt_stride = tb.stride; a.block_table = tb.at;
     a.attn_scale = static_cast<float>(real(p[12]));
     const double cap = real(p[13]);
-    require(cap >= 0.0 && cap < 1e30, name, "softcap must be 0 (none) or positive");
+    require(cap == 0.0 || (cap >= 1.001e-30 && cap <= 0.999e30), name, "softcap must be 0 (none) or between 1e-30 and 1e30");
     a.softcap = static_cast<float>(cap);
     a.window = as_int32(p[15]);
     require(a.window >= 0, name, "window must be positive, or None");
@@ -887,7 +887,7 @@ PyObject* varlen_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
     a.window = as_int32(p[7]);
     require(a.window >= 0, name, "window must be positive, or None");
     const double cap = real(p[8]);
-    require(cap >= 0.0 && cap < 1e30, name, "softcap must be 0 (none) or positive");
+    require(cap == 0.0 || (cap >= 1.001e-30 && cap <= 0.999e30), name, "softcap must be 0 (none) or between 1e-30 and 1e30");
     a.softcap = static_cast<float>(cap);
     if (p[9] != Py_None) {
       const at::Tensor& s = tensor(p[9], name, "alibi_slopes");

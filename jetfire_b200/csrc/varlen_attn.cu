@@ -876,7 +876,7 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   if (!a) return JF_ERR_ARG;
   if (a->dtype != JF_DTYPE_BF16 && a->dtype != JF_DTYPE_FP16) return JF_ERR_ARG;
   if (a->T < 0 || a->n_seqs < 0 || a->H_q <= 0 || a->H_kv <= 0 || a->H_q % a->H_kv != 0 || a->window < 0) return JF_ERR_ARG;
-  if (!(a->softcap >= 0.0f) || a->softcap > 3.0e38f) return JF_ERR_ARG;
+  if (a->softcap != 0.0f && !(a->softcap >= 1.0e-30f && a->softcap <= 1.0e30f)) return JF_ERR_ARG;
   if (a->T > INT32_MAX / 2) return JF_ERR_UNSUPPORTED;
   if (a->T == 0 || a->n_seqs == 0) return JF_OK;
   if (!a->q || !a->k || !a->v || !a->cu_seqlens || !a->out) return JF_ERR_ARG;

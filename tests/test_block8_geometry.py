@@ -49,7 +49,7 @@ def test_every_row_is_written_once_and_every_block_by_one_warp():
             start.append(start[-1] + x)
         lens = [o + x for o, x in zip(old, new)]
         T = start[-1] + rng.choice((0, 0, 5))
-        writes = _append_writes(start, lens, T, rng.choice((1, 4, 16)), 1000)
+        writes = _append_writes(start, lens, T, rng.choice((1, 2, 4, 16)), 1000)
         want = {(s, old[s] + i, start[s] + i) for s in range(n) for i in range(new[s]) if old[s] + i >= 0}
         got = [(s, blk * 16 + r + i, t + i) for s, blk, t, cnt, r in writes for i in range(cnt)]
         assert len(got) == len(set(got)) and set(got) == want
