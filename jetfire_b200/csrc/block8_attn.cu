@@ -34,6 +34,7 @@ constexpr int kStageBytes = 2 * JF_BLOCK_SIZE * JF_HEAD_DIM;
 // The reference of the fp16 weights lies 2^kLift below the maximum it was taken from and may lag the present one by
 // 2^kLag: weights stay below 2^15, and what fp16 flushes to zero is below 2^-33 of the largest (a long row's many small weights add up).
 constexpr float kLift = 9.0f, kLag = 6.0f;
+constexpr float kNone = -3.0e38f;             // the reference of a row that has seen nothing (finite: differences are numbers)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[n][i][k] = 0.0f;
-    m[n][0] = m[n][1] = -INFINITY;
+    m[n][0] = m[n][1] = kNone;
     l[n][0] = l[n][1] = 0.0f;
   }
 
@@ -212,18 +213,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     const int at = begin + warp + i * kWarps;
     return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
   };
-  struct Look { int id; float ks, vs; };
+  struct Look { int id, pos; float ks, vs; };   // pos: 1 more where some of the block's positions are not seen
   auto look_up = [&](int i0) {
-    Look r{-1, 0.0f, 0.0f};
+    Look r{-1, 0, 0.0f, 0.0f};
     if (i0 + lane < mine) {
-      const int64_t id = block_id(P, table_row + position_of(i0 + lane) / JF_BLOCK_SIZE);
+      r.pos = position_of(i0 + lane);
+      const int64_t id = block_id(P, table_row + r.pos / JF_BLOCK_SIZE);
       r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
       if (r.id >= 0) {
         r.ks = P.k_scales[head_row + r.id];
         r.vs = P.v_scales[head_row + r.id];
       }
+      if (!(r.pos + JF_BLOCK_SIZE <= span.len && (r.pos >= span.lo || r.pos + JF_BLOCK_SIZE <= span.prefix))) r.pos += 1;
     }
     return r;
+  };
+  // What was looked up of 64 blocks: id (-1: nothing there), K scale, log2 of the V scale (0 is taken for 2^-100: weightless, but
+  // its positions count), position.
+  int4* entries = reinterpret_cast<int4*>(smem + kWarps * kStages * kStageBytes) + warp * 64;
+  auto note = [&](int i0, const Look& r) {
+    float lg;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(r.vs == 0.0f ? 0x1p-100f : r.vs));
+    entries[(i0 + lane) & 63] = make_int4(r.id, __float_as_int(r.ks), __float_as_int(lg), r.pos);
   };
   // Rings of K and V blocks, kStages each; K runs one block ahead, since the scores of a block are worked out beside the
   // outputs of the one before it.
@@ -249,18 +260,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
 #pragma unroll
     for (int i = 0; i < 4; ++i) cp_async_16(v_ring + slot * 2048 + i * 512 + (v_to ^ (i & 1) << 6), v + i * 512);
   };
-  Look look = look_up(0), next = look;
-  int base = 0;   // first of the blocks that `look` holds; `next` holds the 32 after them
-  auto id_of = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.id : next.id, j & 31); };
-  auto k_scale = [&](int j) { return __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.ks : next.ks, j & 31); };
-  auto log_v_scale = [&](int j) {   // (0 is taken for 2^-100: weightless, but its positions count)
-    const float vs = __shfl_sync(0xFFFFFFFFu, j - base < 32 ? look.vs : next.vs, j & 31);
-    float lg;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(vs == 0.0f ? 0x1p-100f : vs));
-    return lg;
-  };
+  const Look look = look_up(0);
   // (copies arrive in the order of their groups: K of block j is in group j, V of block j in group j + 1)
-  const int id0 = mine > 0 ? id_of(0) : -1, id1 = mine > 1 ? id_of(1) : -1, id2 = mine > 2 ? id_of(2) : -1;
+  const int id0 = __shfl_sync(0xFFFFFFFFu, look.id, 0), id1 = __shfl_sync(0xFFFFFFFFu, look.id, 1), id2 = __shfl_sync(0xFFFFFFFFu, look.id, 2);
   fetch_k(id0, 0);
   cp_async_commit();
   fetch_k(id1, 1);
@@ -327,10 +329,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   }
 
   const float inv_cap = FEAT && P.softcap > 0.0f ? 1.0f / P.softcap : 0.0f;
-  auto whole = [&](int pos) { return pos + JF_BLOCK_SIZE <= span.len && (pos >= span.lo || pos + JF_BLOCK_SIZE <= span.prefix); };
-  // Scores of the warp's i-th block, in units of log2 and with log2 of its V scale on top; -inf where there is nothing to see.
-  auto score = [&](float (&s)[NT][4], int id, float ks, float lvs, int pos, const unsigned char* at) {
-    if (id < 0) {
+  note(0, look);
+  // Scores of a block, in units of log2 and with log2 of its V scale on top; -inf where there is nothing to see.
+  auto score = [&](float (&s)[NT][4], int4 entry, const unsigned char* at) {
+    const float ks = __int_as_float(entry.y), lvs = __int_as_float(entry.z);
+    const int pos = entry.w & ~1;
+    if (entry.x < 0) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           s[n][k] = (s[n][k] - slope[n][k & 1] * static_cast<float>(span.len - 1 - (pos + g + (k >> 1) * 8))) * kLog2e;
       }
     }
-    if (!whole(pos)) {
+    if (entry.w & 1) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int p = pos + g + k * 8;
@@ -406,28 +410,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   cp_async_wait_group<2>();
   __syncwarp();
   float s[NT][4];
-  float lvs = mine > 0 ? log_v_scale(0) : 0.0f;
-  score(s, id0, mine > 0 ? k_scale(0) : 0.0f, lvs, mine > 0 ? position_of(0) : 0, k_ring);
-  int ids[4] = {id0, id1, id2, -1};   // of blocks i .. i + 3
-  int slot = 0;                       // i % kStages
+  int4 now = entries[0];   // block i
+  score(s, now, k_ring);
+  int slot = 0;            // i % kStages
   for (int i = 0; i < mine; ++i) {
-    if ((i & 31) == 0) {
-      if (i > 0) { look = next; base = i; }
-      next = look_up(i + 32);
-    }
-    __syncwarp();              // the slots that are filled now were read in the step before
+    if ((i & 31) == 0) note(i + 32, look_up(i + 32));
+    __syncwarp();          // the slots that are filled now were read in the step before
     const int slot1 = slot + 1 == kStages ? 0 : slot + 1, slot2 = slot1 + 1 == kStages ? 0 : slot1 + 1;
-    ids[3] = i + 3 < mine ? id_of(i + 3) : -1;
-    fetch_k(ids[3], slot);     // (K of block i was read in the step before)
-    fetch_v(ids[2], slot2);
+    fetch_k(entries[(i + 3) & 63].x, slot);   // (K of block i was read in the step before)
+    fetch_v(entries[(i + 2) & 63].x, slot2);
     cp_async_commit();
     cp_async_wait_group<2>();
     __syncwarp();
-    const int id = ids[0], pos = position_of(i);
-    const float ivs = ex2(-lvs);
+    const int4 then = entries[(i + 1) & 63];
+    const float ivs = ex2(-__int_as_float(now.z));
     float ahead[NT][4];
-    const float lvs1 = log_v_scale(i + 1);
-    score(ahead, ids[1], k_scale(i + 1), lvs1, position_of(i + 1), k_ring + slot1 * 2048);
+    score(ahead, then, k_ring + slot1 * 2048);
     const unsigned char* at = v_ring + slot * 2048;
     bool above = false;
 #pragma unroll
@@ -446,7 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
           const float to = fmaxf(m[n][c], top - kLift);
-          const float f = to == m[n][c] ? 1.0f : ex2(m[n][c] - to);
+          const float f = ex2(m[n][c] - to);
           m[n][c] = to;
           l[n][c] *= f;
 #pragma unroll
@@ -459,22 +457,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     uint32_t pb[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
-      const float p0 = ex2(s[n][0] - m0), p1 = ex2(s[n][1] - m1), p2 = ex2(s[n][2] - m0), p3 = ex2(s[n][3] - m1);
+      const float p0 = ex2(s[n][0] - m[n][0]), p1 = ex2(s[n][1] - m[n][1]), p2 = ex2(s[n][2] - m[n][0]), p3 = ex2(s[n][3] - m[n][1]);
       l[n][0] = fmaf(p0 + p2, ivs, l[n][0]);
       l[n][1] = fmaf(p1 + p3, ivs, l[n][1]);
       const __half2 a = __floats2half2_rn(p0, p1), c = __floats2half2_rn(p2, p3);
       pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&a));
       pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&c));
     }
-    if (id >= 0) {
+    if (now.x >= 0) {
       uint32_t r[4][4];
 #pragma unroll
       for (int i2 = 0; i2 < 4; ++i2) {
         const uint4 x = *reinterpret_cast<const uint4*>(at + v_at + (i2 & 1) * JF_HEAD_DIM + (i2 >> 1) * 1024);
         r[i2][0] = bias<CODES>(x.x); r[i2][1] = bias<CODES>(x.y); r[i2][2] = bias<CODES>(x.z); r[i2][3] = bias<CODES>(x.w);
-        if (CODES == JF_CODES_E4M3 && !whole(pos)) {   // a weight of 0 does not make up for a row of NaN codes
-          const int p = pos + 2 * t + (i2 & 1) + (i2 >> 1) * 8;
+        if (CODES == JF_CODES_E4M3 && now.w & 1) {   // a weight of 0 does not make up for a row of NaN codes
+          const int p = (now.w & ~1) + 2 * t + (i2 & 1) + (i2 >> 1) * 8;
           if (p >= span.len || (p < span.lo && p >= span.prefix)) r[i2][0] = r[i2][1] = r[i2][2] = r[i2][3] = 0;
         }
       }
@@ -488,10 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + hl], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
     }
-    ids[0] = ids[1];
-    ids[1] = ids[2];
-    ids[2] = ids[3];
-    lvs = lvs1;
+    now = then;
     slot = slot1;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -521,10 +515,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     float f[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float top = -INFINITY;
+      float top = kNone;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][n * 8 + 2 * t + c]);
-      f[c] = m[n][c] == -INFINITY ? 0.0f : ex2(m[n][c] - top);
+      f[c] = ex2(m[n][c] - top);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)   // tile j: channels 16g + 2j (registers 0, 1) and 16g + 2j + 1
@@ -534,12 +528,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
             make_float2(o[n][j][c] * f[c], o[n][j][2 + c] * f[c]);
   }
   if (threadIdx.x < 8 * NT) {
-    float top = -INFINITY, z = 0.0f;
+    float top = kNone, z = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][threadIdx.x]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
-      if (sm_m[w][threadIdx.x] != -INFINITY) z = fmaf(sm_l[w][threadIdx.x], ex2(sm_m[w][threadIdx.x] - top), z);
+      z = fmaf(sm_l[w][threadIdx.x], ex2(sm_m[w][threadIdx.x] - top), z);
     sm_ml[threadIdx.x] = make_float2(top, z);
   }
   __syncthreads();
@@ -554,7 +548,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     }
     if (cut.n == 1) {
       const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
-      const bool none = ml.x == -INFINITY;
+      const bool none = ml.y == 0.0f;   // (nothing seen: any position that is leaves a weight, or a NaN)
       const float r[4] = {sum.x, sum.y, sum.z, sum.w};
       uint32_t w[4];
 #pragma unroll
@@ -592,7 +586,7 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
   if (n == 1) return;
   const int kvh = h / P.G, in_group = h % P.G, y = kvh * P.groups + in_group / width;
   const int64_t row0 = (static_cast<int64_t>(first) * grid_y + y) * width + in_group % width, step = static_cast<int64_t>(grid_y) * width;
-  float top = -INFINITY;
+  float top = kNone;
   for (int i = threadIdx.x; i < n; i += WARPS * 32) top = fmaxf(top, P.part_ml[(row0 + i * step) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -606,7 +600,7 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
     const int m = min(WARPS * 32, n - i0);
     if (threadIdx.x < m) {
       const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + (row0 + (i0 + threadIdx.x) * step) * 2);
-      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+      const float f = ex2(ml.x - top);
       sm_w[threadIdx.x] = f;
       z = fmaf(ml.y, f, z);
     }
@@ -641,8 +635,8 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
       z += sm_z[k];
     }
     const int64_t row = static_cast<int64_t>(b) * P.H_q + h;
-    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + blockIdx.z * 32 * VEC + threadIdx.x] = Elem<DT>::from_f32(top == -INFINITY ? 0.0f : x / z);
-    if (threadIdx.x == 0 && blockIdx.z == 0 && P.lse) P.lse[row] = top == -INFINITY ? -INFINITY : (top + __log2f(z)) / kLog2e;
+    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + blockIdx.z * 32 * VEC + threadIdx.x] = Elem<DT>::from_f32(z == 0.0f ? 0.0f : x / z);
+    if (threadIdx.x == 0 && blockIdx.z == 0 && P.lse) P.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) / kLog2e;
   }
 }
 
@@ -673,7 +667,7 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
 
 template <int CODES, int DT, int NT, bool FEAT>
 jf_status_t launch_attn(const AttnParams& P, dim3 grid, cudaStream_t s) {
-  constexpr int smem = std::max(kWarps * kStages * kStageBytes, kWarps * 8 * NT * JF_HEAD_DIM * 4);
+  constexpr int smem = std::max(kWarps * (kStages * kStageBytes + 64 * 16), kWarps * 8 * NT * JF_HEAD_DIM * 4);
   auto* kernel = block8_attn_kernel<CODES, DT, NT, FEAT>;
   JF_ENSURE_SMEM(kernel, smem);
   JF_CUDA_TRY(launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, P));

@@ -255,6 +255,21 @@ def test_decode_queries_of_any_size(q_scale):
 
 
 @pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("lens", [[40], [3000]])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_decode_queries_that_are_no_numbers(codes, lens, value):
+    """One element of one head: that head's row is NaN, the others are as ever."""
+    c = Decode(lens, 8, 2, CODES[codes], torch.bfloat16, 35)
+    c.q[0, 3, 77] = value
+    out, lse = c.run()
+    assert torch.isnan(out[0, 3]).all() and torch.isnan(lse[0, 3])
+    c.q[0, 3, 77] = 0.0
+    want, want_lse = c.expected()
+    out[0, 3], lse[0, 3] = want[0, 3].to(out.dtype).cuda(), want_lse[0, 3].float().cuda()
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("codes", CODES)
 def test_decode_block_scales_far_apart(codes):
     c = Decode([900, 64], 8, 2, CODES[codes], torch.bfloat16, 27, v_spread=6.0)
     c.check(*c.run())
