@@ -3,8 +3,8 @@
 //   out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(f(scale q_i.k_j) - slope |i - j|) where i sees j
 //
 // One pass over the keys per row with a running reference m_i and sum l_i; nothing of size rows x keys leaves the chip.
-// A work item is 256 query rows of one head of one sequence: two tiles of 128 rows that share every tile of 128 keys
-// brought into shared memory.  S = Q K^T (fp32) stands in tensor memory, 128 columns per row tile; a thread owns a row: it
+// A work item is two tiles of 128 query rows that share every tile of 128 keys brought into shared memory: the same rows of two
+// query heads of one KV head, or, where a KV head has a single query head, 256 rows of it.  S = Q K^T (fp32) stands in tensor memory, 128 columns per row tile; a thread owns a row: it
 // reads its 128 scores, turns them into weights and writes them back, 16 bits each, over the scores, where they
 // are the first operand of O += P V.  While one row tile's weights are computed the tensor core works on the other's products.
 //
@@ -32,7 +32,6 @@ namespace jf {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128;               // of a tile
-constexpr int kPairRows = 2 * kRows;
 constexpr int kKvStages = 5;
 constexpr int kTileBytes = kKeys * JF_HEAD_DIM * 2;   // 32 KB: two slabs of 64 channels, 128-byte swizzle
 constexpr int kSlabBytes = kTileBytes / 2;
@@ -55,11 +54,15 @@ struct Params {
   int32_t* status;
   int64_t v_stride_t, v_stride_h;
   int32_t T, n_seqs, H_q, H_kv, window;
+  int32_t span, apart;    // rows of a sequence that an item covers; rows between its two tiles (0: same rows, two heads)
+  int32_t G, units;       // query heads of a KV head; items per span of rows
   float scale, softcap;
   bool causal;
 };
 
-struct Item { int row0, len, pair, head, prefix; };   // row0: first row of the sequence; len < 0: no more items
+// row0: first row of the sequence (len < 0: no more items); q0: first row of the item in it; head: of its first tile; two: there is
+// a second tile
+struct Item { int row0, len, q0, head, prefix, two; };
 
 struct Shared {
   uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], half_done[2], o_full[2], item_full[kItems], item_empty[kItems],
@@ -157,8 +160,9 @@ struct Tiles {
   __device__ __forceinline__ bool masked(int t) const { return t >= all_p && (t < all_lo || t >= all_hi); }
   __device__ __forceinline__ bool partly(int t) const { return uses(t) && masked(t); }
 };
-__device__ __forceinline__ Tiles tiles_of(const Params& P, const Item& it, int q0) {
-  if (q0 >= it.len) return Tiles{0, 0, 0, 0, 0, 0};
+__device__ __forceinline__ Tiles tiles_of(const Params& P, const Item& it, int t) {
+  if (t == 1 && !it.two) return Tiles{0, 0, 0, 0, 0, 0};
+  const int q0 = it.q0 + t * P.apart;
   const int r1 = min(q0 + kRows, it.len) - 1;
   return Tiles{(it.prefix + kKeys - 1) / kKeys,
                first_key(P, q0) / kKeys,
@@ -171,7 +175,7 @@ __device__ __forceinline__ Tiles tiles_of(const Params& P, const Item& it, int q
 // of its row tiles.  (From the row's own position backwards: where nearer keys weigh more, references settle early.)
 struct Keys { int a, first, count; };
 __device__ __forceinline__ Keys keys_of(const Params& P, const Item& it) {
-  const int r0 = it.pair * kPairRows, r1 = min(r0 + kPairRows, it.len) - 1;
+  const int r0 = it.q0, r1 = min(r0 + P.span, it.len) - 1;
   const int np = (it.prefix + kKeys - 1) / kKeys, from = first_key(P, r0) / kKeys, to = (end_key(P, it, r1) + kKeys - 1) / kKeys;
   Keys k;
   k.a = min(np, from);
@@ -197,17 +201,18 @@ template <int DT> __device__ __forceinline__ bool no_number(uint32_t half) {
 
 // ---- the roles ------------------------------------------------------------------------------
 
-// Work items of this block: level by level (the l-th 256 rows of every sequence that has them, from the last), heads
+// Work items of this block: level by level (the l-th span of rows of every sequence that has it, from the last), heads
 // fastest, so that long rows come first and heads that share keys run at the same time; every gridDim.x-th is this block's.
 __device__ __forceinline__ bool schedule(const Params& P, Shared& S) {
   const int lane = threadIdx.x & 31;
   int slot = 0, uses_of_slot = 0;
-  auto emit = [&](int row0, int len, int pair, int head, int prefix) {
+  auto emit = [&](int row0, int len, int q0, int unit, int prefix) {
     bool ok = true;
     if (uses_of_slot > 0) ok = wait_warp(&S.item_empty[slot], (uses_of_slot - 1) & 1);
     if (!ok) return false;
     if (lane == 0) {
-      S.item[slot] = Item{row0, len, pair, head, prefix};
+      const int pairs = (P.G + 1) / 2, first = P.apart ? unit : unit / pairs * P.G + unit % pairs * 2;
+      S.item[slot] = Item{row0, len, q0, first, prefix, P.apart ? q0 + P.apart < len : unit % pairs * 2 + 1 < P.G};
       S.bad[slot] = 0;
       mbar_arrive(&S.item_full[slot]);
     }
@@ -228,16 +233,16 @@ __device__ __forceinline__ bool schedule(const Params& P, Shared& S) {
     most = max(most, static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(len))));
   }
   int64_t want = blockIdx.x, before = 0;
-  for (int level = (most + kPairRows - 1) / kPairRows - 1; level >= 0; --level)
+  for (int level = (most + P.span - 1) / P.span - 1; level >= 0; --level)
     for (int c = 0; c < P.n_seqs; c += 32) {
       if (P.n_seqs > 32) bounds(c + lane, row0, len);
-      const unsigned has = __ballot_sync(0xFFFFFFFFu, len > level * kPairRows);
-      const int64_t n = static_cast<int64_t>(__popc(has)) * P.H_q;
+      const unsigned has = __ballot_sync(0xFFFFFFFFu, len > level * P.span);
+      const int64_t n = static_cast<int64_t>(__popc(has)) * P.units;
       while (want < before + n) {
-        const int at = static_cast<int>(want - before), src = __fns(has, 0, at / P.H_q + 1);
+        const int at = static_cast<int>(want - before), src = __fns(has, 0, at / P.units + 1);
         const int r = __shfl_sync(0xFFFFFFFFu, row0, src), l = __shfl_sync(0xFFFFFFFFu, len, src);
         const int prefix = P.prefix ? min(max(P.prefix[c + src], 0), l) : 0;
-        if (!emit(r, l, level, at % P.H_q, prefix)) return false;
+        if (!emit(r, l, level * P.span, at % P.units, prefix)) return false;
         want += gridDim.x;
       }
       before += n;
@@ -271,19 +276,17 @@ __device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem
   ItemReader items;
   Item it;
   Ring ring;
-  const int group = P.H_q / P.H_kv;
   for (int n = 0;; ++n) {
     if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
-    const int q0 = it.pair * kPairRows, kvh = it.head / group;
-    const bool two = q0 + kRows < it.len;
+    const int kvh = it.head / P.G, tiles = it.two ? 2 : 1;
     if (n > 0 && !wait_warp(&S.q_empty, (n - 1) & 1)) return false;
     if (elect_one()) {
-      mbar_expect_tx(&S.q_full, two ? 2 * kTileBytes : kTileBytes);
-      for (int t = 0; t < (two ? 2 : 1); ++t)
+      mbar_expect_tx(&S.q_full, tiles * kTileBytes);
+      for (int t = 0; t < tiles; ++t)
         for (int slab = 0; slab < 2; ++slab)
-          tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head, it.row0 + q0 + t * kRows, &S.q_full);
+          tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head + (P.apart ? 0 : t), it.row0 + it.q0 + t * P.apart, &S.q_full);
     }
     __syncwarp();
     for (int i = 0; i < keys.count; ++i) {
@@ -314,8 +317,7 @@ template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shar
     if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
-    const int q0 = it.pair * kPairRows;
-    const Tiles tiles[2] = {tiles_of(P, it, q0), tiles_of(P, it, q0 + kRows)};
+    const Tiles tiles[2] = {tiles_of(P, it, 0), tiles_of(P, it, 1)};
     int last[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -406,7 +408,7 @@ template <int DT> __device__ __forceinline__ bool clean_values(const Params& P, 
     if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
-    const Tiles upper = tiles_of(P, it, it.pair * kPairRows), lower = tiles_of(P, it, it.pair * kPairRows + kRows);
+    const Tiles upper = tiles_of(P, it, 0), lower = tiles_of(P, it, 1);
     for (int i = 0; i < keys.count; ++i) {
       // every buffer is waited for and passed on, so that none is filled twice in between
       if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
@@ -598,13 +600,13 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float f) {
 // Adds to a row of the result what the cleaned tiles' infinities and NaN do to it.
 template <int DT> __device__ __noinline__ void give_back(const Params& P, const Item it, int row, uint16_t* out) {
   const Keys keys = keys_of(P, it);
-  const Tiles upper = tiles_of(P, it, it.pair * kPairRows), lower = tiles_of(P, it, it.pair * kPairRows + kRows);
+  const Tiles upper = tiles_of(P, it, 0), lower = tiles_of(P, it, 1);
   for (int i = 0; i < keys.count; ++i) {
     const int tile = tile_of(keys, i);
     if (!upper.partly(tile) && !lower.partly(tile)) continue;
     for (int j = tile * kKeys; j < min((tile + 1) * kKeys, it.len); ++j) {
       if (!sees(P, it, row, j)) continue;
-      const uint16_t* v = P.v + (static_cast<int64_t>(it.row0) + j) * P.v_stride_t + it.head / (P.H_q / P.H_kv) * P.v_stride_h;
+      const uint16_t* v = P.v + (static_cast<int64_t>(it.row0) + j) * P.v_stride_t + it.head / P.G * P.v_stride_h;
       for (int k = 0; k < JF_HEAD_DIM; ++k)
         if (no_number<DT>(v[k])) out[k] = Elem<DT>::from_f32(Elem<DT>::to_f32(out[k]) + Elem<DT>::to_f32(v[k]));
     }
@@ -638,9 +640,9 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
     if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
-    const int q0 = it.pair * kPairRows + t * kRows, row = q0 + r;
-    const Tiles tiles = tiles_of(P, it, q0);
-    const float slope2 = FEAT && P.slopes ? P.slopes[it.head] * kLog2e : 0.0f;
+    const int q0 = it.q0 + t * P.apart, row = q0 + r, head = min(it.head + (P.apart ? 0 : t), P.H_q - 1);
+    const Tiles tiles = tiles_of(P, it, t);
+    const float slope2 = FEAT && P.slopes ? P.slopes[head] * kLog2e : 0.0f;
     float m = -INFINITY, l = 0.0f;
     bool have = false;
     for (int i = 0; i < keys.count; ++i) {
@@ -738,7 +740,7 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
     if (have) {
       if (!wait_warp(&S.o_full[t], o_count++ & 1)) return false;
       tc_fence_after();
-      const int64_t at = (static_cast<int64_t>(it.row0) + row) * P.H_q + it.head;
+      const int64_t at = (static_cast<int64_t>(it.row0) + row) * P.H_q + head;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -903,12 +905,18 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   P.T = static_cast<int32_t>(a->T);
   P.n_seqs = a->n_seqs;
   P.H_q = a->H_q;
+  // Two heads with the same keys rather than 256 rows of one: the two tiles of an item then have the same keys to go through, and a
+  // sequence that ends within 128 rows of its last item leaves neither without work.
+  P.G = a->H_q / a->H_kv;
+  P.apart = P.G > 1 ? 0 : kRows;
+  P.span = kRows + P.apart;
+  P.units = P.G > 1 ? a->H_kv * ((P.G + 1) / 2) : a->H_q;
   P.H_kv = a->H_kv;
   P.window = a->window;
   P.scale = a->attn_scale;
   P.softcap = a->softcap;
   P.causal = a->causal != 0;
-  const int64_t most = (a->T / kPairRows + std::min<int64_t>(a->n_seqs, a->T)) * a->H_q;   // work items
+  const int64_t most = (a->T / P.span + std::min<int64_t>(a->n_seqs, a->T)) * P.units;   // work items
   const int grid = static_cast<int>(std::min<int64_t>(num_sms(), most));
   // (the plain form takes the maximum before it scales, so it needs a positive scale)
   const int feat = a->softcap > 0.0f ? 2 : a->alibi_slopes || !(a->attn_scale > 0.0f) ? 1 : 0;
