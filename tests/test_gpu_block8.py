@@ -401,3 +401,32 @@ def test_cache_larger_than_32_bits():
     assert torch.equal(kk[:, :, :8], c.k[:, :, :8]) and torch.equal(ss, c.ks)
     c.table, c.blocks = torch.tensor([[0, 1, 2]]), 3
     c.check(*ops.block8_decode_attn(c.q.cuda(), kd, ks, vd, vs, table, lens, 48, 4, 2, 16, c.scale))
+
+
+def test_two_calls_at_once_on_two_streams():
+    cases = [Decode([3000, 17, 900], 8, 2, torch.int8, torch.bfloat16, 36), Decode([20000], 16, 1, torch.float8_e4m3fn, torch.float16, 37, softcap=5.0)]
+    from jetfire_b200 import ops
+    args, options = [c.device() for c in cases], [c.options() for c in cases]
+    want = [ops.block8_decode_attn(*a, **o) for a, o in zip(args, options)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.block8_decode_attn(*args[i], **options[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+        cases[i].check(*want[i])
+
+
+@pytest.mark.parametrize("options", [dict(softcap=1e-20), dict(softcap=1e-4), dict(softcap=1e20), dict(softcap=3.0, alibi=True)])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0])
+def test_decode_scales_and_caps_of_any_size(options, scale):
+    for codes in CODES.values():
+        c = Decode([500, 30], 8, 2, codes, torch.bfloat16, 38, **options)
+        c.scale = scale
+        c.q = (c.q.float() * 0.5).to(c.q.dtype)
+        c.check(*c.run())

@@ -108,9 +108,17 @@ def test_strided_inputs(layout):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("softcap", [0.0, 3.0, 0.01])
+@pytest.mark.parametrize("alibi", [False, True])
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
-def test_scales(scale):
-    c = Case([400], 2, 2, torch.float16, 45, scale=scale, spread=0.5)
+def test_scales(scale, softcap, alibi):
+    c = Case([400], 2, 1, torch.float16, 45, scale=scale, spread=0.5, softcap=softcap, alibi=alibi)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("softcap", [1e-20, 1e-4, 1e20])
+def test_caps_of_any_size(softcap):
+    c = Case([300], 2, 1, torch.bfloat16, 52, softcap=softcap)
     c.check(*c.run())
 
 
@@ -183,3 +191,23 @@ def test_captured_and_replayed_on_another_stream_with_the_same_bits():
             assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     ops.decode_status_of_copy(record.cpu())
     c.check(out, lse)
+
+
+def test_two_calls_at_once_on_two_streams():
+    from jetfire_b200 import ops
+    cases = [Case([900, 333], 8, 2, torch.bfloat16, 53), Case([1500], 4, 1, torch.bfloat16, 54, window=200, softcap=10.0)]
+    args = [c.device() for c in cases]
+    kw = [dict(), dict(window=200, softcap=10.0)]
+    want = [ops.varlen_prefill_attn(*a, **k) for a, k in zip(args, kw)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.varlen_prefill_attn(*args[i], **kw[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+        cases[i].check(*want[i])
