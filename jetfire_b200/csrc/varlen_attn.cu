@@ -19,8 +19,14 @@
 // would not be: warp 11 looks at every V tile that has masked entries and zeroes infinities and NaN in it; rows that do see
 // them get them back at the end (never, with finite inputs).
 //
-// Bound: the exponentials -- 128 x 128 of them a tile at 16 a cycle and multiprocessor are 1024 cycles, the two products of a tile
-// 512.
+// The weights that meet V are rounded to the operands' type (bf16: 2^-9 of themselves at most, fp16: 2^-12); their sum, the scores and
+// the output are fp32.
+//
+// Bound: per 128 x 128 scores the two products take 1024 cycles of the tensor core, the exponentials 1024 of the special function units (16
+// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 926 to 981 us = 1.12 to 1.19 PFLOP/s, 0.69 to 0.73 of what cuBLAS reaches.  A
+// step of both row tiles is 3500 cycles; with the weights left out it is 2950 (shared-memory reads of the operands and the hand-overs),
+// and a row tile by itself goes through 1750 from its scores to its weights and waits 1020 for the next ones.
+
 #include <cuda.h>
 
 #include <algorithm>
