@@ -59,9 +59,20 @@ def test_every_row_is_written_once_and_every_block_by_one_warp():
             assert r == 0 or (t == start[s] and old[s] % 16 == r)     # rows in front of it were there before the call
 
 
-def _pieces(counts, target, min_piece):
-    piece = max(min_piece, -(-sum(counts) // target))
-    return piece, [max(1, -(-c // piece)) for c in counts]
+def _pieces(counts, target, min_piece, grid, one_wave):
+    cut = lambda piece: [max(1, -(-c // piece)) for c in counts]
+    hi = max(min_piece, -(-sum(counts) // target))
+    if one_wave:
+        lo = max(min_piece, -(-sum(counts) // grid))
+        if (hi - lo) * 8 < hi:
+            return hi, cut(hi)
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if sum(cut(mid)) <= grid:
+                hi = mid
+            else:
+                lo = mid + 1
+    return hi, cut(hi)
 
 
 def test_pieces_fit_the_grid_and_cover_every_block():
@@ -72,10 +83,11 @@ def test_pieces_fit_the_grid_and_cover_every_block():
         counts = [rng.choice((0, most, rng.randint(0, most))) for _ in range(B)]
         wave = rng.choice((1, 18, 37, 74, 296))
         target = max(1, wave - B if 2 * B <= wave else 3 * wave)
-        min_piece = 8
-        piece, n = _pieces(counts, target, min_piece)
+        min_piece = rng.choice((8, 20, 64))
         grid = min(target + B, -(-most // min_piece) * B)
+        piece, n = _pieces(counts, target, min_piece, grid, 1 < B <= 32 and 2 * B <= grid and rng.random() < 0.7)
         assert sum(n) <= grid
         for c, k in zip(counts, n):
-            covered = [min(i * piece + piece, c) - i * piece for i in range(k)]
-            assert sum(max(0, x) for x in covered) == c and (c == 0 or min(covered) > 0)
+            each = -(-c // k)                                     # a sequence's pieces are of one length
+            covered = [min(i * each + each, c) - i * each for i in range(k)]
+            assert each <= piece and sum(max(0, x) for x in covered) == c
