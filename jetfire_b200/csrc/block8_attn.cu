@@ -18,10 +18,11 @@
 //
 // Work: the blocks of every sequence are cut into pieces of one length for the whole batch, chosen on the device from the lengths
 // so that the pieces of a KV head fill about one wave; the pieces' partial results meet in a second kernel.  A
-// sequence of one piece is written by the first kernel itself.
+// sequence of one piece is written by the first kernel itself.  Short sequences are cut into as many pieces as a cluster has blocks,
+// whose results meet in its shared memory.
 //
 // Bound: memory, 256 bytes per (position, KV head).  Four sequences of 65536 positions, 64 / 8 heads, int8: 101 us = 5.3 TB/s (copies of the
-// same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 7 us + 1.5 for the join.
+// same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 6 us.
 #include "jf_common.cuh"
 
 #include <algorithm>
@@ -51,6 +52,7 @@ struct AttnParams {
   int64_t num_blocks, bt_stride;
   int32_t B, H_q, H_kv, G, groups, max_S, max_blocks, window, target, min_piece, pieces;
   float scale, softcap;
+  int32_t cluster;              // blocks that share a sequence, 1 where pieces are looked for
   bool bt_i32, one_wave;
 };
 
@@ -177,7 +179,27 @@ __device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap)
   }
 }
 
-template <int CODES, int DT, int NT, bool FEAT>
+// The blocks of a cluster share a sequence's pieces: no piece has to be looked for, and the results meet in shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {   // the same place in another block's shared memory
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 load4_from(uint32_t at) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ float2 load2_from(uint32_t at) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+  return x;
+}
+
+template <int CODES, int DT, int NT, bool FEAT, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kernel(const __grid_constant__ AttnParams P) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float sm_m[kWarps][8 * NT], sm_l[kWarps][8 * NT];
@@ -187,10 +209,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   const int first_head = kvh * P.G + grp * 8 * NT, heads = min(8 * NT, P.G - grp * 8 * NT);
   pdl_wait();
   pdl_trigger();
-  const Cut cut = find_piece(P, blockIdx.x);
-  if (cut.b < 0) return;
+  Cut cut{0, static_cast<int>(blockIdx.x) / P.cluster, static_cast<int>(blockIdx.x) % P.cluster, P.cluster, 0, 0};
+  if (CLUSTER) {
+    cut.length = P.seq_lens[cut.b];
+    cut.prefix = prefix_of(P, cut.b);
+  } else {
+    cut = find_piece(P, blockIdx.x);
+    if (cut.b < 0) return;
+  }
   const int b = cut.b;
   const Span span = span_of(P, cut.length, cut.prefix);
+  if (CLUSTER) cut.piece = (span.count + cut.n - 1) / cut.n;
   const int begin = cut.index * cut.piece, end = min(begin + cut.piece, span.count);
   // q of the lane's head (column g of each tile), and the slopes of the heads of its score columns 2t and 2t + 1
   uint4 q_raw[NT][4];
@@ -554,9 +583,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     sm_ml[threadIdx.x] = make_float2(top, z);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * (JF_HEAD_DIM / 4); i += kWarps * 32) {
-    const int head = i / (JF_HEAD_DIM / 4), d = i % (JF_HEAD_DIM / 4) * 4;
-    const float2 ml = sm_ml[head];
+  auto write = [&](int head, int d, float4 sum, float2 ml) {
+    const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
+    const bool none = ml.y == 0.0f;   // (nothing seen: any position that is leaves a weight, or a NaN)
+    const float r[4] = {sum.x, sum.y, sum.z, sum.w};
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(none ? 0.0f : r[k] / ml.y);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + row * JF_HEAD_DIM + d) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    if (d == 0 && P.lse) P.lse[row] = none ? -INFINITY : (ml.x + __log2f(ml.y)) / kLog2e;
+  };
+  constexpr int kQuads = JF_HEAD_DIM / 4;
+  for (int i = threadIdx.x; i < heads * kQuads; i += kWarps * 32) {
+    const int head = i / kQuads, d = i % kQuads * 4;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -564,19 +603,42 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
     }
     if (cut.n == 1) {
-      const int64_t row = static_cast<int64_t>(b) * P.H_q + first_head + head;
-      const bool none = ml.y == 0.0f;   // (nothing seen: any position that is leaves a weight, or a NaN)
-      const float r[4] = {sum.x, sum.y, sum.z, sum.w};
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(none ? 0.0f : r[k] / ml.y);
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + row * JF_HEAD_DIM + d) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-      if (d == 0 && P.lse) P.lse[row] = none ? -INFINITY : (ml.x + __log2f(ml.y)) / kLog2e;
+      write(head, d, sum, sm_ml[head]);
+    } else if (CLUSTER) {
+      *reinterpret_cast<float4*>(so + head * JF_HEAD_DIM + d) = sum;   // (no other thread reads these four)
     } else {
       const int64_t row = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (8 * NT) + head;
       *reinterpret_cast<float4*>(P.part_o + row * JF_HEAD_DIM + d) = sum;
-      if (d == 0) *reinterpret_cast<float2*>(P.part_ml + row * 2) = ml;
+      if (d == 0) *reinterpret_cast<float2*>(P.part_ml + row * 2) = sm_ml[head];
     }
+  }
+  if (CLUSTER && cut.n > 1) {
+    cluster_sync();
+    // every block joins its share of the (head, four channels)
+    const int share = (heads * kQuads + cut.n - 1) / cut.n;
+    for (int i = cut.index * share + threadIdx.x; i < min((cut.index + 1) * share, heads * kQuads); i += kWarps * 32) {
+      const int head = i / kQuads, d = i % kQuads * 4;
+      float2 ml[8];
+      float4 x[8];
+      float top = kNone, z = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < cut.n) {
+          ml[r] = load2_from(of_rank(&sm_ml[head], r));
+          x[r] = load4_from(of_rank(so + head * JF_HEAD_DIM + d, r));
+          top = fmaxf(top, ml[r].x);
+        }
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < cut.n) {
+          const float f = ex2(ml[r].x - top);
+          z = fmaf(ml[r].y, f, z);
+          sum = make_float4(fmaf(x[r].x, f, sum.x), fmaf(x[r].y, f, sum.y), fmaf(x[r].z, f, sum.z), fmaf(x[r].w, f, sum.w));
+        }
+      write(head, d, sum, make_float2(top, z));
+    }
+    cluster_sync();   // nobody leaves while its shared memory is read
   }
 }
 
@@ -682,12 +744,48 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
   return true;
 }
 
+// Blocks of a cluster, 0 for pieces and a join.  As many as leave every warp a block, up to eight and while all of them are resident at
+// once, where that is at most kRounds blocks a warp; kFewRounds where pieces could spread over eight times as many multiprocessors.
+// One sequence of 500 positions, 8 KV heads: 7.7 -> 6.0 us, of 4000: 11.7 -> 9.1; 64 of 300: 19.6 -> 17.4; 8 of 2000: 14.9 -> 12.4.  With 2
+// columns, 4000 positions take 9.2 us so and 8.6 in pieces.
+constexpr int kRounds = 6, kFewRounds = 2;
+int cluster_size(const Plan& p, int B, int H_kv, int64_t longest) {
+  const int64_t blocks = (longest + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, columns = static_cast<int64_t>(H_kv) * p.groups * B;
+  const int64_t places = static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1);
+  int c = 1;
+  while (c < 8 && c * kWarps < blocks && 2 * c * columns <= places) c *= 2;
+  const int rounds = 8 * c * columns <= places ? kFewRounds : kRounds;
+  return blocks <= static_cast<int64_t>(c) * kWarps * rounds ? c : 0;
+}
+
 template <int CODES, int DT, int NT, bool FEAT>
 jf_status_t launch_attn(const AttnParams& P, dim3 grid, cudaStream_t s) {
   constexpr int smem = std::max(kWarps * (kStages * kStageBytes + 64 * 16), kWarps * 8 * NT * JF_HEAD_DIM * 4);
-  auto* kernel = block8_attn_kernel<CODES, DT, NT, FEAT>;
+  if (P.cluster == 0) {
+    AttnParams Q = P;
+    Q.cluster = 1;
+    auto* kernel = block8_attn_kernel<CODES, DT, NT, FEAT, false>;
+    JF_ENSURE_SMEM(kernel, smem);
+    JF_CUDA_TRY(launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, Q));
+    return JF_OK;
+  }
+  auto* kernel = block8_attn_kernel<CODES, DT, NT, FEAT, true>;
   JF_ENSURE_SMEM(kernel, smem);
-  JF_CUDA_TRY(launch_pdl(kernel, grid, dim3(kWarps * 32), smem, s, P));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(P.cluster * P.B, grid.y);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = P.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  JF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P));
   return JF_OK;
 }
 template <int CODES, int DT> jf_status_t launch_attn(const AttnParams& P, int nt, bool feat, dim3 grid, cudaStream_t s) {
@@ -742,6 +840,7 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   P.one_wave = a->B > 1 && a->B <= 32 && 2 * a->B <= p.pieces && longest / JF_BLOCK_SIZE * a->B > 32ll * p.target;
   P.scale = a->attn_scale; P.softcap = a->softcap;
   P.bt_i32 = a->bt_is_i32 != 0;
+  P.cluster = cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
   const bool feat = a->softcap > 0.0f || a->alibi_slopes;
   const auto s = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.pieces, a->H_kv * p.groups);
@@ -752,7 +851,7 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   else
     st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_FP16>(P, p.nt, feat, grid, s)
                                    : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
-  if (st != JF_OK || p.pieces == a->B) return st;   // one piece per sequence: nothing to join
+  if (st != JF_OK || P.cluster > 0 || p.pieces == a->B) return st;   // (one piece per sequence: nothing to join)
   const int width = 8 * p.nt, grid_y = a->H_kv * p.groups;
   if (p.pieces / a->B >= kManyPieces)
     JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16

@@ -91,3 +91,27 @@ def test_pieces_fit_the_grid_and_cover_every_block():
             each = -(-c // k)                                     # a sequence's pieces are of one length
             covered = [min(i * each + each, c) - i * each for i in range(k)]
             assert each <= piece and sum(max(0, x) for x in covered) == c
+
+
+def _cluster_size(columns, places, blocks):
+    c = 1
+    while c < 8 and c * 8 < blocks and 2 * c * columns <= places:
+        c *= 2
+    return c if blocks <= c * 8 * (2 if 8 * c * columns <= places else 6) else 0
+
+
+def test_the_blocks_of_a_cluster_share_what_there_is():
+    rng = random.Random(8)
+    for _ in range(4000):
+        columns, places = rng.choice((1, 2, 8, 64, 512)) * rng.randint(1, 70), rng.choice((148, 296))
+        most = rng.choice((1, 8, 9, 65, 250, 385, 8192))
+        c = _cluster_size(columns, places, most)
+        assert c in (0, 1, 2, 4, 8) and (c <= 1 or c * columns <= places) and most <= 8 * c * 6 or c == 0
+        if c == 0:
+            continue
+        count, heads = rng.randint(0, most), rng.randint(1, 16)
+        each = -(-count // c)
+        spans = [(i * each, min(i * each + each, count)) for i in range(c)]   # the last may be empty, with an end in front of its start
+        assert [x for b, e in spans for x in range(b, e)] == list(range(count))
+        share = -(-heads * 32 // c)                                # (head, four channels) that a block joins
+        assert [x for i in range(c) for x in range(i * share, min(i * share + share, heads * 32))] == list(range(heads * 32))

@@ -247,6 +247,16 @@ def test_decode_many_sequences(codes):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("B, H_q, H_kv, longest", [(1, 8, 8, 60), (1, 8, 8, 130), (1, 16, 8, 500), (1, 16, 8, 1030), (2, 8, 1, 900), (9, 8, 8, 700),
+                                                  (40, 8, 8, 300), (3, 32, 2, 2000), (70, 4, 4, 700)])
+def test_decode_clusters_of_every_size(B, H_q, H_kv, longest):
+    """Short sequences are shared by the blocks of a cluster: one, two, four or eight of them, also more than there are blocks of
+    positions."""
+    for codes in CODES.values():
+        c = Decode([longest] + [(i * 97) % (longest + 1) for i in range(1, B)], H_q, H_kv, codes, torch.bfloat16, 39, softcap=8.0 if B == 2 else 0.0)
+        c.check(*c.run())
+
+
 @pytest.mark.parametrize("q_scale", [1e-30, 1e-5, 1e4, 1e30])
 def test_decode_queries_of_any_size(q_scale):
     """bf16 queries far outside fp16's range go through a power of two."""
