@@ -153,6 +153,16 @@ def test_what_a_row_does_not_see_has_no_influence(value, options):
     assert (out[:10] == 5).all() and (out[-60:] == 5).all()
 
 
+@pytest.mark.parametrize("shift", [8, 16, 24])
+def test_an_output_on_any_multiple_of_16_bytes(shift):
+    c = Case([130, 33], 4, 2, torch.bfloat16, 51)
+    T, H, _ = c.q.shape
+    whole = torch.full((T * H * 128 + 32,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, lse = c.run(out=whole[shift:shift + T * H * 128].view(T, H, 128))
+    c.check(out, lse)
+    assert (whole[:shift] == 7.0).all() and (whole[shift + T * H * 128:] == 7.0).all()
+
+
 def test_keys_that_are_no_numbers_reach_only_who_sees_them():
     c = Case([400], 2, 1, torch.float16, 50)
     c.k[250] = float("nan")
