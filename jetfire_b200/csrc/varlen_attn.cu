@@ -558,14 +558,14 @@ template <int DT, bool SCALED> __device__ __forceinline__ void weigh(const float
 }
 
 // The same for scores under a cap whose magnitude stays below it: x = f(s) - ref with f(s) = s (c0 + w q(w)), w = s^2.
-template <int DT> __device__ __forceinline__ void weigh_capped(const float* s, uint32_t* p, uint64_t* sum, const float (&co)[6], float ref) {
+template <int DT, int TERMS> __device__ __forceinline__ void weigh_capped(const float* s, uint32_t* p, uint64_t* sum, const float (&co)[TERMS], float ref) {
   const uint64_t r2 = pair(-ref, -ref);
 #pragma unroll
   for (int c = 0; c < 64; c += 2) {
     const uint64_t x = pair(s[c], s[c + 1]), w = mul2(x, x);
-    uint64_t q = fma2(w, pair(co[5], co[5]), pair(co[4], co[4]));
+    uint64_t q = fma2(w, pair(co[TERMS - 1], co[TERMS - 1]), pair(co[TERMS - 2], co[TERMS - 2]));
 #pragma unroll
-    for (int k = 3; k >= 0; --k) q = fma2(q, w, pair(co[k], co[k]));
+    for (int k = TERMS - 3; k >= 0; --k) q = fma2(q, w, pair(co[k], co[k]));
     float a, b;
     split(fma2(x, q, r2), a, b);
     a = ex2(a);
@@ -632,16 +632,19 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
   const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
   const float sl2 = P.scale * kLog2e;
-  // log2(e) cap tanh(scale s / cap) = s (co[0] + co[1] s^2 + ...) while |s| <= cap_in (the fit of reshape(), in s)
-  float co[6], cap_in = 0.0f;
+  // log2(e) cap tanh(scale s / cap) = s (co[0] + co[1] s^2 + ...) while |s| <= cap_in (the fit of reshape(), in s); up to half of that two
+  // terms fewer are as close (fitted the same way: 6.5e-7): packed documents 338 -> 327 us
+  float co[6], few[4], cap_in = 0.0f;
   if (FEAT == 2) {
     constexpr float fit[6] = {1.0f, -0.333302796f, 0.132884905f, -0.0517682843f, 0.0169064086f, -0.00312657771f};
+    constexpr float near[4] = {1.0f, -0.33328161f, 0.1320536f, -0.04475063f};
     const float in = P.scale / P.softcap, in2 = in * in;
     cap_in = in2 < 1e6f ? fabsf(P.softcap / P.scale) : -1.0f;   // (beyond, powers of in2 leave fp32's range)
     float power = sl2;
 #pragma unroll
     for (int k = 0; k < 6; ++k) {
       co[k] = fit[k] * power;
+      if (k < 4) few[k] = near[k] * power;
       power *= in2;
     }
   }
@@ -695,7 +698,8 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
         if (FEAT == 2 && !masked && slope2 == 0.0f) {
           // the cap keeps the order of scores: the largest is taken before it, and the reference leaves with the last step of f
           const float high = largest<64>(s), low = smallest(s);
-          if (__all_sync(0xFFFFFFFFu, fmaxf(fabsf(high), fabsf(low)) <= cap_in)) {
+          const float most = fmaxf(fabsf(high), fabsf(low));
+          if (__all_sync(0xFFFFFFFFu, most <= cap_in)) {
             const float w = high * high;
             float q = fmaf(w, co[5], co[4]);
 #pragma unroll
@@ -707,7 +711,8 @@ template <int DT, int FEAT> __device__ __forceinline__ bool soften(const Params&
             for (int k = 3; k >= 0; --k) lq = fmaf(lq, lw, co[k]);
             const float top = fmaxf(high * q, low * lq);
             if (__any_sync(0xFFFFFFFFu, top > m + kLag) && !move_to(top)) return false;
-            weigh_capped<DT>(s, p, sum, co, m - kLift);
+            if (__all_sync(0xFFFFFFFFu, most <= 0.5f * cap_in)) weigh_capped<DT, 4>(s, p, sum, few, m - kLift);
+            else weigh_capped<DT, 6>(s, p, sum, co, m - kLift);
             publish(from / 64);
             return true;
           }

@@ -116,6 +116,16 @@ def test_scales(scale, softcap, alibi):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("scale", [128 ** -0.5, -(128 ** -0.5)])
+@pytest.mark.parametrize("softcap", [4.0, 6.0, 9.0, 14.0, 40.0])
+def test_caps_about_the_scores_size(softcap, scale):
+    """Largest scores from a seventh of the cap to beyond it: tiles of every branch of the cap's arithmetic.  (Its relative error of
+    6.7e-7 moves a score of at most 40 by less than 2^-15.)"""
+    for dtype in (torch.bfloat16, torch.float16):
+        c = Case([700], 2, 1, dtype, 53, softcap=softcap, scale=scale)
+        c.check(*c.run())
+
+
 @pytest.mark.parametrize("softcap", [1e-20, 1e-4, 1e20])
 def test_caps_of_any_size(softcap):
     c = Case([300], 2, 1, torch.bfloat16, 52, softcap=softcap)
