@@ -26,6 +26,7 @@
 #include "jf_common.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace jf {
 namespace {
@@ -80,7 +81,7 @@ __device__ __forceinline__ int blocks_of(const AttnParams& P, int b) { return sp
 struct Cut { int piece, b, index, n, length, prefix; };
 // Blocks per piece.  ceil(total / target) always leaves few enough pieces; a batch of at most 32 sequences (a lane holds the blocks of
 // one) that is to fill one wave looks for the shortest pieces that still fit the grid: 32 sequences of very different length took
-// 232 of 296 places before, and 31.5 us instead of 30.1.
+// 232 of 296 places before, and 1.4 us more.
 __device__ __forceinline__ int piece_length(const AttnParams& P, int total, int mine) {
   int hi = max(P.min_piece, (total + P.target - 1) / P.target);
   if (P.one_wave) {
@@ -642,9 +643,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   }
 }
 
-// The pieces of a sequence.  A block of WARPS warps per (head, sequence) and 32 * VEC channels; a warp takes every WARPS-th piece.  Rows
-// of many pieces are spread over four blocks of 32 warps (one sequence of 131072 positions, 8 heads, 293
-// pieces: 4 us instead of 10); many rows take one block of 8 warps (32 sequences, 32 heads: 3 us instead of 12).
+// The pieces of a sequence.  A block of WARPS warps per (head, sequence) and 32 * VEC channels; a warp takes every WARPS-th piece.
 template <int DT, int VEC, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_constant__ AttnParams P, int width, int grid_y) {
   __shared__ float sm_w[WARPS * 32], sm_z[WARPS], sm_top[WARPS], sm_o[WARPS][32 * VEC];
@@ -705,23 +704,27 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
   for (int k = 0; k < VEC; ++k) sm_o[warp][lane * VEC + k] = sum[k];
   if (lane == 0) sm_z[warp] = z;
   __syncthreads();
-  if (threadIdx.x < 32 * VEC) {
+  for (int ch = threadIdx.x; ch < 32 * VEC; ch += WARPS * 32) {
     float x = 0.0f;
     z = 0.0f;
 #pragma unroll
     for (int k = 0; k < WARPS; ++k) {
-      x += sm_o[k][threadIdx.x];
+      x += sm_o[k][ch];
       z += sm_z[k];
     }
     const int64_t row = static_cast<int64_t>(b) * P.H_q + h;
-    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + blockIdx.z * 32 * VEC + threadIdx.x] = Elem<DT>::from_f32(z == 0.0f ? 0.0f : x / z);
-    if (threadIdx.x == 0 && blockIdx.z == 0 && P.lse) P.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) / kLog2e;
+    static_cast<uint16_t*>(P.out)[row * JF_HEAD_DIM + blockIdx.z * 32 * VEC + ch] = Elem<DT>::from_f32(z == 0.0f ? 0.0f : x / z);
+    if (ch == 0 && blockIdx.z == 0 && P.lse) P.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) / kLog2e;
   }
 }
 
 struct Plan { int G, nt, groups, target, min_piece, pieces; uint64_t bytes; };
 constexpr int kMinPiece = 8;   // blocks
-constexpr int kManyPieces = 32;   // of a sequence on average: the join spreads a row over four blocks
+// Pieces of a sequence on average: from kManyPieces on the join spreads a row over four blocks of 16 warps, below kFewPieces it gives it four
+// warps.  Its blocks start late, when those of the first kernel have left their registers, so the fewer they take the sooner all of
+// them run: 32 sequences of up to 8191 positions, four KV heads, 30.5 -> 26.6 us against eight warps a row; two of 46000, 25.9 -> 21.6
+// against blocks of 32 warps (of eight: 22.1, but one of 20000 with one KV head 14.2 and not 11.2).
+constexpr int kManyPieces = 32, kFewPieces = 16;
 
 // Pieces per KV head: one wave of blocks where the batch leaves room for it, three where it does not.
 bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
@@ -853,13 +856,16 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
                                    : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
   if (st != JF_OK || P.cluster > 0 || p.pieces == a->B) return st;   // (one piece per sequence: nothing to join)
   const int width = 8 * p.nt, grid_y = a->H_kv * p.groups;
-  if (p.pieces / a->B >= kManyPieces)
-    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
-                    ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16, 1, 32>, dim3(a->H_q, a->B, 4), dim3(1024), 0, s, P, width, grid_y)
-                    : launch_pdl(block8_join_kernel<JF_DTYPE_FP16, 1, 32>, dim3(a->H_q, a->B, 4), dim3(1024), 0, s, P, width, grid_y));
-  else
-    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16
-                    ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16, 4, 8>, dim3(a->H_q, a->B), dim3(256), 0, s, P, width, grid_y)
-                    : launch_pdl(block8_join_kernel<JF_DTYPE_FP16, 4, 8>, dim3(a->H_q, a->B), dim3(256), 0, s, P, width, grid_y));
+  auto join = [&](auto vec, auto warps, int z) {
+    constexpr int V = decltype(vec)::value, W = decltype(warps)::value;
+    const dim3 rows(a->H_q, a->B, z), block(W * 32);
+    return a->q_dtype == JF_DTYPE_BF16 ? launch_pdl(block8_join_kernel<JF_DTYPE_BF16, V, W>, rows, block, 0, s, P, width, grid_y)
+                                       : launch_pdl(block8_join_kernel<JF_DTYPE_FP16, V, W>, rows, block, 0, s, P, width, grid_y);
+  };
+  using std::integral_constant;
+  const int each = p.pieces / a->B;
+  JF_CUDA_TRY(each >= kManyPieces  ? join(integral_constant<int, 1>(), integral_constant<int, 16>(), 4)
+              : each >= kFewPieces ? join(integral_constant<int, 4>(), integral_constant<int, 8>(), 1)
+                                   : join(integral_constant<int, 4>(), integral_constant<int, 4>(), 1));
   return JF_OK;
 }
