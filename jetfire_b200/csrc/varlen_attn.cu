@@ -23,7 +23,7 @@
 // the output are fp32.
 //
 // Bound: per 128 x 128 scores the two products take 1024 cycles of the tensor core, the exponentials 1024 of the special function units (16
-// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 926 to 981 us = 1.12 to 1.19 PFLOP/s, 0.69 to 0.73 of what cuBLAS reaches.  A
+// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 924 to 963 us = 1.14 to 1.19 PFLOP/s, 0.70 to 0.73 of what cuBLAS reaches.  A
 // step of both row tiles is 3500 cycles; with the weights left out it is 2950 (shared-memory reads of the operands and the hand-overs),
 // and a row tile by itself goes through 1750 from its scores to its weights and waits 1020 for the next ones.
 
