@@ -159,7 +159,7 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // cap * tanh(x / cap) of four scores, for the whole warp the same way: up to |x| = cap by a polynomial fitted for the least
-// relative error (6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).
+// relative error (6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).  A score that is NaN stays one either way.
 __device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap) {
   float most = 0.0f;
 #pragma unroll
@@ -176,7 +176,7 @@ __device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap)
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = cap - __fdividef(2.0f * cap, ex2(fminf(x[k] * inv_cap * (2.0f * kLog2e), 126.0f)) + 1.0f);
+    for (int k = 0; k < 4; ++k) x[k] = cap - __fdividef(2.0f * cap, ex2(min_or_nan(x[k] * inv_cap * (2.0f * kLog2e), 126.0f)) + 1.0f);
   }
 }
 

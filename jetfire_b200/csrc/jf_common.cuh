@@ -246,6 +246,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The smaller of two; a NaN stays one (fminf would return the other).
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // Order-preserving map float -> uint32 (larger float = larger key); -0.0 is folded
 // into +0.0 first so that equal values get equal keys.
 __device__ __forceinline__ uint32_t float_order_key(float x) {
