@@ -513,10 +513,10 @@ template <bool CAP> __device__ __forceinline__ void reshape(float* s, const Para
         q = fma2(q, w, pair(1.0f, 1.0f));
         split(mul2(mul2(z, c2), q), s[c], s[c + 1]);
       }
-    } else {   // cap tanh z = cap - 2 cap / (e^(2z) + 1)
+    } else {   // cap tanh z = cap - 2 cap / (e^(2z) + 1); a NaN stays one
       const float to_e = 2.0f * in * kLog2e;
 #pragma unroll
-      for (int c = 0; c < 64; ++c) s[c] = cap2 - __fdividef(2.0f * cap2, ex2(fminf(s[c] * to_e, 126.0f)) + 1.0f);
+      for (int c = 0; c < 64; ++c) s[c] = cap2 - __fdividef(2.0f * cap2, ex2(min_or_nan(s[c] * to_e, 126.0f)) + 1.0f);
     }
   }
   const float mul = CAP ? 1.0f : sl2;
