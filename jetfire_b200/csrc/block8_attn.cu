@@ -38,6 +38,10 @@ constexpr int kStageBytes = 2 * JF_BLOCK_SIZE * JF_HEAD_DIM;
 // 2^kLag: weights stay below 2^15, and what fp16 flushes to zero is below 2^-33 of the largest (a long row's many small weights add up).
 constexpr float kLift = 9.0f, kLag = 6.0f;
 constexpr float kNone = -3.0e38f;             // the reference of a row that has seen nothing (finite: differences are numbers)
+// The sum counts in units of the weights, the reference follows weights times V scales: over blocks of zeros, whose scale is 2^-107 or
+// 2^-108, a position adds 2^116.  A lane's sum beyond kFull moves the reference up by kDrop, so little that fp16 still holds the
+// weights (two moves last a warp for 2^17 blocks); a warp's sum leaves below kLeave, so that those of all warps and pieces add up.
+constexpr float kFull = 0x1p118f, kDrop = 8.0f, kLeave = 0x1p100f, kDown = 64.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -474,14 +478,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     float ahead[NT][4];
     score(ahead, then, k_ring + slot1 * 2048);
     const unsigned char* at = v_ring + slot * 2048;
-    bool above = false;
+    bool above = false, full = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        above |= s[n][k] > m[n][k & 1] + (kLift + kLag);
-      }
-    if (__any_sync(0xFFFFFFFFu, above)) {
+      for (int k = 0; k < 4; ++k) above |= s[n][k] > m[n][k & 1] + (kLift + kLag);
+      full |= fmaxf(l[n][0], l[n][1]) > kFull;
+    }
+    if (__any_sync(0xFFFFFFFFu, above || full)) {
+      full = __any_sync(0xFFFFFFFFu, full);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -490,7 +495,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-          const float to = fmaxf(m[n][c], top - kLift);
+          float to = fmaxf(m[n][c], top - kLift);
+          if (full) {
+            float most = l[n][c];
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 4));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
+            if (most > kFull) to = fmaxf(to, m[n][c] + kDrop);
+          }
           const float f = ex2(m[n][c] - to);
           m[n][c] = to;
           l[n][c] *= f;
@@ -550,6 +562,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
       x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
       x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+      if (x > kLeave) {
+        const float to = m[n][c] + kDown, f = ex2(m[n][c] - to);
+        m[n][c] = to;
+        x *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o[n][j][c] *= f;
+          o[n][j][2 + c] *= f;
+        }
+      }
       if (g == 0) {
         sm_m[warp][n * 8 + 2 * t + c] = m[n][c];
         sm_l[warp][n * 8 + 2 * t + c] = x;
