@@ -13,7 +13,8 @@
 //
 // A warp goes through its blocks with a running reference m for every head, the sum of its weights and the output
 // unnormalised.  The V scale of a block joins the exponent: w = exp2(s + log2(vs) - m) is what meets the codes, in
-// fp16 (rounded to 11 bits: relative 2^-12 per weight, unbiased), and w / vs in fp32 what the sum gets.  m may lag the
+// fp16 (rounded to 11 bits: relative 2^-11 per weight at most, unbiased), and exp2(s - m) in fp32 what the sum gets (not w / vs: where scales are
+// far apart w is 0 of positions that count; 1 to 2 % of the time).  m may lag the
 // maximum by up to kLag, so that most blocks need one vote and no reduction.
 //
 // Work: the blocks of every sequence are cut into pieces of one length for the whole batch, chosen on the device from the lengths
@@ -60,6 +61,10 @@ struct AttnParams {
   int32_t cluster;              // blocks that share a sequence, 1 where pieces are looked for
   bool bt_i32, one_wave;
 };
+
+// What meets a sum twice, and an output squared, when they go to a reference d above their own.  (V scales up to 2^226 apart put d beyond what one
+// factor can be, while the sum, in units of the weights, is as large as others.)
+__device__ __forceinline__ float half_step(float d) { return ex2(-0.5f * d); }
 
 // What of a sequence is scanned: its first `head` blocks and the `count - head` blocks that end with its last position.
 struct Span { int len, prefix, lo, head, first, count; };
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     cp_async_wait_group<2>();
     __syncwarp();
     const int4 then = entries[(i + 1) & 63];
-    const float ivs = ex2(-__int_as_float(now.z));
+    const float lvs = __int_as_float(now.z);
     float ahead[NT][4];
     score(ahead, then, k_ring + slot1 * 2048);
     const unsigned char* at = v_ring + slot * 2048;
@@ -503,9 +508,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
             most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
             if (most > kFull) to = fmaxf(to, m[n][c] + kDrop);
           }
-          const float f = ex2(m[n][c] - to);
+          const float h = half_step(to - m[n][c]), f = h * h;
           m[n][c] = to;
-          l[n][c] *= f;
+          l[n][c] *= h;
+          l[n][c] *= h;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             o[n][j][c] *= f;
@@ -516,10 +522,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     uint32_t pb[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float p0 = ex2(s[n][0] - m[n][0]), p1 = ex2(s[n][1] - m[n][1]), p2 = ex2(s[n][2] - m[n][0]), p3 = ex2(s[n][3] - m[n][1]);
-      l[n][0] = fmaf(p0 + p2, ivs, l[n][0]);
-      l[n][1] = fmaf(p1 + p3, ivs, l[n][1]);
-      const __half2 a = __floats2half2_rn(p0, p1), c = __floats2half2_rn(p2, p3);
+      const float e0 = s[n][0] - m[n][0], e1 = s[n][1] - m[n][1], e2 = s[n][2] - m[n][0], e3 = s[n][3] - m[n][1];
+      l[n][0] += ex2(e0 - lvs) + ex2(e2 - lvs);
+      l[n][1] += ex2(e1 - lvs) + ex2(e3 - lvs);
+      const __half2 a = __floats2half2_rn(ex2(e0), ex2(e1)), c = __floats2half2_rn(ex2(e2), ex2(e3));
       pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&a));
       pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&c));
     }
@@ -601,8 +607,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][threadIdx.x]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      z = fmaf(sm_l[w][threadIdx.x], ex2(sm_m[w][threadIdx.x] - top), z);
+    for (int w = 0; w < kWarps; ++w) {
+      const float h = half_step(top - sm_m[w][threadIdx.x]);
+      z = fmaf(sm_l[w][threadIdx.x] * h, h, z);
+    }
     sm_ml[threadIdx.x] = make_float2(top, z);
   }
   __syncthreads();
@@ -655,8 +663,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
 #pragma unroll
       for (int r = 0; r < 8; ++r)
         if (r < cut.n) {
-          const float f = ex2(ml[r].x - top);
-          z = fmaf(ml[r].y, f, z);
+          const float h = half_step(top - ml[r].x), f = h * h;
+          z = fmaf(ml[r].y * h, h, z);
           sum = make_float4(fmaf(x[r].x, f, sum.x), fmaf(x[r].y, f, sum.y), fmaf(x[r].z, f, sum.z), fmaf(x[r].w, f, sum.w));
         }
       write(head, d, sum, make_float2(top, z));
@@ -700,9 +708,9 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
     const int m = min(WARPS * 32, n - i0);
     if (threadIdx.x < m) {
       const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + (row0 + (i0 + threadIdx.x) * step) * 2);
-      const float f = ex2(ml.x - top);
-      sm_w[threadIdx.x] = f;
-      z = fmaf(ml.y, f, z);
+      const float h = half_step(top - ml.x);
+      sm_w[threadIdx.x] = h * h;
+      z = fmaf(ml.y * h, h, z);
     }
     __syncthreads();
     const float* o = P.part_o + (row0 + i0 * step) * JF_HEAD_DIM + (blockIdx.z * 32 + lane) * VEC;
