@@ -560,8 +560,12 @@ jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
  * has no influence on it, not even as an infinity or a NaN.
  *
  * Base addresses 16-byte aligned, row and head strides positive multiples of 8 elements (strides of a
- * dimension of size 1 are ignored).  status_record: 16 bytes in device memory, or null; an error that the
- * kernel meets (a wait that ran out) is written there as jf_decode_status_of_copy reads it. */
+ * dimension of size 1 are ignored).  status_record: 16 bytes that the device can write; an error that the
+ * kernel meets (a wait that ran out: rows of out may not have been written) is noted there as
+ * jf_decode_status_of_copy reads it.  Null: in a record of the library's, one a device, in host memory that
+ * lives as long as the process.  An error found there is returned once, by jf_varlen_status or by the next
+ * jf_varlen_attn without a record of its own that is not being captured, which then launches nothing.
+ * jf_varlen_status never waits: after a synchronisation it speaks for all that came before. */
 typedef struct jf_varlen_attn_args {
   int32_t dtype, n_seqs, H_q, H_kv;
   int32_t causal, window;         /* window 0: none */
@@ -580,6 +584,9 @@ typedef struct jf_varlen_attn_args {
 } jf_varlen_attn_args;
 
 jf_status_t jf_varlen_attn(const jf_varlen_attn_args* args, jf_stream_t stream);
+jf_status_t jf_varlen_status(int32_t device);
+/* where that record is (16 bytes, made by the first call that needs it) */
+jf_status_t jf_varlen_record(int32_t device, void** host);
 
 #ifdef __cplusplus
 }

@@ -180,6 +180,8 @@ _SIGS = {
     "jf_block8_workspace_bytes": (C.c_uint64, [C.c_int32] * 4),
     "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
     "jf_varlen_attn": (C.c_int32, [C.POINTER(VarlenAttnArgs), C.c_void_p]),
+    "jf_varlen_status": (C.c_int32, [C.c_int32]),
+    "jf_varlen_record": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
     "jf_alloc_mapped": (C.c_int32, [C.c_uint64, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "jf_free_mapped": (C.c_int32, [C.c_void_p]),
 }

@@ -60,7 +60,8 @@ def score_options(impl, device) -> dict:
 
 
 def native_varlen_prefill(*, q, k, v, out, cu_seqlens, max_seqlen, impl, layer, attn_metadata) -> None:
-    """Attention of a step's prompts by this library's own kernel: a ``prefill_attention`` for ``try_jetfire_mixed``."""
+    """Attention of a step's prompts by this library's own kernel: a ``prefill_attention`` for ``try_jetfire_mixed``.  Raises if a
+    wait inside an earlier one ran out (``ops.varlen_prefill_status``)."""
     direct = out.is_contiguous() and out.data_ptr() % 16 == 0
     got, _ = ops.varlen_prefill_attn(q, k, v, cu_seqlens, float(impl.scale), causal=bool(getattr(attn_metadata, "causal", True)),
                                      out=out if direct else None, **score_options(impl, q.device))
@@ -85,6 +86,9 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
     attn_type = getattr(attn_type, "name", attn_type)
     if attn_type is not None and str(attn_type).upper() != "DECODER":
         return None
+    capturing = query.is_cuda and torch.cuda.is_current_stream_capturing()
+    if query.is_cuda and not capturing:
+        ops.varlen_prefill_status(query.device)        # an error of an earlier step's prompts, as far as it has arrived
     n = int(attn_metadata.seq_lens.numel())
     q = query[:T].reshape(T, H_q, D)
     k, v = key[:T].reshape(T, H_kv, D), value[:T].reshape(T, H_kv, D)
@@ -98,7 +102,7 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
 
     def decode_rows(rows, q_rows, lens_rows, table_rows):
         # (a captured step is replayed with other lengths: up to what the table holds)
-        longest = width if q.is_cuda and torch.cuda.is_current_stream_capturing() else min(int(attn_metadata.max_seq_len), width)
+        longest = width if capturing else min(int(attn_metadata.max_seq_len), width)
         out, _ = store.decode(q_rows, lens_rows, table_rows, max(longest, 1), float(impl.scale), **options)
         out = out.reshape(out.shape[0], *output.shape[1:])
         if isinstance(rows, slice):
@@ -113,7 +117,7 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
         else:          # (rows behind the sequences are padding)
             decode_rows(slice(0, n), q[:n], lens, table)
         return output
-    if q.is_cuda and torch.cuda.is_current_stream_capturing():
+    if capturing:
         return None                                # which rows are prompts is read from the device
     counts = [getattr(attn_metadata, name, None) for name in ("num_decodes", "num_prefills", "num_decode_tokens", "num_prefill_tokens")]
     if all(c is not None for c in counts) and getattr(attn_metadata, "jetfire_prefill_has_context", None) is False:

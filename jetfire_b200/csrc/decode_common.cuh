@@ -247,7 +247,7 @@ constexpr int32_t kWaitDone = 1, kWaitRanOut = 2;
 #ifdef __CUDACC__
 __device__ __forceinline__ void report_status(int32_t* status, int code) {
   status[2] = code;
-  __threadfence();
+  __threadfence_system();   // (a record may lie in host memory)
   *reinterpret_cast<unsigned long long*>(status) = kStatusTag;
 }
 #endif

@@ -30,6 +30,8 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cstring>
+#include <mutex>
 #include <type_traits>
 
 #include "decode_common.cuh"
@@ -844,7 +846,7 @@ varlen_attn_kernel(const __grid_constant__ Params P, const __grid_constant__ CUt
     regs_inc<kRowRegs>();
     ok = soften<DT, FEAT>(P, S, tmem, warp >> 2);
   }
-  if (!ok && P.status) report_status(P.status, JF_ERR_TIMEOUT);
+  if (!ok) report_status(P.status, JF_ERR_TIMEOUT);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -898,8 +900,56 @@ jf_status_t launch(const Params& P, int grid, cudaStream_t s, const CUtensorMap&
   return JF_OK;
 }
 
+// Where the calls that bring no record of their own note a wait that ran out, one a device: host memory that the kernel writes, so that
+// looking at it takes no copy and no wait.  Never freed: captured graphs hold its address.
+struct Record { void *host, *device; };
+constexpr int kDevices = 64;
+std::mutex g_record_mu;
+Record g_records[kDevices];
+
+jf_status_t record_of(int device, bool make, Record& r) {
+  if (device < 0 || device >= kDevices) return JF_ERR_ARG;
+  std::lock_guard<std::mutex> lock(g_record_mu);
+  if (!g_records[device].host && make) {
+    // (a capture that is under way, on any stream, does not mind: nothing of it depends on this)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    JF_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    Record made{};
+    const jf_status_t st = jf_alloc_mapped(256, &made.host, &made.device);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (st != JF_OK) return st;
+    memset(made.host, 0, 256);
+    g_records[device] = made;
+  }
+  r = g_records[device];
+  return JF_OK;
+}
+// An error that is there is taken: it is reported once.
+jf_status_t taken(const Record& r) {
+  if (!r.host) return JF_OK;
+  const jf_status_t st = jf_decode_status_of_copy(r.host);
+  if (st != JF_OK) memset(r.host, 0, JF_STATUS_RECORD_BYTES);
+  return st;
+}
+
 }  // namespace
 }  // namespace jf
+
+extern "C" jf_status_t jf_varlen_record(int32_t device, void** host) {
+  using namespace jf;
+  if (!host) return JF_ERR_ARG;
+  Record r{};
+  const jf_status_t st = record_of(device, true, r);
+  *host = r.host;
+  return st;
+}
+
+extern "C" jf_status_t jf_varlen_status(int32_t device) {
+  using namespace jf;
+  Record r{};
+  const jf_status_t st = record_of(device, false, r);
+  return st == JF_OK ? taken(r) : st;
+}
 
 extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t stream) {
   using namespace jf;
@@ -915,6 +965,17 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   if (!stride_ok(a->T, a->q_stride_t) || !stride_ok(a->H_q, a->q_stride_h) || !stride_ok(a->T, a->k_stride_t) || !stride_ok(a->H_kv, a->k_stride_h) ||
       !stride_ok(a->T, a->v_stride_t) || !stride_ok(a->H_kv, a->v_stride_h))
     return JF_ERR_ARG;
+  const auto s = static_cast<cudaStream_t>(stream);
+  Record own{};
+  if (!a->status_record) {
+    int device = 0;
+    JF_CUDA_TRY(cudaGetDevice(&device));
+    jf_status_t e = record_of(device, true, own);
+    if (e != JF_OK) return e;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    JF_CUDA_TRY(cudaStreamIsCapturing(s, &capture));
+    if (capture == cudaStreamCaptureStatusNone && (e = taken(own)) != JF_OK) return e;
+  }
   CUtensorMap q, k, v;
   jf_status_t st = rows_map(a->q, a->dtype, a->T, a->H_q, a->q_stride_t, a->q_stride_h, &q);
   if (st == JF_OK) st = rows_map(a->k, a->dtype, a->T, a->H_kv, a->k_stride_t, a->k_stride_h, &k);
@@ -927,7 +988,7 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   P.v = static_cast<const uint16_t*>(a->v);
   P.out = static_cast<uint16_t*>(a->out);
   P.lse = a->lse;
-  P.status = static_cast<int32_t*>(a->status_record);
+  P.status = static_cast<int32_t*>(a->status_record ? a->status_record : own.device);
   P.v_stride_t = a->v_stride_t;
   P.v_stride_h = a->v_stride_h;
   P.T = static_cast<int32_t>(a->T);
@@ -948,7 +1009,6 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   const int grid = static_cast<int>(std::min<int64_t>(num_sms(), most));
   // (the plain form takes the maximum before it scales, so it needs a positive scale)
   const int feat = a->softcap > 0.0f ? 2 : a->alibi_slopes || !(a->attn_scale > 0.0f) ? 1 : 0;
-  const auto s = static_cast<cudaStream_t>(stream);
   if (a->dtype == JF_DTYPE_BF16)
     return feat == 0 ? launch<JF_DTYPE_BF16, 0>(P, grid, s, q, k, v) : feat == 1 ? launch<JF_DTYPE_BF16, 1>(P, grid, s, q, k, v)
                                                                             : launch<JF_DTYPE_BF16, 2>(P, grid, s, q, k, v);

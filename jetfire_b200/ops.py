@@ -581,13 +581,23 @@ def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=
     cu_seqlens[i + 1]`` (int32).  Scores as in ``block8_decode_attn``, with ``|i - j|`` for the distance.  Row i
     sees ``j <= i`` (``causal``) closer than ``window``, and the first ``prefix_lens[sequence]`` positions from anywhere;
     what it does not see has no influence, not even as an infinity or a NaN.  Rows of no sequence are not written.
-    Returns ``(out (T, H_q, 128), lse (T, H_q) float32)``.  ``status_record``: 16 cleared bytes on the device in which the
-    kernel notes a wait that ran out (``decode_status_of_copy`` reads a host copy)."""
+    Returns ``(out (T, H_q, 128), lse (T, H_q) float32)``.
+
+    A wait inside the kernel that ran out leaves rows unwritten.  It raises ``JetFireError`` (status ``JF_ERR_TIMEOUT``) once, from
+    ``varlen_prefill_status`` or from the next call of this op on the device that is not being captured.  ``status_record``: 16
+    cleared bytes on the device that take the note instead (``decode_status_of_copy`` reads a host copy)."""
     name = "varlen_prefill_attn"
     st, out, lse = _host.varlen_attn(name, q, k, v, cu_seqlens, attn_scale, causal, _window(window, name), softcap, alibi_slopes,
                                      prefix_lens, out, status_record)
     check(name, st)
     return out, lse
+
+
+def varlen_prefill_status(device=None) -> None:
+    """Raises if a wait inside a ``varlen_prefill_attn`` on ``device`` (default: the current one) ran out since this was last
+    asked.  Never waits: after a synchronisation, of a replayed graph too, it speaks for all that came before."""
+    index = torch.device(device).index if device is not None else None
+    check("varlen_prefill_attn", lib.jf_varlen_status(torch.cuda.current_device() if index is None else index))
 
 
 # ---------------------------------------------------------------------------------------
