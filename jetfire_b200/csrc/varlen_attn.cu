@@ -73,7 +73,7 @@ struct Params {
 struct Item { int row0, len, q0, head, prefix, two; };
 
 struct Shared {
-  uint64_t q_full, q_empty, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], half_done[2], o_full[2], item_full[kItems], item_empty[kItems],
+  uint64_t q_full, q_empty, products_done, kv_full[kKvStages], kv_empty[kKvStages], s_full[2], p_full[2][2], half_done[2], o_full[2], item_full[kItems], item_empty[kItems],
       cleaned[kClean];
   Item item[kItems];
   int bad[kItems];       // V tiles of the item held values that are no numbers
@@ -277,14 +277,17 @@ struct Ring {   // position in the ring of K and V tiles
     stage += n;
     if (stage >= kKvStages) { stage -= kKvStages; ++round; }
   }
+  __device__ __forceinline__ void back() {
+    if (--stage < 0) { stage = kKvStages - 1; --round; }
+  }
 };
 
+// `loaded`: Q tiles asked for; `ring`: one past the last K or V tile asked for.
 __device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, const CUtensorMap* qm, const CUtensorMap* km,
-                                     const CUtensorMap* vm) {
+                                     const CUtensorMap* vm, int& loaded, Ring& ring) {
   ItemReader items;
   Item it;
-  Ring ring;
-  for (int n = 0;; ++n) {
+  for (int& n = loaded;;) {
     if (!items.next(S, it)) return false;
     if (it.len < 0) return true;
     const Keys keys = keys_of(P, it);
@@ -297,6 +300,7 @@ __device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem
           tma_load(q_smem + t * kTileBytes + slab * kSlabBytes, qm, slab * 64, it.head + (P.apart ? 0 : t), it.row0 + it.q0 + t * P.apart, &S.q_full);
     }
     __syncwarp();
+    ++n;
     for (int i = 0; i < keys.count; ++i) {
       const int row = it.row0 + tile_of(keys, i) * kKeys;
       for (int side = 0; side < 2; ++side) {
@@ -312,6 +316,16 @@ __device__ __forceinline__ bool load(const Params& P, Shared& S, uint32_t q_smem
     }
     items.release_warp(S);
   }
+}
+
+// The copies that may be in flight: the block's shared memory stays until they are there, or a wait for one runs out.
+__device__ __forceinline__ bool arrived(Shared& S, int loaded, Ring ring) {
+  if (loaded > 0 && !wait_warp(&S.q_full, (loaded - 1) & 1)) return false;
+  for (int i = 0; i < kKvStages && (ring.round > 0 || ring.stage > 0); ++i) {
+    ring.back();
+    if (!wait_warp(&S.kv_full[ring.stage], ring.round & 1)) return false;
+  }
+  return true;
 }
 
 template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, uint32_t tmem) {
@@ -400,7 +414,7 @@ template <int DT> __device__ __forceinline__ bool multiply(const Params& P, Shar
       ring.step();
     }
     // (the last step moved past a K tile that does not exist)
-    ring.stage = ring.stage == 0 ? (--ring.round, kKvStages - 1) : ring.stage - 1;
+    ring.back();
     items.release_warp(S);
   }
 }
@@ -813,6 +827,7 @@ varlen_attn_kernel(const __grid_constant__ Params P, const __grid_constant__ CUt
   if (threadIdx.x == 0) {
     mbar_init(&S.q_full, 1);
     mbar_init(&S.q_empty, 1);
+    mbar_init(&S.products_done, 1);
     for (int i = 0; i < kKvStages; ++i) { mbar_init(&S.kv_full[i], 1); mbar_init(&S.kv_empty[i], 2); }   // empty: products done, looked over
     for (int t = 0; t < 2; ++t) { mbar_init(&S.s_full[t], 1); mbar_init(&S.p_full[t][0], 4); mbar_init(&S.p_full[t][1], 4); mbar_init(&S.half_done[t], 1); mbar_init(&S.o_full[t], 1); }
     for (int i = 0; i < kItems; ++i) { mbar_init(&S.item_full[i], 1); mbar_init(&S.item_empty[i], 11); }   // 8 + loads, products, cleaning
@@ -829,14 +844,21 @@ varlen_attn_kernel(const __grid_constant__ Params P, const __grid_constant__ CUt
   const uint32_t tmem = S.tmem;
   pdl_wait();
   pdl_trigger();
-  // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
+  // every role ends by itself, a wait that ran out included, loads and products when theirs are through; the error is recorded by whoever
+  // meets it
   bool ok = true;
   if (warp >= 8) {
     regs_dec<kRoleRegs>();
     if (warp == 8) {
-      ok = load(P, S, q_smem, kv_smem, &qm, &km, &vm);
+      int loaded = 0;
+      Ring ring;
+      ok = load(P, S, q_smem, kv_smem, &qm, &km, &vm, loaded, ring);
+      ok &= arrived(S, loaded, ring);
     } else if (warp == 9) {
       ok = multiply<DT>(P, S, q_smem, kv_smem, tmem);
+      if (elect_one()) tc_commit(&S.products_done);
+      __syncwarp();
+      ok &= wait_warp(&S.products_done, 0);
     } else if (warp == 10) {
       ok = schedule(P, S);
     } else {
