@@ -59,6 +59,15 @@ def score_options(impl, device) -> dict:
                 alibi_slopes=slopes.to(device=device, dtype=torch.float32).contiguous() if slopes is not None else None)
 
 
+def served(impl) -> bool:
+    """Whether a layer's attention is one of queries over the layer's own keys and values, with no terms but those of ``score_options``: a
+    decoder's, without a per-head term in the softmax's denominator (``sinks``) and without another layer's cache in place of its own."""
+    attn_type = getattr(impl, "attn_type", None)
+    attn_type = getattr(attn_type, "name", attn_type)
+    return (attn_type is None or str(attn_type).upper() == "DECODER") and getattr(impl, "sinks", None) is None \
+        and getattr(impl, "kv_sharing_target_layer_name", None) is None
+
+
 def native_varlen_prefill(*, q, k, v, out, cu_seqlens, max_seqlen, impl, layer, attn_metadata) -> None:
     """Attention of a step's prompts by this library's own kernel: a ``prefill_attention`` for ``try_jetfire_mixed``.  Raises if a
     wait inside an earlier one ran out (``ops.varlen_prefill_status``)."""
@@ -76,15 +85,14 @@ def _int32(t: torch.Tensor) -> torch.Tensor:
 def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, output, store: JetFireBlock8Store):
     """One step of a layer with an 8-bit cache: append, then attention.  ``query (T, H_q, D)`` or ``(T, H_q * D)``, ``key`` /
     ``value`` likewise with the KV heads, ``output`` like ``query``.  Returns ``output``, or None when the step's attention
-    is not one this path serves -- prompts with cached context, several query tokens over a cache, cascade
-    attention, cross or encoder attention -- and the caller's native attention has to; the tokens are appended either way."""
+    is not one this path serves and the caller's native attention has to.  The tokens are appended all the same where a later step
+    may be served -- after prompts with cached context, several query tokens over a cache, cascade attention -- and
+    not in a layer that never is (``served``)."""
     H_q, H_kv, D = int(layer.num_heads), int(layer.num_kv_heads), int(layer.head_size)
     T = int(attn_metadata.num_actual_tokens)
     if T == 0 or D != store.head_dim or H_kv != store.num_kv_heads:
         return None
-    attn_type = getattr(impl, "attn_type", None)
-    attn_type = getattr(attn_type, "name", attn_type)
-    if attn_type is not None and str(attn_type).upper() != "DECODER":
+    if not served(impl):
         return None
     capturing = query.is_cuda and torch.cuda.is_current_stream_capturing()
     if query.is_cuda and not capturing:

@@ -15,7 +15,7 @@ dummy native KV tensors, prefill activation chunking and scheduler changes.
 """
 from __future__ import annotations
 
-from .block8 import JetFireBlock8Store
+from .block8 import JetFireBlock8Store, served
 from .cache_store import JetFireCacheStore
 from .config import JetFireConfig, get_jetfire_config
 from .jetfire_backend import register_layer_store
@@ -48,8 +48,8 @@ def install_layer_stores(layers: dict, *, num_blocks: int, block_size: int = 16,
     modules, or any stand-in).  Creates one ``JetFireCacheStore`` (``JetFireBlock8Store`` where the configuration
     asks for an 8-bit cache) per layer with vLLM's planned ``num_blocks`` (the scheduler hands out block ids in [0, num_blocks), so the cache must cover
     them all) and registers it under the layer's name.  Layers whose geometry the decode path does
-    not serve (head size other than 128, block size other than 16) are skipped and fall back to
-    vLLM's native attention.  Returns name -> store for the layers that were installed."""
+    not serve (head size other than 128, block size other than 16), and for an 8-bit cache those that ``block8.served`` names,
+    are skipped and fall back to vLLM's native attention.  Returns name -> store for the layers that were installed."""
     import torch
     cfg = cfg or get_jetfire_config()
     dtype = dtype or torch.bfloat16
@@ -58,6 +58,8 @@ def install_layer_stores(layers: dict, *, num_blocks: int, block_size: int = 16,
         if int(getattr(layer, "head_size", 0)) != 128 or int(block_size) != 16:
             continue
         if cfg.block8:
+            if not served(getattr(layer, "impl", layer)):
+                continue
             store = JetFireBlock8Store(num_blocks=int(num_blocks), num_kv_heads=int(layer.num_kv_heads), codes=cfg.block8, device=device,
                                        block_size=int(block_size))
             register_layer_store(name, store)

@@ -1,0 +1,50 @@
+"""Layers and steps that the 8-bit path does not serve go to the native attention, or are refused, instead of being served wrongly.
+On the CPU, with the ops replaced by their plain forms."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from jetfire_b200.adapter import block8 as B8
+from jetfire_b200.adapter import config as jcfg
+from jetfire_b200.adapter import jetfire_backend as jb
+from jetfire_b200.adapter.registry import install_layer_stores
+from test_block8_adapter import D, H_KV, H_Q, Conversation, _impl, _layer, _meta, _plain_ops, _through_the_backend
+
+NOT_SERVED = [dict(sinks=torch.zeros(H_Q)), dict(kv_sharing_target_layer_name="model.layers.0.attn"), dict(attn_type="encoder"),
+              dict(attn_type=SimpleNamespace(name="ENCODER_DECODER"))]
+
+
+@pytest.mark.parametrize("settings", NOT_SERVED)
+def test_layers_with_other_terms_or_another_cache(monkeypatch, settings):
+    """A per-head term in the softmax's denominator, a layer that reads another layer's cache, attention that is no decoder's: nothing
+    is appended and the native attention runs, for prompts and for tokens."""
+    calls = []
+    _plain_ops(monkeypatch, calls)
+    c = Conversation(2, "cpu", seed=11, **settings)
+    impl, call = _through_the_backend(c)
+    try:
+        for news in ([7, 4], [1, 1]):
+            T = sum(news)
+            q, k, v = (torch.zeros(T, h * D, dtype=torch.bfloat16) for h in (H_Q, H_KV, H_KV))
+            out = torch.full((T, H_Q * D), 7.0, dtype=torch.bfloat16)
+            assert call(layer=_layer(), query=q, key=k, value=v, attn_metadata=_meta([0, 0], news, c.table, "cpu"), output=out) is out
+            assert (out == 7.0).all()
+        assert not calls and impl.native == 2
+    finally:
+        jb._STORES.pop("l")
+
+
+@pytest.mark.parametrize("settings", NOT_SERVED)
+@pytest.mark.parametrize("on", ["layer", "impl"])
+def test_such_layers_get_no_cache(settings, on):
+    layer = SimpleNamespace(num_kv_heads=2, head_size=128)
+    for k, v in settings.items():
+        setattr(layer, k, v)
+    if on == "impl":
+        layer = SimpleNamespace(num_kv_heads=2, head_size=128, impl=_impl(**{k: v for k, v in settings.items() if k != "attn_type"}))
+        layer.impl.attn_type = settings.get("attn_type", "decoder")
+    other = SimpleNamespace(num_kv_heads=2, head_size=128, impl=_impl())
+    got = install_layer_stores({"x": layer, "y": other}, num_blocks=4, device="cpu", cfg=jcfg.JetFireConfig(block8="int8"))
+    assert list(got) == ["y"] and jb.get_layer_store("x") is None
+    jb._STORES.pop("y")
