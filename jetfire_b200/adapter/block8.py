@@ -90,10 +90,10 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
     not in a layer that never is (``served``)."""
     H_q, H_kv, D = int(layer.num_heads), int(layer.num_kv_heads), int(layer.head_size)
     T = int(attn_metadata.num_actual_tokens)
-    if T == 0 or D != store.head_dim or H_kv != store.num_kv_heads:
+    if T == 0 or not served(impl):
         return None
-    if not served(impl):
-        return None
+    if D != store.head_dim or H_kv != store.num_kv_heads:
+        raise ValueError(f"the layer's 8-bit cache has {store.num_kv_heads} heads of {store.head_dim}, the layer {H_kv} of {D}")
     capturing = query.is_cuda and torch.cuda.is_current_stream_capturing()
     if query.is_cuda and not capturing:
         ops.varlen_prefill_status(query.device)        # an error of an earlier step's prompts, as far as it has arrived

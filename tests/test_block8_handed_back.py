@@ -48,3 +48,23 @@ def test_such_layers_get_no_cache(settings, on):
     got = install_layer_stores({"x": layer, "y": other}, num_blocks=4, device="cpu", cfg=jcfg.JetFireConfig(block8="int8"))
     assert list(got) == ["y"] and jb.get_layer_store("x") is None
     jb._STORES.pop("y")
+
+
+def _step(store, layer, impl=None, **kw):
+    H_q, H_kv, D = layer.num_heads, layer.num_kv_heads, layer.head_size
+    q, k, v = (torch.zeros(3, h * D, dtype=torch.bfloat16) for h in (H_q, H_kv, H_kv))
+    md = _meta([0], [3], torch.zeros(1, 2, dtype=torch.int32), "cpu")
+    return B8.try_block8_attention(impl=impl or _impl(), layer=layer, query=q, key=k, value=v, attn_metadata=md,
+                                   output=torch.zeros(3, H_q * D, dtype=torch.bfloat16), store=store, **kw)
+
+
+@pytest.mark.parametrize("wrong", [dict(head_size=64), dict(num_kv_heads=4)])
+def test_a_layer_that_does_not_fit_its_cache_is_an_error(monkeypatch, wrong):
+    """It would stay empty beside a layer that never reads it."""
+    calls = []
+    _plain_ops(monkeypatch, calls)
+    store = B8.JetFireBlock8Store(num_blocks=2, num_kv_heads=H_KV, device="cpu")
+    layer = SimpleNamespace(**{**vars(_layer()), **wrong})
+    with pytest.raises(ValueError, match="8-bit cache"):
+        _step(store, layer)
+    assert not calls
