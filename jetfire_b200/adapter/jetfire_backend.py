@@ -35,7 +35,9 @@ class JetFireAttentionImplMixin:
                 output_scale=None, output_block_scale=None):
         store = get_layer_store(getattr(layer, "layer_name", ""))
         if isinstance(store, JetFireBlock8Store):
-            if output is not None and attn_metadata is not None and key is not None and value is not None:
+            # (an output that is to be quantised on its way is not this path's)
+            if output is not None and attn_metadata is not None and key is not None and value is not None \
+                    and output_scale is None and output_block_scale is None:
                 done = try_block8_attention(impl=self, layer=layer, query=query, key=key, value=value,
                                             attn_metadata=attn_metadata, output=output, store=store)
                 if done is not None:

@@ -68,3 +68,20 @@ def test_a_layer_that_does_not_fit_its_cache_is_an_error(monkeypatch, wrong):
     with pytest.raises(ValueError, match="8-bit cache"):
         _step(store, layer)
     assert not calls
+
+
+def test_an_output_that_is_to_be_quantised_goes_to_the_native_attention(monkeypatch):
+    """It would be written without its scale."""
+    calls = []
+    _plain_ops(monkeypatch, calls)
+    c = Conversation(1, "cpu", seed=12)
+    impl, _ = _through_the_backend(c)
+    try:
+        q, k, v = (torch.zeros(3, h * D, dtype=torch.bfloat16) for h in (H_Q, H_KV, H_KV))
+        for scale in (dict(output_scale=torch.ones(1)), dict(output_block_scale=torch.ones(1))):
+            out = torch.full((3, H_Q * D), 7.0).to(torch.float8_e4m3fn)
+            assert impl.forward(_layer(), q, k, v, None, _meta([0], [3], c.table, "cpu"), output=out, **scale) is out
+            assert (out.float() == 7.0).all()
+        assert not calls and impl.native == 2
+    finally:
+        jb._STORES.pop("l")
