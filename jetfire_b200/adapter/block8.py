@@ -72,8 +72,14 @@ def native_varlen_prefill(*, q, k, v, out, cu_seqlens, max_seqlen, impl, layer, 
     """Attention of a step's prompts by this library's own kernel: a ``prefill_attention`` for ``try_jetfire_mixed``.  Raises if a
     wait inside an earlier one ran out (``ops.varlen_prefill_status``)."""
     direct = out.is_contiguous() and out.data_ptr() % 16 == 0
-    got, _ = ops.varlen_prefill_attn(q, k, v, cu_seqlens, float(impl.scale), causal=bool(getattr(attn_metadata, "causal", True)),
-                                     out=out if direct else None, **score_options(impl, q.device))
+    causal, window = bool(getattr(attn_metadata, "causal", True)), getattr(impl, "sliding_window", None)
+    if not causal and isinstance(window, (tuple, list)):     # (left, right): the op sees as far to both sides, or nothing behind
+        left, right = (int(w) for w in window)
+        causal = right == 0
+        if not causal and max(left, -1) != max(right, -1):
+            raise ValueError(f"prompts that see {left} positions before and {right} behind their own (sliding_window) are not served")
+    got, _ = ops.varlen_prefill_attn(q, k, v, cu_seqlens, float(impl.scale), causal=causal, out=out if direct else None,
+                                     **score_options(impl, q.device))
     if not direct:
         out.copy_(got)
 

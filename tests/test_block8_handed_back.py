@@ -85,3 +85,25 @@ def test_an_output_that_is_to_be_quantised_goes_to_the_native_attention(monkeypa
         assert not calls and impl.native == 2
     finally:
         jb._STORES.pop("l")
+
+
+@pytest.mark.parametrize("causal, window, want", [
+    (True, (-1, -1), dict(causal=True, window=None)), (True, (9, 0), dict(causal=True, window=10)), (True, (9, -1), dict(causal=True, window=10)),
+    (False, (-1, -1), dict(causal=False, window=None)), (False, (9, 9), dict(causal=False, window=10)), (False, (9, 0), dict(causal=True, window=10)),
+    (False, (-1, 0), dict(causal=True, window=None)), (False, (9, -1), None), (False, (-1, 5), None), (False, (9, 4), None), (True, 10, dict(causal=True, window=10)),
+    (False, 10, dict(causal=False, window=10)), (False, None, dict(causal=False, window=None))])
+def test_windows_of_prompts_are_the_pair_s_two_sides(monkeypatch, causal, window, want):
+    """(left, right): positions seen before and behind one's own, -1 for all.  What the op has no form for is refused."""
+    seen = {}
+    monkeypatch.setattr(B8.ops, "varlen_prefill_attn", lambda q, *a, out=None, **kw: (seen.update(kw), (q, None))[1])
+    q, k, v = (torch.zeros(3, h, D, dtype=torch.bfloat16) for h in (H_Q, H_KV, H_KV))
+    impl = _impl()
+    impl.sliding_window = window
+    args = dict(q=q, k=k, v=v, out=torch.zeros_like(q), cu_seqlens=torch.tensor([0, 3], dtype=torch.int32), max_seqlen=3, impl=impl, layer=_layer(),
+                attn_metadata=SimpleNamespace(causal=causal))
+    if want is None:
+        with pytest.raises(ValueError, match="sliding_window"):
+            B8.native_varlen_prefill(**args)
+    else:
+        B8.native_varlen_prefill(**args)
+        assert {k: seen[k] for k in ("causal", "window")} == want
