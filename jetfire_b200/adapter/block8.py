@@ -55,8 +55,12 @@ def score_options(impl, device) -> dict:
         left = int(window[0]) if isinstance(window, (tuple, list)) else int(window) - 1
         window = left + 1 if left >= 0 else None
     slopes = getattr(impl, "alibi_slopes", None)
-    return dict(softcap=float(getattr(impl, "logits_soft_cap", None) or 0.0), window=window,
-                alibi_slopes=slopes.to(device=device, dtype=torch.float32).contiguous() if slopes is not None else None)
+    if slopes is not None and (slopes.device != device or slopes.dtype != torch.float32 or not slopes.is_contiguous()):
+        # brought over once and kept where they came from: a captured step cannot wait for the host
+        if device.type == "cuda" and slopes.device.type == "cpu" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("alibi_slopes are on the host: run a step before one is captured")
+        slopes = impl.alibi_slopes = slopes.to(device=device, dtype=torch.float32).contiguous()
+    return dict(softcap=float(getattr(impl, "logits_soft_cap", None) or 0.0), window=window, alibi_slopes=slopes)
 
 
 def served(impl) -> bool:
