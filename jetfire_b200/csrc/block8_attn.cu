@@ -843,7 +843,10 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   if (a->B == 0) return JF_OK;
   Plan p;
   if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;
-  if (!a->q || !a->k_data || !a->v_data || !a->k_scales || !a->v_scales || !a->block_table || !a->seq_lens || !a->out) return JF_ERR_ARG;
+  if (!a->q || !a->seq_lens || !a->out) return JF_ERR_ARG;
+  // (a table without columns and a cache without blocks have no memory; nothing of them is read)
+  if (a->max_blocks > 0 && !a->block_table) return JF_ERR_ARG;
+  if (a->num_blocks > 0 && (!a->k_data || !a->v_data || !a->k_scales || !a->v_scales)) return JF_ERR_ARG;
   if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 8)) return JF_ERR_ARG;
   if (a->num_blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
   if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE) return JF_ERR_UNSUPPORTED;
