@@ -560,7 +560,7 @@ jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
  * has no influence on it, not even as an infinity or a NaN.
  *
  * Base addresses 16-byte aligned, row and head strides positive multiples of 8 elements (strides of a
- * dimension of size 1 are ignored).  status_record: 16 bytes that the device can write; an error that the
+ * dimension of size 1 are ignored); at most 2^18 sequences and 2^24 rows.  status_record: 16 bytes that the device can write; an error that the
  * kernel meets (a wait that ran out: rows of out may not have been written) is noted there as
  * jf_decode_status_of_copy reads it.  Null: in a record of the library's, one a device, in host memory that
  * lives as long as the process.  An error found there is returned once, by jf_varlen_status or by the next

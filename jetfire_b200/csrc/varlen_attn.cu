@@ -51,6 +51,10 @@ constexpr int kThreads = 384;
 constexpr int kRowRegs = 208, kRoleRegs = 80;
 constexpr float kLag = 8.0f;                          // log2
 constexpr uint64_t kWaitNs = 2000000000ull;
+// schedule() goes through all sequences once a level, 0.27 us for 32 of them, and a block's items are up to 148 levels apart: so many
+// keep who waits for one below 0.4 s.  An item of a sequence of so many rows goes through 2^17 key tiles, 9000 cycles each where scores lie beyond a cap: 0.9 s, for which schedule()
+// waits.
+constexpr int kMaxSeqs = 1 << 18, kMaxRows = 1 << 24;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -979,7 +983,7 @@ extern "C" jf_status_t jf_varlen_attn(const jf_varlen_attn_args* a, jf_stream_t 
   if (a->dtype != JF_DTYPE_BF16 && a->dtype != JF_DTYPE_FP16) return JF_ERR_ARG;
   if (a->T < 0 || a->n_seqs < 0 || a->H_q <= 0 || a->H_kv <= 0 || a->H_q % a->H_kv != 0 || a->window < 0) return JF_ERR_ARG;
   if (a->softcap != 0.0f && !(a->softcap >= 1.0e-30f && a->softcap <= 1.0e30f)) return JF_ERR_ARG;
-  if (a->T > INT32_MAX / 2) return JF_ERR_UNSUPPORTED;
+  if (a->T > kMaxRows || a->n_seqs > kMaxSeqs) return JF_ERR_UNSUPPORTED;
   if (a->T == 0 || a->n_seqs == 0) return JF_OK;
   if (!a->q || !a->k || !a->v || !a->cu_seqlens || !a->out) return JF_ERR_ARG;
   if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) || !aligned(a->status_record, 8)) return JF_ERR_ARG;

@@ -578,7 +578,7 @@ def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=
 
     ``q (T, H_q, 128)``, ``k / v (T, H_kv, 128)`` bf16 or fp16; any strides, copied first where tensor copies cannot
     address them (innermost dim not contiguous, rows not 16-byte aligned).  Sequence i owns the rows ``cu_seqlens[i] ..
-    cu_seqlens[i + 1]`` (int32).  Scores as in ``block8_decode_attn``, with ``|i - j|`` for the distance.  Row i
+    cu_seqlens[i + 1]`` (int32; at most 2^18 sequences and 2^24 rows).  Scores as in ``block8_decode_attn``, with ``|i - j|`` for the distance.  Row i
     sees ``j <= i`` (``causal``) closer than ``window``, and the first ``prefix_lens[sequence]`` positions from anywhere;
     what it does not see has no influence, not even as an infinity or a NaN.  Rows of no sequence are not written.
     Returns ``(out (T, H_q, 128), lse (T, H_q) float32)``.
