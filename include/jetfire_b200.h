@@ -507,7 +507,9 @@ int32_t     jf_get_cpu_attn_node(void);
  *   - alibi_slopes[head] * (seq_lens[b] - 1 - j) if alibi_slopes is given;
  *   out = softmax(s).v, lse = log sum exp(s),
  * over the positions j of [seq_lens[b] - window, seq_lens[b]) and [0, prefix_lens[b]) (all of them if
- * window is 0) whose block id is valid; out = 0 and lse = -inf where there is none.  seq_lens is cut to
+ * window is 0) whose block id is valid; out = 0 and lse = -inf where there is none (a table without columns and
+ * a cache without blocks may have null addresses).  A query that holds a NaN or an infinity gives a row of NaN, with
+ * a cap too.  seq_lens is cut to
  * [0, min(max_S, 16 * max_blocks)].  q, out (B, H_q, 128), lse (B, H_q) f32 or null, all contiguous.
  * Two launches at most; workspace as for the entry points above (jf_block8_workspace_bytes, 0 = bad
  * shape), needed no longer than the call's launches.  Block ids are 64-bit or 32-bit integers, rows
@@ -555,7 +557,8 @@ jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
  *   sequence i owns the rows cu_seqlens[i] .. cu_seqlens[i + 1]; out (T, H_q, 128) contiguous; lse
  *   (T, H_q) f32 or null.  Rows of no sequence are not written.
  *
- * Scores as in jf_block8_attn, the distance being |i - j|.  Row i of a sequence sees j <= i (causal) with
+ * Scores as in jf_block8_attn, the distance being |i - j|.  (A score that is NaN stays NaN under a
+ * cap, an infinite one becomes the cap.)  Row i of a sequence sees j <= i (causal) with
  * |i - j| < window (if window > 0), and j < prefix_lens[sequence] (if given).  What a row does not see
  * has no influence on it, not even as an infinity or a NaN.
  *

@@ -23,7 +23,7 @@
 // whose results meet in its shared memory.
 //
 // Bound: memory, 256 bytes per (position, KV head).  Four sequences of 65536 positions, 64 / 8 heads, int8: 101 us = 5.3 TB/s (copies of the
-// same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 6 us.
+// same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 6.2 us.
 #include "jf_common.cuh"
 
 #include <algorithm>
@@ -36,7 +36,8 @@ constexpr int kWarps = 8;
 constexpr int kStages = 3;                    // blocks of K and V in flight per warp
 constexpr int kStageBytes = 2 * JF_BLOCK_SIZE * JF_HEAD_DIM;
 // The reference of the fp16 weights lies 2^kLift below the maximum it was taken from and may lag the present one by
-// 2^kLag: weights stay below 2^15, and what fp16 flushes to zero is below 2^-33 of the largest (a long row's many small weights add up).
+// 2^kLag: weights stay below 2^15, and what fp16 flushes to zero is below 2^-33 of the largest (a long row's many small weights add up;
+// 2^-17 where the sum has moved the reference, see kFull).
 constexpr float kLift = 9.0f, kLag = 6.0f;
 constexpr float kNone = -3.0e38f;             // the reference of a row that has seen nothing (finite: differences are numbers)
 // The sum counts in units of the weights, the reference follows weights times V scales: over blocks of zeros, whose scale is 2^-107 or
@@ -779,7 +780,7 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
 
 // Blocks of a cluster, 0 for pieces and a join.  As many as leave every warp a block, up to eight and while all of them are resident at
 // once, where that is at most kRounds blocks a warp; kFewRounds where pieces could spread over eight times as many multiprocessors.
-// One sequence of 500 positions, 8 KV heads: 7.7 -> 6.0 us, of 4000: 11.7 -> 9.1; 64 of 300: 19.6 -> 17.4; 8 of 2000: 14.9 -> 12.4.  With 2
+// One sequence of 500 positions, 8 KV heads: 7.7 -> 6.0 us (6.2 with what the sums have gained since), of 4000: 11.7 -> 9.1; 64 of 300: 19.6 -> 17.4; 8 of 2000: 14.9 -> 12.4.  With 2
 // columns, 4000 positions take 9.2 us so and 8.6 in pieces.
 constexpr int kRounds = 6, kFewRounds = 2;
 int cluster_size(const Plan& p, int B, int H_kv, int64_t longest) {

@@ -19,11 +19,12 @@
 // would not be: warp 11 looks at every V tile that has masked entries and zeroes infinities and NaN in it; rows that do see
 // them get them back at the end (never, with finite inputs).
 //
-// The weights that meet V are rounded to the operands' type (bf16: 2^-9 of themselves at most, fp16: 2^-12); their sum, the scores and
+// The weights that meet V are rounded to the operands' type (half a step: bf16 2^-8 of themselves at most, fp16 2^-11); their sum, the scores and
 // the output are fp32.
 //
 // Bound: per 128 x 128 scores the two products take 1024 cycles of the tensor core, the exponentials 1024 of the special function units (16
-// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 924 to 963 us = 1.14 to 1.19 PFLOP/s, 0.70 to 0.73 of what cuBLAS reaches.  A
+// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 908 to 940 us by itself = 1.17 to 1.21 PFLOP/s, 0.72 to 0.74 of what cuBLAS reaches, and
+// 1068 among other calls, with the card near its power cap.  A
 // step of both row tiles is 3500 cycles; with the weights left out it is 2950 (shared-memory reads of the operands and the hand-overs),
 // and a row tile by itself goes through 1750 from its scores to its weights and waits 1020 for the next ones.
 
@@ -52,8 +53,8 @@ constexpr int kRowRegs = 208, kRoleRegs = 80;
 constexpr float kLag = 8.0f;                          // log2
 constexpr uint64_t kWaitNs = 2000000000ull;
 // schedule() goes through all sequences once a level, 0.27 us for 32 of them, and a block's items are up to 148 levels apart: so many
-// keep who waits for one below 0.4 s.  An item of a sequence of so many rows goes through 2^17 key tiles, 9000 cycles each where scores lie beyond a cap: 0.9 s, for which schedule()
-// waits.
+// keep who waits for one below 0.4 s.  An item of a sequence of so many rows goes through 2^17 key tiles, 9000 cycles each where scores
+// lie beyond a cap: 0.9 s, for which schedule() waits.
 constexpr int kMaxSeqs = 1 << 18, kMaxRows = 1 << 24;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

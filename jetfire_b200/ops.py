@@ -563,8 +563,8 @@ def block8_decode_attn(q, k_data, k_scales, v_data, v_scales, block_table, seq_l
     ``q (B, H_q, 128)`` stands at position ``seq_lens[b] - 1``.  Scores are ``attn_scale * q.k``, then
     ``softcap * tanh(s / softcap)`` where ``softcap`` is not 0, then ``- alibi_slopes[h] * distance``.  A query sees the
     last ``window`` positions and the first ``prefix_lens[b]``, or everything.  Positions whose block id is not
-    in the cache are not seen; a sequence that sees nothing (length 0) gets zeros and ``lse = -inf``.  ``max_S``
-    bounds the lengths (longer ones are cut to it).  Returns ``(out (B, H_q, 128) like q, lse (B, H_q) float32)``."""
+    in the cache are not seen; a sequence that sees nothing (length 0) gets zeros and ``lse = -inf``.  A query that holds a NaN
+    or an infinity gives a row of NaN, with a cap too.  ``max_S`` bounds the lengths (longer ones are cut to it).  Returns ``(out (B, H_q, 128) like q, lse (B, H_q) float32)``."""
     name = "block8_decode_attn"
     st, out, lse = _host.block8_attn(name, q, k_data, k_scales, v_data, v_scales, block_table, seq_lens, max_S, H_q, H_kv, block_size,
                                      attn_scale, softcap, alibi_slopes, _window(window, name), prefix_lens, workspace, out)
@@ -580,7 +580,8 @@ def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=
     address them (innermost dim not contiguous, rows not 16-byte aligned).  Sequence i owns the rows ``cu_seqlens[i] ..
     cu_seqlens[i + 1]`` (int32; at most 2^18 sequences and 2^24 rows).  Scores as in ``block8_decode_attn``, with ``|i - j|`` for the distance.  Row i
     sees ``j <= i`` (``causal``) closer than ``window``, and the first ``prefix_lens[sequence]`` positions from anywhere;
-    what it does not see has no influence, not even as an infinity or a NaN.  Rows of no sequence are not written.
+    what it does not see has no influence, not even as an infinity or a NaN.  Under a cap a score that is NaN stays NaN and an
+    infinite one becomes the cap.  Rows of no sequence are not written.
     Returns ``(out (T, H_q, 128), lse (T, H_q) float32)``.
 
     A wait inside the kernel that ran out leaves rows unwritten.  It raises ``JetFireError`` (status ``JF_ERR_TIMEOUT``) once, from
