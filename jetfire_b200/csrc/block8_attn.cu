@@ -13,8 +13,8 @@
 //
 // A warp goes through its blocks with a running reference m for every head, the sum of its weights and the output
 // unnormalised.  The V scale of a block joins the exponent: w = exp2(s + log2(vs) - m) is what meets the codes, in
-// fp16 (rounded to 11 bits: relative 2^-11 per weight at most, unbiased), and exp2(s - m) in fp32 what the sum gets (not w / vs: where scales are
-// far apart w is 0 of positions that count; 1 to 2 % of the time).  m may lag the
+// fp16 (rounded to 11 bits: relative 2^-11 per weight at most, unbiased), and exp2(s - m) in fp32 what the sum gets (w / vs would
+// be 1 to 2 % faster, but where scales are far apart w is 0 for positions that count).  m may lag the
 // maximum by up to kLag, so that most blocks need one vote and no reduction.
 //
 // Work: the blocks of every sequence are cut into pieces of one length for the whole batch, chosen on the device from the lengths
@@ -63,8 +63,8 @@ struct AttnParams {
   bool bt_i32, one_wave;
 };
 
-// What meets a sum twice, and an output squared, when they go to a reference d above their own.  (V scales up to 2^226 apart put d beyond what one
-// factor can be, while the sum, in units of the weights, is as large as others.)
+// The root of the factor that takes an output to a reference d above its own; a sum is multiplied by it twice.  (V scales up to 2^226 apart put d
+// beyond what one factor in fp32 can be, while the sum, in units of the weights, is as large as others.)
 __device__ __forceinline__ float half_step(float d) { return ex2(-0.5f * d); }
 
 // What of a sequence is scanned: its first `head` blocks and the `count - head` blocks that end with its last position.
