@@ -549,6 +549,44 @@ jf_status_t jf_block8_append(const void* key, const void* value, int32_t dtype, 
 uint64_t    jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S);
 jf_status_t jf_block8_attn(const jf_block8_attn_args* args, jf_stream_t stream);
 
+/* ---- rotated append, shared prefixes and selected blocks, over the same cache ------------------------
+ * jf_block8_append_rotary is jf_block8_append with the rotation of queries and keys by their positions on the
+ * way and, where bounds is given, the block bounds that jf_block8_sparse_attn selects by.
+ *
+ * Row p of cos_sin (table_rows, rot), fp32 or of the tokens' type, holds the cosines of position p's rot / 2
+ * angles, then their sines; positions[t] is token t's row.  Of the first rot channels (a multiple of 16) a
+ * pair (a, b) -- channels i and i + rot / 2, or 2i and 2i + 1 if interleaved -- becomes
+ *   (a cos - b sin, b cos + a sin),   products and sums rounded to fp32 one by one;
+ * the other channels stay.  Queries are rounded to their type once, keys are quantised from fp32.  A position
+ * outside of the table turns the rotated channels into NaN (0 in the cache).  Query rows
+ * behind query_start_loc[n_seqs] are not written.  query_out (T, H_q, 128) is contiguous, 16-byte aligned, and may be query
+ * itself.  H_q 0: no queries; cos_sin null: no rotation (H_q must be 0 then).
+ * bounds (H_kv, num_blocks, 2, 128) int8 or null: lowest and highest code of each channel over the positions
+ * that a block written by the call then holds; e4m3 codes in units of 448 / 127 scales, rounded outwards. */
+typedef struct jf_block8_rotary_args {
+  int32_t dtype, codes, H_q, H_kv;
+  int32_t n_seqs, max_blocks, bt_is_i32, positions_i32;
+  int32_t rot, interleaved, table_f32, reserved;
+  int64_t T, table_rows, num_blocks, bt_stride;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const void*    query;
+  const void*    key;
+  const void*    value;
+  const void*    positions;
+  const void*    cos_sin;
+  const int32_t* query_start_loc;
+  const int32_t* seq_lens;
+  const void*    block_table;
+  void*          k_data;
+  float*         k_scales;
+  void*          v_data;
+  float*         v_scales;
+  int8_t*        bounds;
+  void*          query_out;
+} jf_block8_rotary_args;
+
+jf_status_t jf_block8_append_rotary(const jf_block8_rotary_args* args, jf_stream_t stream);
+
 /* ---- attention of packed prompts over their own keys and values -----------------------------------
  * What a library's variable-length attention does for the prefill rows of a step (the call of
  * jetfire_vllm/adapter/decode_path.py:1500-1517), in a kernel of this library.

@@ -62,6 +62,21 @@ class Block8AttnArgs(C.Structure):
     ]
 
 
+class Block8RotaryArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("codes", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32),
+        ("n_seqs", C.c_int32), ("max_blocks", C.c_int32), ("bt_is_i32", C.c_int32), ("positions_i32", C.c_int32),
+        ("rot", C.c_int32), ("interleaved", C.c_int32), ("table_f32", C.c_int32), ("reserved", C.c_int32),
+        ("T", C.c_int64), ("table_rows", C.c_int64), ("num_blocks", C.c_int64), ("bt_stride", C.c_int64),
+        ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+        ("query", C.c_void_p), ("key", C.c_void_p), ("value", C.c_void_p), ("positions", C.c_void_p), ("cos_sin", C.c_void_p),
+        ("query_start_loc", C.c_void_p), ("seq_lens", C.c_void_p), ("block_table", C.c_void_p),
+        ("k_data", C.c_void_p), ("k_scales", C.c_void_p), ("v_data", C.c_void_p), ("v_scales", C.c_void_p),
+        ("bounds", C.c_void_p), ("query_out", C.c_void_p),
+    ]
+
+
 class VarlenAttnArgs(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("n_seqs", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32),
@@ -177,6 +192,7 @@ _SIGS = {
     "jf_block8_append": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32] + [C.c_int64] * 4 +
                          [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32] +
                          [C.c_void_p] * 4 + [C.c_int64, C.c_void_p]),
+    "jf_block8_append_rotary": (C.c_int32, [C.POINTER(Block8RotaryArgs), C.c_void_p]),
     "jf_block8_workspace_bytes": (C.c_uint64, [C.c_int32] * 4),
     "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
     "jf_varlen_attn": (C.c_int32, [C.POINTER(VarlenAttnArgs), C.c_void_p]),

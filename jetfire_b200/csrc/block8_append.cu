@@ -10,11 +10,17 @@
 // sequences' bounds (a token leads its block when it is its sequence's first or stands on a multiple of 16), so
 // there is one launch, no scratch and no order among the writers.
 //
+// With a rotation (jf_block8_append_rotary) a key's pair of channels (a, b) becomes (a cos - b sin, b cos + a sin) on the way, in fp32,
+// products and sums rounded one by one, and is quantised from there: no rounding to 16 bits in between.  The same launch rotates
+// the step's queries.  With block bounds the warp that owns a block of K leaves the lowest and highest code of every channel, over
+// all rows the block then holds: rounding keeps the order, so they are found among the scaled numbers and rounded once.
+//
 // Bound: memory -- 2 bytes read and 1 written per element.  8192 tokens, 8 KV heads, bf16 -> int8 (50 MB): 13.6 us = 3.7 TB/s, 16384: 22.1 us = 4.6
 // TB/s; a warp's start (bounds, length, block id, rows: four dependent trips) and 700 instructions a block are what is left.
 #include "jf_common.cuh"
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace jf {
@@ -28,6 +34,16 @@ struct AppendSide {
   int64_t stride_t, stride_h;
   uint8_t* data;
   float* scales;
+};
+struct Rotation {
+  const void *positions, *cos_sin;   // cos_sin null: none
+  int64_t rows;                      // of the table
+  const uint16_t* q;
+  int64_t q_stride_t, q_stride_h;
+  uint16_t* q_out;
+  int8_t* bounds;                    // null: none
+  int32_t H_q, rot, q_rounds, append_blocks;
+  bool pos_i32, interleaved, table_f32;
 };
 struct AppendParams {
   AppendSide side[2];
@@ -111,6 +127,224 @@ template <bool VEC> __device__ __forceinline__ uint4 load8(const uint16_t* p) {
   }
 }
 
+// ---- rotation ---------------------------------------------------------------------------------
+
+// cos of the angles of a lane's eight channels, and sin with the sign of the other channel of the pair.
+struct Turn { float c[8], s[8]; };
+// N neighbouring numbers of the table (`at` counts them; a multiple of N)
+template <int DT, int N> __device__ __forceinline__ void table_row(const Rotation& R, int64_t at, float* x) {
+  if (R.table_f32) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(R.cos_sin) + at + i));
+      x[i] = f.x; x[i + 1] = f.y; x[i + 2] = f.z; x[i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(R.cos_sin) + at + i));
+      unpack2<DT>(w.x, x[i], x[i + 1]);
+      unpack2<DT>(w.y, x[i + 2], x[i + 3]);
+    }
+  }
+}
+// A token whose position is not in the table gets angles that are no numbers.
+template <int DT> __device__ __forceinline__ Turn turn_of(const Rotation& R, int64_t token, int col) {
+  Turn t;
+  const int64_t pos = R.pos_i32 ? static_cast<const int32_t*>(R.positions)[token] : static_cast<const int64_t*>(R.positions)[token];
+  const bool is = pos >= 0 && pos < R.rows;
+  const int half = R.rot / 2;
+  if (!is || col >= R.rot) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t.c[k] = t.s[k] = __int_as_float(0x7FC00000);
+  } else if (R.interleaved) {
+    float c[4], s[4];
+    table_row<DT, 4>(R, pos * R.rot + col / 2, c);
+    table_row<DT, 4>(R, pos * R.rot + half + col / 2, s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      t.c[2 * k] = t.c[2 * k + 1] = c[k];
+      t.s[2 * k] = -s[k];
+      t.s[2 * k + 1] = s[k];
+    }
+  } else {
+    const int at = col < half ? col : col - half;
+    table_row<DT, 8>(R, pos * R.rot + at, t.c);
+    table_row<DT, 8>(R, pos * R.rot + half + at, t.s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t.s[k] = col < half ? -t.s[k] : t.s[k];
+  }
+  return t;
+}
+// A lane's eight channels of a row, rotated; all lanes of the warp (a pair's halves lie in two lanes of the half warp).
+template <int DT> __device__ __forceinline__ void rotate(const Rotation& R, const uint4& raw, const Turn& t, int col, float* v) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  const int lane = threadIdx.x & 31, over = R.rot >> 4;
+  const int from = R.interleaved ? lane : (lane & 16) | ((lane & 15) < over ? ((lane & 15) + over) & 15 : ((lane & 15) - over) & 15);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float a, b, x, y;
+    unpack2<DT>(w[k], a, b);
+    unpack2<DT>(__shfl_sync(0xFFFFFFFFu, w[k], from), x, y);
+    if (R.interleaved) { x = b; y = a; }
+    v[2 * k] = col < R.rot ? __fadd_rn(__fmul_rn(a, t.c[2 * k]), __fmul_rn(x, t.s[2 * k])) : a;
+    v[2 * k + 1] = col < R.rot ? __fadd_rn(__fmul_rn(b, t.c[2 * k + 1]), __fmul_rn(y, t.s[2 * k + 1])) : b;
+  }
+}
+
+// The queries' rows: a warp per token and 2 * q_rounds heads, half a warp a row.
+template <int DT, bool VEC> __device__ __forceinline__ void rotate_queries(const AppendParams& P, const Rotation& R, int64_t item) {
+  const int lane = threadIdx.x & 31, col = (lane & 15) * 8, per = 2 * R.q_rounds, chunks = (R.H_q + per - 1) / per;
+  const int64_t t = item / chunks;
+  if (t >= min(P.T, P.start[P.n_seqs])) return;      // rows of no sequence
+  const int h0 = static_cast<int>(item % chunks) * per + (lane >> 4);
+  const Turn turn = turn_of<DT>(R, t, col);
+  auto rows = [&](auto n_tag, int h) {
+    constexpr int N = decltype(n_tag)::value;
+    uint4 raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      raw[i] = h + 2 * i < R.H_q ? load8<VEC>(R.q + t * R.q_stride_t + (h + 2 * i) * R.q_stride_h + col) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float v[8];
+      rotate<DT>(R, raw[i], turn, col, v);
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+      }
+      if (h + 2 * i < R.H_q) *reinterpret_cast<uint4*>(R.q_out + (t * R.H_q + h + 2 * i) * JF_HEAD_DIM + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  };
+  if (R.q_rounds == 1) rows(std::integral_constant<int, 1>(), h0);
+  else
+    for (int i = 0; i < R.q_rounds; i += 4) rows(std::integral_constant<int, 4>(), h0 + 2 * i);
+}
+
+// ---- blocks -----------------------------------------------------------------------------------
+
+template <int CODES> __device__ __forceinline__ void decode8(uint2 c, float* v) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = decode1<CODES>((k < 4 ? c.x : c.y) >> 8 * (k & 3) & 255u);
+}
+template <int CODES> __device__ __forceinline__ uint2 encode8(const float* v) {
+  return make_uint2(encode4<CODES>(pair(v[0], v[1]), pair(v[2], v[3])), encode4<CODES>(pair(v[4], v[5]), pair(v[6], v[7])));
+}
+
+// What write_block does for a side that is rotated, or whose bounds are kept.
+template <int DT, int CODES, bool VEC>
+__device__ __forceinline__ void write_block_rotated(const AppendParams& P, const Rotation& R, const AppendSide& S, int h, int t, int cnt, int r,
+                                                    int64_t id) {
+  const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
+  const uint16_t* x = S.x + static_cast<int64_t>(t) * S.stride_t + h * S.stride_h + col;
+  float v[8][8];
+  {
+    uint4 raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 2 * i + half;
+      raw[i] = row < cnt ? load8<VEC>(x + row * S.stride_t) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (R.cos_sin) {
+        const int row = 2 * i + half;
+        const Turn turn = turn_of<DT>(R, t + min(row, cnt - 1), col);
+        rotate<DT>(R, raw[i], turn, col, v[i]);
+      } else {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) unpack2<DT>(w[k], v[i][2 * k], v[i][2 * k + 1]);
+      }
+    }
+  }
+  float* scale_at = S.scales + h * P.num_blocks + id;
+  float old = r > 0 ? *scale_at : 0.0f;
+  if (!(old > 0.0f && old < __int_as_float(0x7F800000))) old = 0.0f;   // never written: nothing to keep
+  float top = 0.0f;
+  bool wild = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {   // infinities and NaN do not count
+      const float a = 2 * i + half < cnt ? fabsf(v[i][k]) : 0.0f;
+      const bool fine = a < __int_as_float(0x7F800000);
+      wild |= !fine;
+      top = fmaxf(top, fine ? a : 0.0f);
+    }
+  wild = __any_sync(0xFFFFFFFFu, wild);
+  top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));   // (not negative: ordered as their bits are)
+  const float s = fmaxf(old, scale_for<CODES>(top)), inv = __frcp_rn(s);
+  uint8_t* rows = S.data + ((h * P.num_blocks + id) * JF_BLOCK_SIZE) * JF_HEAD_DIM + col;
+  float lo[8], hi[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    lo[k] = __int_as_float(0x7F800000);
+    hi[k] = -lo[k];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 2 * i + half;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[i][k] = __fmul_rn(v[i][k], inv);
+    if (wild) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = tame<CODES>(v[i][k]);
+    }
+    if (row < cnt) {
+      *reinterpret_cast<uint2*>(rows + (r + row) * JF_HEAD_DIM) = encode8<CODES>(v[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        lo[k] = fminf(lo[k], v[i][k]);
+        hi[k] = fmaxf(hi[k], v[i][k]);
+      }
+    }
+  }
+  const bool grew = s != old;
+  if (r > 0 && (grew || R.bounds)) {
+    const float ratio = __fdiv_rn(old, s);
+    for (int row = half; row < r; row += 2) {
+      uint2* p = reinterpret_cast<uint2*>(rows + row * JF_HEAD_DIM);
+      float w[8];
+      decode8<CODES>(*p, w);
+      if (grew) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = tame<CODES>(__fmul_rn(w[k], ratio));
+        *p = encode8<CODES>(w);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        lo[k] = fminf(lo[k], w[k]);
+        hi[k] = fmaxf(hi[k], w[k]);
+      }
+    }
+  }
+  if (R.bounds) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      lo[k] = fminf(lo[k], __shfl_xor_sync(0xFFFFFFFFu, lo[k], 16));
+      hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xFFFFFFFFu, hi[k], 16));
+      if (half) lo[k] = hi[k];        // half a warp for each of the two
+    }
+    uint2 code = encode8<CODES>(lo);
+    if (CODES == JF_CODES_E4M3) {     // in units of 448 / 127 scales, outwards
+      float w[8];
+      decode8<CODES>(code, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float u = __fdiv_rn(w[k] * 127.0f, 448.0f);
+        w[k] = half ? ceilf(u) : floorf(u);
+      }
+      code = encode8<JF_CODES_INT8>(w);
+    }
+    *reinterpret_cast<uint2*>(R.bounds + ((h * P.num_blocks + id) * 2 + half) * JF_HEAD_DIM + col) = code;
+  }
+  __syncwarp();
+  if (lane == 0 && grew) *scale_at = s;
+}
+
 // Rows t .. t + cnt of the call into rows r .. r + cnt of block `id`; r rows of its sequence are there already.
 template <int DT, int CODES, bool VEC>
 __device__ __forceinline__ void write_block(const AppendParams& P, const AppendSide& S, int h, int t, int cnt, int r, int64_t id) {
@@ -191,8 +425,15 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
 }
 
 // A warp per (chunk of tokens, head, side): it writes every block whose first token of the call stands in the chunk.
-template <int DT, int CODES, bool VEC>   // VEC: rows may be read 16 bytes at a time
-__global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid_constant__ AppendParams P) {
+template <int DT, int CODES, bool VEC, bool ROTARY>   // VEC: rows may be read 16 bytes at a time
+__global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid_constant__ AppendParams P, const __grid_constant__ Rotation R) {
+  if constexpr (ROTARY)
+    if (static_cast<int>(blockIdx.x) >= R.append_blocks) {
+      pdl_wait();
+      pdl_trigger();
+      rotate_queries<DT, VEC>(P, R, static_cast<int64_t>(blockIdx.x - R.append_blocks) * kWarps + (threadIdx.x >> 5));
+      return;
+    }
   const int lane = threadIdx.x & 31;
   const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), rest = item >> 1;
   const int side = item & 1, h = static_cast<int>(rest % static_cast<uint32_t>(P.H));
@@ -225,10 +466,60 @@ __global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid
     if (blk < P.max_blocks) {
       const int64_t at = s * P.bt_stride + blk;
       const int64_t id = P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
-      if (id >= 0 && id < P.num_blocks) write_block<DT, CODES, VEC>(P, S, h, t, cnt, r, id);
+      if (id >= 0 && id < P.num_blocks) {
+        if (ROTARY && side == 0) write_block_rotated<DT, CODES, VEC>(P, R, S, h, t, cnt, r, id);
+        else write_block<DT, CODES, VEC>(P, S, h, t, cnt, r, id);
+      }
     }
     t += cnt;
   }
+}
+
+// Launches what both entry points check; R null: neither rotation nor bounds.
+jf_status_t launch_append(AppendParams& P, const Rotation* R, int dtype, int codes, cudaStream_t s) {
+  const bool there = P.n_seqs > 0 && P.max_blocks > 0 && P.num_blocks > 0;
+  bool vec = aligned(P.side[0].x, 16) && aligned(P.side[1].x, 16) &&
+             (P.side[0].stride_t | P.side[0].stride_h | P.side[1].stride_t | P.side[1].stride_h) % 8 == 0;
+  const int64_t mean = P.T / std::max(P.n_seqs, 1);
+  // Tokens a warp looks through.  16 suit one prompt (8192 tokens, 8 KV heads: 13.7 us, with chunks of four 17.2), but sequences of one
+  // token would wait for one another there (64 of them beside a prompt of 2048: 31.5 us, with chunks of four 10.9), and
+  // which sequences are long is not known here.
+  P.chunk = P.n_seqs < 4 ? 16 : mean >= 8 ? 4 : mean >= 2 ? 2 : 1;
+  const int64_t items = there ? (P.T + int64_t{P.chunk} - 1) / P.chunk * P.H * 2 : 0;
+  int64_t blocks = (items + kWarps - 1) / kWarps;
+  if (items > INT32_MAX) return JF_ERR_UNSUPPORTED;
+  Rotation rot{};
+  if (R) {
+    rot = *R;
+    rot.append_blocks = static_cast<int32_t>(blocks);
+    if (rot.q && P.n_seqs > 0) {
+      vec &= aligned(rot.q, 16) && (rot.q_stride_t | rot.q_stride_h) % 8 == 0;
+      // Rows a warp goes through, two at a time: eight share the angles of their token, where there are warps enough without
+      rot.q_rounds = static_cast<int64_t>(P.T) * rot.H_q >= 16ll * num_sms() * 32 ? 4 : 1;
+      const int64_t chunks = (rot.H_q + 2 * rot.q_rounds - 1) / (2 * rot.q_rounds);
+      blocks += (P.T * chunks + kWarps - 1) / kWarps;
+    }
+  }
+  if (blocks == 0) return JF_OK;
+  if (blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(blocks)), block(kWarps * 32);
+  auto launch = [&](auto dt, auto code) {
+    constexpr int D = decltype(dt)::value, C = decltype(code)::value;
+    if (R)
+      return vec ? launch_pdl(block8_append_kernel<D, C, true, true>, grid, block, 0, s, P, rot)
+                 : launch_pdl(block8_append_kernel<D, C, false, true>, grid, block, 0, s, P, rot);
+    return vec ? launch_pdl(block8_append_kernel<D, C, true, false>, grid, block, 0, s, P, rot)
+               : launch_pdl(block8_append_kernel<D, C, false, false>, grid, block, 0, s, P, rot);
+  };
+  using Bf16 = std::integral_constant<int, JF_DTYPE_BF16>;
+  using Fp16 = std::integral_constant<int, JF_DTYPE_FP16>;
+  using Int8 = std::integral_constant<int, JF_CODES_INT8>;
+  using E4m3 = std::integral_constant<int, JF_CODES_E4M3>;
+  if (dtype == JF_DTYPE_BF16)
+    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Bf16(), Int8()) : launch(Bf16(), E4m3()));
+  else
+    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Fp16(), Int8()) : launch(Fp16(), E4m3()));
+  return JF_OK;
 }
 
 }  // namespace
@@ -258,27 +549,53 @@ extern "C" jf_status_t jf_block8_append(const void* key, const void* value, int3
   P.n_seqs = n_seqs;
   P.max_blocks = max_blocks;
   P.bt_i32 = bt_is_i32 != 0;
-  const bool vec = aligned(key, 16) && aligned(value, 16) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0;
-  const int64_t mean = T / n_seqs;
-  // Tokens a warp looks through.  16 suit one prompt (8192 tokens, 8 KV heads: 13.7 us, with chunks of four 17.2), but sequences of one
-  // token would wait for one another there (64 of them beside a prompt of 2048: 31.5 us, with chunks of four 10.9), and
-  // which sequences are long is not known here.
-  P.chunk = n_seqs < 4 ? 16 : mean >= 8 ? 4 : mean >= 2 ? 2 : 1;
-  const int64_t items = (T + P.chunk - 1) / P.chunk * H_kv * 2, blocks = (items + kWarps - 1) / kWarps;
-  if (items > INT32_MAX) return JF_ERR_UNSUPPORTED;
-  const auto s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(blocks)), block(kWarps * 32);
-  auto launch = [&](auto dt, auto code) {
-    constexpr int D = decltype(dt)::value, C = decltype(code)::value;
-    return vec ? launch_pdl(block8_append_kernel<D, C, true>, grid, block, 0, s, P) : launch_pdl(block8_append_kernel<D, C, false>, grid, block, 0, s, P);
-  };
-  using Bf16 = std::integral_constant<int, JF_DTYPE_BF16>;
-  using Fp16 = std::integral_constant<int, JF_DTYPE_FP16>;
-  using Int8 = std::integral_constant<int, JF_CODES_INT8>;
-  using E4m3 = std::integral_constant<int, JF_CODES_E4M3>;
-  if (dtype == JF_DTYPE_BF16)
-    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Bf16(), Int8()) : launch(Bf16(), E4m3()));
-  else
-    JF_CUDA_TRY(codes == JF_CODES_INT8 ? launch(Fp16(), Int8()) : launch(Fp16(), E4m3()));
-  return JF_OK;
+  return launch_append(P, nullptr, dtype, codes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" jf_status_t jf_block8_append_rotary(const jf_block8_rotary_args* a, jf_stream_t stream) {
+  using namespace jf;
+  if (!a) return JF_ERR_ARG;
+  if (a->T < 0 || a->T > INT32_MAX - 64 || a->H_kv <= 0 || a->H_q < 0 || a->H_q > 65535 || a->n_seqs < 0 || a->max_blocks < 0 || a->num_blocks < 0)
+    return JF_ERR_ARG;
+  if ((a->dtype != JF_DTYPE_BF16 && a->dtype != JF_DTYPE_FP16) || (a->codes != JF_CODES_INT8 && a->codes != JF_CODES_E4M3)) return JF_ERR_ARG;
+  if (a->H_q > 0 && !a->cos_sin) return JF_ERR_ARG;
+  if (a->cos_sin && (a->rot < 16 || a->rot > JF_HEAD_DIM || a->rot % 16 != 0 || a->table_rows < 0 || a->table_rows > INT64_MAX / 1024 ||
+                     !aligned(a->cos_sin, 16)))
+    return JF_ERR_ARG;
+  if (a->T == 0 || a->n_seqs == 0) return JF_OK;
+  if (!a->query_start_loc || !a->seq_lens || (a->cos_sin && !a->positions)) return JF_ERR_ARG;
+  if (a->H_q > 0 && (!a->query || !a->query_out || !aligned(a->query_out, 16))) return JF_ERR_ARG;
+  if (a->max_blocks > 0 && a->num_blocks > 0) {
+    if (!a->key || !a->value || !a->block_table || !a->k_data || !a->v_data || !a->k_scales || !a->v_scales) return JF_ERR_ARG;
+    if (!aligned(a->k_data, 8) || !aligned(a->v_data, 8) || !aligned(a->k_scales, 4) || !aligned(a->v_scales, 4) || !aligned(a->bounds, 8))
+      return JF_ERR_ARG;
+  }
+  AppendParams P{};
+  P.side[0] = {static_cast<const uint16_t*>(a->key), a->k_stride_t, a->k_stride_h, static_cast<uint8_t*>(a->k_data), a->k_scales};
+  P.side[1] = {static_cast<const uint16_t*>(a->value), a->v_stride_t, a->v_stride_h, static_cast<uint8_t*>(a->v_data), a->v_scales};
+  P.start = a->query_start_loc;
+  P.seq_lens = a->seq_lens;
+  P.table = a->block_table;
+  P.bt_stride = a->bt_stride;
+  P.num_blocks = a->num_blocks;
+  P.T = static_cast<int32_t>(a->T);
+  P.H = a->H_kv;
+  P.n_seqs = a->n_seqs;
+  P.max_blocks = a->max_blocks;
+  P.bt_i32 = a->bt_is_i32 != 0;
+  Rotation R{};
+  R.positions = a->positions;
+  R.cos_sin = a->cos_sin;
+  R.rows = a->table_rows;
+  R.q = a->H_q > 0 ? static_cast<const uint16_t*>(a->query) : nullptr;
+  R.q_stride_t = a->q_stride_t;
+  R.q_stride_h = a->q_stride_h;
+  R.q_out = static_cast<uint16_t*>(a->query_out);
+  R.bounds = a->bounds;
+  R.H_q = a->H_q;
+  R.rot = a->rot;
+  R.pos_i32 = a->positions_i32 != 0;
+  R.interleaved = a->interleaved != 0;
+  R.table_f32 = a->table_f32 != 0;
+  return launch_append(P, a->cos_sin || a->bounds ? &R : nullptr, a->dtype, a->codes, static_cast<cudaStream_t>(stream));
 }

@@ -723,16 +723,26 @@ const int32_t* int32_vector(const at::Tensor& t, int64_t n, const char* name, co
   return static_cast<const int32_t*>(ptr(t));
 }
 
-// block8_append(name, key, value, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales)
-PyObject* block8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded([&]() -> PyObject* {
-    expect_args(n, 10, "block8_append");
-    const char* name = text(a[0]);
-    const at::Tensor &key = tensor(a[1], name, "key_tok"), &value = tensor(a[2], name, "value_tok"),
-                     &start = tensor(a[3], name, "query_start_loc"), &lens = tensor(a[4], name, "seq_lens"),
-                     &bt = tensor(a[5], name, "block_table"), &kd = tensor(a[6], name, "k_data"), &ks = tensor(a[7], name, "k_scales"),
-                     &vd = tensor(a[8], name, "v_data"), &vs = tensor(a[9], name, "v_scales");
-    Block8 c;
+// bounds (H_kv, num_blocks, 2, 128)
+int8_t* block_bounds(const at::Tensor& t, const Block8& c, const char* name, bool written) {
+  here(t, name, "bounds");
+  require(t.scalar_type() == at::kChar && t.is_contiguous() && t.dim() == 4 && t.size(0) == c.h_kv && t.size(1) == c.num_blocks && t.size(2) == 2 &&
+              t.size(3) == JF_HEAD_DIM && reinterpret_cast<uintptr_t>(ptr(t)) % 16 == 0,
+          name, "bounds must be contiguous int8 (H_kv, num_blocks, 2, 128), 16-byte aligned");
+  return static_cast<int8_t*>(written ? out_ptr(t) : const_cast<void*>(ptr(t)));
+}
+
+// What an append takes, into the fields that both of its entry points read.
+struct Append {
+  Block8 c;
+  int64_t T = 0;
+  jf_block8_rotary_args a{};
+
+  Append(PyObject* const* p, const char* name) {   // key, value, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales
+    const at::Tensor &key = tensor(p[0], name, "key_tok"), &value = tensor(p[1], name, "value_tok"),
+                     &start = tensor(p[2], name, "query_start_loc"), &lens = tensor(p[3], name, "seq_lens"),
+                     &bt = tensor(p[4], name, "block_table"), &kd = tensor(p[5], name, "k_data"), &ks = tensor(p[6], name, "k_scales"),
+                     &vd = tensor(p[7], name, "v_data"), &vs = tensor(p[8], name, "v_scales");
     c.side(kd, ks, true, name);
     c.side(vd, vs, false, name);
     here(key, name, "key_tok");
@@ -741,21 +751,92 @@ PyObject* block8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
             "key_tok / value_tok must be (T, H_kv, 128)");
     require(key.scalar_type() == value.scalar_type(), name, "key_tok / value_tok differ in dtype");
     require(key.stride(2) == 1 && value.stride(2) == 1, name, "key_tok / value_tok innermost dim must be contiguous");
-    const int dt = dtype_id(key);
+    a.dtype = dtype_id(key);
     const int64_t seqs = lens.dim() == 1 ? lens.size(0) : -1;
     require(seqs >= 0 && seqs < INT32_MAX, name, "seq_lens must be (sequences,) int32");
-    const int32_t* lp = int32_vector(lens, seqs, name, "seq_lens");
-    const int32_t* sp = int32_vector(start, seqs + 1, name, "query_start_loc");
+    a.seq_lens = int32_vector(lens, seqs, name, "seq_lens");
+    a.query_start_loc = int32_vector(start, seqs + 1, name, "query_start_loc");
     const Table tb = block_table(bt, seqs, name);
+    a.codes = c.codes; a.H_kv = c.h_kv; a.num_blocks = c.num_blocks; a.n_seqs = static_cast<int32_t>(seqs);
+    a.block_table = tb.at; a.bt_is_i32 = tb.is_i32; a.bt_stride = tb.stride; a.max_blocks = tb.width;
+    a.T = T = key.size(0);
+    a.key = ptr(key); a.k_stride_t = key.stride(0); a.k_stride_h = key.stride(1);
+    a.value = ptr(value); a.v_stride_t = value.stride(0); a.v_stride_h = value.stride(1);
+    a.k_data = out_ptr(kd); a.v_data = out_ptr(vd);
+    a.k_scales = static_cast<float*>(out_ptr(ks)); a.v_scales = static_cast<float*>(out_ptr(vs));
+  }
+};
+
+// block8_append(name, key, value, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales, bounds | None)
+PyObject* block8_append(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 11, "block8_append");
+    const char* name = text(p[0]);
+    Append x(p + 1, name);
+    jf_block8_rotary_args& a = x.a;
+    if (p[10] != Py_None) a.bounds = block_bounds(tensor(p[10], name, "bounds"), x.c, name, true);
     const jf_stream_t st = current_stream();
-    const void *kp = ptr(key), *vp = ptr(value);
-    const int64_t T = key.size(0), k_t = key.stride(0), k_h = key.stride(1), v_t = value.stride(0), v_h = value.stride(1);
-    void *kdp = out_ptr(kd), *vdp = out_ptr(vd);
-    auto *ksp = static_cast<float*>(out_ptr(ks)), *vsp = static_cast<float*>(out_ptr(vs));
     return PyLong_FromLong(unlocked([&] {
-      return jf_block8_append(kp, vp, dt, T, c.h_kv, k_t, k_h, v_t, v_h, sp, lp, static_cast<int32_t>(seqs), tb.at, tb.is_i32, tb.stride,
-                              tb.width, c.codes, kdp, ksp, vdp, vsp, c.num_blocks, st);
+      return a.bounds ? jf_block8_append_rotary(&a, st)
+                      : jf_block8_append(a.key, a.value, a.dtype, a.T, a.H_kv, a.k_stride_t, a.k_stride_h, a.v_stride_t, a.v_stride_h, a.query_start_loc,
+                                         a.seq_lens, a.n_seqs, a.block_table, a.bt_is_i32, a.bt_stride, a.max_blocks, a.codes, a.k_data, a.k_scales,
+                                         a.v_data, a.v_scales, a.num_blocks, st);
     }));
+  });
+}
+
+// block8_append_rotary(name, query, key, value, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales, positions, cos_sin,
+//                      interleaved, bounds | None, out | None) -> (status, rotated query)
+PyObject* block8_append_rotary(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 16, "block8_append_rotary");
+    const char* name = text(p[0]);
+    const at::Tensor &q = tensor(p[1], name, "query"), &at_row = tensor(p[11], name, "positions"), &table_in = tensor(p[12], name, "cos_sin");
+    Append x(p + 2, name);
+    jf_block8_rotary_args& a = x.a;
+    here(q, name, "query");
+    here(at_row, name, "positions");
+    here(table_in, name, "cos_sin");
+    require(q.dim() == 3 && q.size(0) == x.T && q.size(2) == JF_HEAD_DIM && q.size(1) > 0 && q.size(1) <= 65535, name, "query must be (T, H_q, 128)");
+    require(dtype_id(q) == a.dtype, name, "query and key_tok differ in dtype");
+    require(q.stride(2) == 1, name, "query innermost dim must be contiguous");
+    require((at_row.scalar_type() == at::kLong || at_row.scalar_type() == at::kInt) && at_row.dim() == 1 && at_row.size(0) == x.T && at_row.is_contiguous(),
+            name, "positions must be contiguous int64 or int32 (T,)");
+    require(table_in.dim() == 2 && table_in.size(1) >= 16 && table_in.size(1) <= JF_HEAD_DIM && table_in.size(1) % 16 == 0, name,
+            "cos_sin must be (positions, rot) with rot a multiple of 16, at most 128");
+    require(table_in.scalar_type() == at::kFloat || table_in.scalar_type() == q.scalar_type(), name, "cos_sin must be float32 or of query's dtype");
+    at::Tensor keep;
+    const at::Tensor* table = &contiguous(table_in, keep);
+    if (reinterpret_cast<uintptr_t>(ptr(*table)) % 16 != 0) table = &(keep = table->clone());
+    a.H_q = static_cast<int32_t>(q.size(1));
+    a.positions_i32 = at_row.scalar_type() == at::kInt;
+    a.rot = static_cast<int32_t>(table->size(1));
+    a.interleaved = truth(p[13]);
+    a.table_f32 = table->scalar_type() == at::kFloat;
+    a.table_rows = table->size(0);
+    if (p[14] != Py_None) a.bounds = block_bounds(tensor(p[14], name, "bounds"), x.c, name, true);
+    at::Tensor out;
+    if (p[15] != Py_None) {
+      out = tensor(p[15], name, "out");
+      here(out, name, "out");
+      require(out.is_contiguous() && out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && reinterpret_cast<uintptr_t>(ptr(out)) % 16 == 0,
+              name, "out must be contiguous, 16-byte aligned, of query's dtype and shape");
+    } else {
+      out = at::detail::empty_cuda(q.sizes(), q.scalar_type(), q.device(), c10::nullopt);
+    }
+    jf_status_t r = JF_OK;
+    if (x.T > 0) {
+      a.query = ptr(q); a.q_stride_t = q.stride(0); a.q_stride_h = q.stride(1);
+      a.positions = ptr(at_row);
+      a.cos_sin = ptr(*table);
+      a.query_out = out_ptr(out);
+      // (a table without rows has no memory; nothing of it is read)
+      alignas(16) static const char none[16] = {};
+      if (!a.cos_sin) a.cos_sin = none;
+      const jf_stream_t st = current_stream();
+      r = unlocked([&] { return jf_block8_append_rotary(&a, st); });
+    }
+    return tuple_of(r, {out});
   });
 }
 
@@ -933,7 +1014,7 @@ PyObject* varlen_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     JF_METHOD(quant_write), JF_METHOD(quant_write_kv), JF_METHOD(fused_attn), JF_METHOD(stage_a), JF_METHOD(stage_b),
     JF_METHOD(decode), JF_METHOD(get_workspace), JF_METHOD(blend), JF_METHOD(step_create), JF_METHOD(step_run),
-    JF_METHOD(block8_append), JF_METHOD(block8_attn), JF_METHOD(varlen_attn),
+    JF_METHOD(block8_append), JF_METHOD(block8_append_rotary), JF_METHOD(block8_attn), JF_METHOD(varlen_attn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "tensor-taking half of jetfire_b200.ops", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

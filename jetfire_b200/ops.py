@@ -527,7 +527,7 @@ def int8tc_softmax_v_with_pre_corr_reg_stats(scores, softmax_m, softmax_inv_z, v
 BLOCK8_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 
 
-def block8_append(key_tok, value_tok, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales) -> None:
+def block8_append(key_tok, value_tok, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data, v_scales, *, bounds=None) -> None:
     """In place: the new tokens of a step into a paged cache of 8-bit codes.
 
     ``key_tok / value_tok (T, H_kv, 128)`` bf16 or fp16 (any strides with a contiguous innermost dim);
@@ -538,9 +538,32 @@ def block8_append(key_tok, value_tok, query_start_loc, seq_lens, block_table, k_
     smallest power of two that brings amax to at most 448.  A block that holds earlier positions of its sequence
     keeps the larger scale, its codes rounded to it where it grew.  NaN becomes 0, an infinity the largest code, and neither
     counts in amax.  Rows behind the last sequence and positions without a valid block are skipped.  Every
-    block is written for one sequence only (blocks that sequences share are full and are not written)."""
+    block is written for one sequence only (blocks that sequences share are full and are not written).
+
+    ``bounds (H_kv, num_blocks, 2, 128)`` int8, where given, gets the lowest and highest code of K of every channel in each block
+    that the call writes, over all positions that the block then holds: what ``block8_sparse_decode_attn`` selects by.  Bounds of
+    e4m3 codes are in units of 448 / 127 of the scale, rounded outwards."""
     check("block8_append", _host.block8_append("block8_append", key_tok, value_tok, query_start_loc, seq_lens, block_table,
-                                               k_data, k_scales, v_data, v_scales))
+                                               k_data, k_scales, v_data, v_scales, bounds))
+
+
+def block8_append_rotary(query, key_tok, value_tok, positions, cos_sin, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data,
+                         v_scales, *, interleaved=False, bounds=None, out=None):
+    """``block8_append`` of keys that are rotated by their positions on the way, and the rotated queries of the step.
+
+    ``query (T, H_q, 128)`` and ``key_tok / value_tok (T, H_kv, 128)`` bf16 or fp16 (any strides with a contiguous
+    innermost dim); ``positions (T,)`` int64 or int32: rows of ``cos_sin (positions, rot)``, float32 or of the tokens' dtype,
+    which hold the cosines of ``rot / 2`` angles, then the sines (``rot``: a multiple of 16 up to 128; the channels behind it stay).  A
+    pair of channels ``(a, b)`` -- ``i`` and ``i + rot / 2``, or ``2i`` and ``2i + 1`` where ``interleaved`` -- becomes ``(a cos - b
+    sin, b cos + a sin)``, products and sums rounded to fp32 one by one.  Queries are rounded to their dtype once; keys are
+    quantised from fp32.  A position outside of the table makes the rotated channels NaN (0 in the cache).  The other arguments are
+    those of ``block8_append``.  ``out``: contiguous, 16-byte aligned; it may be ``query``.  Rows behind the last sequence are not written.
+    Returns the rotated queries ``(T, H_q, 128)``."""
+    name = "block8_append_rotary"
+    st, rotated = _host.block8_append_rotary(name, query, key_tok, value_tok, query_start_loc, seq_lens, block_table, k_data, k_scales, v_data,
+                                             v_scales, positions, cos_sin, interleaved, bounds, out)
+    check(name, st)
+    return rotated
 
 
 def block8_workspace_bytes(B, H_q, H_kv, max_S) -> int:
