@@ -587,6 +587,25 @@ typedef struct jf_block8_rotary_args {
 
 jf_status_t jf_block8_append_rotary(const jf_block8_rotary_args* args, jf_stream_t stream);
 
+/* jf_block8_sparse_attn is jf_block8_attn over at most top_blocks blocks of each sequence, chosen by sequence and KV
+ * head.  A sequence of n = ceil(length / 16) <= top_blocks blocks is attended to as a whole; of others the first first_blocks, the last
+ * last_blocks (>= 1), and of those between the ones with the highest scores, ties to the lower number:
+ *   score_j = max_h fl(fl(d_hj * qs_h) * unit_j),   d_hj = sum_c min(q8_hc, 0) lo_jc + max(q8_hc, 0) hi_jc,
+ *   qs_h = max(amax|q_h|, 2^-100) / 127,   q8_h = rint(q_h / qs_h),
+ * h through the query heads of the KV head, lo and hi the block's bounds, unit_j its K scale (e4m3: times 448 / 127), all in
+ * fp32.  A head with an element that is no number has no score, nor has a block without a valid id or with a NaN as its scale; what
+ * has none comes last.  chosen (B, H_kv, top_blocks): the blocks' numbers, rising, then -1.
+ * attn.attn_scale > 0, attn.window 0, no prefix_lens or alibi_slopes; attn.max_S up to 2^22.  Three launches at most. */
+typedef struct jf_block8_sparse_args {
+  jf_block8_attn_args attn;
+  const int8_t* bounds;           /* (H_kv, num_blocks, 2, 128), 16-byte aligned */
+  int32_t*      chosen;
+  int32_t top_blocks, first_blocks, last_blocks, reserved;
+} jf_block8_sparse_args;
+
+uint64_t    jf_block8_sparse_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S, int32_t top_blocks);
+jf_status_t jf_block8_sparse_attn(const jf_block8_sparse_args* args, jf_stream_t stream);
+
 /* ---- attention of packed prompts over their own keys and values -----------------------------------
  * What a library's variable-length attention does for the prefill rows of a step (the call of
  * jetfire_vllm/adapter/decode_path.py:1500-1517), in a kernel of this library.

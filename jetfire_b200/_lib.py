@@ -62,6 +62,11 @@ class Block8AttnArgs(C.Structure):
     ]
 
 
+class Block8SparseArgs(C.Structure):
+    _fields_ = [("attn", Block8AttnArgs), ("bounds", C.c_void_p), ("chosen", C.c_void_p), ("top_blocks", C.c_int32),
+                ("first_blocks", C.c_int32), ("last_blocks", C.c_int32), ("reserved", C.c_int32)]
+
+
 class Block8RotaryArgs(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("codes", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32),
@@ -195,6 +200,8 @@ _SIGS = {
     "jf_block8_append_rotary": (C.c_int32, [C.POINTER(Block8RotaryArgs), C.c_void_p]),
     "jf_block8_workspace_bytes": (C.c_uint64, [C.c_int32] * 4),
     "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
+    "jf_block8_sparse_workspace_bytes": (C.c_uint64, [C.c_int32] * 5),
+    "jf_block8_sparse_attn": (C.c_int32, [C.POINTER(Block8SparseArgs), C.c_void_p]),
     "jf_varlen_attn": (C.c_int32, [C.POINTER(VarlenAttnArgs), C.c_void_p]),
     "jf_varlen_status": (C.c_int32, [C.c_int32]),
     "jf_varlen_record": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),

@@ -24,7 +24,7 @@
 //
 // Bound: memory, 256 bytes per (position, KV head).  Four sequences of 65536 positions, 64 / 8 heads, int8: 101 us = 5.3 TB/s (copies of the
 // same blocks without arithmetic, in an earlier cut of the work, 102; a plain copy runs at 6.5 TB/s); short ones by their dependent trips to memory: 6.2 us.
-#include "jf_common.cuh"
+#include "block8.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -60,7 +60,10 @@ struct AttnParams {
   int32_t B, H_q, H_kv, G, groups, max_S, max_blocks, window, target, min_piece, pieces;
   float scale, softcap;
   int32_t cluster;              // blocks that share a sequence, 1 where pieces are looked for
-  bool bt_i32, one_wave;
+  const int32_t* chosen;        // the blocks to be scanned, (B, H_kv, top), or null: all
+  const void* shared;           // the table of the first shared_blocks blocks of every sequence; the sequence's own follow (max_blocks counts both)
+  int32_t top, shared_blocks;
+  bool bt_i32, one_wave, shared_i32;
 };
 
 // The root of the factor that takes an output to a reference d above its own; a sum is multiplied by it twice.  (V scales up to 2^226 apart put d
@@ -74,7 +77,7 @@ __device__ __forceinline__ Span span_of(const AttnParams& P, int length, int pre
   s.len = max(0, min(length, min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
   const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
   s.prefix = s.lo = s.head = s.first = 0;
-  s.count = blocks;
+  s.count = P.chosen ? min(blocks, P.top) : blocks;
   if (P.window > 0 && P.window < s.len) {
     s.lo = s.len - P.window;
     s.prefix = max(0, min(prefix, s.lo));
@@ -151,6 +154,10 @@ __device__ __forceinline__ int64_t block_id(const AttnParams& P, int64_t at) {
   return P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
 }
 
+__device__ __forceinline__ int64_t shared_id(const AttnParams& P, int at) {
+  return P.shared_i32 ? static_cast<const int32_t*>(P.shared)[at] : static_cast<const int64_t*>(P.shared)[at];
+}
+
 // The lower or upper two of four codes as fp16.  int8: `w` has its sign bits turned over, 0x6400 + u is 1024 + u.
 template <int CODES> __device__ __forceinline__ uint32_t bias(uint32_t w) { return CODES == JF_CODES_INT8 ? w ^ 0x80808080u : w; }
 template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
@@ -162,11 +169,6 @@ template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32
   else
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
   return d;
-}
-__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // cap * tanh(x / cap) of four scores, for the whole warp the same way: up to |x| = cap by a polynomial fitted for the least
 // relative error (6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).  A score that is NaN stays one either way.
@@ -190,15 +192,7 @@ __device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap)
   }
 }
 
-// The blocks of a cluster share a sequence's pieces: no piece has to be looked for, and the results meet in shared memory.
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {   // the same place in another block's shared memory
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  return a;
-}
+// (The blocks of a cluster share a sequence's pieces: no piece has to be looked for, and the results meet in shared memory.)
 __device__ __forceinline__ float4 load4_from(uint32_t at) {
   float4 x;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
@@ -264,8 +258,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   // The warp's blocks: begin + warp, + kWarps, ...; 32 of them are looked up at a time, a lane each.
   const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;
   const int64_t table_row = static_cast<int64_t>(b) * P.bt_stride, head_row = static_cast<int64_t>(kvh) * P.num_blocks;
+  const int32_t* chosen = P.chosen ? P.chosen + (static_cast<int64_t>(b) * P.H_kv + kvh) * P.top : nullptr;
   auto position_of = [&](int i) {   // first position of the warp's i-th block
     const int at = begin + warp + i * kWarps;
+    if (chosen) return chosen[at] * JF_BLOCK_SIZE;
     return (at < span.head ? at : span.first + at - span.head) * JF_BLOCK_SIZE;
   };
   struct Look { int id, pos; float ks, vs; };   // pos: 1 more where some of the block's positions are not seen
@@ -273,7 +269,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     Look r{-1, 0, 0.0f, 0.0f};
     if (i0 + lane < mine) {
       r.pos = position_of(i0 + lane);
-      const int64_t id = block_id(P, table_row + r.pos / JF_BLOCK_SIZE);
+      const int blk = r.pos / JF_BLOCK_SIZE - P.shared_blocks;
+      const int64_t id = blk < 0 ? shared_id(P, blk + P.shared_blocks) : block_id(P, table_row + blk);
       r.id = id < 0 || id >= P.num_blocks ? -1 : static_cast<int>(id);
       if (r.id >= 0) {
         r.ks = P.k_scales[head_row + r.id];
@@ -828,30 +825,29 @@ template <int CODES, int DT> jf_status_t launch_attn(const AttnParams& P, int nt
 }
 
 }  // namespace
-}  // namespace jf
 
-extern "C" uint64_t jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S) {
-  jf::Plan p;
-  return jf::make_plan(B, H_q, H_kv, max_S, p) ? p.bytes : 0;
+uint64_t block8_attn_workspace(int B, int H_q, int H_kv, int max_S) {
+  Plan p;
+  return make_plan(B, H_q, H_kv, max_S, p) ? p.bytes : 0;
 }
 
-extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t stream) {
-  using namespace jf;
-  if (!a) return JF_ERR_ARG;
+jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from, jf_stream_t stream, bool launch) {
   if ((a->q_dtype != JF_DTYPE_BF16 && a->q_dtype != JF_DTYPE_FP16) || (a->codes != JF_CODES_INT8 && a->codes != JF_CODES_E4M3)) return JF_ERR_ARG;
   if (a->B < 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->window < 0) return JF_ERR_ARG;
   if (a->softcap != 0.0f && !(a->softcap >= 1.0e-30f && a->softcap <= 1.0e30f)) return JF_ERR_ARG;
   if (a->B == 0) return JF_OK;
   Plan p;
-  if (!make_plan(a->B, a->H_q, a->H_kv, a->max_S, p)) return JF_ERR_ARG;
+  const int max_S = from.chosen ? static_cast<int>(std::min<int64_t>(a->max_S, int64_t{from.top} * JF_BLOCK_SIZE)) : a->max_S;   // scanned
+  if (!make_plan(a->B, a->H_q, a->H_kv, max_S, p)) return JF_ERR_ARG;
   if (!a->q || !a->seq_lens || !a->out) return JF_ERR_ARG;
   // (a table without columns and a cache without blocks have no memory; nothing of them is read)
   if (a->max_blocks > 0 && !a->block_table) return JF_ERR_ARG;
   if (a->num_blocks > 0 && (!a->k_data || !a->v_data || !a->k_scales || !a->v_scales)) return JF_ERR_ARG;
   if (!aligned(a->q, 16) || !aligned(a->k_data, 16) || !aligned(a->v_data, 16) || !aligned(a->out, 8)) return JF_ERR_ARG;
   if (a->num_blocks > INT32_MAX) return JF_ERR_UNSUPPORTED;
-  if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE) return JF_ERR_UNSUPPORTED;
+  if (a->max_blocks > (INT32_MAX - JF_BLOCK_SIZE) / JF_BLOCK_SIZE - from.shared_blocks) return JF_ERR_UNSUPPORTED;
   if (!a->workspace || a->workspace_bytes < p.bytes || !aligned(a->workspace, 16)) return JF_ERR_WORKSPACE;
+  if (!launch) return JF_OK;
   AttnParams P{};
   P.q = a->q;
   P.k_data = static_cast<const uint8_t*>(a->k_data);
@@ -870,13 +866,15 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
   P.num_blocks = a->num_blocks;
   P.bt_stride = a->bt_stride;
   P.B = a->B; P.H_q = a->H_q; P.H_kv = a->H_kv; P.G = p.G; P.groups = p.groups;
-  P.max_S = a->max_S; P.max_blocks = a->max_blocks; P.window = a->window;
+  P.max_S = a->max_S; P.max_blocks = a->max_blocks + from.shared_blocks; P.window = a->window;
   P.target = p.target; P.min_piece = p.min_piece; P.pieces = p.pieces;
   // (only where a piece is several rounds of a block's warps: the search takes 0.2 us)
-  const int64_t longest = a->window > 0 ? std::min(a->max_S, a->window) : a->max_S;
+  const int64_t longest = a->window > 0 ? std::min(max_S, a->window) : max_S;
   P.one_wave = a->B > 1 && a->B <= 32 && 2 * a->B <= p.pieces && longest / JF_BLOCK_SIZE * a->B > 32ll * p.target;
   P.scale = a->attn_scale; P.softcap = a->softcap;
   P.bt_i32 = a->bt_is_i32 != 0;
+  P.chosen = from.chosen; P.top = from.top;
+  P.shared = from.shared; P.shared_blocks = from.shared_blocks; P.shared_i32 = from.shared_i32;
   P.cluster = cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
   const bool feat = a->softcap > 0.0f || a->alibi_slopes;
   const auto s = static_cast<cudaStream_t>(stream);
@@ -902,4 +900,14 @@ extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t 
               : each >= kFewPieces ? join(integral_constant<int, 4>(), integral_constant<int, 8>(), 1)
                                    : join(integral_constant<int, 4>(), integral_constant<int, 4>(), 1));
   return JF_OK;
+}
+
+}  // namespace jf
+
+extern "C" uint64_t jf_block8_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S) {
+  return jf::block8_attn_workspace(B, H_q, H_kv, max_S);
+}
+
+extern "C" jf_status_t jf_block8_attn(const jf_block8_attn_args* a, jf_stream_t stream) {
+  return a ? jf::block8_attend(a, jf::Block8Source{}, stream, true) : JF_ERR_ARG;
 }

@@ -840,6 +840,82 @@ PyObject* block8_append_rotary(PyObject*, PyObject* const* p, Py_ssize_t n) {
   });
 }
 
+// What every attention over the cache takes: q, k_data, k_scales, v_data, v_scales, then the options below.
+struct Attention {
+  const char* name;
+  Block8 c;
+  jf_block8_attn_args a{};
+  int64_t B = 0;
+  at::Tensor keep, scratch, out, lse;
+
+  // p: q, k_data, k_scales, v_data, v_scales
+  Attention(PyObject* const* p, PyObject* table, PyObject* seq_lens, PyObject* const* sizes, PyObject* scale, PyObject* softcap, const char* of) : name(of) {
+    const at::Tensor &q_in = tensor(p[0], name, "q"), &kd = tensor(p[1], name, "k_data"), &ks = tensor(p[2], name, "k_scales"),
+                     &vd = tensor(p[3], name, "v_data"), &vs = tensor(p[4], name, "v_scales"), &bt = tensor(table, name, "block_table"),
+                     &lens = tensor(seq_lens, name, "seq_lens");
+    c.side(kd, ks, true, name);
+    c.side(vd, vs, false, name);
+    const int32_t max_S = as_int32(sizes[0]), h_q = as_int32(sizes[1]), h_kv = as_int32(sizes[2]);
+    require(as_int32(sizes[3]) == JF_BLOCK_SIZE, name, "block_size must be 16");
+    require(h_kv == c.h_kv, name, "H_kv differs from the cache's");
+    require(h_q > 0 && h_q % h_kv == 0, name, "H_q must be a multiple of H_kv");
+    require(max_S > 0, name, "max_S must be positive");
+    here(q_in, name, "q");
+    B = lens.dim() == 1 ? lens.size(0) : -1;
+    require(B >= 0 && B <= INT32_MAX, name, "seq_lens must be (B,) int32");
+    require(q_in.dim() == 3 && q_in.size(0) == B && q_in.size(1) == h_q && q_in.size(2) == JF_HEAD_DIM, name, "q must be (B, H_q, 128)");
+    q = &contiguous(q_in, keep);
+    if (reinterpret_cast<uintptr_t>(ptr(*q)) % 16 != 0) q = &(keep = q->clone());
+    a.codes = c.codes;
+    a.q_dtype = dtype_id(q_in);
+    a.B = static_cast<int32_t>(B); a.H_q = h_q; a.H_kv = h_kv; a.max_S = max_S;
+    const Table tb = block_table(bt, B, name);
+    a.max_blocks = tb.width; a.bt_is_i32 = tb.is_i32; a.bt_stride = tb.stride; a.block_table = tb.at;
+    a.attn_scale = static_cast<float>(real(scale));
+    const double cap = real(softcap);
+    require(cap == 0.0 || (cap >= 1.001e-30 && cap <= 0.999e30), name, "softcap must be 0 (none) or between 1e-30 and 1e30");
+    a.softcap = static_cast<float>(cap);
+    a.num_blocks = c.num_blocks;
+    a.seq_lens = int32_vector(lens, B, name, "seq_lens");
+    kv[0] = &kd; kv[1] = &ks; kv[2] = &vd; kv[3] = &vs;
+  }
+  void outputs(PyObject* own) {
+    if (own != Py_None) {
+      out = tensor(own, name, "out");
+      here(out, name, "out");
+      require(out.is_contiguous() && out.scalar_type() == q->scalar_type() && out.sizes() == q->sizes(), name,
+              "out must be contiguous, of q's dtype and shape");
+    } else {
+      out = at::detail::empty_cuda({B, a.H_q, JF_HEAD_DIM}, q->scalar_type(), q->device(), c10::nullopt);
+    }
+    lse = at::detail::empty_cuda({B, a.H_q}, at::kFloat, q->device(), c10::nullopt);
+  }
+  // Scratch of `bytes`, the caller's or the library's, and the addresses.
+  void addresses(PyObject* own, uint64_t bytes) {
+    require(bytes > 0, name, "bad shape");
+    if (own != Py_None) {
+      scratch = tensor(own, name, "workspace");
+      here(scratch, name, "workspace");
+      require(scratch.is_contiguous(), name, "workspace must be contiguous");
+    } else {
+      scratch = workspace(bytes, q->device());
+    }
+    const auto base = reinterpret_cast<uintptr_t>(out_ptr(scratch)), at = (base + 255) / 256 * 256;
+    const uint64_t size = static_cast<uint64_t>(scratch.numel()) * scratch.element_size();
+    a.workspace = reinterpret_cast<void*>(at);
+    a.workspace_bytes = size > at - base ? size - (at - base) : 0;
+    a.q = ptr(*q);
+    a.k_data = ptr(*kv[0]);
+    a.k_scales = static_cast<const float*>(ptr(*kv[1]));
+    a.v_data = ptr(*kv[2]);
+    a.v_scales = static_cast<const float*>(ptr(*kv[3]));
+    a.out = out_ptr(out);
+    a.lse = static_cast<float*>(out_ptr(lse));
+  }
+
+  const at::Tensor *q, *kv[4];
+};
+
 // block8_attn(name, q, k_data, k_scales, v_data, v_scales, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale,
 //             softcap, alibi_slopes | None, window (0: none), prefix_lens | None, workspace | None, out | None)
 //   -> (status, out, lse)
@@ -847,82 +923,54 @@ PyObject* block8_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 19, "block8_attn");
     const char* name = text(p[0]);
-    const at::Tensor &q_in = tensor(p[1], name, "q"), &kd = tensor(p[2], name, "k_data"), &ks = tensor(p[3], name, "k_scales"),
-                     &vd = tensor(p[4], name, "v_data"), &vs = tensor(p[5], name, "v_scales"), &bt = tensor(p[6], name, "block_table"),
-                     &lens = tensor(p[7], name, "seq_lens");
-    Block8 c;
-    c.side(kd, ks, true, name);
-    c.side(vd, vs, false, name);
-    const int32_t max_S = as_int32(p[8]), h_q = as_int32(p[9]), h_kv = as_int32(p[10]);
-    require(as_int32(p[11]) == JF_BLOCK_SIZE, name, "block_size must be 16");
-    require(h_kv == c.h_kv, name, "H_kv differs from the cache's");
-    require(h_q > 0 && h_q % h_kv == 0, name, "H_q must be a multiple of H_kv");
-    require(max_S > 0, name, "max_S must be positive");
-    here(q_in, name, "q");
-    const int64_t B = lens.dim() == 1 ? lens.size(0) : -1;
-    require(B >= 0 && B <= INT32_MAX, name, "seq_lens must be (B,) int32");
-    require(q_in.dim() == 3 && q_in.size(0) == B && q_in.size(1) == h_q && q_in.size(2) == JF_HEAD_DIM, name, "q must be (B, H_q, 128)");
-    at::Tensor keep;
-    const at::Tensor* qc = &contiguous(q_in, keep);
-    if (reinterpret_cast<uintptr_t>(ptr(*qc)) % 16 != 0) qc = &(keep = qc->clone());
-    jf_block8_attn_args a{};
-    a.codes = c.codes;
-    a.q_dtype = dtype_id(q_in);
-    a.B = static_cast<int32_t>(B); a.H_q = h_q; a.H_kv = h_kv; a.max_S = max_S;
-    const Table tb = block_table(bt, B, name);
-    a.max_blocks = tb.width; a.bt_is_i32 = tb.is_i32; a.bt_stride = tb.stride; a.block_table = tb.at;
-    a.attn_scale = static_cast<float>(real(p[12]));
-    const double cap = real(p[13]);
-    require(cap == 0.0 || (cap >= 1.001e-30 && cap <= 0.999e30), name, "softcap must be 0 (none) or between 1e-30 and 1e30");
-    a.softcap = static_cast<float>(cap);
+    Attention x(p + 1, p[6], p[7], p + 8, p[12], p[13], name);
+    jf_block8_attn_args& a = x.a;
     a.window = as_int32(p[15]);
     require(a.window >= 0, name, "window must be positive, or None");
-    a.num_blocks = c.num_blocks;
-    a.seq_lens = int32_vector(lens, B, name, "seq_lens");
     if (p[14] != Py_None) {
       const at::Tensor& s = tensor(p[14], name, "alibi_slopes");
       here(s, name, "alibi_slopes");
-      require(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == h_q && s.is_contiguous(), name, "alibi_slopes must be contiguous float32 (H_q,)");
+      require(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == a.H_q && s.is_contiguous(), name, "alibi_slopes must be contiguous float32 (H_q,)");
       a.alibi_slopes = static_cast<const float*>(ptr(s));
     }
-    if (p[16] != Py_None) a.prefix_lens = int32_vector(tensor(p[16], name, "prefix_lens"), B, name, "prefix_lens");
-    const c10::Device device = q_in.device();
-    at::Tensor out;
-    if (p[18] != Py_None) {
-      out = tensor(p[18], name, "out");
-      here(out, name, "out");
-      require(out.is_contiguous() && out.scalar_type() == q_in.scalar_type() && out.sizes() == q_in.sizes(), name,
-              "out must be contiguous, of q's dtype and shape");
-    } else {
-      out = at::detail::empty_cuda({B, h_q, JF_HEAD_DIM}, q_in.scalar_type(), device, c10::nullopt);
-    }
-    at::Tensor lse = at::detail::empty_cuda({B, h_q}, at::kFloat, device, c10::nullopt), scratch;
+    if (p[16] != Py_None) a.prefix_lens = int32_vector(tensor(p[16], name, "prefix_lens"), x.B, name, "prefix_lens");
+    x.outputs(p[18]);
     jf_status_t r = JF_OK;
-    if (B > 0) {
-      const uint64_t bytes = jf_block8_workspace_bytes(a.B, h_q, h_kv, max_S);
-      require(bytes > 0, name, "bad shape");
-      if (p[17] != Py_None) {
-        scratch = tensor(p[17], name, "workspace");
-        here(scratch, name, "workspace");
-        require(scratch.is_contiguous(), name, "workspace must be contiguous");
-      } else {
-        scratch = workspace(bytes, device);
-      }
-      const auto base = reinterpret_cast<uintptr_t>(out_ptr(scratch)), at = (base + 255) / 256 * 256;
-      const uint64_t size = static_cast<uint64_t>(scratch.numel()) * scratch.element_size();
-      a.workspace = reinterpret_cast<void*>(at);
-      a.workspace_bytes = size > at - base ? size - (at - base) : 0;
-      a.q = ptr(*qc);
-      a.k_data = ptr(kd);
-      a.v_data = ptr(vd);
-      a.k_scales = static_cast<const float*>(ptr(ks));
-      a.v_scales = static_cast<const float*>(ptr(vs));
-      a.out = out_ptr(out);
-      a.lse = static_cast<float*>(out_ptr(lse));
+    if (x.B > 0) {
+      x.addresses(p[17], jf_block8_workspace_bytes(a.B, a.H_q, a.H_kv, a.max_S));
       const jf_stream_t st = current_stream();
       r = unlocked([&] { return jf_block8_attn(&a, st); });
     }
-    return tuple_of(r, {out, lse});
+    return tuple_of(r, {x.out, x.lse});
+  });
+}
+
+// block8_sparse_attn(name, q, k_data, k_scales, v_data, v_scales, bounds, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale,
+//                    softcap, top_blocks, first_blocks, last_blocks, workspace | None, out | None) -> (status, out, lse, chosen)
+PyObject* block8_sparse_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 20, "block8_sparse_attn");
+    const char* name = text(p[0]);
+    Attention x(p + 1, p[7], p[8], p + 9, p[13], p[14], name);
+    jf_block8_sparse_args s{};
+    s.top_blocks = as_int32(p[15]);
+    s.first_blocks = as_int32(p[16]);
+    s.last_blocks = as_int32(p[17]);
+    require(s.top_blocks > 0 && s.first_blocks >= 0 && s.last_blocks >= 1 && int64_t{s.first_blocks} + s.last_blocks <= s.top_blocks, name,
+            "top_blocks must hold first_blocks (>= 0) and last_blocks (>= 1)");
+    require(x.a.attn_scale > 0.0f, name, "attn_scale must be positive");
+    s.bounds = block_bounds(tensor(p[6], name, "bounds"), x.c, name, false);
+    x.outputs(p[19]);
+    at::Tensor chosen = at::detail::empty_cuda({x.B, x.a.H_kv, s.top_blocks}, at::kInt, x.q->device(), c10::nullopt);
+    jf_status_t r = JF_OK;
+    if (x.B > 0) {
+      x.addresses(p[18], jf_block8_sparse_workspace_bytes(x.a.B, x.a.H_q, x.a.H_kv, x.a.max_S, s.top_blocks));
+      s.attn = x.a;
+      s.chosen = static_cast<int32_t*>(out_ptr(chosen));
+      const jf_stream_t st = current_stream();
+      r = unlocked([&] { return jf_block8_sparse_attn(&s, st); });
+    }
+    return tuple_of(r, {x.out, x.lse, chosen});
   });
 }
 
@@ -1014,7 +1062,7 @@ PyObject* varlen_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     JF_METHOD(quant_write), JF_METHOD(quant_write_kv), JF_METHOD(fused_attn), JF_METHOD(stage_a), JF_METHOD(stage_b),
     JF_METHOD(decode), JF_METHOD(get_workspace), JF_METHOD(blend), JF_METHOD(step_create), JF_METHOD(step_run),
-    JF_METHOD(block8_append), JF_METHOD(block8_append_rotary), JF_METHOD(block8_attn), JF_METHOD(varlen_attn),
+    JF_METHOD(block8_append), JF_METHOD(block8_append_rotary), JF_METHOD(block8_attn), JF_METHOD(block8_sparse_attn), JF_METHOD(varlen_attn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "tensor-taking half of jetfire_b200.ops", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -595,6 +595,30 @@ def block8_decode_attn(q, k_data, k_scales, v_data, v_scales, block_table, seq_l
     return out, lse
 
 
+def block8_sparse_workspace_bytes(B, H_q, H_kv, max_S, top_blocks) -> int:
+    """Scratch of ``block8_sparse_decode_attn`` for calls of these sizes."""
+    return int(lib.jf_block8_sparse_workspace_bytes(B, H_q, H_kv, max_S, top_blocks))
+
+
+def block8_sparse_decode_attn(q, k_data, k_scales, v_data, v_scales, bounds, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale, *,
+                              top_blocks, first_blocks=1, last_blocks=2, softcap=0.0, workspace=None, out=None):
+    """``block8_decode_attn`` over at most ``top_blocks`` blocks of 16 positions of each sequence, chosen by sequence and KV head.
+
+    A sequence of no more blocks than that is attended to as a whole.  Of others the first ``first_blocks``, the last ``last_blocks``
+    (>= 1: the newest positions) and, of those between, the blocks with the highest scores are chosen, ties to the lower one.  A
+    block's score is an upper bound of ``q.k`` over its positions, the largest over the query heads of the KV head, from the
+    query in 8 bits and ``bounds (H_kv, num_blocks, 2, 128)`` int8, which the appends keep (``block8_append(..., bounds=)``): all its
+    steps are exact or rounded to fp32 one by one, so a choice does not depend on the order of sums.  A query head that holds a NaN or
+    an infinity does not count, nor does a block whose id is not in the cache or whose K scale is NaN (such blocks come last).  ``attn_scale``
+    is positive; there is no window and no bias by distance.  ``max_S`` goes up to 2^22.  Returns ``(out (B, H_q, 128) like q, lse (B, H_q) float32 over the
+    chosen blocks, chosen (B, H_kv, top_blocks) int32)``: the chosen blocks' numbers in the sequence, rising, then -1."""
+    name = "block8_sparse_decode_attn"
+    st, out, lse, chosen = _host.block8_sparse_attn(name, q, k_data, k_scales, v_data, v_scales, bounds, block_table, seq_lens, max_S, H_q, H_kv,
+                                                    block_size, attn_scale, softcap, top_blocks, first_blocks, last_blocks, workspace, out)
+    check(name, st)
+    return out, lse, chosen
+
+
 def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=None, softcap=0.0, alibi_slopes=None,
                         prefix_lens=None, out=None, status_record=None):
     """Attention of packed prompts over their own keys and values, each sequence (document) by itself.

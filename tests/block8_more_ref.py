@@ -67,3 +67,31 @@ class Cache:
 
     def values(self, side):
         return self.code[side] * self.scale[side][..., None, None]
+
+
+def choose(q, lo_hi, ks, ids, n, top, first, last, codes, blocks):
+    """The blocks chosen for one sequence and KV head: ``q (heads, 128)`` float64, ``lo_hi (blocks, 2, 128)`` and ``ks (blocks,)`` of the
+    head, ``ids`` of the sequence's n blocks.  Every step of a score is exact or rounded to fp32."""
+    if n <= top:
+        return list(range(n))
+    ids = ids[:n]
+    is_there = (ids >= 0) & (ids < blocks)
+    at = ids.clamp(0, blocks - 1)
+    unit = R.fl32(ks[at] * (1.0 if codes == torch.int8 else float(torch.tensor(448.0 / 127.0))))
+    score = torch.full((n,), float("-inf"), dtype=torch.float64)
+    near = lo_hi[at].double()
+    for h in range(q.shape[0]):
+        if not bool(torch.isfinite(q[h]).all()):
+            continue
+        step = R.fl32(q[h].abs().max().clamp(min=2.0 ** -100) / 127)
+        q8 = torch.round(R.fl32(q[h] / step))
+        best = (q8.clamp(max=0) * near[:, 0] + q8.clamp(min=0) * near[:, 1]).sum(1)
+        mine = R.fl32(R.fl32(best * step) * unit)
+        score = torch.where(torch.isnan(mine), score, torch.maximum(score, mine))
+    score[~is_there | torch.isnan(unit)] = float("-inf")
+    score[:first] = float("inf")
+    score[n - last:] = float("inf")
+    forced = torch.zeros(n)
+    forced[:first] = forced[n - last:] = 1
+    order = sorted(range(n), key=lambda j: (-forced[j].item(), -score[j].item(), j))
+    return sorted(order[:top])
