@@ -603,6 +603,19 @@ typedef struct jf_block8_sparse_args {
   int32_t top_blocks, first_blocks, last_blocks, reserved;
 } jf_block8_sparse_args;
 
+/* jf_block8_shared_attn is jf_block8_attn of sequences whose first 16 * shared_blocks positions are the same: the blocks of
+ * shared_table (shared_blocks ids, 64-bit or 32-bit), in that order; position 16 * shared_blocks + i of sequence b is in block
+ * attn.block_table[b][i / 16].  attn.seq_lens and attn.max_S count the shared positions; a sequence that ends
+ * within them sees those before its end.  A block shared by the sequences is read once for all of them where they are many.  attn.window 0, no prefix_lens or
+ * alibi_slopes. */
+typedef struct jf_block8_shared_args {
+  jf_block8_attn_args attn;
+  const void* shared_table;
+  int32_t shared_blocks, shared_is_i32;
+} jf_block8_shared_args;
+
+uint64_t    jf_block8_shared_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S, int32_t shared_blocks);
+jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* args, jf_stream_t stream);
 uint64_t    jf_block8_sparse_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S, int32_t top_blocks);
 jf_status_t jf_block8_sparse_attn(const jf_block8_sparse_args* args, jf_stream_t stream);
 

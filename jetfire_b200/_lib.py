@@ -67,6 +67,10 @@ class Block8SparseArgs(C.Structure):
                 ("first_blocks", C.c_int32), ("last_blocks", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Block8SharedArgs(C.Structure):
+    _fields_ = [("attn", Block8AttnArgs), ("shared_table", C.c_void_p), ("shared_blocks", C.c_int32), ("shared_is_i32", C.c_int32)]
+
+
 class Block8RotaryArgs(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32), ("codes", C.c_int32), ("H_q", C.c_int32), ("H_kv", C.c_int32),
@@ -202,6 +206,8 @@ _SIGS = {
     "jf_block8_attn": (C.c_int32, [C.POINTER(Block8AttnArgs), C.c_void_p]),
     "jf_block8_sparse_workspace_bytes": (C.c_uint64, [C.c_int32] * 5),
     "jf_block8_sparse_attn": (C.c_int32, [C.POINTER(Block8SparseArgs), C.c_void_p]),
+    "jf_block8_shared_workspace_bytes": (C.c_uint64, [C.c_int32] * 5),
+    "jf_block8_shared_attn": (C.c_int32, [C.POINTER(Block8SharedArgs), C.c_void_p]),
     "jf_varlen_attn": (C.c_int32, [C.POINTER(VarlenAttnArgs), C.c_void_p]),
     "jf_varlen_status": (C.c_int32, [C.c_int32]),
     "jf_varlen_record": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),

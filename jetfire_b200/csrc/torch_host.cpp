@@ -974,6 +974,34 @@ PyObject* block8_sparse_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   });
 }
 
+// block8_shared_attn(name, q, k_data, k_scales, v_data, v_scales, shared_table, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale,
+//                    softcap, workspace | None, out | None) -> (status, out, lse)
+PyObject* block8_shared_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 17, "block8_shared_attn");
+    const char* name = text(p[0]);
+    Attention x(p + 1, p[7], p[8], p + 9, p[13], p[14], name);
+    const at::Tensor& shared = tensor(p[6], name, "shared_table");
+    here(shared, name, "shared_table");
+    require((shared.scalar_type() == at::kLong || shared.scalar_type() == at::kInt) && shared.dim() == 1 && shared.is_contiguous() &&
+                shared.size(0) <= INT32_MAX,
+            name, "shared_table must be contiguous int64 or int32 (blocks,)");
+    jf_block8_shared_args s{};
+    s.shared_blocks = static_cast<int32_t>(shared.size(0));
+    s.shared_is_i32 = shared.scalar_type() == at::kInt;
+    x.outputs(p[16]);
+    jf_status_t r = JF_OK;
+    if (x.B > 0) {
+      x.addresses(p[15], jf_block8_shared_workspace_bytes(x.a.B, x.a.H_q, x.a.H_kv, x.a.max_S, s.shared_blocks));
+      s.attn = x.a;
+      s.shared_table = ptr(shared);
+      const jf_stream_t st = current_stream();
+      r = unlocked([&] { return jf_block8_shared_attn(&s, st); });
+    }
+    return tuple_of(r, {x.out, x.lse});
+  });
+}
+
 // ---- packed prompts -------------------------------------------------------------------------
 
 // (T, H, 128) as the kernel's tensor copies can address it, or a contiguous copy.
@@ -1062,7 +1090,7 @@ PyObject* varlen_attn(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     JF_METHOD(quant_write), JF_METHOD(quant_write_kv), JF_METHOD(fused_attn), JF_METHOD(stage_a), JF_METHOD(stage_b),
     JF_METHOD(decode), JF_METHOD(get_workspace), JF_METHOD(blend), JF_METHOD(step_create), JF_METHOD(step_run),
-    JF_METHOD(block8_append), JF_METHOD(block8_append_rotary), JF_METHOD(block8_attn), JF_METHOD(block8_sparse_attn), JF_METHOD(varlen_attn),
+    JF_METHOD(block8_append), JF_METHOD(block8_append_rotary), JF_METHOD(block8_attn), JF_METHOD(block8_sparse_attn), JF_METHOD(block8_shared_attn), JF_METHOD(varlen_attn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "tensor-taking half of jetfire_b200.ops", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

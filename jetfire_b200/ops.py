@@ -595,6 +595,26 @@ def block8_decode_attn(q, k_data, k_scales, v_data, v_scales, block_table, seq_l
     return out, lse
 
 
+def block8_shared_workspace_bytes(B, H_q, H_kv, max_S, shared_blocks) -> int:
+    """Scratch of ``block8_shared_prefix_attn`` for calls of these sizes (``shared_blocks``: entries of ``shared_table``)."""
+    return int(lib.jf_block8_shared_workspace_bytes(B, H_q, H_kv, max_S, shared_blocks))
+
+
+def block8_shared_prefix_attn(q, k_data, k_scales, v_data, v_scales, shared_table, block_table, seq_lens, max_S, H_q, H_kv, block_size, attn_scale, *,
+                              softcap=0.0, workspace=None, out=None):
+    """``block8_decode_attn`` of sequences that share their first positions, which are read and multiplied once for all.
+
+    ``shared_table (n,)`` int64 or int32: the blocks of the first ``16 n`` positions, the same for every sequence; ``block_table (B,
+    max_blocks)``: the blocks of each sequence's positions from ``16 n`` on.  ``seq_lens`` and ``max_S`` count the shared positions; a
+    sequence that ends within them sees those before its end.  A call captured in a graph is for one ``n``.  There is no window and no bias by distance; the
+    other arguments and the results are those of ``block8_decode_attn``."""
+    name = "block8_shared_prefix_attn"
+    st, out, lse = _host.block8_shared_attn(name, q, k_data, k_scales, v_data, v_scales, shared_table, block_table, seq_lens, max_S, H_q, H_kv, block_size,
+                                            attn_scale, softcap, workspace, out)
+    check(name, st)
+    return out, lse
+
+
 def block8_sparse_workspace_bytes(B, H_q, H_kv, max_S, top_blocks) -> int:
     """Scratch of ``block8_sparse_decode_attn`` for calls of these sizes."""
     return int(lib.jf_block8_sparse_workspace_bytes(B, H_q, H_kv, max_S, top_blocks))
