@@ -12,6 +12,13 @@ struct Block8Source {
   const void* shared = nullptr;      // ids of the blocks that come before those of the table, the same for all sequences
   int32_t shared_blocks = 0;
   bool shared_i32 = false;
+  // Partial results of the positions before, which are joined with those of the table's blocks: lengths count `behind` blocks
+  // that the table does not have.  Layout and geometry: block8_shared.cu.
+  int32_t behind = 0;
+  const float* part_o = nullptr;
+  const float4* part_ml = nullptr;
+  int64_t units = 0;
+  int32_t grid = 0, tiles = 0, pairs = 0, row_tiles = 0;
 };
 // jf_block8_attn with such blocks; its checks only where `launch` is false.
 jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from, jf_stream_t stream, bool launch);

@@ -63,7 +63,8 @@ struct AttnParams {
   const int32_t* chosen;        // the blocks to be scanned, (B, H_kv, top), or null: all
   const void* shared;           // the table of the first shared_blocks blocks of every sequence; the sequence's own follow (max_blocks counts both)
   int32_t top, shared_blocks;
-  bool bt_i32, one_wave, shared_i32;
+  int32_t behind;               // positions before those of the table, whose partial results are elsewhere
+  bool bt_i32, one_wave, shared_i32, partial;   // partial: no piece is written out by itself
 };
 
 // The root of the factor that takes an output to a reference d above its own; a sum is multiplied by it twice.  (V scales up to 2^226 apart put d
@@ -74,7 +75,7 @@ __device__ __forceinline__ float half_step(float d) { return ex2(-0.5f * d); }
 struct Span { int len, prefix, lo, head, first, count; };
 __device__ __forceinline__ Span span_of(const AttnParams& P, int length, int prefix) {
   Span s;
-  s.len = max(0, min(length, min(P.max_S, P.max_blocks * JF_BLOCK_SIZE)));
+  s.len = max(0, min(min(length, P.max_S) - P.behind, P.max_blocks * JF_BLOCK_SIZE));
   const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
   s.prefix = s.lo = s.head = s.first = 0;
   s.count = P.chosen ? min(blocks, P.top) : blocks;
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
       const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 * NT + head) * JF_HEAD_DIM + d);
       sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
     }
-    if (cut.n == 1) {
+    if (cut.n == 1 && !P.partial) {
       write(head, d, sum, sm_ml[head]);
     } else if (CLUSTER) {
       *reinterpret_cast<float4*>(so + head * JF_HEAD_DIM + d) = sum;   // (no other thread reads these four)
@@ -746,6 +747,98 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
   }
 }
 
+// The pieces of a sequence and the partial results of the positions before them (part_o, part_ml of `from`): a warp per (sequence,
+// head), four channels a lane.  A result there has references of its own for its output and for its sum.
+template <int DT>
+__global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ Block8Source from, int width,
+                                                                 int grid_y) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int b = static_cast<int>(row / P.H_q), h = static_cast<int>(row % P.H_q);
+  pdl_wait();
+  pdl_trigger();
+  if (b >= P.B) return;
+  int total = 0, first = 0, n = 0;
+  for (int i = lane; i < P.B; i += 32) total += blocks_of(P, i);
+  const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total), total);
+  for (int i = lane; i <= b; i += 32) {
+    const int k = max(1, (blocks_of(P, i) + piece - 1) / piece);
+    if (i < b) first += k; else n = k;
+  }
+  first = __reduce_add_sync(0xFFFFFFFFu, first);
+  n = __reduce_add_sync(0xFFFFFFFFu, n);
+  const int kvh = h / P.G, in_group = h % P.G, y = kvh * P.groups + in_group / width;
+  const int64_t own0 = (static_cast<int64_t>(first) * grid_y + y) * width + in_group % width, step = static_cast<int64_t>(grid_y) * width;
+  // the results of the row's pair of row tiles: those of the thread blocks that hold some of its units, and where it is a single tile of both groups
+  const int64_t in_head = static_cast<int64_t>(b) * P.G + in_group;
+  const int tile = static_cast<int>(in_head / 128), r = static_cast<int>(in_head % 128), pair = tile / 2;
+  const bool two = pair * 2 + 1 < from.row_tiles;
+  const int64_t item = static_cast<int64_t>(kvh) * from.pairs + pair, u0 = item * from.tiles, u1 = u0 + from.tiles - 1;
+  const int64_t c0 = ((u0 + 1) * from.grid - 1) / from.units, c1 = ((u1 + 1) * from.grid - 1) / from.units;
+  const int per = two ? 1 : 2, m = static_cast<int>(c1 - c0 + 1) * per;
+  auto result = [&](int i) {   // row of part_o and part_ml
+    const int64_t c = c0 + i / per;
+    return ((c + item) * 2 + (two ? tile & 1 : i % per)) * 128 + r;
+  };
+  // references
+  float top_o = kNone, top_l = kNone;
+  for (int i = lane; i < n + m; i += 32) {
+    if (i < n) {
+      const float x = P.part_ml[(own0 + i * step) * 2];
+      top_o = fmaxf(top_o, x);
+      top_l = fmaxf(top_l, x);
+    } else {
+      const float4 x = from.part_ml[result(i - n)];
+      top_o = fmaxf(top_o, x.x);
+      top_l = fmaxf(top_l, x.y);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top_o = fmaxf(top_o, __shfl_xor_sync(0xFFFFFFFFu, top_o, o));
+    top_l = fmaxf(top_l, __shfl_xor_sync(0xFFFFFFFFu, top_l, o));
+  }
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float z = 0.0f;
+  for (int i0 = 0; i0 < n + m; i0 += 32) {
+    const int i = i0 + lane;
+    float w = 0.0f;
+    int64_t at = -1;
+    if (i < n) {
+      const float2 x = *reinterpret_cast<const float2*>(P.part_ml + (own0 + i * step) * 2);
+      const float f = half_step(top_l - x.x), e = half_step(top_o - x.x);
+      z = fmaf(x.y * f, f, z);
+      w = e * e;
+      if (x.y != 0.0f) at = own0 + i * step;
+    } else if (i < n + m) {
+      const int64_t where = result(i - n);
+      const float4 x = from.part_ml[where];
+      const float f = half_step(top_l - x.y), e = half_step(top_o - x.x);
+      z = fmaf(x.z * f, f, z);
+      w = e * e;
+      if (x.z != 0.0f) at = where;     // (a group without tiles left no output)
+    }
+    const int some = min(32, n + m - i0);
+    for (int k = 0; k < some; ++k) {
+      const float f = __shfl_sync(0xFFFFFFFFu, w, k);
+      const int64_t where = __shfl_sync(0xFFFFFFFFu, at, k);
+      if (where < 0) continue;
+      const float4 x = *reinterpret_cast<const float4*>((i0 + k < n ? P.part_o : from.part_o) + where * JF_HEAD_DIM + lane * 4);
+      sum = make_float4(fmaf(x.x, f, sum.x), fmaf(x.y, f, sum.y), fmaf(x.z, f, sum.z), fmaf(x.w, f, sum.w));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
+  const bool none = z == 0.0f;
+  const float f = half_step(top_l - top_o);
+  const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = Elem<DT>::from_f32(none ? 0.0f : e[k] / z * f * f);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + row * JF_HEAD_DIM + lane * 4) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+  if (lane == 0 && P.lse) P.lse[row] = none ? -INFINITY : (top_l + __log2f(z)) / kLog2e;
+}
+
 struct Plan { int G, nt, groups, target, min_piece, pieces; uint64_t bytes; };
 constexpr int kMinPiece = 8;   // blocks
 // Pieces of a sequence on average: from kManyPieces on the join spreads a row over four blocks of 16 warps, below kFewPieces it gives it four
@@ -837,7 +930,9 @@ jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from
   if (a->softcap != 0.0f && !(a->softcap >= 1.0e-30f && a->softcap <= 1.0e30f)) return JF_ERR_ARG;
   if (a->B == 0) return JF_OK;
   Plan p;
-  const int max_S = from.chosen ? static_cast<int>(std::min<int64_t>(a->max_S, int64_t{from.top} * JF_BLOCK_SIZE)) : a->max_S;   // scanned
+  const int max_S = from.chosen   ? static_cast<int>(std::min<int64_t>(a->max_S, int64_t{from.top} * JF_BLOCK_SIZE))   // scanned
+                    : from.part_o ? std::max(a->max_S - from.behind * JF_BLOCK_SIZE, 1)
+                                  : a->max_S;
   if (!make_plan(a->B, a->H_q, a->H_kv, max_S, p)) return JF_ERR_ARG;
   if (!a->q || !a->seq_lens || !a->out) return JF_ERR_ARG;
   // (a table without columns and a cache without blocks have no memory; nothing of them is read)
@@ -874,8 +969,10 @@ jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from
   P.scale = a->attn_scale; P.softcap = a->softcap;
   P.bt_i32 = a->bt_is_i32 != 0;
   P.chosen = from.chosen; P.top = from.top;
+  P.behind = from.behind * JF_BLOCK_SIZE;
+  P.partial = from.part_o != nullptr;
   P.shared = from.shared; P.shared_blocks = from.shared_blocks; P.shared_i32 = from.shared_i32;
-  P.cluster = cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
+  P.cluster = P.partial ? 0 : cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
   const bool feat = a->softcap > 0.0f || a->alibi_slopes;
   const auto s = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.pieces, a->H_kv * p.groups);
@@ -886,8 +983,14 @@ jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from
   else
     st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_FP16>(P, p.nt, feat, grid, s)
                                    : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
-  if (st != JF_OK || P.cluster > 0 || p.pieces == a->B) return st;   // (one piece per sequence: nothing to join)
   const int width = 8 * p.nt, grid_y = a->H_kv * p.groups;
+  if (st == JF_OK && P.partial) {
+    const dim3 rows(static_cast<unsigned>((int64_t{a->B} * a->H_q + 7) / 8));
+    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16 ? launch_pdl(block8_join_shared_kernel<JF_DTYPE_BF16>, rows, dim3(256), 0, s, P, from, width, grid_y)
+                                            : launch_pdl(block8_join_shared_kernel<JF_DTYPE_FP16>, rows, dim3(256), 0, s, P, from, width, grid_y));
+    return JF_OK;
+  }
+  if (st != JF_OK || P.cluster > 0 || p.pieces == a->B) return st;   // (one piece per sequence: nothing to join)
   auto join = [&](auto vec, auto warps, int z) {
     constexpr int V = decltype(vec)::value, W = decltype(warps)::value;
     const dim3 rows(a->H_q, a->B, z), block(W * 32);

@@ -1,17 +1,634 @@
-// Decode attention of sequences that share their first positions, over the 8-bit cache.
+// Decode attention of sequences that share their first positions, over the 8-bit cache, on the fifth-generation tensor cores.
+//
+//   out_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(f(scale q_r.k_j)),   r through the query heads of a KV head in all sequences
+//
+// The shared positions meet all rows of a KV head in one product, so that they are read, and turned into operands, once for
+// 256 rows.  The codes become fp16, which holds them exactly, on their way through registers into the operands' shared-memory layout; a row's
+// query is fp16 under a power of two that brings its largest element to [2^13, 2^14) (what that rounds is 2^-38 of it).  The
+// scales stay out of the products, in fp32: a block's K scale multiplies its 16 scores, its V scale joins their exponent.
+//
+// A row keeps two references.  w = exp2(x + log2 vs - R) is the weight that meets V's codes (fp16: half a step is 2^-11 of it), x the
+// score in units of log2; R lags the maximum of x + log2 vs by up to 2^kLag.  The sum of exp2(x - m) is formed block by block from the
+// same exponentials, times exp2(R - log2 vs - m): one more of them for 16 positions.  Where V scales lie so far apart (beyond
+// 2^kSpread) that a weight could vanish while its position counts, those tiles take an exponential more for every position.
+//
+//   warps 0-3, 4-7   scores -> weights of row tile 0, 1 (a thread a row); the rescaling of O; the partial result
+//   warps 8-11       codes -> fp16 operands: 128 positions of K, then of V, two buffers each
+//   warp 12          issues the matrix products
+//
+// Work is a line of units -- (KV head, pair of row tiles, 128 positions) -- cut into pieces of one length, one for each thread block, so that all
+// multiprocessors end together; where a piece passes from one pair of row tiles to the next it leaves two partial results.  A single row
+// tile (128 rows or fewer) is worked on by both groups of warps, in turn on its tiles of positions.  What the sequences have behind the shared positions goes
+// through block8_attn.cu's kernel, whose partial results are joined with these ones.
+//
+// Bound: the tensor pipe and the exponentials in turn where there are 256 rows, else the conversion.
 #include "block8.cuh"
+#include "decode_common.cuh"
+#include "tensor_common.cuh"
 
 #include <algorithm>
+#include <type_traits>
+
+namespace jf {
+namespace {
+
+constexpr int kRows = 128, kKeys = 128;                // of a tile
+constexpr int kTileBlocks = kKeys / JF_BLOCK_SIZE;
+constexpr int kCodeBytes = kKeys * JF_HEAD_DIM;        // of a tile as it lies in the cache
+constexpr int kStaged = 2;                             // K or V tiles on their way from memory
+constexpr int kNotes = 8;
+constexpr int kThreads = 512;
+// Registers a thread: the rows' warpgroups, the converting one, the one that issues; together what the block is launched with.
+constexpr int kRowRegs = 200, kConvertRegs = 72, kIssueRegs = 40;
+constexpr float kLag = 8.0f, kLift = 7.0f;             // log2; weights stay below 2^15
+constexpr float kSumLag = 24.0f, kSpread = 64.0f;
+constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSmemBytes = 2 * kTileBytes + 4 * kTileBytes + kStaged * kCodeBytes + 1024;
+
+struct SharedParams {
+  const uint16_t* q;
+  const uint8_t *k_data, *v_data;
+  const float *k_scales, *v_scales;
+  const void* table;
+  const int32_t* seq_lens;
+  float* part_o;          // [piece, row tile of the pair][128][128]
+  float4* part_ml;        // R - lift, m, sum
+  int32_t* status;
+  int64_t num_blocks, units;
+  int32_t H_q, G, rows, row_tiles, pairs, tiles, blocks, max_S;   // rows: of a KV head; blocks: shared ones; tiles: of positions
+  float scale, softcap;
+  bool i32;
+};
+
+// What a tile's rows need to know of it: its blocks' K scales, log2 of their V scales.
+struct alignas(16) Note {
+  float ks[kTileBlocks], lvs[kTileBlocks];
+  float lvs_lo, lvs_hi;
+  uint32_t dead;          // a bit for each block that is not there
+  uint32_t odd;           // a K scale that is not above zero
+};
+struct Shared {
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2], note_full[kNotes], products_done;
+  Note note[kNotes];
+  uint32_t tmem;
+};
+
+// The units of a thread block, item by item (an item: a KV head and a pair of row tiles).
+struct Segment { int64_t u, end; int item, first, n; };   // n tiles of positions from `first` on
+__device__ __forceinline__ Segment units_of(const SharedParams& P) {
+  const int64_t c = blockIdx.x, all = gridDim.x;
+  return Segment{c * P.units / all, (c + 1) * P.units / all, 0, 0, 0};
+}
+__device__ __forceinline__ bool next_segment(const SharedParams& P, Segment& s) {
+  s.u += s.n;
+  if (s.u >= s.end) return false;
+  s.item = static_cast<int>(s.u / P.tiles);
+  s.first = static_cast<int>(s.u - static_cast<int64_t>(s.item) * P.tiles);
+  s.n = static_cast<int>(min(static_cast<int64_t>(P.tiles - s.first), s.end - s.u));
+  return true;
+}
+__device__ __forceinline__ bool two_tiles(const SharedParams& P, const Segment& s) { return s.item % P.pairs * 2 + 1 < P.row_tiles; }
+// Whether group t of rows has anything to do in a segment.
+__device__ __forceinline__ bool has_jobs(const SharedParams& P, const Segment& s, int t) { return t < s.n || two_tiles(P, s); }
+
+// ---- codes -> operands --------------------------------------------------------------------------
+template <int CODES> __device__ __forceinline__ uint32_t flip(uint32_t w) { return CODES == JF_CODES_INT8 ? w ^ 0x80808080u : w; }
+template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {   // two of four codes as fp16
+  uint32_t d;
+  if (CODES == JF_CODES_INT8)   // (sign bits turned over: 0x6400 + u is 1024 + u)
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(prmt(w, 0x64646464u, HIGH ? 0x4342u : 0x4140u)), "r"(0x64806480u));
+  else if (HIGH)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
+  return d;
+}
+
+template <int CODES> __device__ __forceinline__ bool convert(const SharedParams& P, Shared& S, unsigned char* kv, unsigned char* staged) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, tid = threadIdx.x & 127;
+  const Segment range = units_of(P);
+  const int64_t begin = range.u, sides = 2 * (range.end - range.u);
+  // four units' blocks are looked up at a time, a lane each, a round ahead
+  struct Look { int id; float ks, vs; };
+  auto look_up = [&](int64_t u0) {
+    Look r{-1, 0.0f, 0.0f};
+    const int64_t u = u0 + (lane >> 3);
+    if (u < range.end) {
+      const int item = static_cast<int>(u / P.tiles), block = static_cast<int>(u - static_cast<int64_t>(item) * P.tiles) * kTileBlocks + (lane & 7);
+      if (block < P.blocks) {
+        const int64_t id = P.i32 ? static_cast<const int32_t*>(P.table)[block] : static_cast<const int64_t*>(P.table)[block];
+        const int64_t row = static_cast<int64_t>(item / P.pairs) * P.num_blocks;
+        if (id >= 0 && id < P.num_blocks) {
+          r.id = static_cast<int>(id);
+          r.ks = P.k_scales[row + id];
+          r.vs = P.v_scales[row + id];
+        }
+      }
+    }
+    return r;
+  };
+  int64_t at = begin;          // first unit of `now`
+  Look now = look_up(begin), then = look_up(begin + 4);
+  // A thread copies the bytes that it converts: 16 of each block, so a wait for its own copies is enough.
+  auto fetch = [&](int64_t n) {
+    if (n < sides) {
+      const int64_t u = begin + (n >> 1);
+      const int off = static_cast<int>(u - at), head = static_cast<int>(u / P.tiles) / P.pairs;
+      const uint8_t* base = (n & 1 ? P.v_data : P.k_data) + static_cast<int64_t>(head) * P.num_blocks * (JF_BLOCK_SIZE * JF_HEAD_DIM) + tid * 16;
+      unsigned char* to = staged + (n % kStaged) * kCodeBytes + tid * 16;
+#pragma unroll
+      for (int i = 0; i < kTileBlocks; ++i) {
+        const int id = __shfl_sync(0xFFFFFFFFu, off < 4 ? now.id : then.id, (off & 3) * 8 + i);
+        if (id >= 0) cp_async_16(to + i * 2048, base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM));
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int n = 0; n < kStaged; ++n) fetch(n);
+  // where a thread's 16 channels go: two chunks of 16 bytes of a row; the upper half of a row's threads takes them in the other order, so
+  // that eight threads meet all banks
+  const int row = tid >> 3, cc = tid & 7, j0 = (cc & 3) * 2, sw = row & 7;
+  const uint32_t base = (cc >> 2) * kSlabBytes + row * 128;
+  const uint32_t lo_at = base + ((j0 ^ sw) << 4), hi_at = base + (((j0 + 1) ^ sw) << 4);
+  for (int64_t n = 0; n < sides; ++n) {
+    const int64_t g = n >> 1;
+    const int side = static_cast<int>(n & 1), slot = static_cast<int>(g & 1);
+    if (begin + g >= at + 4) {
+      now = then;
+      at += 4;
+      then = look_up(at + 4);
+    }
+    if (g >= 2 && !wait_warp(side ? &S.v_empty[slot] : &S.k_empty[slot], static_cast<uint32_t>((g >> 1) - 1) & 1u)) {
+      cp_async_wait_all();
+      return false;
+    }
+    const int off = static_cast<int>(begin + g - at) * 8;
+    if (side == 0 && warp == 0) {   // the note of this tile
+      const int id = __shfl_sync(0xFFFFFFFFu, now.id, (off + lane) & 31);
+      const float ks = __shfl_sync(0xFFFFFFFFu, now.ks, (off + lane) & 31), vs = __shfl_sync(0xFFFFFFFFu, now.vs, (off + lane) & 31);
+      const bool mine = lane < kTileBlocks, is = mine && id >= 0;
+      float lg;
+      asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(vs == 0.0f ? 0x1p-100f : vs));   // (weightless, but its positions count)
+      Note& note = S.note[g % kNotes];
+      if (mine) {
+        note.ks[lane] = is ? ks : 1.0f;
+        note.lvs[lane] = is ? lg : 0.0f;
+      }
+      const unsigned dead = __ballot_sync(0xFFFFFFFFu, mine && !is), odd = __ballot_sync(0xFFFFFFFFu, is && !(ks > 0.0f));
+      float lo = is ? lg : 3.0e38f, hi = is ? lg : -3.0e38f;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+      }
+      if (lane == 0) {
+        note.lvs_lo = lo;
+        note.lvs_hi = hi;
+        note.dead = dead;
+        note.odd = odd;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.note_full[g % kNotes]);
+    }
+    cp_async_wait_group<kStaged - 1>();
+    const unsigned char* from = staged + (n % kStaged) * kCodeBytes + tid * 16;
+    unsigned char* to = kv + (side * 2 + slot) * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < kTileBlocks; ++i) {
+      const bool is = __shfl_sync(0xFFFFFFFFu, now.id, off + i) >= 0;
+      uint4 x = *reinterpret_cast<const uint4*>(from + i * 2048);
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (is) {
+        x.x = flip<CODES>(x.x); x.y = flip<CODES>(x.y); x.z = flip<CODES>(x.z); x.w = flip<CODES>(x.w);
+        a = make_uint4(widen<CODES, false>(x.x), widen<CODES, true>(x.x), widen<CODES, false>(x.y), widen<CODES, true>(x.y));
+        b = make_uint4(widen<CODES, false>(x.z), widen<CODES, true>(x.z), widen<CODES, false>(x.w), widen<CODES, true>(x.w));
+      }
+      const bool swap = cc >= 4;
+      *reinterpret_cast<uint4*>(to + i * 2048 + (swap ? hi_at : lo_at)) = swap ? b : a;
+      *reinterpret_cast<uint4*>(to + i * 2048 + (swap ? lo_at : hi_at)) = swap ? a : b;
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(side ? &S.v_full[slot] : &S.k_full[slot]);
+    fetch(n + kStaged);
+  }
+  cp_async_wait_all();
+  return true;
+}
+
+// ---- the products -------------------------------------------------------------------------------
+// Jobs of a segment: with two row tiles (positions i, row tile 0), (i, 1), (i + 1, 0), ...; with one (i, group 0), (i + 1, group 1), ...
+// The scores of job j + 2, which goes to the same group as job j, are asked for behind the products of its weights with V.
+__device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, uint32_t tmem) {
+  constexpr uint32_t qk = instruction<JF_DTYPE_FP16>(false), pv = instruction<JF_DTYPE_FP16>(true);
+  const uint64_t q_op = operand(q_smem, 16), k_op = operand(kv_smem, 16), v_op = operand(kv_smem + 2 * kTileBytes, kSlabBytes);
+  Segment s = units_of(P);
+  uint32_t base = 0, p_count[2] = {0, 0}, q_count[2] = {0, 0};   // tiles of positions, weights, queries so far
+  while (next_segment(P, s)) {
+    const bool two = two_tiles(P, s);
+    const int jobs = two ? 2 * s.n : s.n;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (has_jobs(P, s, t) && !wait_warp(&S.q_full[t], q_count[t]++ & 1)) return false;
+    auto scores = [&](int j) {
+      const int t = j & 1;
+      const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
+      if (!wait_warp(&S.k_full[slot], g >> 1 & 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = q_op + t * (kTileBytes >> 4), b = k_op + slot * (kTileBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = ((k >> 2) * kSlabBytes + (k & 3) * 32) >> 4;
+          mma_ss(tmem + t * 128, a + off, b + off, qk, k > 0);
+        }
+        tc_commit(&S.s_full[t]);
+        if (!two || t == 1) tc_commit(&S.k_empty[slot]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int j = 0; j < min(jobs, 2); ++j)
+      if (!scores(j)) return false;
+    for (int j = 0; j < jobs; ++j) {
+      const int t = j & 1;
+      const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
+      if (!wait_warp(&S.v_full[slot], g >> 1 & 1)) return false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {   // the weights come in two halves
+        if (!wait_warp(&S.p_full[t][h], p_count[t] & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t b = v_op + slot * (kTileBytes >> 4);
+#pragma unroll
+          for (int k = h * 4; k < h * 4 + 4; ++k)
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
+          if (h == 1) {
+            if (!two || t == 1) tc_commit(&S.v_empty[slot]);
+            if (j + 2 >= jobs) tc_commit(&S.o_full[t]);
+          }
+        }
+        __syncwarp();
+      }
+      ++p_count[t];
+      if (j + 2 < jobs && !scores(j + 2)) return false;
+    }
+    base += s.n;
+  }
+  return true;
+}
+
+// ---- scores -> weights ----------------------------------------------------------------------------
+// The largest of 16 scores; a NaN if there is one.
+__device__ __forceinline__ float largest16(const float* s) {
+  float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]);
+  a = max3(a, s[6], s[7]);
+  b = max3(b, s[8], s[9]);
+  a = max3(a, s[10], s[11]);
+  b = max3(b, s[12], s[13]);
+  return max3(max3(a, b, s[14]), s[15], s[15]);
+}
+// cap * tanh(x / cap) of 64 scores, in units of log2 (cap2: the cap in these units), for the whole warp the same way: up to
+// |x| = cap by a polynomial (relative error 6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).  A NaN stays one.
+__device__ __forceinline__ void cap64(float* x, float cap2, float inv) {
+  float most = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 64; ++c) most = fmaxf(most, fabsf(x[c]));
+  if (__all_sync(0xFFFFFFFFu, most <= cap2)) {
+    const uint64_t i2 = pair(inv, inv);
+#pragma unroll
+    for (int c = 0; c < 64; c += 2) {
+      const uint64_t v = pair(x[c], x[c + 1]), z = mul2(v, i2), w = mul2(z, z);
+      uint64_t q = fma2(w, pair(-0.00312657771f, -0.00312657771f), pair(0.0169064086f, 0.0169064086f));
+      q = fma2(q, w, pair(-0.0517682843f, -0.0517682843f));
+      q = fma2(q, w, pair(0.132884905f, 0.132884905f));
+      q = fma2(q, w, pair(-0.333302796f, -0.333302796f));
+      q = fma2(q, w, pair(1.0f, 1.0f));
+      split(mul2(v, q), x[c], x[c + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 64; ++c) x[c] = cap2 - __fdividef(2.0f * cap2, ex2(min_or_nan(x[c] * inv * (2.0f * kLog2e), 126.0f)) + 1.0f);
+  }
+}
+
+template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedParams& P, Shared& S, unsigned char* q_smem, uint32_t tmem, int t) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, r = warp * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+  const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+  const float cap2 = CAP ? P.softcap * kLog2e : 0.0f, inv_cap = CAP ? 1.0f / cap2 : 0.0f;
+  // The row's query as fp16 into the operand's place; what brings its products to scores in units of log2, and the positions that it sees.
+  // (more than there are: all of them)
+  struct Row { float f; int len; bool idle; };   // idle: no lane of the warp has a row
+  auto load_query = [&](const Segment& s) {
+    const int tile = s.item % P.pairs * 2 + (two_tiles(P, s) ? t : 0), row = tile * kRows + r;
+    Row to{0.0f, INT32_MAX, tile * kRows + warp * 32 >= P.rows};
+    if (!has_jobs(P, s, t)) return to;   // (its queries would not be waited for)
+    uint4 x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = make_uint4(0, 0, 0, 0);
+    if (row < P.rows) {
+      const int b = row / P.G, head = s.item / P.pairs * P.G + row % P.G;
+      const uint4* from = reinterpret_cast<const uint4*>(P.q + (static_cast<int64_t>(b) * P.H_q + head) * JF_HEAD_DIM);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __ldg(from + i);
+      const int len = max(min(P.seq_lens[b], P.max_S), 0);
+      if (len < P.blocks * JF_BLOCK_SIZE) to.len = len;
+    }
+    float amax = 0.0f, odd = 0.0f;   // odd: NaN if an element is no number, else 0
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float y = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16 * e));
+          amax = fmaxf(amax, fabsf(y));
+          odd = fmaf(y, 0.0f, odd);
+        }
+    }
+    constexpr int TOP = 13;
+    const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127, 127), TOP - 126);
+    const float up = copysignf(__uint_as_float(static_cast<uint32_t>(TOP - e + 127) << 23), P.scale);
+    to.f = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) * fabsf(P.scale) * kLog2e + odd;
+    unsigned char* out = q_smem + r * 128;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float lo = Elem<DT>::to_f32(static_cast<uint16_t>(w[k])) * up, hi = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)) * up;
+        h[k] = odd == 0.0f ? round2<JF_DTYPE_FP16>(lo, hi) : 0u;
+      }
+      *reinterpret_cast<uint4*>(out + (i >> 3) * kSlabBytes + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.q_full[t]);
+    return to;
+  };
+
+  Segment s = units_of(P);
+  uint32_t base = 0, s_count = 0, o_count = 0;
+  bool more = next_segment(P, s);
+  Row row = more ? load_query(s) : Row{0.0f, 0, true};
+  while (more) {
+    const bool two = two_tiles(P, s);
+    float R = kNone, m = kNone, l = 0.0f, lvs_top = -3.0e38f;
+    bool have = false;
+    for (int i = two ? 0 : t; i < s.n; i += two ? 1 : 2) {
+      const uint32_t g = base + i;
+      const Note& note = S.note[g % kNotes];
+      const int end = (s.first + i + 1) * kKeys;
+      if (!wait_warp(&S.note_full[g % kNotes], g / kNotes & 1)) return false;
+      if (!wait_warp(&S.s_full[t], s_count++ & 1)) return false;
+      tc_fence_after();
+      if (row.idle) {   // (whatever the weights of rows that are none are)
+        __syncwarp();
+        if (lane < 2) mbar_arrive(&S.p_full[t][lane]);
+        have = true;
+        continue;
+      }
+      uint32_t u[128];
+      float* x = reinterpret_cast<float*>(u);
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld32(s_at + c, u + c);
+      float f[kTileBlocks], lvs[kTileBlocks];
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; ++b) {
+        f[b] = note.ks[b] * row.f;
+        lvs[b] = note.lvs[b];
+      }
+      const uint32_t dead = note.dead;
+      lvs_top = fmaxf(lvs_top, note.lvs_hi);
+      const bool wide = lvs_top - note.lvs_lo > kSpread;
+      const bool masked = __any_sync(0xFFFFFFFFu, row.len < end) || dead != 0;
+      const bool scaled = CAP || masked || wide || note.odd != 0;
+      tc_wait_ld();
+      if (scaled) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int c = h * 64; c < h * 64 + 64; c += 2) split(mul2(pair(x[c], x[c + 1]), pair(f[c / 16], f[c / 16])), x[c], x[c + 1]);
+          if (CAP) cap64(x + h * 64, cap2, inv_cap);
+          if (masked) {
+            const int left = row.len - (end - kKeys);
+#pragma unroll
+            for (int c = h * 64; c < h * 64 + 64; ++c) x[c] = c < left && !(dead >> (c / 16) & 1u) ? x[c] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) f[b] = 1.0f;
+      }
+      float top_x = -INFINITY, top_w = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; ++b) {
+        const float y = largest16(x + b * 16) * f[b];
+        top_x = max3(top_x, y, y);
+        top_w = max3(top_w, y + lvs[b], y + lvs[b]);
+      }
+      if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag))) {
+        const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
+        R = to;
+        if (have) rescale(o_at, by);
+      }
+      if (__any_sync(0xFFFFFFFFu, top_x > m + kSumLag)) {
+        const float to = top_x > m + kSumLag ? top_x : m;
+        l *= ex2(m - to);
+        m = to;
+      }
+      const float ref = R - kLift;
+      if (wide) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) l += ex2(x[c] - m);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int b = h * 4; b < h * 4 + 4; ++b) {
+          const uint64_t f2 = pair(f[b], f[b]), c2 = pair(lvs[b] - ref, lvs[b] - ref);
+          uint64_t sum = 0;
+#pragma unroll
+          for (int c = b * 16; c < b * 16 + 16; c += 2) {
+            float a, d;
+            split(fma2(pair(x[c], x[c + 1]), f2, c2), a, d);
+            a = ex2(a);
+            d = ex2(d);
+            sum = add2(sum, pair(a, d));
+            p[(c - h * 64) / 2] = round2<JF_DTYPE_FP16>(a, d);
+          }
+          if (!wide) {
+            float a, d;
+            split(sum, a, d);
+            l = fmaf(a + d, ex2(ref - lvs[b] - m), l);
+          }
+        }
+        tmem_st32(s_at + h * 32, p);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[t][h]);
+      }
+      have = true;
+    }
+    // the next queries, then the partial result
+    const int64_t piece = (static_cast<int64_t>(blockIdx.x) + s.item) * 2 + t;
+    base += s.n;
+    const float ref = R - kLift;
+    const bool idle = row.idle;
+    more = next_segment(P, s);
+    if (more) row = load_query(s);
+    if (have) {
+      if (!wait_warp(&S.o_full[t], o_count++ & 1)) return false;
+      tc_fence_after();
+      float* out = P.part_o + (piece * kRows + r) * JF_HEAD_DIM;
+#pragma unroll 1
+      for (int c = idle ? 4 : 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_at + c * 32, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c * 32 + k), JF_W8(o, k) : "memory");
+      }
+      tc_fence_before();
+    }
+    P.part_ml[piece * kRows + r] = make_float4(ref, m, l, 0.0f);
+    __syncwarp();
+  }
+  return true;
+}
+
+template <int DT, int CODES, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid_constant__ SharedParams P) {
+  extern __shared__ unsigned char raw[];
+  __shared__ Shared S;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // (known to be the same for all lanes)
+  unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  unsigned char *kv = smem + 2 * kTileBytes, *staged = kv + 4 * kTileBytes;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.q_full[i], 4);
+      mbar_init(&S.k_full[i], 4);
+      mbar_init(&S.v_full[i], 4);
+      mbar_init(&S.k_empty[i], 1);
+      mbar_init(&S.v_empty[i], 1);
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.p_full[i][0], 4);
+      mbar_init(&S.p_full[i][1], 4);
+      mbar_init(&S.o_full[i], 1);
+    }
+    for (int i = 0; i < kNotes; ++i) mbar_init(&S.note_full[i], 1);
+    mbar_init(&S.products_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem;
+  pdl_wait();
+  pdl_trigger();
+  // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
+  bool ok = true;
+  if (warp >= 12) {
+    regs_dec<kIssueRegs>();
+    if (warp == 12) {
+      ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
+      if (elect_one()) tc_commit(&S.products_done);
+      __syncwarp();
+      ok &= wait_warp(&S.products_done, 0);
+    }
+  } else if (warp >= 8) {
+    regs_dec<kConvertRegs>();
+    ok = convert<CODES>(P, S, kv, staged);
+  } else {
+    regs_inc<kRowRegs>();
+    ok = soften<DT, CAP>(P, S, smem + (warp >> 2) * kTileBytes, tmem, warp >> 2);
+  }
+  if (!ok) report_status(P.status, JF_ERR_TIMEOUT);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+
+struct Plan {
+  int G, row_tiles, pairs, tiles, grid;
+  int64_t items, units;
+  uint64_t own, o_bytes, bytes;   // scratch of the own positions' part, of the outputs, of all
+};
+constexpr int kFewRows = 16;      // rows of a KV head up to which the shared positions go through block8_attn.cu's kernel
+
+bool tensor_form(int B, int H_q, int H_kv, int shared_blocks) { return shared_blocks > 0 && int64_t{B} * (H_q / H_kv) > kFewRows; }
+
+bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) {
+  if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_S <= 0 || H_q % H_kv != 0 || shared_blocks < 0 || shared_blocks > INT32_MAX / JF_BLOCK_SIZE - 1) return false;
+  p = Plan{};
+  if (!tensor_form(B, H_q, H_kv, shared_blocks)) {
+    p.bytes = block8_attn_workspace(B, H_q, H_kv, max_S);
+    return p.bytes > 0;
+  }
+  p.G = H_q / H_kv;
+  const int64_t rows = int64_t{B} * p.G;
+  if (rows > INT32_MAX / 2 || H_q > 65535 || B > 65535) return false;
+  p.row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
+  p.pairs = (p.row_tiles + 1) / 2;
+  const int seen = std::min(shared_blocks, (max_S + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE);   // of the shared blocks
+  p.tiles = (seen + kTileBlocks - 1) / kTileBlocks;
+  p.items = int64_t{H_kv} * p.pairs;
+  if (p.items > INT32_MAX / 4) return false;
+  p.units = p.items * p.tiles;
+  p.grid = static_cast<int>(std::min<int64_t>(num_sms(), p.units));
+  p.own = (block8_attn_workspace(B, H_q, H_kv, std::max(max_S - shared_blocks * JF_BLOCK_SIZE, 1)) + 255) / 256 * 256;
+  if (p.own == 0) return false;
+  const uint64_t part_rows = static_cast<uint64_t>(p.grid + p.items) * 2 * kRows;
+  p.o_bytes = part_rows * JF_HEAD_DIM * sizeof(float);
+  p.bytes = p.own + p.o_bytes + part_rows * sizeof(float4);
+  return true;
+}
+
+template <int DT, int CODES, bool CAP> jf_status_t launch(const SharedParams& P, int grid, cudaStream_t s) {
+  auto* kernel = block8_shared_kernel<DT, CODES, CAP>;
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, block8_shared_kernel<DT, CODES, CAP>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  // (a warpgroup that asks for more than the block has waits for good)
+  if (regs * kThreads < 128 * (2 * kRowRegs + kConvertRegs + kIssueRegs)) return JF_ERR_UNSUPPORTED;
+  JF_ENSURE_SMEM(kernel, kSmemBytes);
+  JF_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmemBytes, s, P));
+  return JF_OK;
+}
+template <int DT, int CODES> jf_status_t launch(const SharedParams& P, int grid, cudaStream_t s) {
+  return P.softcap > 0.0f ? launch<DT, CODES, true>(P, grid, s) : launch<DT, CODES, false>(P, grid, s);
+}
+
+}  // namespace
+}  // namespace jf
 
 extern "C" uint64_t jf_block8_shared_workspace_bytes(int32_t B, int32_t H_q, int32_t H_kv, int32_t max_S, int32_t shared_blocks) {
-  if (shared_blocks < 0) return 0;
-  return jf::block8_attn_workspace(B, H_q, H_kv, max_S);
+  jf::Plan p;
+  return jf::make_plan(B, H_q, H_kv, max_S, shared_blocks, p) ? p.bytes : 0;
 }
 
 extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_stream_t stream) {
   using namespace jf;
   if (!a) return JF_ERR_ARG;
-  const jf_block8_attn_args& at = a->attn;
+  jf_block8_attn_args at = a->attn;
   if (a->shared_blocks < 0 || at.window != 0 || at.prefix_lens || at.alibi_slopes) return JF_ERR_ARG;
   if (a->shared_blocks > INT32_MAX / JF_BLOCK_SIZE - 1) return JF_ERR_UNSUPPORTED;
   if (at.B > 0 && a->shared_blocks > 0 && !a->shared_table) return JF_ERR_ARG;
@@ -19,5 +636,54 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   from.shared = a->shared_table;
   from.shared_blocks = a->shared_blocks;
   from.shared_i32 = a->shared_is_i32 != 0;
+  at.workspace_bytes = UINT64_MAX;   // (what is needed is another plan's)
+  const jf_status_t checked = block8_attend(&at, from, stream, false);
+  if (checked != JF_OK || at.B == 0) return checked;
+  at.workspace_bytes = a->attn.workspace_bytes;
+  Plan p;
+  if (!make_plan(at.B, at.H_q, at.H_kv, at.max_S, a->shared_blocks, p)) return JF_ERR_ARG;
+  if (at.workspace_bytes < p.bytes) return JF_ERR_WORKSPACE;
+  if (!tensor_form(at.B, at.H_q, at.H_kv, a->shared_blocks)) return block8_attend(&at, from, stream, true);
+  const auto s = static_cast<cudaStream_t>(stream);
+  SharedParams P{};
+  jf_status_t st = wait_record(s, &P.status);
+  if (st != JF_OK) return st;
+  P.q = static_cast<const uint16_t*>(at.q);
+  P.k_data = static_cast<const uint8_t*>(at.k_data);
+  P.v_data = static_cast<const uint8_t*>(at.v_data);
+  P.k_scales = at.k_scales;
+  P.v_scales = at.v_scales;
+  P.table = a->shared_table;
+  P.seq_lens = at.seq_lens;
+  P.part_o = reinterpret_cast<float*>(static_cast<char*>(at.workspace) + p.own);
+  P.part_ml = reinterpret_cast<float4*>(static_cast<char*>(at.workspace) + p.own + p.o_bytes);
+  P.num_blocks = at.num_blocks;
+  P.units = p.units;
+  P.H_q = at.H_q;
+  P.G = p.G;
+  P.rows = at.B * p.G;
+  P.row_tiles = p.row_tiles;
+  P.pairs = p.pairs;
+  P.tiles = p.tiles;
+  P.blocks = std::min(a->shared_blocks, p.tiles * kTileBlocks);
+  P.max_S = at.max_S;
+  P.scale = at.attn_scale;
+  P.softcap = at.softcap;
+  P.i32 = a->shared_is_i32 != 0;
+  if (at.q_dtype == JF_DTYPE_BF16)
+    st = at.codes == JF_CODES_INT8 ? launch<JF_DTYPE_BF16, JF_CODES_INT8>(P, p.grid, s) : launch<JF_DTYPE_BF16, JF_CODES_E4M3>(P, p.grid, s);
+  else
+    st = at.codes == JF_CODES_INT8 ? launch<JF_DTYPE_FP16, JF_CODES_INT8>(P, p.grid, s) : launch<JF_DTYPE_FP16, JF_CODES_E4M3>(P, p.grid, s);
+  if (st != JF_OK) return st;
+  from = Block8Source{};
+  from.behind = a->shared_blocks;
+  from.part_o = P.part_o;
+  from.part_ml = P.part_ml;
+  from.units = p.units;
+  from.grid = p.grid;
+  from.tiles = p.tiles;
+  from.pairs = p.pairs;
+  from.row_tiles = p.row_tiles;
+  at.workspace_bytes = p.own;
   return block8_attend(&at, from, stream, true);
 }
