@@ -15,6 +15,9 @@
 //   warps 0-3, 4-7   scores -> weights of row tile 0, 1 (a thread a row); the rescaling of O; the partial result
 //   warps 8-11       codes -> fp16 operands: 128 positions of K, then of V, two buffers each
 //   warp 12          issues the matrix products
+//   warp 13          looks blocks up and copies their codes into shared memory, 2048 bytes at a time
+// A row's scores are read from tensor memory 64 at a time, in loops, once for the maximum and once for the weights: held in registers and
+// unrolled they made the code twice what the instruction caches take (256 sequences over 65536 positions: 721 us and more).
 //
 // Work is a line of units -- (KV head, pair of row tiles, 128 positions) -- cut into pieces of one length, one for each thread block, so that all
 // multiprocessors end together; where a piece passes from one pair of row tiles to the next it leaves two partial results.  A single row
@@ -38,8 +41,6 @@ constexpr int kCodeBytes = kKeys * JF_HEAD_DIM;        // of a tile as it lies i
 constexpr int kStaged = 2;                             // K or V tiles on their way from memory
 constexpr int kNotes = 8;
 constexpr int kThreads = 512;
-// Registers a thread: the rows' warpgroups, the converting one, the one that issues; together what the block is launched with.
-constexpr int kRowRegs = 200, kConvertRegs = 72, kIssueRegs = 40;
 constexpr float kLag = 8.0f, kLift = 7.0f;             // log2; weights stay below 2^15
 constexpr float kSumLag = 24.0f, kSpread = 64.0f;
 constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
@@ -55,8 +56,8 @@ struct SharedParams {
   float* part_o;          // [piece, row tile of the pair][128][128]
   float4* part_ml;        // R - lift, m, sum
   int32_t* status;
-  int64_t num_blocks, units;
-  int32_t H_q, G, rows, row_tiles, pairs, tiles, blocks, max_S;   // rows: of a KV head; blocks: shared ones; tiles: of positions
+  int64_t num_blocks;
+  int32_t units, H_q, G, rows, row_tiles, pairs, tiles, blocks, max_S;   // rows: of a KV head; blocks: shared ones; tiles: of positions
   float scale, softcap;
   bool i32;
 };
@@ -69,23 +70,22 @@ struct alignas(16) Note {
   uint32_t odd;           // a K scale that is not above zero
 };
 struct Shared {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2], note_full[kNotes], products_done;
+  uint64_t code_full[kStaged], code_empty[kStaged], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2],
+      o_full[2], note_full[kNotes], products_done;
   Note note[kNotes];
   uint32_t tmem;
+  int begin, end;         // units of this thread block
 };
 
 // The units of a thread block, item by item (an item: a KV head and a pair of row tiles).
-struct Segment { int64_t u, end; int item, first, n; };   // n tiles of positions from `first` on
-__device__ __forceinline__ Segment units_of(const SharedParams& P) {
-  const int64_t c = blockIdx.x, all = gridDim.x;
-  return Segment{c * P.units / all, (c + 1) * P.units / all, 0, 0, 0};
-}
+struct Segment { int u, end, item, first, n; };   // n tiles of positions from `first` on
+__device__ __forceinline__ Segment units_of(const Shared& S) { return Segment{S.begin, S.end, 0, 0, 0}; }
 __device__ __forceinline__ bool next_segment(const SharedParams& P, Segment& s) {
   s.u += s.n;
   if (s.u >= s.end) return false;
-  s.item = static_cast<int>(s.u / P.tiles);
-  s.first = static_cast<int>(s.u - static_cast<int64_t>(s.item) * P.tiles);
-  s.n = static_cast<int>(min(static_cast<int64_t>(P.tiles - s.first), s.end - s.u));
+  s.item = s.u / P.tiles;
+  s.first = s.u - s.item * P.tiles;
+  s.n = min(P.tiles - s.first, s.end - s.u);
   return true;
 }
 __device__ __forceinline__ bool two_tiles(const SharedParams& P, const Segment& s) { return s.item % P.pairs * 2 + 1 < P.row_tiles; }
@@ -105,17 +105,18 @@ template <int CODES, bool HIGH> __device__ __forceinline__ uint32_t widen(uint32
   return d;
 }
 
-template <int CODES> __device__ __forceinline__ bool convert(const SharedParams& P, Shared& S, unsigned char* kv, unsigned char* staged) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, tid = threadIdx.x & 127;
-  const Segment range = units_of(P);
-  const int64_t begin = range.u, sides = 2 * (range.end - range.u);
+// Codes of the tiles in turn, K then V, and each tile's note.  `sent`: K and V tiles asked for.
+__device__ __forceinline__ bool load(const SharedParams& P, Shared& S, unsigned char* staged, int& sent) {
+  const int lane = threadIdx.x & 31;
+  const Segment range = units_of(S);
+  const int sides = 2 * (range.end - range.u);
   // four units' blocks are looked up at a time, a lane each, a round ahead
   struct Look { int id; float ks, vs; };
-  auto look_up = [&](int64_t u0) {
+  auto look_up = [&](int u0) {
     Look r{-1, 0.0f, 0.0f};
-    const int64_t u = u0 + (lane >> 3);
+    const int u = u0 + (lane >> 3);
     if (u < range.end) {
-      const int item = static_cast<int>(u / P.tiles), block = static_cast<int>(u - static_cast<int64_t>(item) * P.tiles) * kTileBlocks + (lane & 7);
+      const int item = u / P.tiles, block = (u - item * P.tiles) * kTileBlocks + (lane & 7);
       if (block < P.blocks) {
         const int64_t id = P.i32 ? static_cast<const int32_t*>(P.table)[block] : static_cast<const int64_t*>(P.table)[block];
         const int64_t row = static_cast<int64_t>(item / P.pairs) * P.num_blocks;
@@ -128,47 +129,21 @@ template <int CODES> __device__ __forceinline__ bool convert(const SharedParams&
     }
     return r;
   };
-  int64_t at = begin;          // first unit of `now`
-  Look now = look_up(begin), then = look_up(begin + 4);
-  // A thread copies the bytes that it converts: 16 of each block, so a wait for its own copies is enough.
-  auto fetch = [&](int64_t n) {
-    if (n < sides) {
-      const int64_t u = begin + (n >> 1);
-      const int off = static_cast<int>(u - at), head = static_cast<int>(u / P.tiles) / P.pairs;
-      const uint8_t* base = (n & 1 ? P.v_data : P.k_data) + static_cast<int64_t>(head) * P.num_blocks * (JF_BLOCK_SIZE * JF_HEAD_DIM) + tid * 16;
-      unsigned char* to = staged + (n % kStaged) * kCodeBytes + tid * 16;
-#pragma unroll
-      for (int i = 0; i < kTileBlocks; ++i) {
-        const int id = __shfl_sync(0xFFFFFFFFu, off < 4 ? now.id : then.id, (off & 3) * 8 + i);
-        if (id >= 0) cp_async_16(to + i * 2048, base + static_cast<int64_t>(id) * (JF_BLOCK_SIZE * JF_HEAD_DIM));
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int n = 0; n < kStaged; ++n) fetch(n);
-  // where a thread's 16 channels go: two chunks of 16 bytes of a row; the upper half of a row's threads takes them in the other order, so
-  // that eight threads meet all banks
-  const int row = tid >> 3, cc = tid & 7, j0 = (cc & 3) * 2, sw = row & 7;
-  const uint32_t base = (cc >> 2) * kSlabBytes + row * 128;
-  const uint32_t lo_at = base + ((j0 ^ sw) << 4), hi_at = base + (((j0 + 1) ^ sw) << 4);
-  for (int64_t n = 0; n < sides; ++n) {
-    const int64_t g = n >> 1;
-    const int side = static_cast<int>(n & 1), slot = static_cast<int>(g & 1);
-    if (begin + g >= at + 4) {
+  Look now = look_up(range.u), then = look_up(range.u + 4);
+#pragma unroll 1
+  for (int& n = sent; n < sides; ++n) {
+    const int g = n >> 1, u = range.u + g;
+    const int side = n & 1, slot = n % kStaged, off = (g & 3) * 8;
+    if (side == 0 && g > 0 && off == 0) {
       now = then;
-      at += 4;
-      then = look_up(at + 4);
+      then = look_up(u + 4);
     }
-    if (g >= 2 && !wait_warp(side ? &S.v_empty[slot] : &S.k_empty[slot], static_cast<uint32_t>((g >> 1) - 1) & 1u)) {
-      cp_async_wait_all();
-      return false;
-    }
-    const int off = static_cast<int>(begin + g - at) * 8;
-    if (side == 0 && warp == 0) {   // the note of this tile
-      const int id = __shfl_sync(0xFFFFFFFFu, now.id, (off + lane) & 31);
+    if (n >= kStaged && !wait_warp(&S.code_empty[slot], static_cast<uint32_t>(n / kStaged - 1) & 1u)) return false;
+    const int id = __shfl_sync(0xFFFFFFFFu, now.id, (off + lane) & 31);
+    const bool mine = lane < kTileBlocks, is = mine && id >= 0;
+    const unsigned there = __ballot_sync(0xFFFFFFFFu, is);
+    if (side == 0) {
       const float ks = __shfl_sync(0xFFFFFFFFu, now.ks, (off + lane) & 31), vs = __shfl_sync(0xFFFFFFFFu, now.vs, (off + lane) & 31);
-      const bool mine = lane < kTileBlocks, is = mine && id >= 0;
       float lg;
       asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(vs == 0.0f ? 0x1p-100f : vs));   // (weightless, but its positions count)
       Note& note = S.note[g % kNotes];
@@ -176,7 +151,7 @@ template <int CODES> __device__ __forceinline__ bool convert(const SharedParams&
         note.ks[lane] = is ? ks : 1.0f;
         note.lvs[lane] = is ? lg : 0.0f;
       }
-      const unsigned dead = __ballot_sync(0xFFFFFFFFu, mine && !is), odd = __ballot_sync(0xFFFFFFFFu, is && !(ks > 0.0f));
+      const unsigned odd = __ballot_sync(0xFFFFFFFFu, is && !(ks > 0.0f));
       float lo = is ? lg : 3.0e38f, hi = is ? lg : -3.0e38f;
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) {
@@ -186,35 +161,70 @@ template <int CODES> __device__ __forceinline__ bool convert(const SharedParams&
       if (lane == 0) {
         note.lvs_lo = lo;
         note.lvs_hi = hi;
-        note.dead = dead;
+        note.dead = ~there & 255u;
         note.odd = odd;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.note_full[g % kNotes]);
     }
-    cp_async_wait_group<kStaged - 1>();
-    const unsigned char* from = staged + (n % kStaged) * kCodeBytes + tid * 16;
+    if (lane == 0) mbar_expect_tx(&S.code_full[slot], __popc(there) * (JF_BLOCK_SIZE * JF_HEAD_DIM));
+    __syncwarp();
+    if (is) {
+      const int head = u / P.tiles / P.pairs;
+      bulk_g2s(staged + slot * kCodeBytes + lane * (JF_BLOCK_SIZE * JF_HEAD_DIM),
+               (side ? P.v_data : P.k_data) + (static_cast<int64_t>(head) * P.num_blocks + id) * (JF_BLOCK_SIZE * JF_HEAD_DIM),
+               JF_BLOCK_SIZE * JF_HEAD_DIM, &S.code_full[slot]);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+// The copies that may be in flight: the block's shared memory stays until they are there, or a wait for one runs out.
+__device__ __forceinline__ bool arrived(Shared& S, int sent) {
+  for (int n = max(sent - kStaged, 0); n < sent; ++n)
+    if (!wait_warp(&S.code_full[n % kStaged], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
+  return true;
+}
+
+template <int CODES> __device__ __forceinline__ bool convert(const SharedParams& P, Shared& S, unsigned char* kv, const unsigned char* staged) {
+  const int lane = threadIdx.x & 31, tid = threadIdx.x & 127;
+  const Segment range = units_of(S);
+  const int sides = 2 * (range.end - range.u);
+  // A thread has the same 16 channels of one row of every block: two chunks of 16 bytes of the operand's row.  Eight threads that read or write
+  // together have half of a row and the other half of the next one, which the swizzle puts on all banks.
+  const int row = tid >> 4 << 1 | (tid >> 2 & 1), cc = ((tid >> 2 ^ tid >> 3) & 1) << 2 | (tid & 3), j0 = (cc & 3) * 2, sw = row & 7;
+  const uint32_t base = (cc >> 2) * kSlabBytes + row * 128;
+  const uint32_t lo_at = base + ((j0 ^ sw) << 4), hi_at = base + (((j0 + 1) ^ sw) << 4);
+#pragma unroll 1
+  for (int n = 0; n < sides; ++n) {
+    const int g = n >> 1, side = n & 1, slot = g & 1, stage = n % kStaged;
+    if (!wait_warp(&S.code_full[stage], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
+    const unsigned char* from = staged + stage * kCodeBytes + row * JF_HEAD_DIM + cc * 16;
+    uint4 x[kTileBlocks];
+#pragma unroll
+    for (int i = 0; i < kTileBlocks; ++i) x[i] = *reinterpret_cast<const uint4*>(from + i * 2048);
+    const uint32_t dead = S.note[g % kNotes].dead;
+    if (dead) {
+#pragma unroll
+      for (int i = 0; i < kTileBlocks; ++i)
+        if (dead >> i & 1u) x[i] = make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.code_empty[stage]);
+    if (g >= 2 && !wait_warp(side ? &S.v_empty[slot] : &S.k_empty[slot], static_cast<uint32_t>((g >> 1) - 1) & 1u)) return false;
     unsigned char* to = kv + (side * 2 + slot) * kTileBytes;
 #pragma unroll
     for (int i = 0; i < kTileBlocks; ++i) {
-      const bool is = __shfl_sync(0xFFFFFFFFu, now.id, off + i) >= 0;
-      uint4 x = *reinterpret_cast<const uint4*>(from + i * 2048);
-      uint4 a = make_uint4(0, 0, 0, 0), b = a;
-      if (is) {
-        x.x = flip<CODES>(x.x); x.y = flip<CODES>(x.y); x.z = flip<CODES>(x.z); x.w = flip<CODES>(x.w);
-        a = make_uint4(widen<CODES, false>(x.x), widen<CODES, true>(x.x), widen<CODES, false>(x.y), widen<CODES, true>(x.y));
-        b = make_uint4(widen<CODES, false>(x.z), widen<CODES, true>(x.z), widen<CODES, false>(x.w), widen<CODES, true>(x.w));
-      }
-      const bool swap = cc >= 4;
-      *reinterpret_cast<uint4*>(to + i * 2048 + (swap ? hi_at : lo_at)) = swap ? b : a;
-      *reinterpret_cast<uint4*>(to + i * 2048 + (swap ? lo_at : hi_at)) = swap ? a : b;
+      const uint32_t w[4] = {flip<CODES>(x[i].x), flip<CODES>(x[i].y), flip<CODES>(x[i].z), flip<CODES>(x[i].w)};
+      *reinterpret_cast<uint4*>(to + i * 2048 + lo_at) =
+          make_uint4(widen<CODES, false>(w[0]), widen<CODES, true>(w[0]), widen<CODES, false>(w[1]), widen<CODES, true>(w[1]));
+      *reinterpret_cast<uint4*>(to + i * 2048 + hi_at) =
+          make_uint4(widen<CODES, false>(w[2]), widen<CODES, true>(w[2]), widen<CODES, false>(w[3]), widen<CODES, true>(w[3]));
     }
     fence_proxy_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(side ? &S.v_full[slot] : &S.k_full[slot]);
-    fetch(n + kStaged);
   }
-  cp_async_wait_all();
   return true;
 }
 
@@ -224,16 +234,16 @@ template <int CODES> __device__ __forceinline__ bool convert(const SharedParams&
 __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint32_t q_smem, uint32_t kv_smem, uint32_t tmem) {
   constexpr uint32_t qk = instruction<JF_DTYPE_FP16>(false), pv = instruction<JF_DTYPE_FP16>(true);
   const uint64_t q_op = operand(q_smem, 16), k_op = operand(kv_smem, 16), v_op = operand(kv_smem + 2 * kTileBytes, kSlabBytes);
-  Segment s = units_of(P);
-  uint32_t base = 0, p_count[2] = {0, 0}, q_count[2] = {0, 0};   // tiles of positions, weights, queries so far
+  Segment s = units_of(S);
+  uint32_t base = 0, p_count0 = 0, p_count1 = 0, q_count0 = 0, q_count1 = 0;   // tiles of positions, weights, queries so far
   while (next_segment(P, s)) {
     const bool two = two_tiles(P, s);
     const int jobs = two ? 2 * s.n : s.n;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (has_jobs(P, s, t) && !wait_warp(&S.q_full[t], q_count[t]++ & 1)) return false;
-    auto scores = [&](int j) {
-      const int t = j & 1;
+    if (!wait_warp(&S.q_full[0], q_count0++ & 1)) return false;
+    if (jobs > 1 && !wait_warp(&S.q_full[1], q_count1++ & 1)) return false;
+    // (the group as a constant: arrays and addresses that depend on it stay out of memory)
+    auto scores = [&](auto t_tag, int j) {
+      constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
       if (!wait_warp(&S.k_full[slot], g >> 1 & 1)) return false;
       tc_fence_after();
@@ -250,18 +260,16 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
       __syncwarp();
       return true;
     };
-    for (int j = 0; j < min(jobs, 2); ++j)
-      if (!scores(j)) return false;
-    for (int j = 0; j < jobs; ++j) {
-      const int t = j & 1;
+    auto job = [&](auto t_tag, int j, uint32_t parity) {
+      constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
       if (!wait_warp(&S.v_full[slot], g >> 1 & 1)) return false;
+      const uint64_t b = v_op + slot * (kTileBytes >> 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // the weights come in two halves
-        if (!wait_warp(&S.p_full[t][h], p_count[t] & 1)) return false;
+        if (!wait_warp(&S.p_full[t][h], parity)) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t b = v_op + slot * (kTileBytes >> 4);
 #pragma unroll
           for (int k = h * 4; k < h * 4 + 4; ++k)
             mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
@@ -272,8 +280,15 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
         }
         __syncwarp();
       }
-      ++p_count[t];
-      if (j + 2 < jobs && !scores(j + 2)) return false;
+      return j + 2 >= jobs || scores(t_tag, j + 2);
+    };
+    using First = std::integral_constant<int, 0>;
+    using Second = std::integral_constant<int, 1>;
+    if (!scores(First(), 0) || (jobs > 1 && !scores(Second(), 1))) return false;
+#pragma unroll 1
+    for (int j = 0; j < jobs; j += 2) {
+      if (!job(First(), j, p_count0++ & 1)) return false;
+      if (j + 1 < jobs && !job(Second(), j + 1, p_count1++ & 1)) return false;
     }
     base += s.n;
   }
@@ -326,45 +341,55 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
     const int tile = s.item % P.pairs * 2 + (two_tiles(P, s) ? t : 0), row = tile * kRows + r;
     Row to{0.0f, INT32_MAX, tile * kRows + warp * 32 >= P.rows};
     if (!has_jobs(P, s, t)) return to;   // (its queries would not be waited for)
-    uint4 x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = make_uint4(0, 0, 0, 0);
+    const uint4* from = nullptr;
     if (row < P.rows) {
       const int b = row / P.G, head = s.item / P.pairs * P.G + row % P.G;
-      const uint4* from = reinterpret_cast<const uint4*>(P.q + (static_cast<int64_t>(b) * P.H_q + head) * JF_HEAD_DIM);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __ldg(from + i);
+      from = reinterpret_cast<const uint4*>(P.q + (static_cast<int64_t>(b) * P.H_q + head) * JF_HEAD_DIM);
       const int len = max(min(P.seq_lens[b], P.max_S), 0);
       if (len < P.blocks * JF_BLOCK_SIZE) to.len = len;
     }
     float amax = 0.0f, odd = 0.0f;   // odd: NaN if an element is no number, else 0
+    uint4 x[4];
+    auto read = [&](int i) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      for (int k = 0; k < 4; ++k) x[k] = from ? __ldg(from + i + k) : make_uint4(0, 0, 0, 0);
+    };
+    // (twice through the row, in loops: the code runs once a segment and comes from far)
+#pragma unroll 1
+    for (int i = 0; i < 16; i += 4) {
+      read(i);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float y = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16 * e));
-          amax = fmaxf(amax, fabsf(y));
-          odd = fmaf(y, 0.0f, odd);
-        }
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float y = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16 * e));
+            amax = fmaxf(amax, fabsf(y));
+            odd = fmaf(y, 0.0f, odd);
+          }
+      }
     }
     constexpr int TOP = 13;
     const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127, 127), TOP - 126);
     const float up = copysignf(__uint_as_float(static_cast<uint32_t>(TOP - e + 127) << 23), P.scale);
     to.f = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) * fabsf(P.scale) * kLog2e + odd;
     unsigned char* out = q_smem + r * 128;
+#pragma unroll 1
+    for (int i = 0; i < 16; i += 4) {
+      read(i);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t h[4];
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+        uint32_t h[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float lo = Elem<DT>::to_f32(static_cast<uint16_t>(w[k])) * up, hi = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)) * up;
-        h[k] = odd == 0.0f ? round2<JF_DTYPE_FP16>(lo, hi) : 0u;
+        for (int k = 0; k < 4; ++k) {
+          const float lo = Elem<DT>::to_f32(static_cast<uint16_t>(w[k])) * up, hi = Elem<DT>::to_f32(static_cast<uint16_t>(w[k] >> 16)) * up;
+          h[k] = odd == 0.0f ? round2<JF_DTYPE_FP16>(lo, hi) : 0u;
+        }
+        *reinterpret_cast<uint4*>(out + (i >> 3) * kSlabBytes + ((((i + j) & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
-      *reinterpret_cast<uint4*>(out + (i >> 3) * kSlabBytes + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     fence_proxy_async();
     __syncwarp();
@@ -372,11 +397,10 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
     return to;
   };
 
-  Segment s = units_of(P);
+  Segment s = units_of(S);
   uint32_t base = 0, s_count = 0, o_count = 0;
-  bool more = next_segment(P, s);
-  Row row = more ? load_query(s) : Row{0.0f, 0, true};
-  while (more) {
+  Row row{0.0f, 0, true};
+  for (bool more = true; more;) {   // (the first time round there is nothing but queries to be loaded)
     const bool two = two_tiles(P, s);
     float R = kNone, m = kNone, l = 0.0f, lvs_top = -3.0e38f;
     bool have = false;
@@ -393,44 +417,52 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
         have = true;
         continue;
       }
-      uint32_t u[128];
-      float* x = reinterpret_cast<float*>(u);
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) tmem_ld32(s_at + c, u + c);
-      float f[kTileBlocks], lvs[kTileBlocks];
-#pragma unroll
-      for (int b = 0; b < kTileBlocks; ++b) {
-        f[b] = note.ks[b] * row.f;
-        lvs[b] = note.lvs[b];
-      }
-      const uint32_t dead = note.dead;
       lvs_top = fmaxf(lvs_top, note.lvs_hi);
+      const uint32_t dead = note.dead;
       const bool wide = lvs_top - note.lvs_lo > kSpread;
       const bool masked = __any_sync(0xFFFFFFFFu, row.len < end) || dead != 0;
-      const bool scaled = CAP || masked || wide || note.odd != 0;
-      tc_wait_ld();
-      if (scaled) {
+      const bool scaled = CAP || masked || wide || note.odd != 0;   // scores are brought to units of log2 one by one, and written back
+      float top_x = -INFINITY, top_w = -INFINITY;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t u[64];
+        float* x = reinterpret_cast<float*>(u);
+        tmem_ld32(s_at + h * 64, u);
+        tmem_ld32(s_at + h * 64 + 32, u + 32);
+        float f[4], lvs[4];
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&note.ks[h * 4]);
+        *reinterpret_cast<float4*>(lvs) = *reinterpret_cast<const float4*>(&note.lvs[h * 4]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int b = 0; b < 4; ++b) f[b] *= row.f;
+        tc_wait_ld();
+        if (scaled) {
 #pragma unroll
-          for (int c = h * 64; c < h * 64 + 64; c += 2) split(mul2(pair(x[c], x[c + 1]), pair(f[c / 16], f[c / 16])), x[c], x[c + 1]);
-          if (CAP) cap64(x + h * 64, cap2, inv_cap);
+          for (int k = 0; k < 64; k += 2) split(mul2(pair(x[k], x[k + 1]), pair(f[k / 16], f[k / 16])), x[k], x[k + 1]);
+          if (CAP) cap64(x, cap2, inv_cap);
           if (masked) {
-            const int left = row.len - (end - kKeys);
+            const int left = row.len - (end - kKeys) - h * 64;
 #pragma unroll
-            for (int c = h * 64; c < h * 64 + 64; ++c) x[c] = c < left && !(dead >> (c / 16) & 1u) ? x[c] : -INFINITY;
+            for (int w = 0; w < 2; ++w) {
+              const int some = left - w * 32;
+              const uint32_t gone = (dead >> (h * 4 + w * 2) & 1u ? 0xFFFFu : 0u) | (dead >> (h * 4 + w * 2 + 1) & 1u ? 0xFFFF0000u : 0u);
+              const uint32_t seen = (some >= 32 ? ~0u : some <= 0 ? 0u : (1u << some) - 1u) & ~gone;
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[w * 32 + k] = seen >> k & 1u ? x[w * 32 + k] : -INFINITY;
+            }
           }
+          tmem_st32(s_at + h * 64, u);
+          tmem_st32(s_at + h * 64 + 32, u + 32);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) f[b] = 1.0f;
         }
 #pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b) f[b] = 1.0f;
+        for (int b = 0; b < 4; b += 2) {
+          const float y0 = largest16(x + b * 16) * f[b], y1 = largest16(x + b * 16 + 16) * f[b + 1];
+          top_x = max3(top_x, y0, y1);
+          top_w = max3(top_w, y0 + lvs[b], y1 + lvs[b + 1]);
+        }
       }
-      float top_x = -INFINITY, top_w = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < kTileBlocks; ++b) {
-        const float y = largest16(x + b * 16) * f[b];
-        top_x = max3(top_x, y, y);
-        top_w = max3(top_w, y + lvs[b], y + lvs[b]);
-      }
+      if (scaled) tc_wait_st();
       if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag))) {
         const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
         R = to;
@@ -442,31 +474,40 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
         m = to;
       }
       const float ref = R - kLift;
-      if (wide) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) l += ex2(x[c] - m);
-      }
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
+        uint32_t u[64], p[32];
+        const float* x = reinterpret_cast<const float*>(u);
+        tmem_ld32(s_at + h * 64, u);
+        tmem_ld32(s_at + h * 64 + 32, u + 32);
+        float f[4], lvs[4];
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&note.ks[h * 4]);
+        *reinterpret_cast<float4*>(lvs) = *reinterpret_cast<const float4*>(&note.lvs[h * 4]);
 #pragma unroll
-        for (int b = h * 4; b < h * 4 + 4; ++b) {
+        for (int b = 0; b < 4; ++b) f[b] = scaled ? 1.0f : f[b] * row.f;
+        tc_wait_ld();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
           const uint64_t f2 = pair(f[b], f[b]), c2 = pair(lvs[b] - ref, lvs[b] - ref);
           uint64_t sum = 0;
 #pragma unroll
-          for (int c = b * 16; c < b * 16 + 16; c += 2) {
+          for (int k = b * 16; k < b * 16 + 16; k += 2) {
             float a, d;
-            split(fma2(pair(x[c], x[c + 1]), f2, c2), a, d);
+            split(fma2(pair(x[k], x[k + 1]), f2, c2), a, d);
             a = ex2(a);
             d = ex2(d);
             sum = add2(sum, pair(a, d));
-            p[(c - h * 64) / 2] = round2<JF_DTYPE_FP16>(a, d);
+            p[k / 2] = round2<JF_DTYPE_FP16>(a, d);
           }
           if (!wide) {
             float a, d;
             split(sum, a, d);
             l = fmaf(a + d, ex2(ref - lvs[b] - m), l);
           }
+        }
+        if (wide) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) l += ex2(x[k] - m);
         }
         tmem_st32(s_at + h * 32, p);
         tc_wait_st();
@@ -478,6 +519,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
     }
     // the next queries, then the partial result
     const int64_t piece = (static_cast<int64_t>(blockIdx.x) + s.item) * 2 + t;
+    const bool any = s.n > 0;
     base += s.n;
     const float ref = R - kLift;
     const bool idle = row.idle;
@@ -498,7 +540,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
       }
       tc_fence_before();
     }
-    P.part_ml[piece * kRows + r] = make_float4(ref, m, l, 0.0f);
+    if (any) P.part_ml[piece * kRows + r] = make_float4(ref, m, l, 0.0f);
     __syncwarp();
   }
   return true;
@@ -523,8 +565,14 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
       mbar_init(&S.p_full[i][1], 4);
       mbar_init(&S.o_full[i], 1);
     }
+    for (int i = 0; i < kStaged; ++i) {
+      mbar_init(&S.code_full[i], 1);
+      mbar_init(&S.code_empty[i], 4);
+    }
     for (int i = 0; i < kNotes; ++i) mbar_init(&S.note_full[i], 1);
     mbar_init(&S.products_done, 1);
+    S.begin = static_cast<int>(static_cast<int64_t>(blockIdx.x) * P.units / gridDim.x);
+    S.end = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * P.units / gridDim.x);
     fence_barrier_init();
   }
   if (warp == 12) {
@@ -539,20 +587,19 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   pdl_trigger();
   // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
   bool ok = true;
-  if (warp >= 12) {
-    regs_dec<kIssueRegs>();
-    if (warp == 12) {
-      ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
-      if (elect_one()) tc_commit(&S.products_done);
-      __syncwarp();
-      ok &= wait_warp(&S.products_done, 0);
-    }
-  } else if (warp >= 8) {
-    regs_dec<kConvertRegs>();
-    ok = convert<CODES>(P, S, kv, staged);
-  } else {
-    regs_inc<kRowRegs>();
+  if (warp < 8) {
     ok = soften<DT, CAP>(P, S, smem + (warp >> 2) * kTileBytes, tmem, warp >> 2);
+  } else if (warp < 12) {
+    ok = convert<CODES>(P, S, kv, staged);
+  } else if (warp == 12) {
+    ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
+    if (elect_one()) tc_commit(&S.products_done);
+    __syncwarp();
+    ok &= wait_warp(&S.products_done, 0);
+  } else if (warp == 13) {
+    int sent = 0;
+    ok = load(P, S, staged, sent);
+    ok &= arrived(S, sent);
   }
   if (!ok) report_status(P.status, JF_ERR_TIMEOUT);
   __syncwarp();
@@ -590,8 +637,8 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) 
   const int seen = std::min(shared_blocks, (max_S + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE);   // of the shared blocks
   p.tiles = (seen + kTileBlocks - 1) / kTileBlocks;
   p.items = int64_t{H_kv} * p.pairs;
-  if (p.items > INT32_MAX / 4) return false;
   p.units = p.items * p.tiles;
+  if (p.units > INT32_MAX / 2) return false;
   p.grid = static_cast<int>(std::min<int64_t>(num_sms(), p.units));
   p.own = (block8_attn_workspace(B, H_q, H_kv, std::max(max_S - shared_blocks * JF_BLOCK_SIZE, 1)) + 255) / 256 * 256;
   if (p.own == 0) return false;
@@ -603,12 +650,6 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) 
 
 template <int DT, int CODES, bool CAP> jf_status_t launch(const SharedParams& P, int grid, cudaStream_t s) {
   auto* kernel = block8_shared_kernel<DT, CODES, CAP>;
-  static const int regs = [] {
-    cudaFuncAttributes f{};
-    return cudaFuncGetAttributes(&f, block8_shared_kernel<DT, CODES, CAP>) == cudaSuccess ? f.numRegs : 0;
-  }();
-  // (a warpgroup that asks for more than the block has waits for good)
-  if (regs * kThreads < 128 * (2 * kRowRegs + kConvertRegs + kIssueRegs)) return JF_ERR_UNSUPPORTED;
   JF_ENSURE_SMEM(kernel, kSmemBytes);
   JF_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmemBytes, s, P));
   return JF_OK;
@@ -658,7 +699,7 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   P.part_o = reinterpret_cast<float*>(static_cast<char*>(at.workspace) + p.own);
   P.part_ml = reinterpret_cast<float4*>(static_cast<char*>(at.workspace) + p.own + p.o_bytes);
   P.num_blocks = at.num_blocks;
-  P.units = p.units;
+  P.units = static_cast<int32_t>(p.units);
   P.H_q = at.H_q;
   P.G = p.G;
   P.rows = at.B * p.G;

@@ -50,6 +50,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* x) {
       "%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::JF_W8(x, 0), JF_W8(x, 8), JF_W8(x, 16), JF_W8(x, 24), "r"(at)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::JF_W8(x, 0), JF_W8(x, 8), "r"(at)
+      : "memory");
+}
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -59,6 +64,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // Bounded.  Most waits end within a few attempts; the clock that bounds the others is read only after that (a read of it
 // in front of every wait that did not end at once took 0.4 us of each step).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
   for (int i = 0; i < 1000; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait(bar, parity, kTensorWaitNs);
