@@ -12,12 +12,15 @@
 // same exponentials, times exp2(R - log2 vs - m): one more of them for 16 positions.  Where V scales lie so far apart (beyond
 // 2^kSpread) that a weight could vanish while its position counts, those tiles take an exponential more for every position.
 //
-//   warps 0-3, 4-7   scores -> weights of row tile 0, 1 (a thread a row); the rescaling of O; the partial result
-//   warps 8-11       codes -> fp16 operands: 128 positions of K, then of V, two buffers each
-//   warp 12          issues the matrix products
-//   warp 13          looks blocks up and copies their codes into shared memory, 2048 bytes at a time
-// A row's scores are read from tensor memory 64 at a time, in loops, once for the maximum and once for the weights: held in registers and
-// unrolled they made the code twice what the instruction caches take (256 sequences over 65536 positions: 721 us and more).
+//   warps 0-15       scores -> weights: 8 for a row tile, 4 (a thread a row) for each half of a tile's 128 positions; the rescaling of O;
+//                    the partial result
+//   warps 16-19      codes -> fp16 operands: 128 positions of K, then of V, two buffers each
+//   warp 20          issues the matrix products
+//   warp 21          looks blocks up and copies their codes into shared memory, 2048 bytes at a time
+// The product of a tile's weights with V comes in two halves, the first before the second, and a row's reference may move between any two of
+// them: the two threads of a row hand it to one another, the first half's after its maximum to the second's, that to the first half's of the next
+// tile.  (A thread for all 128 positions left the special function units idle for more than half of the time: 727 us for 256 sequences over 65536
+// positions.  Code unrolled for 128 scores was twice what the instruction caches take: 966.)
 //
 // Work is a line of units -- (KV head, pair of row tiles, 128 positions) -- cut into pieces of one length, one for each thread block, so that all
 // multiprocessors end together; where a piece passes from one pair of row tiles to the next it leaves two partial results.  A single row
@@ -40,12 +43,12 @@ constexpr int kTileBlocks = kKeys / JF_BLOCK_SIZE;
 constexpr int kCodeBytes = kKeys * JF_HEAD_DIM;        // of a tile as it lies in the cache
 constexpr int kStaged = 2;                             // K or V tiles on their way from memory
 constexpr int kNotes = 8;
-constexpr int kThreads = 512;
+constexpr int kThreads = 768;
 constexpr float kLag = 8.0f, kLift = 7.0f;             // log2; weights stay below 2^15
 constexpr float kSumLag = 24.0f, kSpread = 64.0f;
 constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSmemBytes = 2 * kTileBytes + 4 * kTileBytes + kStaged * kCodeBytes + 1024;
+constexpr int kSmemBytes = 227 * 1024;                 // 6 operands, the codes and Shared leave 992 bytes to bring the first to a multiple of 1024
 
 struct SharedParams {
   const uint16_t* q;
@@ -54,7 +57,7 @@ struct SharedParams {
   const void* table;
   const int32_t* seq_lens;
   float* part_o;          // [piece, row tile of the pair][128][128]
-  float4* part_ml;        // R - lift, m, sum
+  float4* part_ml;        // [..][128][half]: R - lift (of the first half), m, sum
   int32_t* status;
   int64_t num_blocks;
   int32_t units, H_q, G, rows, row_tiles, pairs, tiles, blocks, max_S;   // rows: of a KV head; blocks: shared ones; tiles: of positions
@@ -71,11 +74,15 @@ struct alignas(16) Note {
 };
 struct Shared {
   uint64_t code_full[kStaged], code_empty[kStaged], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2],
-      o_full[2], note_full[kNotes], products_done;
+      pv_done[2][2], moved[2][2][4], note_full[kNotes], products_done;
   Note note[kNotes];
+  float reference[2][kRows];
   uint32_t tmem;
   int begin, end;         // units of this thread block
 };
+
+constexpr int kUsedBytes = 6 * kTileBytes + kStaged * kCodeBytes + static_cast<int>(sizeof(Shared));
+static_assert(kUsedBytes <= kSmemBytes, "");
 
 // The units of a thread block, item by item (an item: a KV head and a pair of row tiles).
 struct Segment { int u, end, item, first, n; };   // n tiles of positions from `first` on
@@ -245,7 +252,7 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
     auto scores = [&](auto t_tag, int j) {
       constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
-      if (!wait_warp(&S.k_full[slot], g >> 1 & 1)) return false;
+      if ((!two || t == 0) && !wait_warp(&S.k_full[slot], g >> 1 & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = q_op + t * (kTileBytes >> 4), b = k_op + slot * (kTileBytes >> 4);
@@ -263,7 +270,7 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
     auto job = [&](auto t_tag, int j, uint32_t parity) {
       constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
-      if (!wait_warp(&S.v_full[slot], g >> 1 & 1)) return false;
+      if ((!two || t == 0) && !wait_warp(&S.v_full[slot], g >> 1 & 1)) return false;
       const uint64_t b = v_op + slot * (kTileBytes >> 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // the weights come in two halves
@@ -272,11 +279,9 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
         if (elect_one()) {
 #pragma unroll
           for (int k = h * 4; k < h * 4 + 4; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
-          if (h == 1) {
-            if (!two || t == 1) tc_commit(&S.v_empty[slot]);
-            if (j + 2 >= jobs) tc_commit(&S.o_full[t]);
-          }
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + h * 64 + (k & 3) * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
+          tc_commit(&S.pv_done[t][h]);
+          if (h == 1 && (!two || t == 1)) tc_commit(&S.v_empty[slot]);
         }
         __syncwarp();
       }
@@ -305,16 +310,16 @@ __device__ __forceinline__ float largest16(const float* s) {
   b = max3(b, s[12], s[13]);
   return max3(max3(a, b, s[14]), s[15], s[15]);
 }
-// cap * tanh(x / cap) of 64 scores, in units of log2 (cap2: the cap in these units), for the whole warp the same way: up to
+// cap * tanh(x / cap) of 32 scores, in units of log2 (cap2: the cap in these units), for the whole warp the same way: up to
 // |x| = cap by a polynomial (relative error 6.6e-7), beyond it as cap - 2 cap / (e^(2x / cap) + 1).  A NaN stays one.
-__device__ __forceinline__ void cap64(float* x, float cap2, float inv) {
+__device__ __forceinline__ void cap32(float* x, float cap2, float inv) {
   float most = 0.0f;
 #pragma unroll
-  for (int c = 0; c < 64; ++c) most = fmaxf(most, fabsf(x[c]));
+  for (int c = 0; c < 32; ++c) most = fmaxf(most, fabsf(x[c]));
   if (__all_sync(0xFFFFFFFFu, most <= cap2)) {
     const uint64_t i2 = pair(inv, inv);
 #pragma unroll
-    for (int c = 0; c < 64; c += 2) {
+    for (int c = 0; c < 32; c += 2) {
       const uint64_t v = pair(x[c], x[c + 1]), z = mul2(v, i2), w = mul2(z, z);
       uint64_t q = fma2(w, pair(-0.00312657771f, -0.00312657771f), pair(0.0169064086f, 0.0169064086f));
       q = fma2(q, w, pair(-0.0517682843f, -0.0517682843f));
@@ -325,14 +330,14 @@ __device__ __forceinline__ void cap64(float* x, float cap2, float inv) {
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < 64; ++c) x[c] = cap2 - __fdividef(2.0f * cap2, ex2(min_or_nan(x[c] * inv * (2.0f * kLog2e), 126.0f)) + 1.0f);
+    for (int c = 0; c < 32; ++c) x[c] = cap2 - __fdividef(2.0f * cap2, ex2(min_or_nan(x[c] * inv * (2.0f * kLog2e), 126.0f)) + 1.0f);
   }
 }
 
-template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedParams& P, Shared& S, unsigned char* q_smem, uint32_t tmem, int t) {
+template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedParams& P, Shared& S, unsigned char* q_smem, uint32_t tmem, int t, int half) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, r = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-  const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+  const uint32_t s_at = tmem + lanes + t * 128 + half * 64, o_at = tmem + lanes + 256 + t * 128;   // of this half; of the row
   const float cap2 = CAP ? P.softcap * kLog2e : 0.0f, inv_cap = CAP ? 1.0f / cap2 : 0.0f;
   // The row's query as fp16 into the operand's place; what brings its products to scores in units of log2, and the positions that it sees.
   // (more than there are: all of them)
@@ -377,7 +382,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
     to.f = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) * fabsf(P.scale) * kLog2e + odd;
     unsigned char* out = q_smem + r * 128;
 #pragma unroll 1
-    for (int i = 0; i < 16; i += 4) {
+    for (int i = half * 8; i < half * 8 + 8; i += 4) {   // (half of the row for each of its two threads)
       read(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -398,141 +403,137 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
   };
 
   Segment s = units_of(S);
-  uint32_t base = 0, s_count = 0, o_count = 0;
+  uint32_t base = 0, tiles = 0, turns = 0;   // tiles of positions so far: of the block, of this group, of those with rows of this warp
   Row row{0.0f, 0, true};
   for (bool more = true; more;) {   // (the first time round there is nothing but queries to be loaded)
     const bool two = two_tiles(P, s);
     float R = kNone, m = kNone, l = 0.0f, lvs_top = -3.0e38f;
     bool have = false;
+#pragma unroll 1
     for (int i = two ? 0 : t; i < s.n; i += two ? 1 : 2) {
       const uint32_t g = base + i;
       const Note& note = S.note[g % kNotes];
       const int end = (s.first + i + 1) * kKeys;
       if (!wait_warp(&S.note_full[g % kNotes], g / kNotes & 1)) return false;
-      if (!wait_warp(&S.s_full[t], s_count++ & 1)) return false;
-      tc_fence_after();
-      if (row.idle) {   // (whatever the weights of rows that are none are)
-        __syncwarp();
-        if (lane < 2) mbar_arrive(&S.p_full[t][lane]);
-        have = true;
-        continue;
-      }
       lvs_top = fmaxf(lvs_top, note.lvs_hi);
-      const uint32_t dead = note.dead;
+      const uint32_t dead = note.dead >> half * 4 & 15u;
       const bool wide = lvs_top - note.lvs_lo > kSpread;
       const bool masked = __any_sync(0xFFFFFFFFu, row.len < end) || dead != 0;
       const bool scaled = CAP || masked || wide || note.odd != 0;   // scores are brought to units of log2 one by one, and written back
-      float top_x = -INFINITY, top_w = -INFINITY;
+      if (!wait_warp(&S.s_full[t], tiles & 1)) return false;
+      tc_fence_after();
+      if (!row.idle) {   // (whatever the weights of rows that are none are)
+        float top_x = -INFINITY, top_w = -INFINITY;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        uint32_t u[64];
-        float* x = reinterpret_cast<float*>(u);
-        tmem_ld32(s_at + h * 64, u);
-        tmem_ld32(s_at + h * 64 + 32, u + 32);
-        float f[4], lvs[4];
-        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&note.ks[h * 4]);
-        *reinterpret_cast<float4*>(lvs) = *reinterpret_cast<const float4*>(&note.lvs[h * 4]);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t u[32];
+          float* x = reinterpret_cast<float*>(u);
+          tmem_ld32(s_at + c * 32, u);
+          float2 f = *reinterpret_cast<const float2*>(&note.ks[half * 4 + c * 2]);
+          const float2 lvs = *reinterpret_cast<const float2*>(&note.lvs[half * 4 + c * 2]);
+          f = make_float2(f.x * row.f, f.y * row.f);
+          tc_wait_ld();
+          if (scaled) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) f[b] *= row.f;
-        tc_wait_ld();
-        if (scaled) {
+            for (int k = 0; k < 32; k += 2) split(mul2(pair(x[k], x[k + 1]), k < 16 ? pair(f.x, f.x) : pair(f.y, f.y)), x[k], x[k + 1]);
+            if (CAP) cap32(x, cap2, inv_cap);
+            if (masked) {
+              const int left = row.len - (end - kKeys) - half * 64 - c * 32;
+              const uint32_t gone = (dead >> (c * 2) & 1u ? 0xFFFFu : 0u) | (dead >> (c * 2 + 1) & 1u ? 0xFFFF0000u : 0u);
+              const uint32_t seen = (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u) & ~gone;
 #pragma unroll
-          for (int k = 0; k < 64; k += 2) split(mul2(pair(x[k], x[k + 1]), pair(f[k / 16], f[k / 16])), x[k], x[k + 1]);
-          if (CAP) cap64(x, cap2, inv_cap);
-          if (masked) {
-            const int left = row.len - (end - kKeys) - h * 64;
+              for (int k = 0; k < 32; ++k) x[k] = seen >> k & 1u ? x[k] : -INFINITY;
+            }
+            tmem_st32(s_at + c * 32, u);
+            f = make_float2(1.0f, 1.0f);
+          }
+          const float y0 = largest16(x) * f.x, y1 = largest16(x + 16) * f.y;
+          top_x = max3(top_x, y0, y1);
+          top_w = max3(top_w, y0 + lvs.x, y1 + lvs.y);
+        }
+        if (scaled) tc_wait_st();
+        // the row's reference from the other half's thread
+        if (half == 1 ? !wait_warp(&S.moved[t][0][warp], turns & 1) : turns > 0 && !wait_warp(&S.moved[t][1][warp], (turns - 1) & 1)) return false;
+        if (half == 1 || have) R = S.reference[t][r];
+        else S.reference[t][r] = R;
+        if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag))) {
+          const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
+          R = to;
+          S.reference[t][r] = R;
+          if (half == 1 || have) {
+            // (the first half's product has to be through; that of the tile before is, since these scores came behind it)
+            if (half == 1 && !wait_warp(&S.pv_done[t][0], tiles & 1)) return false;
+            tc_fence_after();
+            rescale(o_at, by);
+            tc_wait_st();
+            tc_fence_before();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.moved[t][half][warp]);
+        ++turns;
+        if (__any_sync(0xFFFFFFFFu, top_x > m + kSumLag)) {
+          const float to = top_x > m + kSumLag ? top_x : m;
+          l *= ex2(m - to);
+          m = to;
+        }
+        const float ref = R - kLift;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t u[32], p[16];
+          const float* x = reinterpret_cast<const float*>(u);
+          tmem_ld32(s_at + c * 32, u);
+          const float2 ks = *reinterpret_cast<const float2*>(&note.ks[half * 4 + c * 2]), lv = *reinterpret_cast<const float2*>(&note.lvs[half * 4 + c * 2]);
+          tc_wait_ld();
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const int some = left - w * 32;
-              const uint32_t gone = (dead >> (h * 4 + w * 2) & 1u ? 0xFFFFu : 0u) | (dead >> (h * 4 + w * 2 + 1) & 1u ? 0xFFFF0000u : 0u);
-              const uint32_t seen = (some >= 32 ? ~0u : some <= 0 ? 0u : (1u << some) - 1u) & ~gone;
+          for (int b = 0; b < 2; ++b) {
+            const float f = scaled ? 1.0f : (b ? ks.y : ks.x) * row.f, lvs = b ? lv.y : lv.x;
+            const uint64_t f2 = pair(f, f), c2 = pair(lvs - ref, lvs - ref);
+            uint64_t sum = 0;
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[w * 32 + k] = seen >> k & 1u ? x[w * 32 + k] : -INFINITY;
+            for (int k = b * 16; k < b * 16 + 16; k += 2) {
+              float a, d;
+              split(fma2(pair(x[k], x[k + 1]), f2, c2), a, d);
+              a = ex2(a);
+              d = ex2(d);
+              sum = add2(sum, pair(a, d));
+              p[k / 2] = round2<JF_DTYPE_FP16>(a, d);
+            }
+            if (!wide) {
+              float a, d;
+              split(sum, a, d);
+              l = fmaf(a + d, ex2(fminf(ref - lvs - m, 126.0f)), l);   // (beyond, where the other half's scores are far above, the weights are zero)
+            } else {
+#pragma unroll
+              for (int k = b * 16; k < b * 16 + 16; ++k) l += ex2(x[k] - m);
             }
           }
-          tmem_st32(s_at + h * 64, u);
-          tmem_st32(s_at + h * 64 + 32, u + 32);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) f[b] = 1.0f;
+          tmem_st16(s_at + c * 16, p);
         }
-#pragma unroll
-        for (int b = 0; b < 4; b += 2) {
-          const float y0 = largest16(x + b * 16) * f[b], y1 = largest16(x + b * 16 + 16) * f[b + 1];
-          top_x = max3(top_x, y0, y1);
-          top_w = max3(top_w, y0 + lvs[b], y1 + lvs[b + 1]);
-        }
-      }
-      if (scaled) tc_wait_st();
-      if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag))) {
-        const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
-        R = to;
-        if (have) rescale(o_at, by);
-      }
-      if (__any_sync(0xFFFFFFFFu, top_x > m + kSumLag)) {
-        const float to = top_x > m + kSumLag ? top_x : m;
-        l *= ex2(m - to);
-        m = to;
-      }
-      const float ref = R - kLift;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        uint32_t u[64], p[32];
-        const float* x = reinterpret_cast<const float*>(u);
-        tmem_ld32(s_at + h * 64, u);
-        tmem_ld32(s_at + h * 64 + 32, u + 32);
-        float f[4], lvs[4];
-        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&note.ks[h * 4]);
-        *reinterpret_cast<float4*>(lvs) = *reinterpret_cast<const float4*>(&note.lvs[h * 4]);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) f[b] = scaled ? 1.0f : f[b] * row.f;
-        tc_wait_ld();
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint64_t f2 = pair(f[b], f[b]), c2 = pair(lvs[b] - ref, lvs[b] - ref);
-          uint64_t sum = 0;
-#pragma unroll
-          for (int k = b * 16; k < b * 16 + 16; k += 2) {
-            float a, d;
-            split(fma2(pair(x[k], x[k + 1]), f2, c2), a, d);
-            a = ex2(a);
-            d = ex2(d);
-            sum = add2(sum, pair(a, d));
-            p[k / 2] = round2<JF_DTYPE_FP16>(a, d);
-          }
-          if (!wide) {
-            float a, d;
-            split(sum, a, d);
-            l = fmaf(a + d, ex2(ref - lvs[b] - m), l);
-          }
-        }
-        if (wide) {
-#pragma unroll
-          for (int k = 0; k < 64; ++k) l += ex2(x[k] - m);
-        }
-        tmem_st32(s_at + h * 32, p);
         tc_wait_st();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.p_full[t][h]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.p_full[t][half]);
       have = true;
+      ++tiles;
     }
-    // the next queries, then the partial result
+    // the next queries, then the partial result: half of the channels for each of a row's threads, and each one's sum
     const int64_t piece = (static_cast<int64_t>(blockIdx.x) + s.item) * 2 + t;
-    const bool any = s.n > 0;
+    const bool any = s.n > 0, idle = row.idle;
     base += s.n;
-    const float ref = R - kLift;
-    const bool idle = row.idle;
     more = next_segment(P, s);
     if (more) row = load_query(s);
-    if (have) {
-      if (!wait_warp(&S.o_full[t], o_count++ & 1)) return false;
+    if (have && !idle) {
+      if (half == 0 && !wait_warp(&S.moved[t][1][warp], (turns - 1) & 1)) return false;
+      R = S.reference[t][r];
+      if (!wait_warp(&S.pv_done[t][1], (tiles - 1) & 1)) return false;
       tc_fence_after();
-      float* out = P.part_o + (piece * kRows + r) * JF_HEAD_DIM;
+      float* out = P.part_o + (piece * kRows + r) * JF_HEAD_DIM + half * 64;
 #pragma unroll 1
-      for (int c = idle ? 4 : 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t o[32];
-        tmem_ld32(o_at + c * 32, o);
+        tmem_ld32(o_at + half * 64 + c * 32, o);
         tc_wait_ld();
 #pragma unroll
         for (int k = 0; k < 32; k += 8)
@@ -540,7 +541,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
       }
       tc_fence_before();
     }
-    if (any) P.part_ml[piece * kRows + r] = make_float4(ref, m, l, 0.0f);
+    if (any) P.part_ml[(piece * kRows + r) * 2 + half] = make_float4(R - kLift, m, l, 0.0f);
     __syncwarp();
   }
   return true;
@@ -549,21 +550,27 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
 template <int DT, int CODES, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid_constant__ SharedParams P) {
   extern __shared__ unsigned char raw[];
-  __shared__ Shared S;
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // (known to be the same for all lanes)
-  unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  unsigned char *kv = smem + 2 * kTileBytes, *staged = kv + 4 * kTileBytes;
+  const uint32_t up = (1024u - (smem_u32(raw) & 1023u)) & 1023u;
+  if (up > kSmemBytes - kUsedBytes) {   // (nothing static is in front of it: it starts on a multiple of 1024)
+    if (threadIdx.x == 0) report_status(P.status, JF_ERR_STATE);
+    return;
+  }
+  unsigned char *smem = raw + up, *kv = smem + 2 * kTileBytes, *staged = kv + 4 * kTileBytes;
+  Shared& S = *reinterpret_cast<Shared*>(staged + kStaged * kCodeBytes);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&S.q_full[i], 4);
+      mbar_init(&S.q_full[i], 8);
       mbar_init(&S.k_full[i], 4);
       mbar_init(&S.v_full[i], 4);
       mbar_init(&S.k_empty[i], 1);
       mbar_init(&S.v_empty[i], 1);
       mbar_init(&S.s_full[i], 1);
+      for (int k = 0; k < 8; ++k) mbar_init(&S.moved[i][k >> 2][k & 3], 1);
       mbar_init(&S.p_full[i][0], 4);
       mbar_init(&S.p_full[i][1], 4);
-      mbar_init(&S.o_full[i], 1);
+      mbar_init(&S.pv_done[i][0], 1);
+      mbar_init(&S.pv_done[i][1], 1);
     }
     for (int i = 0; i < kStaged; ++i) {
       mbar_init(&S.code_full[i], 1);
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
     S.end = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * P.units / gridDim.x);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 20) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -587,16 +594,16 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   pdl_trigger();
   // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
   bool ok = true;
-  if (warp < 8) {
-    ok = soften<DT, CAP>(P, S, smem + (warp >> 2) * kTileBytes, tmem, warp >> 2);
-  } else if (warp < 12) {
+  if (warp < 16) {
+    ok = soften<DT, CAP>(P, S, smem + (warp >> 3) * kTileBytes, tmem, warp >> 3, warp >> 2 & 1);
+  } else if (warp < 20) {
     ok = convert<CODES>(P, S, kv, staged);
-  } else if (warp == 12) {
+  } else if (warp == 20) {
     ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
     if (elect_one()) tc_commit(&S.products_done);
     __syncwarp();
     ok &= wait_warp(&S.products_done, 0);
-  } else if (warp == 13) {
+  } else if (warp == 21) {
     int sent = 0;
     ok = load(P, S, staged, sent);
     ok &= arrived(S, sent);
@@ -605,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
@@ -644,7 +651,7 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) 
   if (p.own == 0) return false;
   const uint64_t part_rows = static_cast<uint64_t>(p.grid + p.items) * 2 * kRows;
   p.o_bytes = part_rows * JF_HEAD_DIM * sizeof(float);
-  p.bytes = p.own + p.o_bytes + part_rows * sizeof(float4);
+  p.bytes = p.own + p.o_bytes + part_rows * 2 * sizeof(float4);
   return true;
 }
 

@@ -61,13 +61,27 @@ template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setm
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Bounded.  Most waits end within a few attempts; the clock that bounds the others is read only after that (a read of it
-// in front of every wait that did not end at once took 0.4 us of each step).
+// Bounded.  An attempt lasts 120 cycles or so; the loop is four instructions, since warps that wait take issue slots from those that compute (the
+// loop as the compiler makes it was 20, and half of what a kernel with many roles issued).  Most waits end within a few attempts; the
+// clock that bounds the others is read only after that (a read of it in front of every wait that did not end at once took
+// 0.4 us of each step).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-#pragma unroll 1
-  for (int i = 0; i < 1000; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, kTensorWaitNs);
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 0;\n"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 q, n, 1000;\n\t"
+      "@q bra AGAIN;\n"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0 || mbar_wait(bar, parity, kTensorWaitNs);
 }
 // by a whole warp, which goes on or gives up together
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)); }
@@ -78,9 +92,9 @@ __device__ __forceinline__ uint64_t operand(uint32_t smem, uint32_t lead_bytes) 
   return static_cast<uint64_t>(smem >> 4 & 0x3FFFu) | static_cast<uint64_t>(lead_bytes >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
          1ull << 46 | 2ull << 61;
 }
-template <int DT> __device__ constexpr uint32_t instruction(bool b_mn_major) {
+template <int DT> __device__ constexpr uint32_t instruction(bool b_mn_major, uint32_t columns = 128u) {
   constexpr uint32_t type = DT == JF_DTYPE_BF16 ? 1u : 0u;
-  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
+  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | (columns >> 3) << 17 | (128u >> 4) << 24;
 }
 
 // ---- arithmetic on pairs ----------------------------------------------------------------------
