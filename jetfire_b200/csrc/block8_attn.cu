@@ -788,9 +788,9 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
       top_o = fmaxf(top_o, x);
       top_l = fmaxf(top_l, x);
     } else {
-      const float4* x = from.part_ml + result(i - n) * 2;   // (the sum in two halves)
-      top_o = fmaxf(top_o, x[0].x);
-      top_l = fmaxf(top_l, fmaxf(x[0].y, x[1].y));
+      const float4 x = from.part_ml[result(i - n)];
+      top_o = fmaxf(top_o, x.x);
+      top_l = fmaxf(top_l, x.y);
     }
   }
 #pragma unroll
@@ -812,11 +812,11 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
       if (x.y != 0.0f) at = own0 + i * step;
     } else if (i < n + m) {
       const int64_t where = result(i - n);
-      const float4 x0 = from.part_ml[where * 2], x1 = from.part_ml[where * 2 + 1];
-      const float f0 = half_step(top_l - x0.y), f1 = half_step(top_l - x1.y), e = half_step(top_o - x0.x);
-      z = fmaf(x0.z * f0, f0, fmaf(x1.z * f1, f1, z));
+      const float4 x = from.part_ml[where];
+      const float f = half_step(top_l - x.y), e = half_step(top_o - x.x);
+      z = fmaf(x.z * f, f, z);
       w = e * e;
-      if (x0.z != 0.0f || x1.z != 0.0f) at = where;     // (a group without tiles left no output)
+      if (x.z != 0.0f) at = where;     // (a group without tiles left no output)
     }
     const int some = min(32, n + m - i0);
     for (int k = 0; k < some; ++k) {

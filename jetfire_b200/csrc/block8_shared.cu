@@ -12,15 +12,12 @@
 // same exponentials, times exp2(R - log2 vs - m): one more of them for 16 positions.  Where V scales lie so far apart (beyond
 // 2^kSpread) that a weight could vanish while its position counts, those tiles take an exponential more for every position.
 //
-//   warps 0-15       scores -> weights: 8 for a row tile, 4 (a thread a row) for each half of a tile's 128 positions; the rescaling of O;
-//                    the partial result
-//   warps 16-19      codes -> fp16 operands: 128 positions of K, then of V, two buffers each
-//   warp 20          issues the matrix products
-//   warp 21          looks blocks up and copies their codes into shared memory, 2048 bytes at a time
-// The product of a tile's weights with V comes in two halves, the first before the second, and a row's reference may move between any two of
-// them: the two threads of a row hand it to one another, the first half's after its maximum to the second's, that to the first half's of the next
-// tile.  (A thread for all 128 positions left the special function units idle for more than half of the time: 727 us for 256 sequences over 65536
-// positions.  Code unrolled for 128 scores was twice what the instruction caches take: 966.)
+//   warps 0-3, 4-7   scores -> weights of row tile 0, 1 (a thread a row); the rescaling of O; the partial result
+//   warps 8, 9       codes -> fp16 operands: 128 positions of K, then of V, two buffers each
+//   warp 10          issues the matrix products
+//   warp 11          looks blocks up and copies their codes into shared memory, 2048 bytes at a time
+// What is not on the common path is kept small (the code that all of these go through has to fit the instruction caches: at 123 KB a unit took
+// 8300 cycles on the GPCs that have all their multiprocessors at work, 5000 on the others).
 //
 // Work is a line of units -- (KV head, pair of row tiles, 128 positions) -- cut into pieces of one length, one for each thread block, so that all
 // multiprocessors end together; where a piece passes from one pair of row tiles to the next it leaves two partial results.  A single row
@@ -43,7 +40,9 @@ constexpr int kTileBlocks = kKeys / JF_BLOCK_SIZE;
 constexpr int kCodeBytes = kKeys * JF_HEAD_DIM;        // of a tile as it lies in the cache
 constexpr int kStaged = 2;                             // K or V tiles on their way from memory
 constexpr int kNotes = 8;
-constexpr int kThreads = 768;
+constexpr int kThreads = 384;
+// Registers a thread: the rows' warpgroups, the other one; together no more than the block is launched with (launch() checks that).
+constexpr int kRowRegs = 208, kRoleRegs = 80;
 constexpr float kLag = 8.0f, kLift = 7.0f;             // log2; weights stay below 2^15
 constexpr float kSumLag = 24.0f, kSpread = 64.0f;
 constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
@@ -57,13 +56,33 @@ struct SharedParams {
   const void* table;
   const int32_t* seq_lens;
   float* part_o;          // [piece, row tile of the pair][128][128]
-  float4* part_ml;        // [..][128][half]: R - lift (of the first half), m, sum
+  float4* part_ml;        // R - lift, m, sum
   int32_t* status;
   int64_t num_blocks;
   int32_t units, H_q, G, rows, row_tiles, pairs, tiles, blocks, max_S;   // rows: of a KV head; blocks: shared ones; tiles: of positions
   float scale, softcap;
   bool i32;
 };
+
+// Bounded: 2^24 attempts, a second or so.  (No wait here is for more than the work on a few tiles.)
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 0;\n"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 q, n, 16777216;\n\t"
+      "@q bra AGAIN;\n"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xFFFFFFFFu, done != 0);
+}
 
 // What a tile's rows need to know of it: its blocks' K scales, log2 of their V scales.
 struct alignas(16) Note {
@@ -74,9 +93,8 @@ struct alignas(16) Note {
 };
 struct Shared {
   uint64_t code_full[kStaged], code_empty[kStaged], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2],
-      pv_done[2][2], moved[2][2][4], note_full[kNotes], products_done;
+      o_full[2], note_full[kNotes], products_done;
   Note note[kNotes];
-  float reference[2][kRows];
   uint32_t tmem;
   int begin, end;         // units of this thread block
 };
@@ -145,7 +163,7 @@ __device__ __forceinline__ bool load(const SharedParams& P, Shared& S, unsigned 
       now = then;
       then = look_up(u + 4);
     }
-    if (n >= kStaged && !wait_warp(&S.code_empty[slot], static_cast<uint32_t>(n / kStaged - 1) & 1u)) return false;
+    if (n >= kStaged && !await(&S.code_empty[slot], static_cast<uint32_t>(n / kStaged - 1) & 1u)) return false;
     const int id = __shfl_sync(0xFFFFFFFFu, now.id, (off + lane) & 31);
     const bool mine = lane < kTileBlocks, is = mine && id >= 0;
     const unsigned there = __ballot_sync(0xFFFFFFFFu, is);
@@ -189,45 +207,48 @@ __device__ __forceinline__ bool load(const SharedParams& P, Shared& S, unsigned 
 // The copies that may be in flight: the block's shared memory stays until they are there, or a wait for one runs out.
 __device__ __forceinline__ bool arrived(Shared& S, int sent) {
   for (int n = max(sent - kStaged, 0); n < sent; ++n)
-    if (!wait_warp(&S.code_full[n % kStaged], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
+    if (!await(&S.code_full[n % kStaged], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
   return true;
 }
 
 template <int CODES> __device__ __forceinline__ bool convert(const SharedParams& P, Shared& S, unsigned char* kv, const unsigned char* staged) {
-  const int lane = threadIdx.x & 31, tid = threadIdx.x & 127;
+  const int lane = threadIdx.x & 31, tid = threadIdx.x & 63;
   const Segment range = units_of(S);
   const int sides = 2 * (range.end - range.u);
-  // A thread has the same 16 channels of one row of every block: two chunks of 16 bytes of the operand's row.  Eight threads that read or write
-  // together have half of a row and the other half of the next one, which the swizzle puts on all banks.
+  // A thread has the same 16 channels of rows r and r + 8 of every block: two chunks of 16 bytes of the operand's row.  Eight threads that read or
+  // write together have half of a row and the other half of the next one, which the swizzle puts on all banks.
   const int row = tid >> 4 << 1 | (tid >> 2 & 1), cc = ((tid >> 2 ^ tid >> 3) & 1) << 2 | (tid & 3), j0 = (cc & 3) * 2, sw = row & 7;
   const uint32_t base = (cc >> 2) * kSlabBytes + row * 128;
   const uint32_t lo_at = base + ((j0 ^ sw) << 4), hi_at = base + (((j0 + 1) ^ sw) << 4);
 #pragma unroll 1
   for (int n = 0; n < sides; ++n) {
     const int g = n >> 1, side = n & 1, slot = g & 1, stage = n % kStaged;
-    if (!wait_warp(&S.code_full[stage], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
-    const unsigned char* from = staged + stage * kCodeBytes + row * JF_HEAD_DIM + cc * 16;
-    uint4 x[kTileBlocks];
-#pragma unroll
-    for (int i = 0; i < kTileBlocks; ++i) x[i] = *reinterpret_cast<const uint4*>(from + i * 2048);
+    if (!await(&S.code_full[stage], static_cast<uint32_t>(n / kStaged) & 1u)) return false;
+    if (g >= 2 && !await(side ? &S.v_empty[slot] : &S.k_empty[slot], static_cast<uint32_t>((g >> 1) - 1) & 1u)) return false;
     const uint32_t dead = S.note[g % kNotes].dead;
-    if (dead) {
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* from = staged + stage * kCodeBytes + h * (kCodeBytes / 2) + row * JF_HEAD_DIM + cc * 16;
+      unsigned char* to = kv + (side * 2 + slot) * kTileBytes + h * (kSlabBytes / 2);
+      uint4 x[kTileBlocks];
 #pragma unroll
-      for (int i = 0; i < kTileBlocks; ++i)
-        if (dead >> i & 1u) x[i] = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kTileBlocks; ++i) x[i] = *reinterpret_cast<const uint4*>(from + i * 1024);
+      if (dead) {
+#pragma unroll
+        for (int i = 0; i < kTileBlocks; ++i)
+          if (dead >> (h * 4 + i / 2) & 1u) x[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kTileBlocks; ++i) {
+        const uint32_t w[4] = {flip<CODES>(x[i].x), flip<CODES>(x[i].y), flip<CODES>(x[i].z), flip<CODES>(x[i].w)};
+        *reinterpret_cast<uint4*>(to + i * 1024 + lo_at) =
+            make_uint4(widen<CODES, false>(w[0]), widen<CODES, true>(w[0]), widen<CODES, false>(w[1]), widen<CODES, true>(w[1]));
+        *reinterpret_cast<uint4*>(to + i * 1024 + hi_at) =
+            make_uint4(widen<CODES, false>(w[2]), widen<CODES, true>(w[2]), widen<CODES, false>(w[3]), widen<CODES, true>(w[3]));
+      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&S.code_empty[stage]);
-    if (g >= 2 && !wait_warp(side ? &S.v_empty[slot] : &S.k_empty[slot], static_cast<uint32_t>((g >> 1) - 1) & 1u)) return false;
-    unsigned char* to = kv + (side * 2 + slot) * kTileBytes;
-#pragma unroll
-    for (int i = 0; i < kTileBlocks; ++i) {
-      const uint32_t w[4] = {flip<CODES>(x[i].x), flip<CODES>(x[i].y), flip<CODES>(x[i].z), flip<CODES>(x[i].w)};
-      *reinterpret_cast<uint4*>(to + i * 2048 + lo_at) =
-          make_uint4(widen<CODES, false>(w[0]), widen<CODES, true>(w[0]), widen<CODES, false>(w[1]), widen<CODES, true>(w[1]));
-      *reinterpret_cast<uint4*>(to + i * 2048 + hi_at) =
-          make_uint4(widen<CODES, false>(w[2]), widen<CODES, true>(w[2]), widen<CODES, false>(w[3]), widen<CODES, true>(w[3]));
-    }
     fence_proxy_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(side ? &S.v_full[slot] : &S.k_full[slot]);
@@ -246,13 +267,13 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
   while (next_segment(P, s)) {
     const bool two = two_tiles(P, s);
     const int jobs = two ? 2 * s.n : s.n;
-    if (!wait_warp(&S.q_full[0], q_count0++ & 1)) return false;
-    if (jobs > 1 && !wait_warp(&S.q_full[1], q_count1++ & 1)) return false;
+    if (!await(&S.q_full[0], q_count0++ & 1)) return false;
+    if (jobs > 1 && !await(&S.q_full[1], q_count1++ & 1)) return false;
     // (the group as a constant: arrays and addresses that depend on it stay out of memory)
     auto scores = [&](auto t_tag, int j) {
       constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
-      if ((!two || t == 0) && !wait_warp(&S.k_full[slot], g >> 1 & 1)) return false;
+      if ((!two || t == 0) && !await(&S.k_full[slot], g >> 1 & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = q_op + t * (kTileBytes >> 4), b = k_op + slot * (kTileBytes >> 4);
@@ -270,18 +291,18 @@ __device__ __forceinline__ bool multiply(const SharedParams& P, Shared& S, uint3
     auto job = [&](auto t_tag, int j, uint32_t parity) {
       constexpr int t = decltype(t_tag)::value;
       const uint32_t g = base + (two ? j >> 1 : j), slot = g & 1;
-      if ((!two || t == 0) && !wait_warp(&S.v_full[slot], g >> 1 & 1)) return false;
+      if ((!two || t == 0) && !await(&S.v_full[slot], g >> 1 & 1)) return false;
       const uint64_t b = v_op + slot * (kTileBytes >> 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // the weights come in two halves
-        if (!wait_warp(&S.p_full[t][h], parity)) return false;
+        if (!await(&S.p_full[t][h], parity)) return false;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int k = h * 4; k < h * 4 + 4; ++k)
-            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + h * 64 + (k & 3) * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
-          tc_commit(&S.pv_done[t][h]);
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, b + k * (2048 >> 4), pv, j >= 2 || k > 0);
           if (h == 1 && (!two || t == 1)) tc_commit(&S.v_empty[slot]);
+          if (h == 1 && j + 2 >= jobs) tc_commit(&S.o_full[t]);
         }
         __syncwarp();
       }
@@ -334,10 +355,10 @@ __device__ __forceinline__ void cap32(float* x, float cap2, float inv) {
   }
 }
 
-template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedParams& P, Shared& S, unsigned char* q_smem, uint32_t tmem, int t, int half) {
+template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedParams& P, Shared& S, unsigned char* q_smem, uint32_t tmem, int t) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3, r = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-  const uint32_t s_at = tmem + lanes + t * 128 + half * 64, o_at = tmem + lanes + 256 + t * 128;   // of this half; of the row
+  const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
   const float cap2 = CAP ? P.softcap * kLog2e : 0.0f, inv_cap = CAP ? 1.0f / cap2 : 0.0f;
   // The row's query as fp16 into the operand's place; what brings its products to scores in units of log2, and the positions that it sees.
   // (more than there are: all of them)
@@ -382,7 +403,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
     to.f = __uint_as_float(static_cast<uint32_t>(e - TOP + 127) << 23) * fabsf(P.scale) * kLog2e + odd;
     unsigned char* out = q_smem + r * 128;
 #pragma unroll 1
-    for (int i = half * 8; i < half * 8 + 8; i += 4) {   // (half of the row for each of its two threads)
+    for (int i = 0; i < 16; i += 4) {
       read(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -403,7 +424,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
   };
 
   Segment s = units_of(S);
-  uint32_t base = 0, tiles = 0, turns = 0;   // tiles of positions so far: of the block, of this group, of those with rows of this warp
+  uint32_t base = 0, tiles = 0, ends = 0;   // tiles of positions so far: of the block, of this group; segments with some
   Row row{0.0f, 0, true};
   for (bool more = true; more;) {   // (the first time round there is nothing but queries to be loaded)
     const bool two = two_tiles(P, s);
@@ -414,126 +435,129 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
       const uint32_t g = base + i;
       const Note& note = S.note[g % kNotes];
       const int end = (s.first + i + 1) * kKeys;
-      if (!wait_warp(&S.note_full[g % kNotes], g / kNotes & 1)) return false;
+      if (!await(&S.note_full[g % kNotes], g / kNotes & 1)) return false;
       lvs_top = fmaxf(lvs_top, note.lvs_hi);
-      const uint32_t dead = note.dead >> half * 4 & 15u;
+      const uint32_t dead = note.dead;
       const bool wide = lvs_top - note.lvs_lo > kSpread;
       const bool masked = __any_sync(0xFFFFFFFFu, row.len < end) || dead != 0;
-      const bool scaled = CAP || masked || wide || note.odd != 0;   // scores are brought to units of log2 one by one, and written back
-      if (!wait_warp(&S.s_full[t], tiles & 1)) return false;
+      const bool scaled = CAP || masked || wide || note.odd != 0;
+      if (!await(&S.s_full[t], tiles++ & 1)) return false;
       tc_fence_after();
-      if (!row.idle) {   // (whatever the weights of rows that are none are)
-        float top_x = -INFINITY, top_w = -INFINITY;
+      if (row.idle) {   // (whatever the weights of rows that are none are)
+        __syncwarp();
+        if (lane < 2) mbar_arrive(&S.p_full[t][lane]);
+        have = true;
+        continue;
+      }
+      if (scaled) {   // scores are brought to units of log2 one by one, and written back
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t u[32];
           float* x = reinterpret_cast<float*>(u);
           tmem_ld32(s_at + c * 32, u);
-          float2 f = *reinterpret_cast<const float2*>(&note.ks[half * 4 + c * 2]);
-          const float2 lvs = *reinterpret_cast<const float2*>(&note.lvs[half * 4 + c * 2]);
-          f = make_float2(f.x * row.f, f.y * row.f);
-          tc_wait_ld();
-          if (scaled) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) split(mul2(pair(x[k], x[k + 1]), k < 16 ? pair(f.x, f.x) : pair(f.y, f.y)), x[k], x[k + 1]);
-            if (CAP) cap32(x, cap2, inv_cap);
-            if (masked) {
-              const int left = row.len - (end - kKeys) - half * 64 - c * 32;
-              const uint32_t gone = (dead >> (c * 2) & 1u ? 0xFFFFu : 0u) | (dead >> (c * 2 + 1) & 1u ? 0xFFFF0000u : 0u);
-              const uint32_t seen = (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u) & ~gone;
-#pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = seen >> k & 1u ? x[k] : -INFINITY;
-            }
-            tmem_st32(s_at + c * 32, u);
-            f = make_float2(1.0f, 1.0f);
-          }
-          const float y0 = largest16(x) * f.x, y1 = largest16(x + 16) * f.y;
-          top_x = max3(top_x, y0, y1);
-          top_w = max3(top_w, y0 + lvs.x, y1 + lvs.y);
-        }
-        if (scaled) tc_wait_st();
-        // the row's reference from the other half's thread
-        if (half == 1 ? !wait_warp(&S.moved[t][0][warp], turns & 1) : turns > 0 && !wait_warp(&S.moved[t][1][warp], (turns - 1) & 1)) return false;
-        if (half == 1 || have) R = S.reference[t][r];
-        else S.reference[t][r] = R;
-        if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag))) {
-          const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
-          R = to;
-          S.reference[t][r] = R;
-          if (half == 1 || have) {
-            // (the first half's product has to be through; that of the tile before is, since these scores came behind it)
-            if (half == 1 && !wait_warp(&S.pv_done[t][0], tiles & 1)) return false;
-            tc_fence_after();
-            rescale(o_at, by);
-            tc_wait_st();
-            tc_fence_before();
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.moved[t][half][warp]);
-        ++turns;
-        if (__any_sync(0xFFFFFFFFu, top_x > m + kSumLag)) {
-          const float to = top_x > m + kSumLag ? top_x : m;
-          l *= ex2(m - to);
-          m = to;
-        }
-        const float ref = R - kLift;
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          uint32_t u[32], p[16];
-          const float* x = reinterpret_cast<const float*>(u);
-          tmem_ld32(s_at + c * 32, u);
-          const float2 ks = *reinterpret_cast<const float2*>(&note.ks[half * 4 + c * 2]), lv = *reinterpret_cast<const float2*>(&note.lvs[half * 4 + c * 2]);
+          const float2 ks = *reinterpret_cast<const float2*>(&note.ks[c * 2]);
+          const float f0 = ks.x * row.f, f1 = ks.y * row.f;
           tc_wait_ld();
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float f = scaled ? 1.0f : (b ? ks.y : ks.x) * row.f, lvs = b ? lv.y : lv.x;
-            const uint64_t f2 = pair(f, f), c2 = pair(lvs - ref, lvs - ref);
-            uint64_t sum = 0;
+          for (int k = 0; k < 32; k += 2) split(mul2(pair(x[k], x[k + 1]), k < 16 ? pair(f0, f0) : pair(f1, f1)), x[k], x[k + 1]);
+          if (CAP) cap32(x, cap2, inv_cap);
+          if (masked) {
+            const int left = row.len - (end - kKeys) - c * 32;
+            const uint32_t gone = (dead >> (c * 2) & 1u ? 0xFFFFu : 0u) | (dead >> (c * 2 + 1) & 1u ? 0xFFFF0000u : 0u);
+            const uint32_t seen = (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u) & ~gone;
 #pragma unroll
-            for (int k = b * 16; k < b * 16 + 16; k += 2) {
-              float a, d;
-              split(fma2(pair(x[k], x[k + 1]), f2, c2), a, d);
-              a = ex2(a);
-              d = ex2(d);
-              sum = add2(sum, pair(a, d));
-              p[k / 2] = round2<JF_DTYPE_FP16>(a, d);
-            }
-            if (!wide) {
-              float a, d;
-              split(sum, a, d);
-              l = fmaf(a + d, ex2(fminf(ref - lvs - m, 126.0f)), l);   // (beyond, where the other half's scores are far above, the weights are zero)
-            } else {
-#pragma unroll
-              for (int k = b * 16; k < b * 16 + 16; ++k) l += ex2(x[k] - m);
-            }
+            for (int k = 0; k < 32; ++k) x[k] = seen >> k & 1u ? x[k] : -INFINITY;
           }
-          tmem_st16(s_at + c * 16, p);
+          tmem_st32(s_at + c * 32, u);
         }
         tc_wait_st();
-        tc_fence_before();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.p_full[t][half]);
+      uint32_t u[128];
+      float* x = reinterpret_cast<float*>(u);
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld32(s_at + c, u + c);
+      float f[kTileBlocks], lvs[kTileBlocks];
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; b += 4) {
+        *reinterpret_cast<float4*>(f + b) = *reinterpret_cast<const float4*>(&note.ks[b]);
+        *reinterpret_cast<float4*>(lvs + b) = *reinterpret_cast<const float4*>(&note.lvs[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; ++b) f[b] = scaled ? 1.0f : f[b] * row.f;
+      tc_wait_ld();
+      float top_x = -INFINITY, top_w = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; b += 2) {
+        const float y0 = largest16(x + b * 16) * f[b], y1 = largest16(x + b * 16 + 16) * f[b + 1];
+        top_x = max3(top_x, y0, y1);
+        top_w = max3(top_w, y0 + lvs[b], y1 + lvs[b + 1]);
+      }
+      if (__any_sync(0xFFFFFFFFu, !(top_w <= R + kLag) || top_x > m + kSumLag)) {
+        const float to = !(top_w <= R + kLag) ? fmaxf(R, top_w) : R, by = ex2(R - to);   // (what other rows do does not move a row)
+        R = to;
+        if (have && __any_sync(0xFFFFFFFFu, by != 1.0f)) rescale(o_at, by);
+        const float sum_to = top_x > m + kSumLag ? top_x : m;
+        l *= ex2(m - sum_to);
+        m = sum_to;
+      }
+      const float ref = R - kLift;
+      if (wide) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(s_at + c * 32, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) l += ex2(__uint_as_float(v[k]) - m);
+        }
+      }
+      float sums[kTileBlocks];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int b = h * 4; b < h * 4 + 4; ++b) {
+          const uint64_t f2 = pair(f[b], f[b]), c2 = pair(lvs[b] - ref, lvs[b] - ref);
+          uint64_t sum = 0;
+#pragma unroll
+          for (int k = b * 16; k < b * 16 + 16; k += 2) {
+            float a, d;
+            split(fma2(pair(x[k], x[k + 1]), f2, c2), a, d);
+            a = ex2(a);
+            d = ex2(d);
+            sum = add2(sum, pair(a, d));
+            p[(k - h * 64) / 2] = round2<JF_DTYPE_FP16>(a, d);
+          }
+          float a, d;
+          split(sum, a, d);
+          sums[b] = a + d;
+        }
+        tmem_st32(s_at + h * 32, p);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[t][h]);
+      }
+      if (!wide) {
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) l = fmaf(sums[b], ex2(ref - lvs[b] - m), l);
+      }
       have = true;
-      ++tiles;
     }
-    // the next queries, then the partial result: half of the channels for each of a row's threads, and each one's sum
+    // the next queries, then the partial result
     const int64_t piece = (static_cast<int64_t>(blockIdx.x) + s.item) * 2 + t;
     const bool any = s.n > 0, idle = row.idle;
     base += s.n;
     more = next_segment(P, s);
     if (more) row = load_query(s);
-    if (have && !idle) {
-      if (half == 0 && !wait_warp(&S.moved[t][1][warp], (turns - 1) & 1)) return false;
-      R = S.reference[t][r];
-      if (!wait_warp(&S.pv_done[t][1], (tiles - 1) & 1)) return false;
+    if (have) {
+      if (!await(&S.o_full[t], ends++ & 1)) return false;
       tc_fence_after();
-      float* out = P.part_o + (piece * kRows + r) * JF_HEAD_DIM + half * 64;
+      float* out = P.part_o + (piece * kRows + r) * JF_HEAD_DIM;
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
+      for (int c = idle ? 4 : 0; c < 4; ++c) {
         uint32_t o[32];
-        tmem_ld32(o_at + half * 64 + c * 32, o);
+        tmem_ld32(o_at + c * 32, o);
         tc_wait_ld();
 #pragma unroll
         for (int k = 0; k < 32; k += 8)
@@ -541,7 +565,7 @@ template <int DT, bool CAP> __device__ __forceinline__ bool soften(const SharedP
       }
       tc_fence_before();
     }
-    if (any) P.part_ml[(piece * kRows + r) * 2 + half] = make_float4(R - kLift, m, l, 0.0f);
+    if (any) P.part_ml[piece * kRows + r] = make_float4(R - kLift, m, l, 0.0f);
     __syncwarp();
   }
   return true;
@@ -560,21 +584,19 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   Shared& S = *reinterpret_cast<Shared*>(staged + kStaged * kCodeBytes);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&S.q_full[i], 8);
-      mbar_init(&S.k_full[i], 4);
-      mbar_init(&S.v_full[i], 4);
+      mbar_init(&S.q_full[i], 4);
+      mbar_init(&S.k_full[i], 2);
+      mbar_init(&S.v_full[i], 2);
       mbar_init(&S.k_empty[i], 1);
       mbar_init(&S.v_empty[i], 1);
       mbar_init(&S.s_full[i], 1);
-      for (int k = 0; k < 8; ++k) mbar_init(&S.moved[i][k >> 2][k & 3], 1);
       mbar_init(&S.p_full[i][0], 4);
       mbar_init(&S.p_full[i][1], 4);
-      mbar_init(&S.pv_done[i][0], 1);
-      mbar_init(&S.pv_done[i][1], 1);
+      mbar_init(&S.o_full[i], 1);
     }
     for (int i = 0; i < kStaged; ++i) {
       mbar_init(&S.code_full[i], 1);
-      mbar_init(&S.code_empty[i], 4);
+      mbar_init(&S.code_empty[i], 2);
     }
     for (int i = 0; i < kNotes; ++i) mbar_init(&S.note_full[i], 1);
     mbar_init(&S.products_done, 1);
@@ -582,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
     S.end = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * P.units / gridDim.x);
     fence_barrier_init();
   }
-  if (warp == 20) {
+  if (warp == 10) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -594,25 +616,29 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   pdl_trigger();
   // every role ends by itself, a wait that ran out included; the error is recorded by whoever meets it
   bool ok = true;
-  if (warp < 16) {
-    ok = soften<DT, CAP>(P, S, smem + (warp >> 3) * kTileBytes, tmem, warp >> 3, warp >> 2 & 1);
-  } else if (warp < 20) {
-    ok = convert<CODES>(P, S, kv, staged);
-  } else if (warp == 20) {
-    ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
-    if (elect_one()) tc_commit(&S.products_done);
-    __syncwarp();
-    ok &= wait_warp(&S.products_done, 0);
-  } else if (warp == 21) {
-    int sent = 0;
-    ok = load(P, S, staged, sent);
-    ok &= arrived(S, sent);
+  if (warp < 8) {
+    regs_inc<kRowRegs>();
+    ok = soften<DT, CAP>(P, S, smem + (warp >> 2) * kTileBytes, tmem, warp >> 2);
+  } else {
+    regs_dec<kRoleRegs>();
+    if (warp < 10) {
+      ok = convert<CODES>(P, S, kv, staged);
+    } else if (warp == 10) {
+      ok = multiply(P, S, smem_u32(smem), smem_u32(kv), tmem);
+      if (elect_one()) tc_commit(&S.products_done);
+      __syncwarp();
+      ok &= await(&S.products_done, 0);
+    } else {
+      int sent = 0;
+      ok = load(P, S, staged, sent);
+      ok &= arrived(S, sent);
+    }
   }
   if (!ok) report_status(P.status, JF_ERR_TIMEOUT);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 20) {
+  if (warp == 10) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
@@ -651,12 +677,18 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) 
   if (p.own == 0) return false;
   const uint64_t part_rows = static_cast<uint64_t>(p.grid + p.items) * 2 * kRows;
   p.o_bytes = part_rows * JF_HEAD_DIM * sizeof(float);
-  p.bytes = p.own + p.o_bytes + part_rows * 2 * sizeof(float4);
+  p.bytes = p.own + p.o_bytes + part_rows * sizeof(float4);
   return true;
 }
 
 template <int DT, int CODES, bool CAP> jf_status_t launch(const SharedParams& P, int grid, cudaStream_t s) {
   auto* kernel = block8_shared_kernel<DT, CODES, CAP>;
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, block8_shared_kernel<DT, CODES, CAP>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  // (a warpgroup that asks for more than the block has waits for good)
+  if (regs * kThreads < 128 * (2 * kRowRegs + kRoleRegs)) return JF_ERR_UNSUPPORTED;
   JF_ENSURE_SMEM(kernel, kSmemBytes);
   JF_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmemBytes, s, P));
   return JF_OK;
