@@ -213,7 +213,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y / P.groups, grp = blockIdx.y % P.groups;
   const int first_head = kvh * P.G + grp * 8 * NT, heads = min(8 * NT, P.G - grp * 8 * NT);
-  pdl_wait();
+  // (Behind block8_shared.cu's kernel, which has waited for what is in front of it before it lets this one start, and whose results are not
+  // read here: the wait comes at the end, so that blocks may start where that kernel's have left.)
+  if (!P.partial) pdl_wait();
   pdl_trigger();
   Cut cut{0, static_cast<int>(blockIdx.x) / P.cluster, static_cast<int>(blockIdx.x) % P.cluster, P.cluster, 0, 0};
   if (CLUSTER) {
@@ -221,7 +223,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     cut.prefix = prefix_of(P, cut.b);
   } else {
     cut = find_piece(P, blockIdx.x);
-    if (cut.b < 0) return;
+    if (cut.b < 0) {
+      if (P.partial) pdl_wait();
+      return;
+    }
   }
   const int b = cut.b;
   const Span span = span_of(P, cut.length, cut.prefix);
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     }
     if (cut.n == 1 && !P.partial) {
       write(head, d, sum, sm_ml[head]);
-    } else if (CLUSTER) {
+    } else if (CLUSTER && !P.partial) {
       *reinterpret_cast<float4*>(so + head * JF_HEAD_DIM + d) = sum;   // (no other thread reads these four)
     } else {
       const int64_t row = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (8 * NT) + head;
@@ -670,6 +675,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) block8_attn_kern
     }
     cluster_sync();   // nobody leaves while its shared memory is read
   }
+  if (P.partial) pdl_wait();
 }
 
 // The pieces of a sequence.  A block of WARPS warps per (head, sequence) and 32 * VEC channels; a warp takes every WARPS-th piece.
@@ -758,15 +764,18 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
   pdl_wait();
   pdl_trigger();
   if (b >= P.B) return;
-  int total = 0, first = 0, n = 0;
-  for (int i = lane; i < P.B; i += 32) total += blocks_of(P, i);
-  const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total), total);
-  for (int i = lane; i <= b; i += 32) {
-    const int k = max(1, (blocks_of(P, i) + piece - 1) / piece);
-    if (i < b) first += k; else n = k;
+  int total = 0, first = b, n = 1;   // pieces of the sequence: one where no piece had to be looked for
+  if (P.cluster == 0) {
+    first = n = 0;
+    for (int i = lane; i < P.B; i += 32) total += blocks_of(P, i);
+    const int piece = piece_length(P, __reduce_add_sync(0xFFFFFFFFu, total), total);
+    for (int i = lane; i <= b; i += 32) {
+      const int k = max(1, (blocks_of(P, i) + piece - 1) / piece);
+      if (i < b) first += k; else n = k;
+    }
+    first = __reduce_add_sync(0xFFFFFFFFu, first);
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
   }
-  first = __reduce_add_sync(0xFFFFFFFFu, first);
-  n = __reduce_add_sync(0xFFFFFFFFu, n);
   const int kvh = h / P.G, in_group = h % P.G, y = kvh * P.groups + in_group / width;
   const int64_t own0 = (static_cast<int64_t>(first) * grid_y + y) * width + in_group % width, step = static_cast<int64_t>(grid_y) * width;
   // the results of the row's pair of row tiles: those of the thread blocks that hold some of its units, and where it is a single tile of both groups
@@ -819,12 +828,19 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
       if (x.z != 0.0f) at = where;     // (a group without tiles left no output)
     }
     const int some = min(32, n + m - i0);
-    for (int k = 0; k < some; ++k) {
-      const float f = __shfl_sync(0xFFFFFFFFu, w, k);
-      const int64_t where = __shfl_sync(0xFFFFFFFFu, at, k);
-      if (where < 0) continue;
-      const float4 x = *reinterpret_cast<const float4*>((i0 + k < n ? P.part_o : from.part_o) + where * JF_HEAD_DIM + lane * 4);
-      sum = make_float4(fmaf(x.x, f, sum.x), fmaf(x.y, f, sum.y), fmaf(x.z, f, sum.z), fmaf(x.w, f, sum.w));
+    for (int k0 = 0; k0 < some; k0 += 8) {   // eight results in flight
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t where = __shfl_sync(0xFFFFFFFFu, at, k0 + k);
+        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (where >= 0) x[k] = *reinterpret_cast<const float4*>((i0 + k0 + k < n ? P.part_o : from.part_o) + where * JF_HEAD_DIM + lane * 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
+        sum = make_float4(fmaf(x[k].x, f, sum.x), fmaf(x[k].y, f, sum.y), fmaf(x[k].z, f, sum.z), fmaf(x[k].w, f, sum.w));
+      }
     }
   }
 #pragma unroll
@@ -873,6 +889,7 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
 // One sequence of 500 positions, 8 KV heads: 7.7 -> 6.0 us (6.2 with what the sums have gained since), of 4000: 11.7 -> 9.1; 64 of 300: 19.6 -> 17.4; 8 of 2000: 14.9 -> 12.4.  With 2
 // columns, 4000 positions take 9.2 us so and 8.6 in pieces.
 constexpr int kRounds = 6, kFewRounds = 2;
+constexpr int kOwnRounds = 8;
 int cluster_size(const Plan& p, int B, int H_kv, int64_t longest) {
   const int64_t blocks = (longest + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, columns = static_cast<int64_t>(H_kv) * p.groups * B;
   const int64_t places = static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1);
@@ -972,10 +989,12 @@ jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from
   P.behind = from.behind * JF_BLOCK_SIZE;
   P.partial = from.part_o != nullptr;
   P.shared = from.shared; P.shared_blocks = from.shared_blocks; P.shared_i32 = from.shared_i32;
-  P.cluster = P.partial ? 0 : cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
+  // (partial results: a block for a sequence and KV head, where that is a few rounds of blocks a warp)
+  const int64_t own_blocks = (static_cast<int64_t>(std::min<int64_t>(max_S, int64_t{a->max_blocks} * JF_BLOCK_SIZE)) + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
+  P.cluster = P.partial ? own_blocks <= kWarps * kOwnRounds : cluster_size(p, a->B, a->H_kv, a->prefix_lens ? a->max_S : longest);   // (a prefix may be as long as the sequence)
   const bool feat = a->softcap > 0.0f || a->alibi_slopes;
   const auto s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(p.pieces, a->H_kv * p.groups);
+  const dim3 grid(p.pieces, a->H_kv * p.groups);   // (clusters: launch_attn)
   jf_status_t st;
   if (a->q_dtype == JF_DTYPE_BF16)
     st = a->codes == JF_CODES_INT8 ? launch_attn<JF_CODES_INT8, JF_DTYPE_BF16>(P, p.nt, feat, grid, s)
