@@ -753,17 +753,20 @@ __global__ void __launch_bounds__(WARPS * 32) block8_join_kernel(const __grid_co
   }
 }
 
-// The pieces of a sequence and the partial results of the positions before them (part_o, part_ml of `from`): a warp per (sequence,
+// The pieces of a sequence and the partial results of the positions before them (part_o, part_ml of `from`): WARPS warps per (sequence,
 // head), four channels a lane.  A result there has references of its own for its output and for its sum.
-template <int DT>
+template <int DT, int WARPS>
 __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ Block8Source from, int width,
                                                                  int grid_y) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  constexpr int ROWS = 8 / WARPS;
+  __shared__ float2 sm_top[8], sm_z[8];
+  __shared__ float4 sm_o[WARPS > 1 ? 8 : 1][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WARPS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + warp / WARPS;
   const int b = static_cast<int>(row / P.H_q), h = static_cast<int>(row % P.H_q);
   pdl_wait();
   pdl_trigger();
-  if (b >= P.B) return;
+  if (b >= P.B) return;   // (with several warps a row there is a row for every block)
   int total = 0, first = b, n = 1;   // pieces of the sequence: one where no piece had to be looked for
   if (P.cluster == 0) {
     first = n = 0;
@@ -791,7 +794,7 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
   };
   // references
   float top_o = kNone, top_l = kNone;
-  for (int i = lane; i < n + m; i += 32) {
+  for (int i = part * 32 + lane; i < n + m; i += WARPS * 32) {
     if (i < n) {
       const float x = P.part_ml[(own0 + i * step) * 2];
       top_o = fmaxf(top_o, x);
@@ -807,10 +810,20 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
     top_o = fmaxf(top_o, __shfl_xor_sync(0xFFFFFFFFu, top_o, o));
     top_l = fmaxf(top_l, __shfl_xor_sync(0xFFFFFFFFu, top_l, o));
   }
+  if (WARPS > 1) {
+    if (lane == 0) sm_top[warp] = make_float2(top_o, top_l);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      top_o = fmaxf(top_o, sm_top[k].x);
+      top_l = fmaxf(top_l, sm_top[k].y);
+    }
+  }
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float z = 0.0f;
-  for (int i0 = 0; i0 < n + m; i0 += 32) {
-    const int i = i0 + lane;
+  // (results part, part + WARPS, ...: a lane looks at one, then all lanes take their channels of each)
+  for (int i0 = 0; i0 * WARPS < n + m; i0 += 32) {
+    const int i = (i0 + lane) * WARPS + part;
     float w = 0.0f;
     int64_t at = -1;
     if (i < n) {
@@ -827,14 +840,14 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
       w = e * e;
       if (x.z != 0.0f) at = where;     // (a group without tiles left no output)
     }
-    const int some = min(32, n + m - i0);
+    const int some = min(32, (n + m - i0 * WARPS + WARPS - 1) / WARPS);
     for (int k0 = 0; k0 < some; k0 += 8) {   // eight results in flight
       float4 x[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int64_t where = __shfl_sync(0xFFFFFFFFu, at, k0 + k);
         x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (where >= 0) x[k] = *reinterpret_cast<const float4*>((i0 + k0 + k < n ? P.part_o : from.part_o) + where * JF_HEAD_DIM + lane * 4);
+        if (where >= 0) x[k] = *reinterpret_cast<const float4*>(((i0 + k0 + k) * WARPS + part < n ? P.part_o : from.part_o) + where * JF_HEAD_DIM + lane * 4);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -845,6 +858,20 @@ __global__ void __launch_bounds__(256) block8_join_shared_kernel(const __grid_co
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
+  if (WARPS > 1) {
+    if (lane == 0) sm_z[warp].x = z;
+    sm_o[warp][lane] = sum;
+    __syncthreads();
+    if (warp > 0) return;
+    z = 0.0f;
+    sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      z += sm_z[k].x;
+      const float4 x = sm_o[k][lane];
+      sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+    }
+  }
   const bool none = z == 0.0f;
   const float f = half_step(top_l - top_o);
   const float e[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -890,6 +917,7 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
 // columns, 4000 positions take 9.2 us so and 8.6 in pieces.
 constexpr int kRounds = 6, kFewRounds = 2;
 constexpr int kOwnRounds = 8;
+constexpr int kManyResults = 16;
 int cluster_size(const Plan& p, int B, int H_kv, int64_t longest) {
   const int64_t blocks = (longest + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, columns = static_cast<int64_t>(H_kv) * p.groups * B;
   const int64_t places = static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1);
@@ -1004,9 +1032,21 @@ jf_status_t block8_attend(const jf_block8_attn_args* a, const Block8Source& from
                                    : launch_attn<JF_CODES_E4M3, JF_DTYPE_FP16>(P, p.nt, feat, grid, s);
   const int width = 8 * p.nt, grid_y = a->H_kv * p.groups;
   if (st == JF_OK && P.partial) {
-    const dim3 rows(static_cast<unsigned>((int64_t{a->B} * a->H_q + 7) / 8));
-    JF_CUDA_TRY(a->q_dtype == JF_DTYPE_BF16 ? launch_pdl(block8_join_shared_kernel<JF_DTYPE_BF16>, rows, dim3(256), 0, s, P, from, width, grid_y)
-                                            : launch_pdl(block8_join_shared_kernel<JF_DTYPE_FP16>, rows, dim3(256), 0, s, P, from, width, grid_y));
+    // Eight warps a row where a row has many results and the rows do not fill the multiprocessors: 8 / 1 heads, 16 sequences over 65536 shared
+    // positions (128 rows of 297 results) 74 -> 32 us, 32 / 8 heads, 32 over 4096 (1024 of 37) 33 -> 30; 64 over 4096 would go from 36 to 42.
+    const int64_t results = (from.grid + int64_t{a->H_kv} * from.pairs) / (int64_t{a->H_kv} * from.pairs) * (from.row_tiles & 1 ? 2 : 1);
+    auto join = [&](auto dt, auto warps) {
+      constexpr int D = decltype(dt)::value, W = decltype(warps)::value;
+      const dim3 rows(static_cast<unsigned>((int64_t{a->B} * a->H_q * W + 7) / 8));
+      return launch_pdl(block8_join_shared_kernel<D, W>, rows, dim3(256), 0, s, P, from, width, grid_y);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Eight = std::integral_constant<int, 8>;
+    using Bf16 = std::integral_constant<int, JF_DTYPE_BF16>;
+    using Fp16 = std::integral_constant<int, JF_DTYPE_FP16>;
+    const bool many = results > kManyResults && int64_t{a->B} * a->H_q <= 8 * num_sms();
+    if (a->q_dtype == JF_DTYPE_BF16) JF_CUDA_TRY(many ? join(Bf16(), Eight()) : join(Bf16(), One()));
+    else JF_CUDA_TRY(many ? join(Fp16(), Eight()) : join(Fp16(), One()));
     return JF_OK;
   }
   if (st != JF_OK || P.cluster > 0 || p.pieces == a->B) return st;   // (one piece per sequence: nothing to join)

@@ -651,14 +651,22 @@ struct Plan {
   int64_t items, units;
   uint64_t own, o_bytes, bytes;   // scratch of the own positions' part, of the outputs, of all
 };
-constexpr int kFewRows = 16;      // rows of a KV head up to which the shared positions go through block8_attn.cu's kernel
+constexpr int kLeastUnits = 2;    // of a thread block
+// Blocks that the sequences would read one after the other, each the shared ones for itself: up to here they do, in block8_attn.cu's kernel.  (The way
+// by the tensor cores is 14 us of launches, loads and joins before it is worth anything.  Back to back, 32 / 8 heads: 64 sequences over 256 positions
+// 18 and 28 us, 8 over 4096 22 and 19 (from cold caches 27 and 27), 32 over 1024 27 and 26, 16 over 4096 32 and 23, 16 over 16384 90 and 30; 8 / 1 heads: 4
+// over 65536 21 and 26, 8 over 65536 30 and 27.)
+constexpr int64_t kFewBlocks = 20000;
 
-bool tensor_form(int B, int H_q, int H_kv, int shared_blocks) { return shared_blocks > 0 && int64_t{B} * (H_q / H_kv) > kFewRows; }
+bool tensor_form(int B, int H_kv, int max_S, int shared_blocks) {
+  const int seen = std::min(shared_blocks, (max_S - 1) / JF_BLOCK_SIZE + 1);
+  return int64_t{B} * H_kv * seen > kFewBlocks;
+}
 
 bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) {
   if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_S <= 0 || H_q % H_kv != 0 || shared_blocks < 0 || shared_blocks > INT32_MAX / JF_BLOCK_SIZE - 1) return false;
   p = Plan{};
-  if (!tensor_form(B, H_q, H_kv, shared_blocks)) {
+  if (!tensor_form(B, H_kv, max_S, shared_blocks)) {
     p.bytes = block8_attn_workspace(B, H_q, H_kv, max_S);
     return p.bytes > 0;
   }
@@ -667,12 +675,12 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) 
   if (rows > INT32_MAX / 2 || H_q > 65535 || B > 65535) return false;
   p.row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
   p.pairs = (p.row_tiles + 1) / 2;
-  const int seen = std::min(shared_blocks, (max_S + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE);   // of the shared blocks
+  const int seen = std::min(shared_blocks, (max_S - 1) / JF_BLOCK_SIZE + 1);   // of the shared blocks
   p.tiles = (seen + kTileBlocks - 1) / kTileBlocks;
   p.items = int64_t{H_kv} * p.pairs;
   p.units = p.items * p.tiles;
   if (p.units > INT32_MAX / 2) return false;
-  p.grid = static_cast<int>(std::min<int64_t>(num_sms(), p.units));
+  p.grid = static_cast<int>(std::min<int64_t>(num_sms(), (p.units + kLeastUnits - 1) / kLeastUnits));
   p.own = (block8_attn_workspace(B, H_q, H_kv, std::max(max_S - shared_blocks * JF_BLOCK_SIZE, 1)) + 255) / 256 * 256;
   if (p.own == 0) return false;
   const uint64_t part_rows = static_cast<uint64_t>(p.grid + p.items) * 2 * kRows;
@@ -723,7 +731,7 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   Plan p;
   if (!make_plan(at.B, at.H_q, at.H_kv, at.max_S, a->shared_blocks, p)) return JF_ERR_ARG;
   if (at.workspace_bytes < p.bytes) return JF_ERR_WORKSPACE;
-  if (!tensor_form(at.B, at.H_q, at.H_kv, a->shared_blocks)) return block8_attend(&at, from, stream, true);
+  if (!tensor_form(at.B, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
   const auto s = static_cast<cudaStream_t>(stream);
   SharedParams P{};
   jf_status_t st = wait_record(s, &P.status);
