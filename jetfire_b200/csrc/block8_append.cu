@@ -42,7 +42,7 @@ struct Rotation {
   int64_t q_stride_t, q_stride_h;
   uint16_t* q_out;
   int8_t* bounds;                    // null: none
-  int32_t H_q, rot, q_rounds, append_blocks;
+  int32_t H_q, rot, q_rounds, k_blocks, append_blocks;   // k_blocks: thread blocks of K, V's come behind them, the queries' behind append_blocks
   bool pos_i32, interleaved, table_f32;
 };
 struct AppendParams {
@@ -149,9 +149,11 @@ template <int DT, int N> __device__ __forceinline__ void table_row(const Rotatio
   }
 }
 // A token whose position is not in the table gets angles that are no numbers.
-template <int DT> __device__ __forceinline__ Turn turn_of(const Rotation& R, int64_t token, int col) {
+__device__ __forceinline__ int64_t position_of(const Rotation& R, int64_t token) {
+  return R.pos_i32 ? static_cast<const int32_t*>(R.positions)[token] : static_cast<const int64_t*>(R.positions)[token];
+}
+template <int DT> __device__ __forceinline__ Turn turn_of(const Rotation& R, int64_t pos, int col) {
   Turn t;
-  const int64_t pos = R.pos_i32 ? static_cast<const int32_t*>(R.positions)[token] : static_cast<const int64_t*>(R.positions)[token];
   const bool is = pos >= 0 && pos < R.rows;
   const int half = R.rot / 2;
   if (!is || col >= R.rot) {
@@ -171,6 +173,34 @@ template <int DT> __device__ __forceinline__ Turn turn_of(const Rotation& R, int
     const int at = col < half ? col : col - half;
     table_row<DT, 8>(R, pos * R.rot + at, t.c);
     table_row<DT, 8>(R, pos * R.rot + half + at, t.s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t.s[k] = col < half ? -t.s[k] : t.s[k];
+  }
+  return t;
+}
+// The same of a token whose row of the table stands in shared memory, in fp32 (NaN where it is not in the table).
+__device__ __forceinline__ Turn turn_of(const Rotation& R, const float* row, int col) {
+  Turn t;
+  const int half = R.rot / 2;
+  if (col >= R.rot) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t.c[k] = t.s[k] = 0.0f;
+  } else if (R.interleaved) {
+    const float4 c = *reinterpret_cast<const float4*>(row + col / 2), s = *reinterpret_cast<const float4*>(row + half + col / 2);
+    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      t.c[2 * k] = t.c[2 * k + 1] = cs[k];
+      t.s[2 * k] = -sn[k];
+      t.s[2 * k + 1] = sn[k];
+    }
+  } else {
+    const int at = col < half ? col : col - half;
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      *reinterpret_cast<float4*>(t.c + k) = *reinterpret_cast<const float4*>(row + at + k);
+      *reinterpret_cast<float4*>(t.s + k) = *reinterpret_cast<const float4*>(row + half + at + k);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) t.s[k] = col < half ? -t.s[k] : t.s[k];
   }
@@ -196,31 +226,45 @@ template <int DT> __device__ __forceinline__ void rotate(const Rotation& R, cons
 template <int DT, bool VEC> __device__ __forceinline__ void rotate_queries(const AppendParams& P, const Rotation& R, int64_t item) {
   const int lane = threadIdx.x & 31, col = (lane & 15) * 8, per = 2 * R.q_rounds, chunks = (R.H_q + per - 1) / per;
   const int64_t t = item / chunks;
-  if (t >= min(P.T, P.start[P.n_seqs])) return;      // rows of no sequence
-  const int h0 = static_cast<int>(item % chunks) * per + (lane >> 4);
-  const Turn turn = turn_of<DT>(R, t, col);
-  auto rows = [&](auto n_tag, int h) {
+  if (t >= P.T) return;
+  const int last = P.start[P.n_seqs];
+  const int h0 = static_cast<int>(item - t * chunks) * per + (lane >> 4);
+  const uint16_t* from = R.q + t * R.q_stride_t + col;
+  const int64_t pos = position_of(R, t);
+  auto rows = [&](auto n_tag) {
     constexpr int N = decltype(n_tag)::value;
-    uint4 raw[N];
+    uint4 raw[N], then[N];
+    auto read = [&](uint4* to, int h) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      raw[i] = h + 2 * i < R.H_q ? load8<VEC>(R.q + t * R.q_stride_t + (h + 2 * i) * R.q_stride_h + col) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < N; ++i) to[i] = h + 2 * i < R.H_q ? load8<VEC>(from + (h + 2 * i) * R.q_stride_h) : make_uint4(0, 0, 0, 0);
+    };
+    read(raw, h0);      // (on their way while the angles are looked up)
+    const Turn turn = turn_of<DT>(R, pos, col);
+    if (t >= last) return;   // rows of no sequence
+#pragma unroll 1
+    for (int h = h0;;) {
+      const bool more = N > 1 && h + 2 * N < h0 + per;
+      if (more) read(then, h + 2 * N);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float v[8];
-      rotate<DT>(R, raw[i], turn, col, v);
-      uint32_t w[4];
+      for (int i = 0; i < N; ++i) {
+        float v[8];
+        rotate<DT>(R, raw[i], turn, col, v);
+        uint32_t w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
-        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+        for (int k = 0; k < 4; ++k) {
+          if (DT == JF_DTYPE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
+        }
+        if (h + 2 * i < R.H_q) *reinterpret_cast<uint4*>(R.q_out + (t * R.H_q + h + 2 * i) * JF_HEAD_DIM + col) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      if (h + 2 * i < R.H_q) *reinterpret_cast<uint4*>(R.q_out + (t * R.H_q + h + 2 * i) * JF_HEAD_DIM + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (!more) break;
+      h += 2 * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = then[i];
     }
   };
-  if (R.q_rounds == 1) rows(std::integral_constant<int, 1>(), h0);
-  else
-    for (int i = 0; i < R.q_rounds; i += 4) rows(std::integral_constant<int, 4>(), h0 + 2 * i);
+  if (R.q_rounds == 1) rows(std::integral_constant<int, 1>());
+  else rows(std::integral_constant<int, 4>());
 }
 
 // ---- blocks -----------------------------------------------------------------------------------
@@ -233,116 +277,138 @@ template <int CODES> __device__ __forceinline__ uint2 encode8(const float* v) {
   return make_uint2(encode4<CODES>(pair(v[0], v[1]), pair(v[2], v[3])), encode4<CODES>(pair(v[4], v[5]), pair(v[6], v[7])));
 }
 
-// What write_block does for a side that is rotated, or whose bounds are kept.
+// What write_block does for a side that is rotated, or whose bounds are kept; `at`: the block's place in the table; the warp's lanes hold the
+// positions of the tokens from `first` on, `turns` their angles where there are more than a few.  The block's rows, their angles, its id, and what it holds of earlier rows are all asked for before one of
+// them is waited for.  Sixteen rows are rotated twice, once for their maximum and once to be stored (64 values a lane held in between
+// left room for 16 warps on a multiprocessor); up to two, a token of a decode step, once.
 template <int DT, int CODES, bool VEC>
 __device__ __forceinline__ void write_block_rotated(const AppendParams& P, const Rotation& R, const AppendSide& S, int h, int t, int cnt, int r,
-                                                    int64_t id) {
+                                                    int64_t at, int first, int64_t pos, const float* turns) {
   const int lane = threadIdx.x & 31, half = lane >> 4, col = (lane & 15) * 8;
   const uint16_t* x = S.x + static_cast<int64_t>(t) * S.stride_t + h * S.stride_h + col;
-  float v[8][8];
-  {
-    uint4 raw[8];
+  auto body = [&](auto rounds_tag) {
+    constexpr int N = decltype(rounds_tag)::value;
+    const int64_t id = P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
+    uint4 raw[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int row = 2 * i + half;
       raw[i] = row < cnt ? load8<VEC>(x + row * S.stride_t) : make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    auto angles = [&](int i) {
+      const int token = t - first + min(2 * i + half, cnt - 1);
+      return turns ? turn_of(R, turns + token * R.rot, col) : turn_of<DT>(R, __shfl_sync(0xFFFFFFFFu, pos, token), col);
+    };
+    Turn turn;
+    auto rotated = [&](int i, float* v) {
       if (R.cos_sin) {
-        const int row = 2 * i + half;
-        const Turn turn = turn_of<DT>(R, t + min(row, cnt - 1), col);
-        rotate<DT>(R, raw[i], turn, col, v[i]);
+        if (N > 1) turn = angles(i);
+        rotate<DT>(R, raw[i], turn, col, v);
       } else {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) unpack2<DT>(w[k], v[i][2 * k], v[i][2 * k + 1]);
+        for (int k = 0; k < 4; ++k) unpack2<DT>(w[k], v[2 * k], v[2 * k + 1]);
+      }
+    };
+    if (N == 1 && R.cos_sin) turn = angles(0);
+    if (id < 0 || id >= P.num_blocks) return;
+    float* scale_at = S.scales + h * P.num_blocks + id;
+    uint8_t* rows = S.data + ((h * P.num_blocks + id) * JF_BLOCK_SIZE) * JF_HEAD_DIM + col;
+    float old = r > 0 ? *scale_at : 0.0f;
+    uint2 was[8];      // earlier rows of the block (of a few tokens: of many, they are the exception and looked at when their turn comes)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (N == 1 && 2 * i + half < r) was[i] = *reinterpret_cast<const uint2*>(rows + (2 * i + half) * JF_HEAD_DIM);
+    if (!(old > 0.0f && old < __int_as_float(0x7F800000))) old = 0.0f;   // never written: nothing to keep
+    float top = 0.0f, v[8];
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      rotated(i, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {   // infinities and NaN do not count
+        const float a = 2 * i + half < cnt ? fabsf(v[k]) : 0.0f;
+        const bool fine = a < __int_as_float(0x7F800000);
+        wild |= !fine;
+        top = fmaxf(top, fine ? a : 0.0f);
       }
     }
-  }
-  float* scale_at = S.scales + h * P.num_blocks + id;
-  float old = r > 0 ? *scale_at : 0.0f;
-  if (!(old > 0.0f && old < __int_as_float(0x7F800000))) old = 0.0f;   // never written: nothing to keep
-  float top = 0.0f;
-  bool wild = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {   // infinities and NaN do not count
-      const float a = 2 * i + half < cnt ? fabsf(v[i][k]) : 0.0f;
-      const bool fine = a < __int_as_float(0x7F800000);
-      wild |= !fine;
-      top = fmaxf(top, fine ? a : 0.0f);
-    }
-  wild = __any_sync(0xFFFFFFFFu, wild);
-  top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));   // (not negative: ordered as their bits are)
-  const float s = fmaxf(old, scale_for<CODES>(top)), inv = __frcp_rn(s);
-  uint8_t* rows = S.data + ((h * P.num_blocks + id) * JF_BLOCK_SIZE) * JF_HEAD_DIM + col;
-  float lo[8], hi[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    lo[k] = __int_as_float(0x7F800000);
-    hi[k] = -lo[k];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = 2 * i + half;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[i][k] = __fmul_rn(v[i][k], inv);
-    if (wild) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = tame<CODES>(v[i][k]);
-    }
-    if (row < cnt) {
-      *reinterpret_cast<uint2*>(rows + (r + row) * JF_HEAD_DIM) = encode8<CODES>(v[i]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        lo[k] = fminf(lo[k], v[i][k]);
-        hi[k] = fmaxf(hi[k], v[i][k]);
-      }
-    }
-  }
-  const bool grew = s != old;
-  if (r > 0 && (grew || R.bounds)) {
-    const float ratio = __fdiv_rn(old, s);
-    for (int row = half; row < r; row += 2) {
-      uint2* p = reinterpret_cast<uint2*>(rows + row * JF_HEAD_DIM);
-      float w[8];
-      decode8<CODES>(*p, w);
-      if (grew) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = tame<CODES>(__fmul_rn(w[k], ratio));
-        *p = encode8<CODES>(w);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        lo[k] = fminf(lo[k], w[k]);
-        hi[k] = fmaxf(hi[k], w[k]);
-      }
-    }
-  }
-  if (R.bounds) {
+    wild = __any_sync(0xFFFFFFFFu, wild);
+    top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));   // (not negative: ordered as their bits are)
+    const float s = fmaxf(old, scale_for<CODES>(top)), inv = __frcp_rn(s);
+    float lo[8], hi[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      lo[k] = fminf(lo[k], __shfl_xor_sync(0xFFFFFFFFu, lo[k], 16));
-      hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xFFFFFFFFu, hi[k], 16));
-      if (half) lo[k] = hi[k];        // half a warp for each of the two
+      lo[k] = __int_as_float(0x7F800000);
+      hi[k] = -lo[k];
     }
-    uint2 code = encode8<CODES>(lo);
-    if (CODES == JF_CODES_E4M3) {     // in units of 448 / 127 scales, outwards
-      float w[8];
-      decode8<CODES>(code, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = 2 * i + half;
+      if (N > 1) rotated(i, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(v[k], inv);
+      if (wild) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = tame<CODES>(v[k]);
+      }
+      if (row < cnt) {
+        *reinterpret_cast<uint2*>(rows + (r + row) * JF_HEAD_DIM) = encode8<CODES>(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          lo[k] = fminf(lo[k], v[k]);
+          hi[k] = fmaxf(hi[k], v[k]);
+        }
+      }
+    }
+    const bool grew = s != old;
+    if (r > 0 && (grew || R.bounds)) {
+      const float ratio = __fdiv_rn(old, s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 2 * i + half;
+        if (row >= r) continue;
+        float w[8];
+        if (N > 1) was[i] = *reinterpret_cast<const uint2*>(rows + row * JF_HEAD_DIM);
+        decode8<CODES>(was[i], w);
+        if (grew) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] = tame<CODES>(__fmul_rn(w[k], ratio));
+          *reinterpret_cast<uint2*>(rows + row * JF_HEAD_DIM) = encode8<CODES>(w);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          lo[k] = fminf(lo[k], w[k]);
+          hi[k] = fmaxf(hi[k], w[k]);
+        }
+      }
+    }
+    __syncwarp();
+    if (R.bounds) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float u = __fdiv_rn(w[k] * 127.0f, 448.0f);
-        w[k] = half ? ceilf(u) : floorf(u);
+        lo[k] = fminf(lo[k], __shfl_xor_sync(0xFFFFFFFFu, lo[k], 16));
+        hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xFFFFFFFFu, hi[k], 16));
+        if (half) lo[k] = hi[k];        // half a warp for each of the two
       }
-      code = encode8<JF_CODES_INT8>(w);
+      uint2 code = encode8<CODES>(lo);
+      if (CODES == JF_CODES_E4M3) {     // in units of 448 / 127 scales, outwards
+        float w[8];
+        decode8<CODES>(code, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float u = __fdiv_rn(w[k] * 127.0f, 448.0f);
+          w[k] = half ? ceilf(u) : floorf(u);
+        }
+        code = encode8<JF_CODES_INT8>(w);
+      }
+      *reinterpret_cast<uint2*>(R.bounds + ((h * P.num_blocks + id) * 2 + half) * JF_HEAD_DIM + col) = code;
     }
-    *reinterpret_cast<uint2*>(R.bounds + ((h * P.num_blocks + id) * 2 + half) * JF_HEAD_DIM + col) = code;
-  }
-  __syncwarp();
-  if (lane == 0 && grew) *scale_at = s;
+    __syncwarp();
+    if (lane == 0 && grew) *scale_at = s;
+  };
+  if (cnt <= 2) body(std::integral_constant<int, 1>());
+  else body(std::integral_constant<int, 8>());
 }
 
 // Rows t .. t + cnt of the call into rows r .. r + cnt of block `id`; r rows of its sequence are there already.
@@ -424,26 +490,72 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
   if (lane == 0 && s != old) *scale_at = s;
 }
 
-// A warp per (chunk of tokens, head, side): it writes every block whose first token of the call stands in the chunk.
-template <int DT, int CODES, bool VEC, bool ROTARY>   // VEC: rows may be read 16 bytes at a time
-__global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid_constant__ AppendParams P, const __grid_constant__ Rotation R) {
-  if constexpr (ROTARY)
+// A warp per (chunk of tokens, head, side): it writes every block whose first token of the call stands in the chunk.  With a rotation the
+// warps of a thread block take heads of K of one chunk, whose tokens' angles they bring to shared memory together (kStaged); of chunks of one
+// token each warp finds its own, in a kernel whose registers are not held down for the sake of more blocks on a multiprocessor
+// (four sequences of a token 9.8 us from cold caches and not 13.0, 8192 tokens 98 and not 102).
+enum { kPlain, kDirect, kStaged };
+constexpr int kTurns = 31;   // tokens: the chunk's and 15 more
+template <int DT, int CODES, bool VEC, int ROTARY>   // VEC: rows may be read 16 bytes at a time
+__global__ void __launch_bounds__(kWarps * 32, ROTARY == kStaged ? 5 : 1) block8_append_kernel(const __grid_constant__ AppendParams P, const __grid_constant__ Rotation R) {
+  __shared__ __align__(16) float sm_turns[ROTARY == kStaged ? kTurns * JF_HEAD_DIM : 1];
+  const float* turns = nullptr;
+  const int lane = threadIdx.x & 31;
+  int side, h, t;
+  if constexpr (ROTARY) {
     if (static_cast<int>(blockIdx.x) >= R.append_blocks) {
       pdl_wait();
       pdl_trigger();
       rotate_queries<DT, VEC>(P, R, static_cast<int64_t>(blockIdx.x - R.append_blocks) * kWarps + (threadIdx.x >> 5));
       return;
     }
-  const int lane = threadIdx.x & 31;
-  const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), rest = item >> 1;
-  const int side = item & 1, h = static_cast<int>(rest % static_cast<uint32_t>(P.H));
-  const int64_t from = static_cast<int64_t>(rest / static_cast<uint32_t>(P.H)) * P.chunk;
-  if (from >= P.T) { pdl_wait(); return; }
-  int t = static_cast<int>(from);
-  const int end = min(t + P.chunk, P.T);
+    int64_t from;
+    if (static_cast<int>(blockIdx.x) < R.k_blocks) {
+      const int per = (P.H + kWarps - 1) / kWarps;
+      side = 0;
+      h = static_cast<int>(blockIdx.x) % per * kWarps + (threadIdx.x >> 5);
+      from = static_cast<int64_t>(static_cast<int>(blockIdx.x) / per) * P.chunk;
+    } else {
+      const int item = static_cast<int>(blockIdx.x - R.k_blocks) * kWarps + static_cast<int>(threadIdx.x >> 5);
+      side = 1;
+      h = item % P.H;
+      from = static_cast<int64_t>(item / P.H) * P.chunk;
+    }
+    if (from >= P.T) { pdl_wait(); return; }
+    t = static_cast<int>(from);
+    pdl_wait();
+    pdl_trigger();
+    if (ROTARY == kStaged && side == 0 && R.cos_sin) {
+      const int pieces = R.rot / 4, all = min(P.chunk + 15, P.T - t) * pieces;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < all; i += kWarps * 32) {
+        const int token = i / pieces, piece = (i - token * pieces) * 4;
+        const int64_t pos = position_of(R, t + token);
+        float x[4];
+        if (pos >= 0 && pos < R.rows) table_row<DT, 4>(R, pos * R.rot + piece, x);
+        else x[0] = x[1] = x[2] = x[3] = __int_as_float(0x7FC00000);
+        *reinterpret_cast<float4*>(sm_turns + token * R.rot + piece) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+      __syncthreads();
+      turns = sm_turns;
+    }
+    if (h >= P.H) return;
+  } else {
+    const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), rest = item >> 1;
+    side = item & 1;
+    h = static_cast<int>(rest % static_cast<uint32_t>(P.H));
+    const int64_t from = static_cast<int64_t>(rest / static_cast<uint32_t>(P.H)) * P.chunk;
+    if (from >= P.T) { pdl_wait(); return; }
+    t = static_cast<int>(from);
+    pdl_wait();
+    pdl_trigger();
+  }
+  const int first = t, end = min(t + P.chunk, P.T);
   const AppendSide& S = P.side[side];
-  pdl_wait();
-  pdl_trigger();
+  // positions of the tokens that may be in the chunk's blocks: its own and 15 more
+  int64_t pos_of_lane = 0;
+  if constexpr (ROTARY)
+    if (side == 0 && R.cos_sin && !turns) pos_of_lane = position_of(R, min(t + lane, P.T - 1));
   // sequences that end at or before t
   int s = 0;
   for (int i = lane; i < P.n_seqs; i += 32) s += P.start[i + 1] <= t;
@@ -465,10 +577,11 @@ __global__ void __launch_bounds__(kWarps * 32) block8_append_kernel(const __grid
     const int64_t blk = pos >> 4;
     if (blk < P.max_blocks) {
       const int64_t at = s * P.bt_stride + blk;
-      const int64_t id = P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
-      if (id >= 0 && id < P.num_blocks) {
-        if (ROTARY && side == 0) write_block_rotated<DT, CODES, VEC>(P, R, S, h, t, cnt, r, id);
-        else write_block<DT, CODES, VEC>(P, S, h, t, cnt, r, id);
+      if (ROTARY && side == 0) {
+        write_block_rotated<DT, CODES, VEC>(P, R, S, h, t, cnt, r, at, first, pos_of_lane, turns);
+      } else {
+        const int64_t id = P.bt_i32 ? static_cast<const int32_t*>(P.table)[at] : static_cast<const int64_t*>(P.table)[at];
+        if (id >= 0 && id < P.num_blocks) write_block<DT, CODES, VEC>(P, S, h, t, cnt, r, id);
       }
     }
     t += cnt;
@@ -491,11 +604,16 @@ jf_status_t launch_append(AppendParams& P, const Rotation* R, int dtype, int cod
   Rotation rot{};
   if (R) {
     rot = *R;
+    const int64_t chunks_of = there ? (P.T + int64_t{P.chunk} - 1) / P.chunk : 0, k = chunks_of * ((P.H + kWarps - 1) / kWarps);
+    blocks = k + (chunks_of * P.H + kWarps - 1) / kWarps;
+    if (blocks > INT32_MAX / 2) return JF_ERR_UNSUPPORTED;
+    rot.k_blocks = static_cast<int32_t>(k);
     rot.append_blocks = static_cast<int32_t>(blocks);
     if (rot.q && P.n_seqs > 0) {
       vec &= aligned(rot.q, 16) && (rot.q_stride_t | rot.q_stride_h) % 8 == 0;
-      // Rows a warp goes through, two at a time: eight share the angles of their token, where there are warps enough without
-      rot.q_rounds = static_cast<int64_t>(P.T) * rot.H_q >= 16ll * num_sms() * 32 ? 4 : 1;
+      // Pairs of rows that a warp goes through with the angles of their token: as many as leave warps enough (8192 tokens, 64 heads: 4 129 us, 16 114)
+      const int64_t pairs = static_cast<int64_t>(P.T) * rot.H_q / 2, enough = 64ll * num_sms();
+      rot.q_rounds = pairs >= 16 * enough ? 16 : pairs >= 4 * enough ? 4 : 1;
       const int64_t chunks = (rot.H_q + 2 * rot.q_rounds - 1) / (2 * rot.q_rounds);
       blocks += (P.T * chunks + kWarps - 1) / kWarps;
     }
@@ -505,11 +623,14 @@ jf_status_t launch_append(AppendParams& P, const Rotation* R, int dtype, int cod
   const dim3 grid(static_cast<unsigned>(blocks)), block(kWarps * 32);
   auto launch = [&](auto dt, auto code) {
     constexpr int D = decltype(dt)::value, C = decltype(code)::value;
+    if (R && P.chunk > 1)
+      return vec ? launch_pdl(block8_append_kernel<D, C, true, kStaged>, grid, block, 0, s, P, rot)
+                 : launch_pdl(block8_append_kernel<D, C, false, kStaged>, grid, block, 0, s, P, rot);
     if (R)
-      return vec ? launch_pdl(block8_append_kernel<D, C, true, true>, grid, block, 0, s, P, rot)
-                 : launch_pdl(block8_append_kernel<D, C, false, true>, grid, block, 0, s, P, rot);
-    return vec ? launch_pdl(block8_append_kernel<D, C, true, false>, grid, block, 0, s, P, rot)
-               : launch_pdl(block8_append_kernel<D, C, false, false>, grid, block, 0, s, P, rot);
+      return vec ? launch_pdl(block8_append_kernel<D, C, true, kDirect>, grid, block, 0, s, P, rot)
+                 : launch_pdl(block8_append_kernel<D, C, false, kDirect>, grid, block, 0, s, P, rot);
+    return vec ? launch_pdl(block8_append_kernel<D, C, true, kPlain>, grid, block, 0, s, P, rot)
+               : launch_pdl(block8_append_kernel<D, C, false, kPlain>, grid, block, 0, s, P, rot);
   };
   using Bf16 = std::integral_constant<int, JF_DTYPE_BF16>;
   using Fp16 = std::integral_constant<int, JF_DTYPE_FP16>;
