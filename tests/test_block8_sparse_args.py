@@ -34,7 +34,10 @@ def test_status(L):
 def test_workspace_bytes(L):
     w, dense = L.lib.jf_block8_sparse_workspace_bytes, L.lib.jf_block8_workspace_bytes
     assert w(1, 8, 2, 100, 0) == 0 and w(1, 8, 3, 100, 4) == 0 and w(1, 8, 2, 0, 4) == 0
-    assert w(4, 64, 8, 65536, 128) == dense(4, 64, 8, 2048) and w(4, 64, 8, 100, 2 ** 31 - 1) == dense(4, 64, 8, 100)
+    # the attention's over the chosen blocks, and four bytes for each block of a row
+    up = lambda x: (x + 255) // 256 * 256
+    assert w(4, 64, 8, 65536, 128) == up(dense(4, 64, 8, 2048)) + 4 * 8 * 4096 * 4
+    assert w(4, 64, 8, 100, 2 ** 31 - 1) == up(dense(4, 64, 8, 100)) + 4 * 8 * 8 * 4
 
 
 def test_the_op_refuses(L):

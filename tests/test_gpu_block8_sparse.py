@@ -264,3 +264,23 @@ def test_a_decode_loop_in_a_graph(codes):
                 at = c.table[b, blk]
                 assert torch.equal(c.bounds[:, at].double(), M.bounds_of(k[:, at], min(16, n - blk * 16), code))
         c.check(*got)
+
+
+def test_a_row_longer_than_shared_memory():
+    """50000 blocks: the choice exactly, the outputs as the decode attention gives them over a table of the chosen blocks."""
+    from jetfire_b200 import ops
+    n, top = 50000, 300
+    g = torch.Generator(device="cuda").manual_seed(6)
+    kd, vd = (torch.randint(-127, 128, (1, n * 16, 128), dtype=torch.int8, device="cuda", generator=g) for _ in range(2))
+    ks, vs = (torch.rand(1, n, device="cuda", generator=g) * 0.02 + 0.001 for _ in range(2))
+    rows = kd.view(1, n, 16, 128)
+    bounds = torch.stack([rows.amin(2), rows.amax(2)], 2)
+    table = torch.randperm(n, device="cuda", generator=g)[None]
+    q = torch.randn(1, 4, 128, device="cuda", generator=g).bfloat16()
+    lens = torch.tensor([n * 16 - 5], dtype=torch.int32, device="cuda")
+    out, lse, chosen = ops.block8_sparse_decode_attn(q, kd, ks, vd, vs, bounds, table, lens, n * 16, 4, 1, 16, 0.05, top_blocks=top)
+    pick = M.choose(q[0].double().cpu(), bounds[0].cpu(), ks[0].double().cpu(), table[0].cpu(), n, top, 1, 2, torch.int8, n)
+    assert chosen[0, 0].tolist() == pick
+    want, want_lse = ops.block8_decode_attn(q, kd, ks, vd, vs, table[:, chosen[0, 0].long()].contiguous(), lens - (n - top) * 16, top * 16, 4, 1, 16, 0.05)
+    tol = 2 * ((2 ** -11 + 2 ** -14) * 127 * 0.021 + 2 ** -8 * want.float().abs())
+    assert ((out.float() - want.float()).abs() <= tol).all() and (lse - want_lse).abs().max() <= 2 ** -12
