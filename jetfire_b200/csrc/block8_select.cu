@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kScoreWarps = 8, kTile = 16;        // blocks of a warp's tile
 constexpr int kWarps = 16, kThreads = kWarps * 32; // of the choosing kernel
+constexpr int kScoreBlocks = 3;                   // of a multiprocessor: warps take more tiles rather than that there are several waves of blocks
 constexpr int kBins = 2048;
 constexpr int kMaxBlocks = 1 << 18;
 constexpr int kMaxKeys = 49152;                   // of a row in shared memory; longer rows are read from where they are
@@ -84,7 +85,7 @@ template <int DT> __device__ __forceinline__ void round_queries(const SelectPara
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kScoreWarps * 32) block8_score_kernel(const __grid_constant__ SelectParams P) {
+__global__ void __launch_bounds__(kScoreWarps * 32, kScoreBlocks) block8_score_kernel(const __grid_constant__ SelectParams P) {
   __shared__ Queries S;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, b = blockIdx.z;
@@ -356,7 +357,7 @@ extern "C" jf_status_t jf_block8_sparse_attn(const jf_block8_sparse_args* a, jf_
   const auto s = static_cast<cudaStream_t>(stream);
   if (blocks > a->top_blocks) {   // (else there is nothing to choose)
     const int64_t tiles = (blocks + kScoreWarps * kTile - 1) / (kScoreWarps * kTile) * at.B * at.H_kv;
-    P.tiles = tiles > 16 * num_sms() ? 4 : tiles > 8 * num_sms() ? 2 : 1;
+    P.tiles = static_cast<int>(std::min<int64_t>((tiles + kScoreBlocks * num_sms() - 1) / (kScoreBlocks * num_sms()), 16));
     const int each = kScoreWarps * kTile * P.tiles;
     const dim3 grid(static_cast<unsigned>((blocks + each - 1) / each), at.H_kv, at.B), block(kScoreWarps * 32);
     JF_CUDA_TRY(at.q_dtype == JF_DTYPE_BF16 ? launch_pdl(block8_score_kernel<JF_DTYPE_BF16>, grid, block, 0, s, P)
