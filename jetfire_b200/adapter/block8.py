@@ -4,7 +4,10 @@ For layers that need more than the 2 to 4 bits of the release modes.  ``JetFireB
 layer's cache (codes, one scale per block of 16 positions and KV head); ``try_block8_attention``
 serves a step of it: every new token is appended, sequences with one query token attend over the
 cache (``ops.block8_decode_attn``), prompts attend over the step's own keys and values
-(``ops.varlen_prefill_attn``), both with the implementation's score cap, distance bias and window.
+(``ops.varlen_prefill_attn``), both with the implementation's score cap, distance bias and window.  A decode step of
+sequences that share a prefix (vLLM's cascade steps) reads the prefix once for all of them (``ops.block8_shared_prefix_attn``); a store made
+for it keeps block bounds and lets a decode token attend to its best blocks only (``ops.block8_sparse_decode_attn``; a choice of the
+user's, ``JETFIRE_BLOCK8_TOP``).
 
 Nothing of the decode part waits on the host: a step of decode sequences can be captured in a graph.
 """
@@ -13,16 +16,19 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from .config import BLOCK8_CODES
+from .config import BLOCK8_CODES, BLOCK8_FIRST, BLOCK8_LAST
 from .mixed_batch import split_mixed_batch
 
 
 class JetFireBlock8Store:
     """Cache of one layer: ``k_data / v_data (H_kv, num_blocks * 16, 128)`` int8 or float8_e4m3fn, ``k_scales /
-    v_scales (H_kv, num_blocks)`` float32."""
+    v_scales (H_kv, num_blocks)`` float32.  ``top_blocks``: blocks that a decode token attends to (0: all); the store then keeps
+    ``bounds (H_kv, num_blocks, 2, 128)`` int8 to choose them by."""
 
     def __init__(self, *, num_blocks: int, num_kv_heads: int, head_dim: int = 128, codes: str = "int8", device="cuda",
-                 block_size: int = 16):
+                 block_size: int = 16, top_blocks: int = 0):
+        if top_blocks != 0 and top_blocks < BLOCK8_FIRST + BLOCK8_LAST:
+            raise ValueError(f"top_blocks must be 0 or at least {BLOCK8_FIRST + BLOCK8_LAST}, got {top_blocks}")
         if head_dim != 128 or block_size != 16:
             raise ValueError("the 8-bit cache is built for head_dim 128 and block_size 16")
         if codes not in BLOCK8_CODES:
@@ -36,15 +42,35 @@ class JetFireBlock8Store:
         self.v_data = torch.zeros(self.num_kv_heads, self.num_slots, head_dim, **data)
         self.k_scales = torch.zeros(self.num_kv_heads, self.num_blocks, dtype=torch.float32, device=self.device)
         self.v_scales = torch.zeros(self.num_kv_heads, self.num_blocks, dtype=torch.float32, device=self.device)
+        self.top_blocks = int(top_blocks)
+        self.bounds = torch.zeros(self.num_kv_heads, self.num_blocks, 2, head_dim, dtype=torch.int8, device=self.device) if top_blocks else None
 
     def append(self, key, value, query_start_loc, seq_lens, block_table) -> None:
         """``key / value (T, H_kv, 128)``: the new tokens of a step, ``seq_lens`` counting them already."""
-        ops.block8_append(key, value, query_start_loc, seq_lens, block_table, self.k_data, self.k_scales, self.v_data, self.v_scales)
+        kept = dict(bounds=self.bounds) if self.bounds is not None else {}
+        ops.block8_append(key, value, query_start_loc, seq_lens, block_table, self.k_data, self.k_scales, self.v_data, self.v_scales, **kept)
 
-    def decode(self, q, seq_lens, block_table, max_S, scale, **options):
-        """Attention of one query token per sequence (``ops.block8_decode_attn``)."""
-        return ops.block8_decode_attn(q, self.k_data, self.k_scales, self.v_data, self.v_scales, block_table, seq_lens, max_S,
-                                      int(q.shape[1]), self.num_kv_heads, self.block_size, scale, **options)
+    def append_rotary(self, query, key, value, positions, cos_sin, query_start_loc, seq_lens, block_table, *, interleaved=False, out=None):
+        """``append`` of keys that are rotated by their positions on the way; returns the rotated queries (``ops.block8_append_rotary``)."""
+        return ops.block8_append_rotary(query, key, value, positions, cos_sin, query_start_loc, seq_lens, block_table, self.k_data, self.k_scales,
+                                        self.v_data, self.v_scales, interleaved=interleaved, bounds=self.bounds, out=out)
+
+    def decode(self, q, seq_lens, block_table, max_S, scale, *, shared_blocks=0, **options):
+        """Attention of one query token per sequence: over the best blocks where the store chooses (``ops.block8_sparse_decode_attn``), else with
+        the first ``shared_blocks`` blocks of the first row, the same for all sequences, read once (``ops.block8_shared_prefix_attn``),
+        else over everything (``ops.block8_decode_attn``, which also serves layers with a window or a bias by distance)."""
+        cache = (q, self.k_data, self.k_scales, self.v_data, self.v_scales)
+        sizes = (seq_lens, max_S, int(q.shape[1]), self.num_kv_heads, self.block_size, scale)
+        if any(options.get(name) is not None for name in ("window", "alibi_slopes", "prefix_lens")):
+            return ops.block8_decode_attn(*cache, block_table, *sizes, **options)
+        options = {k: v for k, v in options.items() if v is not None}
+        if self.top_blocks and scale > 0:
+            out, lse, _ = ops.block8_sparse_decode_attn(*cache, self.bounds, block_table, *sizes, top_blocks=self.top_blocks, first_blocks=BLOCK8_FIRST,
+                                                        last_blocks=BLOCK8_LAST, **options)
+            return out, lse
+        if shared_blocks and q.shape[0]:
+            return ops.block8_shared_prefix_attn(*cache, block_table[0, :shared_blocks], block_table[:, shared_blocks:], *sizes, **options)
+        return ops.block8_decode_attn(*cache, block_table, *sizes, **options)
 
 
 def score_options(impl, device) -> dict:
@@ -96,7 +122,7 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
     """One step of a layer with an 8-bit cache: append, then attention.  ``query (T, H_q, D)`` or ``(T, H_q * D)``, ``key`` /
     ``value`` likewise with the KV heads, ``output`` like ``query``.  Returns ``output``, or None when the step's attention
     is not one this path serves and the caller's native attention has to.  The tokens are appended all the same where a later step
-    may be served -- after prompts with cached context, several query tokens over a cache, cascade attention -- and
+    may be served -- after prompts with cached context, several query tokens over a cache, cascade steps other than of decode tokens -- and
     not in a layer that never is (``served``)."""
     H_q, H_kv, D = int(layer.num_heads), int(layer.num_kv_heads), int(layer.head_size)
     T = int(attn_metadata.num_actual_tokens)
@@ -112,8 +138,12 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
     k, v = key[:T].reshape(T, H_kv, D), value[:T].reshape(T, H_kv, D)
     start, lens, table = _int32(attn_metadata.query_start_loc[:n + 1]), _int32(attn_metadata.seq_lens), attn_metadata.block_table[:n]
     store.append(k, v, start, lens, table)
-    if int(getattr(impl, "dcp_world_size", 1) or 1) > 1 or getattr(attn_metadata, "use_cascade", False) \
-            or not bool(getattr(attn_metadata, "causal", True)):
+    shared = 0      # blocks that all sequences begin with
+    if getattr(attn_metadata, "use_cascade", False):
+        shared = min(int(getattr(attn_metadata, "common_prefix_len", 0) or 0) // store.block_size, int(table.shape[1]))
+        if shared == 0 or int(attn_metadata.max_query_len) != 1:
+            return None
+    if int(getattr(impl, "dcp_world_size", 1) or 1) > 1 or not bool(getattr(attn_metadata, "causal", True)):
         return None
     options = score_options(impl, q.device)
     width = int(table.shape[1]) * store.block_size
@@ -121,7 +151,7 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
     def decode_rows(rows, q_rows, lens_rows, table_rows):
         # (a captured step is replayed with other lengths: up to what the table holds)
         longest = width if capturing else min(int(attn_metadata.max_seq_len), width)
-        out, _ = store.decode(q_rows, lens_rows, table_rows, max(longest, 1), float(impl.scale), **options)
+        out, _ = store.decode(q_rows, lens_rows, table_rows, max(longest, 1), float(impl.scale), shared_blocks=shared, **options)
         out = out.reshape(out.shape[0], *output.shape[1:])
         if isinstance(rows, slice):
             output[rows].copy_(out)

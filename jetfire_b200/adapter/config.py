@@ -40,6 +40,7 @@ SUPPORTED_TOP_K = (32, 64, 128, 256, 512, 1024, 2048, 4096)
 
 
 BLOCK8_CODES = ("int8", "e4m3")
+BLOCK8_FIRST, BLOCK8_LAST = 1, 2   # of the chosen blocks: the sequence's first, and its last
 NUMA_AUTO, NUMA_OFF = -2, -1   # the GPU's own node when the host has several / leave it to first touch
 
 
@@ -57,6 +58,7 @@ class JetFireConfig:
     stream_signal: str = "flags"          # how a stream-ordered step meets the host: "flags" or "callbacks"
     gpu_correction_share: float = 0.0     # fraction of the correction's rows the GPU computes from the mapped mirror
     block8: str | None = None             # codes of an 8-bit cache in place of the packed one and its mirror
+    block8_top: int = 0                   # blocks of it that a decode token attends to, chosen by their bounds (0: all)
 
     @property
     def scheme(self) -> QuantScheme:
@@ -130,11 +132,16 @@ def get_jetfire_config() -> JetFireConfig:
     block8 = (os.environ.get("JETFIRE_BLOCK8") or "off").strip().lower()
     if block8 not in ("off", *BLOCK8_CODES):
         raise ValueError(f"JETFIRE_BLOCK8 must be 'off' or one of {BLOCK8_CODES}, got {block8!r}")
+    block8_top = _int_env("JETFIRE_BLOCK8_TOP", 0)
+    if block8_top != 0 and block8_top < BLOCK8_FIRST + BLOCK8_LAST:
+        raise ValueError(f"JETFIRE_BLOCK8_TOP must be 0 or at least {BLOCK8_FIRST + BLOCK8_LAST}, got {block8_top}")
+    if block8_top and block8 == "off":
+        raise ValueError("JETFIRE_BLOCK8_TOP chooses among the blocks of an 8-bit cache: JETFIRE_BLOCK8 is off")
     _CONFIG = JetFireConfig(mode=mode, top_k=top_k, group_size=group, cpu_attn_threads=threads,
                             max_batch_size=_int_env("JETFIRE_MAX_BATCH_SIZE", 32),
                             slots_i32=_int_env("JETFIRE_SLOTS_I32", 1) != 0, numa_node=_numa_env(),
                             stream_ordered=_int_env("JETFIRE_STREAM_ORDERED", 1) != 0, stream_signal=signal,
-                            gpu_correction_share=share, block8=None if block8 == "off" else block8)
+                            gpu_correction_share=share, block8=None if block8 == "off" else block8, block8_top=block8_top)
     return _CONFIG
 
 

@@ -61,7 +61,7 @@ def install_layer_stores(layers: dict, *, num_blocks: int, block_size: int = 16,
             if not served(getattr(layer, "impl", layer)):
                 continue
             store = JetFireBlock8Store(num_blocks=int(num_blocks), num_kv_heads=int(layer.num_kv_heads), codes=cfg.block8, device=device,
-                                       block_size=int(block_size))
+                                       block_size=int(block_size), top_blocks=cfg.block8_top)
             register_layer_store(name, store)
             out[name] = store
             continue
