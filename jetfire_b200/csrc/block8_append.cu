@@ -497,7 +497,7 @@ __device__ __forceinline__ void write_block(const AppendParams& P, const AppendS
 enum { kPlain, kDirect, kStaged };
 constexpr int kTurns = 31;   // tokens: the chunk's and 15 more
 template <int DT, int CODES, bool VEC, int ROTARY>   // VEC: rows may be read 16 bytes at a time
-__global__ void __launch_bounds__(kWarps * 32, ROTARY == kStaged ? 5 : 1) block8_append_kernel(const __grid_constant__ AppendParams P, const __grid_constant__ Rotation R) {
+__global__ void __launch_bounds__(kWarps * 32, ROTARY == kStaged ? 5 : ROTARY == kDirect ? 1 : 0) block8_append_kernel(const __grid_constant__ AppendParams P, const __grid_constant__ Rotation R) {
   __shared__ __align__(16) float sm_turns[ROTARY == kStaged ? kTurns * JF_HEAD_DIM : 1];
   const float* turns = nullptr;
   const int lane = threadIdx.x & 31;
