@@ -606,8 +606,10 @@ typedef struct jf_block8_sparse_args {
 /* jf_block8_shared_attn is jf_block8_attn of sequences whose first 16 * shared_blocks positions are the same: the blocks of
  * shared_table (shared_blocks ids, 64-bit or 32-bit), in that order; position 16 * shared_blocks + i of sequence b is in block
  * attn.block_table[b][i / 16].  attn.seq_lens and attn.max_S count the shared positions; a sequence that ends
- * within them sees those before its end.  A block shared by the sequences is read once for all of them where they are many.  attn.window 0, no prefix_lens or
- * alibi_slopes. */
+ * within them sees those before its end (but for e4m3 codes and V scales that are no numbers, which no append writes: in shared blocks they
+ * may reach every sequence).  Where the sequences are many and the shared positions long, these meet all rows of a KV head in one
+ * product, and are read once for 256 rows.  attn.window 0, no prefix_lens or alibi_slopes.  A wait that ran out is noted in the
+ * library's record, as by jf_varlen_attn without one of its own, and returned likewise.  Three launches at most. */
 typedef struct jf_block8_shared_args {
   jf_block8_attn_args attn;
   const void* shared_table;
@@ -637,7 +639,7 @@ jf_status_t jf_block8_sparse_attn(const jf_block8_sparse_args* args, jf_stream_t
  * kernel meets (a wait that ran out: rows of out may not have been written) is noted there as
  * jf_decode_status_of_copy reads it.  Null: in a record of the library's, one a device, in host memory that
  * lives as long as the process.  An error found there is returned once, by jf_varlen_status or by the next
- * jf_varlen_attn without a record of its own that is not being captured, which then launches nothing.
+ * jf_varlen_attn without a record of its own (or jf_block8_shared_attn) that is not being captured, which then launches nothing.
  * jf_varlen_status never waits: after a synchronisation it speaks for all that came before. */
 typedef struct jf_varlen_attn_args {
   int32_t dtype, n_seqs, H_q, H_kv;

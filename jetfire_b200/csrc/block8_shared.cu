@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // (known to be the same for all lanes)
   const uint32_t up = (1024u - (smem_u32(raw) & 1023u)) & 1023u;
   if (up > kSmemBytes - kUsedBytes) {   // (nothing static is in front of it: it starts on a multiple of 1024)
+    pdl_wait();
     if (threadIdx.x == 0) report_status(P.status, JF_ERR_STATE);
     return;
   }

@@ -606,8 +606,10 @@ def block8_shared_prefix_attn(q, k_data, k_scales, v_data, v_scales, shared_tabl
 
     ``shared_table (n,)`` int64 or int32: the blocks of the first ``16 n`` positions, the same for every sequence; ``block_table (B,
     max_blocks)``: the blocks of each sequence's positions from ``16 n`` on.  ``seq_lens`` and ``max_S`` count the shared positions; a
-    sequence that ends within them sees those before its end.  A call captured in a graph is for one ``n``.  There is no window and no bias by distance; the
-    other arguments and the results are those of ``block8_decode_attn``."""
+    sequence that ends within them sees those before its end (but for e4m3 codes and V scales that are no numbers, which no append writes: in shared
+    blocks they may reach every sequence).  A call captured in a graph is for one ``n``.  There is no window and no bias by distance; the
+    other arguments and the results are those of ``block8_decode_attn``.  A wait inside the kernels that ran out (rows are then wrong) raises
+    ``JetFireError`` from the next call of this op or ``varlen_prefill_attn`` that is not being captured, or from ``varlen_prefill_status``."""
     name = "block8_shared_prefix_attn"
     st, out, lse = _host.block8_shared_attn(name, q, k_data, k_scales, v_data, v_scales, shared_table, block_table, seq_lens, max_S, H_q, H_kv, block_size,
                                             attn_scale, softcap, workspace, out)
@@ -662,8 +664,8 @@ def varlen_prefill_attn(q, k, v, cu_seqlens, attn_scale, *, causal=True, window=
 
 
 def varlen_prefill_status(device=None) -> None:
-    """Raises if a wait inside a ``varlen_prefill_attn`` on ``device`` (default: the current one) ran out since this was last
-    asked.  Never waits: after a synchronisation, of a replayed graph too, it speaks for all that came before."""
+    """Raises if a wait inside a ``varlen_prefill_attn`` or ``block8_shared_prefix_attn`` on ``device`` (default: the current one) ran out since
+    this was last asked.  Never waits: after a synchronisation, of a replayed graph too, it speaks for all that came before."""
     index = torch.device(device).index if device is not None else None
     check("varlen_prefill_attn", lib.jf_varlen_status(torch.cuda.current_device() if index is None else index))
 
