@@ -5,14 +5,18 @@
 // is an upper bound of q.k over block j, but for the query's rounding: lo and hi are the lowest and highest code of channel c in the
 // block (block bounds, kept by the append), unit_j what a code of 1 stands for, h runs through the query heads of
 // the KV head.  The sum is one integer product of 256 channels, exact, on the tensor cores (mma.s8: 16 blocks x 8
-// heads); it and the two factors that follow, in fp32, have one value whatever the order, so the choice is the same on every run and in every plain form.  Ties go to the lower block.
+// heads); it and the two factors that follow, in fp32, have one value whatever the order, so the choice is the same on every run
+// and in every plain form.  Ties go to the lower block.
 //
 // One kernel scores, 16 blocks a warp at a time, and leaves the scores as integers ordered like them; a second one, a block a row, brings a row's
 // integers to shared memory and finds the limit above which blocks are chosen: histograms of 2048 bins over the range it must lie in, until one
 // value is left or all that are left are taken.  A warp goes through a stretch of the row, so the list comes out in rising order by
 // counting votes, and what reads it adds up in the same order always.
 //
-// Bound: the scores by memory (260 bytes a block and KV head, 256 of them in one piece), the choice by latency: MEASURED
+// Bound: the scores by memory (260 bytes a block and KV head, 256 of them in one piece): 4 x 4096 blocks, 8 KV heads, 34 MB, 11.9 us from cold caches =
+// 2.9 TB/s, three dependent trips and two or four tiles a warp.  The choice by latency: a row of 4096 scores 4 us with warm caches (loads 0.7, the limit 1.7,
+// the list 1.9).  With the attention over 128 of 4096 blocks of four sequences the call takes 25 us back to back, over all of them
+// jf_block8_attn takes 101.  (Both in one kernel, a cluster a row with histograms over distributed shared memory: 31.)
 #include "block8.cuh"
 
 #include <algorithm>
@@ -192,6 +196,7 @@ __global__ void __launch_bounds__(kThreads) block8_choose_kernel(const __grid_co
     hi = max(hi, k);
   };
   // (rows begin on multiples of 16 bytes)
+#pragma unroll 2
   for (int i = threadIdx.x; i < n / 4; i += kThreads) {
     const uint4 k = *reinterpret_cast<const uint4*>(global + i * 4);
     if (STAGED) *reinterpret_cast<uint4*>(staged + i * 4) = k;
@@ -226,6 +231,7 @@ __global__ void __launch_bounds__(kThreads) block8_choose_kernel(const __grid_co
       for (int i = 0; i < kEach; ++i) S.count[threadIdx.x + i * kThreads] = 0;
       if (threadIdx.x == 0) S.bin = -1;
       __syncthreads();
+#pragma unroll 4
       for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint32_t k = keys[i];
         if (k >= from && k <= above) atomicAdd(&S.count[(k - from) >> shift], 1u);
@@ -280,6 +286,7 @@ __global__ void __launch_bounds__(kThreads) block8_choose_kernel(const __grid_co
   // ---- the list: keys beyond `above`, and the first `need` of those in [from, above] (all of them, or of one value).  A warp has a stretch of the row.
   const int stretch = (n + kWarps * 32 - 1) / (kWarps * 32) * 32, k0 = min(warp * stretch, n), k1 = min(k0 + stretch, n);
   int over = 0, ties = 0;
+#pragma unroll 4
   for (int i = k0; i < k1; i += 32) {
     const uint32_t k = i + lane < k1 ? keys[i + lane] : 0u;
     over += __popc(__ballot_sync(0xFFFFFFFFu, k > above));
@@ -297,6 +304,7 @@ __global__ void __launch_bounds__(kThreads) block8_choose_kernel(const __grid_co
     }
   at += min(number, need);
   const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
   for (int i = k0; i < k1; i += 32) {
     const uint32_t k = i + lane < k1 ? keys[i + lane] : 0u;
     const bool tie = k >= from && k <= above;

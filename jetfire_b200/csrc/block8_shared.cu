@@ -24,7 +24,9 @@
 // tile (128 rows or fewer) is worked on by both groups of warps, in turn on its tiles of positions.  What the sequences have behind the shared positions goes
 // through block8_attn.cu's kernel, whose partial results are joined with these ones.
 //
-// Bound: the tensor pipe and the exponentials in turn where there are 256 rows, else the conversion.
+// Bound: the tensor pipe and the exponentials in turn, and shared memory, which the operands, the codes and their conversion share.  A unit of 256 rows
+// takes 4400 cycles (3900 without copies and conversion): 256 sequences over 65536 positions, 64 / 8 heads, int8, 530 us = 1.04 PFLOP/s, 0.63 of what
+// cuBLAS reaches; the whole call 575 us against 4240 through block8_attn.cu.
 #include "block8.cuh"
 #include "decode_common.cuh"
 #include "tensor_common.cuh"
