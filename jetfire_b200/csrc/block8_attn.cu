@@ -193,7 +193,15 @@ __device__ __forceinline__ void soften4(float (&x)[4], float cap, float inv_cap)
   }
 }
 
-// (The blocks of a cluster share a sequence's pieces: no piece has to be looked for, and the results meet in shared memory.)
+// The blocks of a cluster share a sequence's pieces: no piece has to be looked for, and the results meet in shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {   // the same place in another block's shared memory
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
 __device__ __forceinline__ float4 load4_from(uint32_t at) {
   float4 x;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");

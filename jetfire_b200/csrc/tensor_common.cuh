@@ -50,11 +50,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* x) {
       "%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::JF_W8(x, 0), JF_W8(x, 8), JF_W8(x, 16), JF_W8(x, 24), "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::JF_W8(x, 0), JF_W8(x, 8), "r"(at)
-      : "memory");
-}
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -92,9 +87,9 @@ __device__ __forceinline__ uint64_t operand(uint32_t smem, uint32_t lead_bytes) 
   return static_cast<uint64_t>(smem >> 4 & 0x3FFFu) | static_cast<uint64_t>(lead_bytes >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
          1ull << 46 | 2ull << 61;
 }
-template <int DT> __device__ constexpr uint32_t instruction(bool b_mn_major, uint32_t columns = 128u) {
+template <int DT> __device__ constexpr uint32_t instruction(bool b_mn_major) {
   constexpr uint32_t type = DT == JF_DTYPE_BF16 ? 1u : 0u;
-  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | (columns >> 3) << 17 | (128u >> 4) << 24;
+  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
 }
 
 // ---- arithmetic on pairs ----------------------------------------------------------------------

@@ -23,8 +23,8 @@
 // the output are fp32.
 //
 // Bound: per 128 x 128 scores the two products take 1024 cycles of the tensor core, the exponentials 1024 of the special function units (16
-// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 908 to 940 us by itself = 1.17 to 1.21 PFLOP/s, 0.72 to 0.74 of what cuBLAS reaches, and
-// 1068 among other calls, with the card near its power cap.  A
+// a cycle).  One prompt of 8192 tokens, 64 / 8 heads, bf16, takes 883 to 902 us by itself = 1.22 to 1.25 PFLOP/s, 0.74 to 0.76 of what cuBLAS reaches, and
+// 1010 among other calls, with the card near its power cap.  A
 // step of both row tiles is 3500 cycles; with the weights left out it is 2950 (shared-memory reads of the operands and the hand-overs),
 // and a row tile by itself goes through 1750 from its scores to its weights and waits 1020 for the next ones.
 
