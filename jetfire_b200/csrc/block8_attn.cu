@@ -924,8 +924,10 @@ bool make_plan(int B, int H_q, int H_kv, int max_S, Plan& p) {
 // One sequence of 500 positions, 8 KV heads: 7.7 -> 6.0 us (6.2 with what the sums have gained since), of 4000: 11.7 -> 9.1; 64 of 300: 19.6 -> 17.4; 8 of 2000: 14.9 -> 12.4.  With 2
 // columns, 4000 positions take 9.2 us so and 8.6 in pieces.
 constexpr int kRounds = 6, kFewRounds = 2;
+// Blocks a warp up to which a sequence's part behind a shared prefix is one block's work, found without a search: 256 sequences of up to 509
+// positions, 8 KV heads, 86 -> 63 us.
 constexpr int kOwnRounds = 8;
-constexpr int kManyResults = 16;
+constexpr int kManyResults = 16;   // of a row, see where it is used
 int cluster_size(const Plan& p, int B, int H_kv, int64_t longest) {
   const int64_t blocks = (longest + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE, columns = static_cast<int64_t>(H_kv) * p.groups * B;
   const int64_t places = static_cast<int64_t>(num_sms()) * (p.nt == 1 ? 2 : 1);

@@ -654,7 +654,8 @@ struct Plan {
   int64_t items, units;
   uint64_t own, o_bytes, bytes;   // scratch of the own positions' part, of the outputs, of all
 };
-constexpr int kLeastUnits = 2;    // of a thread block
+// Units of a thread block at least: 8 to 64 sequences over 2048 positions, 32 / 8 heads, take 29 to 42 us with one, 26 to 40 with two, 34 to 54 with six.
+constexpr int kLeastUnits = 2;
 // Blocks that the sequences would read one after the other, each the shared ones for itself: up to here they do, in block8_attn.cu's kernel.  (The way
 // by the tensor cores is 14 us of launches, loads and joins before it is worth anything.  Back to back, 32 / 8 heads: 64 sequences over 256 positions
 // 18 and 28 us, 8 over 4096 22 and 19 (from cold caches 27 and 27), 32 over 1024 27 and 26, 16 over 4096 32 and 23, 16 over 16384 90 and 30; 8 / 1 heads: 4
