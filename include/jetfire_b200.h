@@ -609,7 +609,8 @@ typedef struct jf_block8_sparse_args {
  * within them sees those before its end (but for e4m3 codes and V scales that are no numbers, which no append writes: in shared blocks they
  * may reach every sequence).  Where the sequences are many and the shared positions long, these meet all rows of a KV head in one
  * product, and are read once for 256 rows.  attn.window 0, no prefix_lens or alibi_slopes.  A wait that ran out is noted in the
- * library's record, as by jf_varlen_attn without one of its own, and returned likewise.  Three launches at most. */
+ * library's record, as by jf_varlen_attn without one of its own, and returned likewise.  attn.workspace is aligned to 32 bytes at
+ * least.  Three launches at most. */
 typedef struct jf_block8_shared_args {
   jf_block8_attn_args attn;
   const void* shared_table;

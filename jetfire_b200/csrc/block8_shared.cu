@@ -49,6 +49,7 @@ constexpr float kLag = 8.0f, kLift = 7.0f;             // log2; weights stay bel
 constexpr float kSumLag = 24.0f, kSpread = 64.0f;
 constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr size_t kWorkspaceAlign = 32;                 // partial outputs are written 32 bytes at a time
 constexpr int kSmemBytes = 227 * 1024;                 // 6 operands, the codes and Shared leave 992 bytes to bring the first to a multiple of 1024
 
 struct SharedParams {
@@ -734,7 +735,7 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   at.workspace_bytes = a->attn.workspace_bytes;
   Plan p;
   if (!make_plan(at.B, at.H_q, at.H_kv, at.max_S, a->shared_blocks, p)) return JF_ERR_ARG;
-  if (at.workspace_bytes < p.bytes) return JF_ERR_WORKSPACE;
+  if (at.workspace_bytes < p.bytes || !aligned(at.workspace, kWorkspaceAlign)) return JF_ERR_WORKSPACE;
   if (!tensor_form(at.B, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
   const auto s = static_cast<cudaStream_t>(stream);
   SharedParams P{};
