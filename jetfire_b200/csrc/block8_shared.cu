@@ -736,11 +736,11 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   Plan p;
   if (!make_plan(at.B, at.H_q, at.H_kv, at.max_S, a->shared_blocks, p)) return JF_ERR_ARG;
   if (at.workspace_bytes < p.bytes || !aligned(at.workspace, kWorkspaceAlign)) return JF_ERR_WORKSPACE;
-  if (!tensor_form(at.B, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
   const auto s = static_cast<cudaStream_t>(stream);
   SharedParams P{};
-  jf_status_t st = wait_record(s, &P.status);
+  jf_status_t st = wait_record(s, &P.status);   // (an error of an earlier call is returned whichever way this one goes)
   if (st != JF_OK) return st;
+  if (!tensor_form(at.B, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
   P.q = static_cast<const uint16_t*>(at.q);
   P.k_data = static_cast<const uint8_t*>(at.k_data);
   P.v_data = static_cast<const uint8_t*>(at.v_data);
