@@ -75,7 +75,7 @@ __device__ __forceinline__ float half_step(float d) { return ex2(-0.5f * d); }
 struct Span { int len, prefix, lo, head, first, count; };
 __device__ __forceinline__ Span span_of(const AttnParams& P, int length, int prefix) {
   Span s;
-  s.len = max(0, min(min(length, P.max_S) - P.behind, P.max_blocks * JF_BLOCK_SIZE));
+  s.len = min(max(min(length, P.max_S), P.behind) - P.behind, P.max_blocks * JF_BLOCK_SIZE);   // (a length may be any number)
   const int blocks = (s.len + JF_BLOCK_SIZE - 1) / JF_BLOCK_SIZE;
   s.prefix = s.lo = s.head = s.first = 0;
   s.count = P.chosen ? min(blocks, P.top) : blocks;
