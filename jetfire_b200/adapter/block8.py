@@ -9,7 +9,8 @@ sequences that share a prefix (vLLM's cascade steps) reads the prefix once for a
 for it keeps block bounds and lets a decode token attend to its best blocks only (``ops.block8_sparse_decode_attn``; a choice of the
 user's, ``JETFIRE_BLOCK8_TOP``).
 
-Nothing of the decode part waits on the host: a step of decode sequences can be captured in a graph.
+Nothing of the decode part waits on the host: a step of decode sequences can be captured in a graph.  What they share is known on the
+host only and may be another prefix when the graph is replayed, so a captured cascade step goes through every sequence's whole table.
 """
 from __future__ import annotations
 
@@ -143,6 +144,8 @@ def try_block8_attention(*, impl, layer, query, key, value, attn_metadata, outpu
         shared = min(int(getattr(attn_metadata, "common_prefix_len", 0) or 0) // store.block_size, int(table.shape[1]))
         if shared == 0 or int(attn_metadata.max_query_len) != 1:
             return None
+        if capturing:      # (replayed with sequences that share something else, or nothing: everything is in their tables too)
+            shared = 0
     if int(getattr(impl, "dcp_world_size", 1) or 1) > 1 or not bool(getattr(attn_metadata, "causal", True)):
         return None
     options = score_options(impl, q.device)
