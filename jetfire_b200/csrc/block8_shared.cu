@@ -657,21 +657,28 @@ struct Plan {
 };
 // Units of a thread block at least: 8 to 64 sequences over 2048 positions, 32 / 8 heads, take 29 to 42 us with one, 26 to 40 with two, 34 to 54 with six.
 constexpr int kLeastUnits = 2;
-// Blocks that the sequences would read one after the other, each the shared ones for itself: up to here they do, in block8_attn.cu's kernel.  (The way
-// by the tensor cores is 14 us of launches, loads and joins before it is worth anything.  Back to back, 32 / 8 heads: 64 sequences over 256 positions
-// 18 and 28 us, 8 over 4096 22 and 19 (from cold caches 27 and 27), 32 over 1024 27 and 26, 16 over 4096 32 and 23, 16 over 16384 90 and 30; 8 / 1 heads: 4
-// over 65536 21 and 26, 8 over 65536 30 and 27.)
-constexpr int64_t kFewBlocks = 20000;
+// Whether the shared positions go through the tensor cores, or once for every sequence through block8_attn.cu's kernel.  That one takes 5.5e-4 us
+// for a block of a KV head and a sequence (5/3 of it for every 16 query heads, where a KV head has more than 8), this one 1.6e-3 us for a block of a KV head
+// and 9 us more of launches, loads and joins: what three sequences read is not worth it, what a fourth and others do from 16000 blocks on.  Back to
+// back, us, decode kernel / this one:
+//   32 / 8 heads, 65536 positions: 1 sequence 34 / 67, 2 48 / 68, 3 65 / 68, 4 82 / 68, 8 168 / 69; 16384: 3 25 / 26, 4 29 / 26, 8 51 / 27;
+//     4096: 4 14 / 16, 8 22 / 19, 16 33 / 23; 32 over 1024 27 / 26, over 2048 42 / 29; 64 over 512 23 / 28, over 1024 49 / 29; 128 over 512 39 / 41
+//   8 / 1: 4 over 131072 30 / 33, 8 over 32768 21 / 24, 8 over 65536 30 / 27, 16 over 16384 21 / 22, 16 over 32768 30 / 29
+//   32 / 2: 1 over 131072 27 / 41, 2 41 / 43, 3 57 / 45; 4 over 32768 27 / 26, over 65536 41 / 34; 8 over 8192 20 / 22, over 16384 27 / 26; 16 over 4096 22 / 23, over 8192 30 / 24
+//   40 / 1: 1 over 131072 34 / 37, 2 over 32768 23 / 26, over 65536 34 / 30, 4 over 16384 23 / 20, 16 over 4096 25 / 23
+// From cold caches a call takes 7 to 9 us more by the decode kernel, 8 to 20 by this one.
+constexpr int64_t kFewBlocks = 16000;
 
-bool tensor_form(int B, int H_kv, int max_S, int shared_blocks) {
-  const int seen = std::min(shared_blocks, (max_S - 1) / JF_BLOCK_SIZE + 1);
-  return int64_t{B} * H_kv * seen > kFewBlocks;
+bool tensor_form(int B, int H_q, int H_kv, int max_S, int shared_blocks) {
+  const int seen = std::min(shared_blocks, (max_S - 1) / JF_BLOCK_SIZE + 1), G = H_q / H_kv;
+  const int64_t thirds = int64_t{B} * (G <= 8 ? 3 : 5 * ((G + 15) / 16));
+  return (thirds - 9) * H_kv * seen > 3 * kFewBlocks;
 }
 
 bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) {
   if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_S <= 0 || H_q % H_kv != 0 || shared_blocks < 0 || shared_blocks > INT32_MAX / JF_BLOCK_SIZE - 1) return false;
   p = Plan{};
-  if (!tensor_form(B, H_kv, max_S, shared_blocks)) {
+  if (!tensor_form(B, H_q, H_kv, max_S, shared_blocks)) {
     p.bytes = block8_attn_workspace(B, H_q, H_kv, max_S);
     return p.bytes > 0;
   }
@@ -740,7 +747,7 @@ extern "C" jf_status_t jf_block8_shared_attn(const jf_block8_shared_args* a, jf_
   SharedParams P{};
   jf_status_t st = wait_record(s, &P.status);   // (an error of an earlier call is returned whichever way this one goes)
   if (st != JF_OK) return st;
-  if (!tensor_form(at.B, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
+  if (!tensor_form(at.B, at.H_q, at.H_kv, at.max_S, a->shared_blocks)) return block8_attend(&at, from, stream, true);
   P.q = static_cast<const uint16_t*>(at.q);
   P.k_data = static_cast<const uint8_t*>(at.k_data);
   P.v_data = static_cast<const uint8_t*>(at.v_data);
