@@ -50,7 +50,7 @@ constexpr float kSumLag = 24.0f, kSpread = 64.0f;
 constexpr float kNone = -3.0e38f;                      // the reference of a row that has seen nothing (finite: differences are numbers)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr size_t kWorkspaceAlign = 32;                 // partial outputs are written 32 bytes at a time
-constexpr int kSmemBytes = 227 * 1024;                 // 6 operands, the codes and Shared leave 992 bytes to bring the first to a multiple of 1024
+constexpr int kSmemBytes = 227 * 1024;
 
 struct SharedParams {
   const uint16_t* q;
@@ -103,7 +103,7 @@ struct Shared {
 };
 
 constexpr int kUsedBytes = 6 * kTileBytes + kStaged * kCodeBytes + static_cast<int>(sizeof(Shared));
-static_assert(kUsedBytes <= kSmemBytes, "");
+static_assert(kUsedBytes + 1023 <= kSmemBytes, "the operands start on a multiple of 1024, wherever shared memory does");
 
 // The units of a thread block, item by item (an item: a KV head and a pair of row tiles).
 struct Segment { int u, end, item, first, n; };   // n tiles of positions from `first` on
@@ -579,11 +579,6 @@ __global__ void __launch_bounds__(kThreads, 1) block8_shared_kernel(const __grid
   extern __shared__ unsigned char raw[];
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // (known to be the same for all lanes)
   const uint32_t up = (1024u - (smem_u32(raw) & 1023u)) & 1023u;
-  if (up > kSmemBytes - kUsedBytes) {   // (nothing static is in front of it: it starts on a multiple of 1024)
-    pdl_wait();
-    if (threadIdx.x == 0) report_status(P.status, JF_ERR_STATE);
-    return;
-  }
   unsigned char *smem = raw + up, *kv = smem + 2 * kTileBytes, *staged = kv + 4 * kTileBytes;
   Shared& S = *reinterpret_cast<Shared*>(staged + kStaged * kCodeBytes);
   if (threadIdx.x == 0) {
