@@ -653,21 +653,21 @@ struct Plan {
 // Units of a thread block at least: 8 to 64 sequences over 2048 positions, 32 / 8 heads, take 29 to 42 us with one, 26 to 40 with two, 34 to 54 with six.
 constexpr int kLeastUnits = 2;
 // Whether the shared positions go through the tensor cores, or once for every sequence through block8_attn.cu's kernel.  That one takes 5.5e-4 us
-// for a block of a KV head and a sequence (5/3 of it for every 16 query heads, where a KV head has more than 8), this one 1.6e-3 us for a block of a KV head
-// and 9 us more of launches, loads and joins: what three sequences read is not worth it, what a fourth and others do from 16000 blocks on.  Back to
-// back, us, decode kernel / this one:
+// for a block of a KV head and a sequence (1.5 times that for every 16 query heads, where a KV head has more than 8).  This one takes what three such readings
+// do for a block of a KV head, what 10 more do for a sequence's own positions and its part of the join, and 7 us of launches and loads.  Back to back, us,
+// decode kernel / this one:
 //   32 / 8 heads, 65536 positions: 1 sequence 34 / 67, 2 48 / 68, 3 65 / 68, 4 82 / 68, 8 168 / 69; 16384: 3 25 / 26, 4 29 / 26, 8 51 / 27;
-//     4096: 4 14 / 16, 8 22 / 19, 16 33 / 23; 32 over 1024 27 / 26, over 2048 42 / 29; 64 over 512 23 / 28, over 1024 49 / 29; 128 over 512 39 / 41
-//   8 / 1: 4 over 131072 30 / 33, 8 over 32768 21 / 24, 8 over 65536 30 / 27, 16 over 16384 21 / 22, 16 over 32768 30 / 29
-//   32 / 2: 1 over 131072 27 / 41, 2 41 / 43, 3 57 / 45; 4 over 32768 27 / 26, over 65536 41 / 34; 8 over 8192 20 / 22, over 16384 27 / 26; 16 over 4096 22 / 23, over 8192 30 / 24
+//     4096: 4 14 / 16, 8 22 / 19, 16 33 / 23; 32 over 1024 27 / 26, over 2048 42 / 29; 64 over 512 23 / 28, over 1024 49 / 29; 128 over 512 39 / 41, 256 over 256 56 / 61
+//   8 / 1: 4 over 131072 30 / 33, 8 over 32768 21 / 24, over 65536 30 / 27, 16 over 16384 21 / 22, over 32768 30 / 29; 64 over 2048 14 / 22, 256 over 1024 39 / 27
+//   32 / 2: 1 over 131072 27 / 41, 2 41 / 43, 3 57 / 45; 3 over 65536 34 / 34, 4 41 / 34; 8 over 8192 20 / 22, over 16384 27 / 26; 16 over 4096 22 / 23, over 8192 30 / 24
 //   40 / 1: 1 over 131072 34 / 37, 2 over 32768 23 / 26, over 65536 34 / 30, 4 over 16384 23 / 20, 16 over 4096 25 / 23
 // From cold caches a call takes 7 to 9 us more by the decode kernel, 8 to 20 by this one.
-constexpr int64_t kFewBlocks = 16000;
+constexpr int64_t kFewBlocks = 13500;
 
 bool tensor_form(int B, int H_q, int H_kv, int max_S, int shared_blocks) {
   const int seen = std::min(shared_blocks, (max_S - 1) / JF_BLOCK_SIZE + 1), G = H_q / H_kv;
-  const int64_t thirds = int64_t{B} * (G <= 8 ? 3 : 5 * ((G + 15) / 16));
-  return (thirds - 9) * H_kv * seen > 3 * kFewBlocks;
+  const int64_t halves = int64_t{B} * (G <= 8 ? 2 : 3 * ((G + 15) / 16));   // of a reading
+  return H_kv * ((halves - 6) * seen - 20ll * B) > 2 * kFewBlocks;
 }
 
 bool make_plan(int B, int H_q, int H_kv, int max_S, int shared_blocks, Plan& p) {

@@ -24,11 +24,12 @@ def test_one_sequence_of_sixteen_heads(L, positions):
 
 
 @pytest.mark.parametrize("B, H_q, H_kv, positions", [(4, 32, 8, 65536), (8, 32, 8, 16384), (16, 32, 8, 4096), (64, 64, 8, 2048), (256, 64, 8, 65536),
-                                                     (8, 8, 1, 65536), (4, 32, 2, 65536), (2, 40, 1, 131072), (90, 64, 8, 480)])
+                                                     (8, 8, 1, 65536), (4, 32, 2, 65536), (2, 40, 1, 131072), (90, 64, 8, 480), (256, 8, 1, 1024)])
 def test_many_or_long(L, B, H_q, H_kv, positions):
     assert not _by_decode(L, B, H_q, H_kv, positions)
 
 
-@pytest.mark.parametrize("B, H_q, H_kv, positions", [(4, 32, 8, 2048), (64, 32, 8, 512), (16, 8, 1, 16384), (100, 64, 8, 0), (4, 32, 2, 16384), (2, 40, 1, 16384)])
+@pytest.mark.parametrize("B, H_q, H_kv, positions", [(4, 32, 8, 2048), (64, 32, 8, 512), (16, 8, 1, 16384), (100, 64, 8, 0), (4, 32, 2, 16384), (2, 40, 1, 16384), (1, 40, 1, 131072),
+                                                     (256, 64, 8, 256), (256, 32, 8, 128)])
 def test_short(L, B, H_q, H_kv, positions):
     assert _by_decode(L, B, H_q, H_kv, positions)
