@@ -595,7 +595,8 @@ jf_status_t jf_block8_append_rotary(const jf_block8_rotary_args* args, jf_stream
  * h through the query heads of the KV head, lo and hi the block's bounds, unit_j its K scale (e4m3: times 448 / 127), all in
  * fp32.  A head with an element that is no number has no score, nor has a block without a valid id or with a NaN as its scale; what
  * has none comes last.  chosen (B, H_kv, top_blocks): the blocks' numbers, rising, then -1.
- * attn.attn_scale > 0, attn.window 0, no prefix_lens or alibi_slopes; attn.max_S up to 2^22.  Three launches at most. */
+ * attn.attn_scale > 0, attn.window 0, no prefix_lens or alibi_slopes; attn.max_S up to 2^22.  Four launches at most: scores, choice,
+ * attention, and a join where the chosen blocks are more than the attention goes through in one. */
 typedef struct jf_block8_sparse_args {
   jf_block8_attn_args attn;
   const int8_t* bounds;           /* (H_kv, num_blocks, 2, 128), 16-byte aligned */

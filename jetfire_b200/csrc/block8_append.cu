@@ -16,7 +16,10 @@
 // all rows the block then holds: rounding keeps the order, so they are found among the scaled numbers and rounded once.
 //
 // Rotated: 8192 tokens, 64 / 8 heads, bf16 -> int8 with bounds (324 MB) 96 us from cold caches = 3.4 TB/s: the queries' rows alone 58, K and V
-// alone 53 (K's warps rotate in fp32, twice); four sequences of a token, 32 / 8 heads, 3.8 us back to back.
+// alone 53.  K's staged warps have 96 registers and spill 180 to 192 bytes a thread, and V's and the
+// queries' run with the same 20 warps a multiprocessor: 44 % of the issue slots are used, it is latency that is left.  Four sequences of a token, 32 / 8 heads,
+// 3.8 us back to back.  Bounds without a rotation go through the same kernels: 8192 tokens, 8 KV heads, 36 us from cold caches and 14.7 back to back (without
+// bounds 18 and 8.3; e4m3 37 and 15.5), 64 single tokens 11.7 and 3.9 (9.5 and 3.1; e4m3 12.9 and 5.3).
 //
 // Bound: memory -- 2 bytes read and 1 written per element.  8192 tokens, 8 KV heads, bf16 -> int8 (50 MB): 13.6 us = 3.7 TB/s, 16384: 22.1 us = 4.6
 // TB/s; a warp's start (bounds, length, block id, rows: four dependent trips) and 700 instructions a block are what is left.

@@ -159,10 +159,13 @@ __device__ __forceinline__ void bulk_g2s_u32(uint32_t dst, const void* src, uint
 }
 // Programmatic dependent launch.  A kernel launched with launch_pdl may start while the
 // kernel before it in the stream is still running (after that kernel's CTAs have all called
-// pdl_trigger or exited); it must call pdl_wait before it touches any global memory, which
-// returns once the earlier kernel has completed and its writes are visible.  Without the
-// launch attribute both are no-ops.  Only work that needs no global memory (barrier
-// initialisation, address arithmetic) is placed ahead of pdl_wait.
+// pdl_trigger or exited); it must call pdl_wait before it touches global memory that the earlier
+// kernel writes or reads, which returns once that kernel has completed and its writes are visible.
+// Without the launch attribute both are no-ops.  Ahead of pdl_wait comes work that needs no global
+// memory (barrier initialisation, address arithmetic).  A kernel that touches some there says why it
+// may: the one before it is of the same call, every block of that one calls pdl_wait before
+// pdl_trigger, and it neither writes what is read nor reads what is written ahead of the wait.  Every
+// block calls pdl_wait at some point, since the kernel behind relies on all that came before.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
